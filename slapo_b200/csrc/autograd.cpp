@@ -1,6 +1,6 @@
 // Differentiable front ends of the kernels: the autograd nodes of linear, bias + activation,
-// bias + dropout + residual, the normalisations, flash attention and T5's relative bias, as C++
-// functions.
+// bias + dropout + residual, the normalisations, flash attention, T5's relative bias and the token
+// table's lookup, as C++ functions.
 //
 // A layer of a small model is a few kernels of some microseconds each; a Python autograd function
 // costs about 30 us per direction on the host (argument packing, the interpreter, one operator
@@ -394,6 +394,28 @@ tensor_list RelBiasFn::backward(AutogradContext* ctx, tensor_list grads) {
   return {RelBiasSumFn::apply(grads[0], s[1], s[0].detach()), Tensor()};
 }
 
+// Rows of a table by token ids; the ids are what the backward needs.
+struct EmbeddingFn : public Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, int64_t start,
+                        const optional<int64_t>& padding, double scale) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = weight.size(0);
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["scale"] = scale;
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, double)>("slapo_b200::embedding_fwd");
+    return f.call(ids, weight, start, scale);
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, int64_t, const optional<int64_t>&, double)>(
+        "slapo_b200::embedding_bwd");
+    return {f.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
+                   ctx->saved_data["start"].toInt(), ctx->saved_data["padding"].toOptional<int64_t>(),
+                   ctx->saved_data["scale"].toDouble()),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ------------------------------------------------------------------------ //
 // A bias that starts anywhere, as the kernels read it: 16 bytes at a time.  (A copy that is differentiated.)
 Tensor aligned(const Tensor& bias) {
@@ -444,6 +466,11 @@ Tensor flash(const Tensor& q, const optional<Tensor>& k, const optional<Tensor>&
   return FlashFn::apply(q, k, v, key_bias, rel, causal, scale, p);
 }
 
+Tensor embedding(const Tensor& ids, const Tensor& weight, int64_t start, const optional<int64_t>& padding,
+                 double scale) {
+  return EmbeddingFn::apply(weight, ids, start, padding, scale);
+}
+
 Tensor rel_bias(const Tensor& table, const Tensor& buckets) { return RelBiasFn::apply(table, buckets); }
 
 }  // namespace
@@ -458,6 +485,7 @@ void register_autograd_ops(torch::Library& m) {
   m.def("dropout_add_norm(Tensor x, Tensor? bias, Tensor residual, Tensor weight, Tensor? ln_bias, float p, float eps) -> (Tensor, Tensor)",
         &dropout_add_norm);
   m.def("rel_bias(Tensor table, Tensor buckets) -> Tensor", &rel_bias);
+  m.def("embedding(Tensor ids, Tensor weight, int start, int? padding, float scale) -> Tensor", &embedding);
   m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p) -> Tensor",
         &flash);
 }

@@ -299,6 +299,8 @@ void register_gemm_ops(torch::Library& m);
 void register_attn_ops(torch::Library& m);
 void register_comm_ops(torch::Library& m);
 void register_loss_ops(torch::Library& m);
+void register_optim_ops(torch::Library& m);
+void register_embed_ops(torch::Library& m);
 void register_autograd_ops(torch::Library& m);
 
 TORCH_LIBRARY(slapo_b200, m) {
@@ -327,5 +329,7 @@ TORCH_LIBRARY(slapo_b200, m) {
   register_attn_ops(m);
   register_comm_ops(m);
   register_loss_ops(m);
+  register_optim_ops(m);
+  register_embed_ops(m);
   register_autograd_ops(m);
 }

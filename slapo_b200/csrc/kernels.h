@@ -32,6 +32,47 @@ void launch_fused_adamw(void* param, const void* grad, float* master, float* exp
                         float weight_decay, float bc1, float bc2, int dtype, cudaStream_t stream,
                         const float* hyper = nullptr);
 
+// Token table (embedding.cu): out[t] = scale * w[ids[t] - start], rows of zeros for ids outside of [start, start + rows)
+int launch_embedding_fwd(const void* ids, bool ids64, const void* w, void* out, int64_t tokens, int64_t rows,
+                         int64_t cols, int64_t row_stride, int64_t start, float scale, int dtype,
+                         cudaStream_t stream);
+// Its gradient: dw [rows, cols] contiguous, every row written; tokens with id `padding` have none.
+// Scratch in 32-bit words: ids and places twice (`sorted` each), the rows' ranges, shares of frequent rows.
+struct EmbedGradPlan {
+  int64_t sorted, range, shares, part;
+  int share;          // sorted tokens to a share
+  int64_t words() const { return 4 * sorted + range + part; }
+};
+EmbedGradPlan embedding_bwd_plan(int64_t tokens, int64_t rows, int64_t cols);
+int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, int32_t* scratch,
+                         const EmbedGradPlan& plan, int64_t tokens, int64_t rows, int64_t cols, int64_t start,
+                         int64_t padding, float scale, int dtype, cudaStream_t stream);
+
+// AdamW over many tensors (adamw_multi.cu).  Pointers of one tensor of n values in row order; master: fp32 weights
+// or null (then `param` is what is updated); m, v: moments, fp32 or with m_scale and v_scale 8 bits in blocks of 256;
+// aligned: all on 16 bytes (8-bit moments on 8), so that vectors of eight can be read
+struct AdamwTensor {
+  void* param;
+  const void* grad;
+  float* master;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  int64_t n;
+  float lr, weight_decay;
+  int aligned;
+};
+struct AdamwScalars {
+  float beta1, one_beta1, beta2, one_beta2, eps;
+  float inv_bc1, inv_sqrt_bc2;        // 1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t): where `step` is null
+  const int64_t* step;                // t on the device, or null
+  double beta1_d, beta2_d;
+  const float* grad_scale;            // factor on every gradient, or null
+};
+int launch_adamw_multi(const AdamwTensor* t, int n, const AdamwScalars& s, bool bits8, int dtype,
+                       cudaStream_t stream);
+
 // C[M,N] = act(A B^T + bias); a_mn / b_mn select M/N-major operands (see gemm.cu).
 // Returns 0 on success, >0 when the launch was refused on the host.
 // `epi`: an activation (A and B K-major) or its derivative (B N-major) in the epilogue, as a layer's forward and

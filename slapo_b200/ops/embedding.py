@@ -1,4 +1,9 @@
-"""Vocabulary-parallel embedding whose forward needs no all-reduce.
+"""Token tables.
+
+``FusedEmbedding`` is ``nn.Embedding`` on ``csrc/embedding.cu``: the lookup with a factor, and a gradient
+that sorts the tokens instead of adding atomically.
+
+``FusedVocabParallelEmbedding`` is a vocabulary-parallel embedding whose forward needs no all-reduce.
 
 With the vocabulary split over the tensor-parallel group, exactly one rank
 owns the row of every token id.  ``FusedVocabParallelEmbedding`` lets that
@@ -15,14 +20,43 @@ the tokens: the owner of a row stores it into that one rank (the
 reduce-scatter of the recipe's hooks, slapo/model_schedule/gpt2.py:343-355 and
 424-432 of the reference, without looking up or adding zeros).  The backward
 first gathers the token-sharded output gradient with the peer-load gather
-kernel, then accumulates locally as before.
+kernel, then accumulates locally as before.  (Locally: ``csrc/embedding.cu`` on the shard's
+ids, the others' give nothing.)
 """
 from __future__ import annotations
 
 import torch
 from torch import nn
 
+from . import functional as NF
 from . import native
+
+
+class FusedEmbedding(nn.Embedding):
+    """``nn.Embedding`` whose rows are multiplied by ``scale``, with the fused lookup and gradient.
+
+    Ids outside of the table give zeros (see :func:`slapo_b200.ops.functional.embedding`).  ``max_norm``,
+    ``scale_grad_by_freq`` and ``sparse`` are not supported."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
+        self.scale = float(scale)
+
+    @classmethod
+    def from_embedding(cls, emb: nn.Embedding, scale=1.0):
+        """The same table (the same parameter) as a fused module."""
+        if emb.max_norm is not None or emb.scale_grad_by_freq or emb.sparse:
+            raise ValueError("max_norm, scale_grad_by_freq and sparse are not supported")
+        new = cls(emb.num_embeddings, emb.embedding_dim, emb.padding_idx, scale, device="meta",
+                  dtype=emb.weight.dtype)
+        new.weight = emb.weight
+        return new
+
+    def forward(self, ids):
+        return NF.embedding(ids, self.weight, self.padding_idx, self.scale)
+
+    def extra_repr(self):
+        return super().extra_repr() + (f", scale={self.scale}" if self.scale != 1.0 else "")
 
 
 class _VocabEmbedFn(torch.autograd.Function):
@@ -57,8 +91,6 @@ class _VocabEmbedFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         (flat,) = ctx.saved_tensors
-        local = flat - ctx.lo
-        own = (local >= 0) & (local < ctx.rows)
         if ctx.sp_axis is not None:
             # every rank needs the gradient rows of the ids it owns, whoever kept the token
             from ..parallel.fused_tp import peer_gather
@@ -71,8 +103,7 @@ class _VocabEmbedFn(torch.autograd.Function):
                 full = full.view(world, b, s // world, -1).permute(1, 0, 2, 3)
             grad = full.reshape(flat.numel(), -1)
         g = grad.reshape(flat.numel(), -1)
-        grad_w = torch.zeros(ctx.rows, g.shape[1], dtype=torch.float32, device=g.device)
-        grad_w.index_add_(0, local[own], g[own].float())
+        grad_w = native.ops().embedding_bwd(g, flat, ctx.rows, ctx.lo, None, 1.0)
         return None, grad_w.to(ctx.dtype), None
 
 

@@ -149,6 +149,32 @@ def mlp(x, w1, b1, w2, b2, act: str, p: float):
 
 
 # ---------------------------------------------------------------------- #
+# token table
+def embedding(ids, weight, padding_idx=None, scale: float = 1.0, vocab_start: int = 0):
+    """``scale * weight[ids - vocab_start]`` for int64 or int32 ``ids`` of any shape.
+
+    Ids outside of ``[vocab_start, vocab_start + rows)`` give zeros and no gradient, so that a shard of a
+    table takes the ids of all (no id is an error).  Tokens with id ``padding_idx`` have no gradient.  The
+    gradient of a row is summed in fp32 in the order of its tokens and rounded once, the same every time."""
+    if weight.dim() != 2:
+        raise ValueError(f"a 2-D table is required, not {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"ids of int64 or int32 are required, not {ids.dtype}")
+    if padding_idx is not None and padding_idx < 0:
+        raise ValueError(f"padding_idx is an id, not counted from the end: {padding_idx}")
+    if _native_ok(weight):
+        return _nodes().embedding(ids, weight, vocab_start, padding_idx, float(scale))
+    row = ids.long() - vocab_start
+    own = (row >= 0) & (row < weight.shape[0])
+    out = weight[torch.where(own, row, torch.zeros_like(row))] if weight.shape[0] else \
+        weight.new_zeros(*ids.shape, weight.shape[1])
+    if padding_idx is not None:
+        out = torch.where((ids != padding_idx)[..., None], out, out.detach())
+    out = torch.where(own[..., None], out, torch.zeros_like(out))
+    return out if scale == 1.0 else (out.float() * scale).to(out.dtype)
+
+
+# ---------------------------------------------------------------------- #
 # dropout family
 def effective_dropout_p(p: float) -> float:
     """Dropout probability the CUDA kernels actually apply.  They draw 7-bit

@@ -1,0 +1,175 @@
+"""AdamW over many tensors: the plain form against the formula in 64 bits and against torch.optim.AdamW, the
+8-bit moments' format, the optimizer's bookkeeping and what it refuses."""
+import copy
+import math
+
+import pytest
+import torch
+
+from slapo_b200.op import FusedAdamW, dequantize_moment, multi_tensor_adamw, quantize_moment
+from slapo_b200.ops.adamw import STATE_BLOCK, state_blocks
+
+
+def _model():
+    torch.manual_seed(3)
+    return torch.nn.Sequential(torch.nn.Linear(13, 7), torch.nn.LayerNorm(7), torch.nn.Linear(7, 5))
+
+
+def _grads(model, seed):
+    g = torch.Generator().manual_seed(seed)
+    for p in model.parameters():
+        p.grad = torch.randn(p.shape, generator=g).to(p.dtype)
+
+
+def test_follows_torch_adamw():
+    a, b = _model(), _model()
+    groups = lambda m: [{"params": [m[0].weight, m[2].weight], "weight_decay": 0.1},    # noqa: E731
+                        {"params": [m[0].bias, m[2].bias, *m[1].parameters()], "weight_decay": 0.0,
+                         "lr": 3e-3}]
+    mine = FusedAdamW(groups(a), lr=1e-2, betas=(0.8, 0.95))
+    ref = torch.optim.AdamW(groups(b), lr=1e-2, betas=(0.8, 0.95))
+    for step in range(5):
+        _grads(a, step)
+        _grads(b, step)
+        mine.step()
+        ref.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        # (a step moves a weight by at most about lr; a few roundings of 2^-24 of it and of the weight)
+        torch.testing.assert_close(p, q, rtol=16 * 2.0 ** -24, atol=5 * 1e-2 * 16 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("second", [False, True])
+@pytest.mark.parametrize("n", [1, 255, 256, 257, 1000])
+def test_8bit_moments_keep_their_precision(n, second):
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g))
+    if second:
+        x = x * x
+    codes, scale = quantize_moment(x, second)
+    assert codes.dtype == torch.float8_e4m3fn and scale.shape == (state_blocks(n),)
+    mantissa, _ = torch.frexp(scale)
+    assert bool((mantissa == 0.5).all())                      # powers of two
+    held = x.double().sqrt() if second else x.double()
+    value = codes.double() * scale.double().repeat_interleave(STATE_BLOCK)[:n]
+    factor = scale.double().repeat_interleave(STATE_BLOCK)[:n]
+    # half a step: 2^-4 of the value, or 2^-10 of the factor (the square root itself is rounded to 2^-24);
+    # what would be rounded to zero is held as 2^-9 of it
+    least = factor * (2.0 ** -9 if second else 2.0 ** -10)
+    bound = torch.maximum(held.abs() * 2.0 ** -4, least) * (1 + 2.0 ** -22)
+    assert bool(((value - held).abs() <= bound).all())
+    assert bool((codes.float().abs() <= 448).all())
+    if second:
+        assert bool((value[held > 0] > 0).all())
+    again, scale2 = quantize_moment(dequantize_moment(codes, scale, second), second)
+    assert torch.equal(again.float(), codes.float()) or not torch.equal(scale, scale2)
+
+
+def test_8bit_factor_is_the_smallest_that_fits():
+    for top, want in ((448.0, 1.0), (448.5, 2.0), (224.0, 0.5), (1.0, 2.0 ** -8), (0.0, 2.0 ** -126),
+                      (2.0 ** -130, 2.0 ** -126)):
+        x = torch.zeros(300)
+        x[7] = -top
+        _, scale = quantize_moment(x)
+        assert scale.tolist() == [want, 2.0 ** -126], (top, scale)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_state_dict_round_trip(bits, dtype):
+    a = _model().to(dtype)
+    opt = FusedAdamW(a.parameters(), lr=1e-2, state_bits=bits)
+    for step in range(3):
+        _grads(a, step)
+        opt.step()
+    b = copy.deepcopy(a)
+    other = FusedAdamW(b.parameters(), lr=5.0, state_bits=bits)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for p, q in zip(a.parameters(), b.parameters()):
+        for name, value in opt.state[p].items():
+            got = other.state[q][name]
+            if torch.is_tensor(value):
+                assert got.dtype == value.dtype and torch.equal(got.float(), value.float()), name
+                assert got.data_ptr() != value.data_ptr()
+            else:
+                assert got == value
+    _grads(a, 9)
+    _grads(b, 9)
+    opt.step()
+    other.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q)
+    with pytest.raises(ValueError, match="bits"):
+        FusedAdamW(b.parameters(), state_bits=40 - bits).load_state_dict(opt.state_dict())
+
+
+def test_parameters_without_a_gradient_are_left_alone():
+    m = _model()
+    opt = FusedAdamW(m.parameters(), lr=1e-2)
+    _grads(m, 0)
+    m[2].weight.grad = None
+    before = m[2].weight.detach().clone()
+    opt.step()
+    assert torch.equal(before, m[2].weight) and m[2].weight not in opt.state
+    _grads(m, 1)
+    opt.step()
+    assert opt.state[m[2].weight]["step"] == 1 and opt.state[m[0].weight]["step"] == 2
+
+
+def test_closure_and_grad_scale():
+    a, b = _model(), _model()
+    x = torch.randn(4, 13)
+    one, two = FusedAdamW(a.parameters(), lr=1e-2), FusedAdamW(b.parameters(), lr=1e-2)
+
+    def closure():
+        one.zero_grad()
+        loss = a(x).square().sum()
+        loss.backward()
+        return loss
+
+    loss = one.step(closure)
+    assert loss.requires_grad
+    (b(x).square().sum() * 4.0).backward()
+    two.step(grad_scale=torch.full((1,), 0.25))
+    for p, q in zip(a.parameters(), b.parameters()):
+        torch.testing.assert_close(p, q, rtol=2.0 ** -20, atol=1e-2 * 2.0 ** -18)
+
+
+def test_masters_keep_what_the_type_loses():
+    p = torch.nn.Parameter(torch.ones(8, dtype=torch.bfloat16))
+    q = torch.nn.Parameter(torch.ones(8, dtype=torch.bfloat16))
+    keep, lose = FusedAdamW([p], lr=1e-4, weight_decay=0.0), FusedAdamW([q], lr=1e-4, weight_decay=0.0,
+                                                                      master_weights=False)
+    for _ in range(100):
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+        keep.step()
+        lose.step()
+    assert bool((q == 1).all()) and bool((p < 1).all())
+    # 100 differences just below 1, each rounded by up to 2^-25, and updates of 1e-4 off by some 2^-22 of it
+    torch.testing.assert_close(keep.state[p]["master"], torch.full((8,), 0.99), rtol=0,
+                               atol=100 * 2.0 ** -25 + 100 * 1e-4 * 2.0 ** -22)
+
+
+def test_refusals():
+    w = torch.nn.Parameter(torch.zeros(4, 4))
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8),
+               dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            FusedAdamW([w], **kw)
+    t = torch.nn.Parameter(torch.zeros(4, 3).t())
+    t.grad = torch.zeros_like(t)
+    with pytest.raises(ValueError, match="contiguous"):
+        FusedAdamW([t]).step()
+    w.grad = torch.zeros(4, 4).to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        FusedAdamW([w]).step()
+    z = lambda: [torch.zeros(3)]     # noqa: E731
+    with pytest.raises(ValueError, match="both"):
+        multi_tensor_adamw(z(), z(), z(), z(), lr=1.0, step=1, exp_avg_scales=z())
+    with pytest.raises(ValueError, match="count from 1"):
+        multi_tensor_adamw(z(), z(), z(), z(), lr=1.0, step=0)
+    with pytest.raises(ValueError, match="values required"):
+        multi_tensor_adamw(z(), z(), z(), z(), lr=[1.0, 2.0], step=1)
+    with pytest.raises(ValueError, match="gradients"):
+        multi_tensor_adamw(z(), [], z(), z(), lr=1.0, step=1)
+    multi_tensor_adamw([], [], [], [], lr=1.0, step=1)
+    assert math.isfinite(float(w.sum()))

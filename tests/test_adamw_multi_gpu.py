@@ -1,0 +1,271 @@
+"""AdamW over many tensors on the GPU: against the formula in 64 bits, 8-bit moments to the bit against the
+plain form, odd lengths and addresses, captured steps and refusals."""
+import copy
+
+import pytest
+import torch
+
+from slapo_b200.op import FusedAdamW, dequantize_moment, multi_tensor_adamw, quantize_moment
+from slapo_b200.ops import native
+from slapo_b200.ops.adamw import _reference_step, state_blocks
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [1, 7, 8, 255, 256, 257, 2047, 2048, 2049, 5000, 0, 70001]
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def _tensors(sizes, dtype, bits, master, offset=0, seed=0):
+    """Lists of a step's tensors; each begins ``offset`` elements into memory of its own."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def make(values):
+        at = torch.empty(values.numel() + offset, device="cuda", dtype=values.dtype)
+        at = at[offset:]
+        at.copy_(values.reshape(-1))
+        return at
+
+    t = {"params": [], "grads": [], "exp_avgs": [], "exp_avg_sqs": []}
+    if master:
+        t["masters"] = []
+    if bits == 8:
+        t["exp_avg_scales"], t["exp_avg_sq_scales"] = [], []
+    for n in sizes:
+        w = torch.randn(n, generator=g, device="cuda") * 0.05
+        m = torch.randn(n, generator=g, device="cuda") * 1e-3
+        v = (m * 1.5) ** 2 + 1e-8
+        t["params"].append(make(w.to(dtype)))
+        t["grads"].append(make((torch.randn(n, generator=g, device="cuda") * 2e-3).to(dtype)))
+        if master:
+            t["masters"].append(make(w))
+        for name, x, second in (("exp_avgs", m, False), ("exp_avg_sqs", v, True)):
+            if bits == 8:
+                codes, scale = quantize_moment(x, second)
+                t[name].append(make(codes))
+                t[name[:-1] + "_scales"].append(scale)
+            else:
+                t[name].append(make(x))
+    return t
+
+
+def _copy(t):
+    return {k: [x.clone() for x in v] for k, v in t.items()}
+
+
+@pytest.mark.parametrize("offset", [0, 1, 4])
+@pytest.mark.parametrize("dtype,master", [(torch.bfloat16, True), (torch.bfloat16, False),
+                                          (torch.float16, True), (torch.float16, False),
+                                          (torch.float32, False)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_against_64_bits(bits, dtype, master, offset):
+    t = _tensors(SIZES, dtype, bits, master, offset)
+    old = _copy(t)
+    lrs = [1e-2 * (1 + i) for i in range(len(SIZES))]
+    decays = [0.1 * (i % 3) for i in range(len(SIZES))]
+    b1, b2, eps, step = 0.9, 0.99, 1e-6, 3
+    gs = torch.full((1,), 0.5, device="cuda")
+    multi_tensor_adamw(**t, lr=lrs, betas=(b1, b2), eps=eps, weight_decay=decays, step=step, grad_scale=gs)
+    for i, n in enumerate(SIZES):
+        g = old["grads"][i].double() * 0.5
+        if bits == 8:
+            m = dequantize_moment(old["exp_avgs"][i], old["exp_avg_scales"][i]).double()
+            v = dequantize_moment(old["exp_avg_sqs"][i], old["exp_avg_sq_scales"][i], second=True).double()
+        else:
+            m, v = old["exp_avgs"][i].double(), old["exp_avg_sqs"][i].double()
+        size = m.abs() * b1 + g.abs() * (1 - b1)
+        m, v = m * b1 + g * (1 - b1), v * b2 + g * g * (1 - b2)
+        w = (old["masters"] if master else old["params"])[i].double()
+        denom = (v / (1 - b2 ** step)).sqrt() + eps
+        update = m / (1 - b1 ** step) / denom + decays[i] * w
+        want = w - lrs[i] * update
+        # the moment: three roundings of 2^-24 and the constants' two; the quotient: some ten of 2^-23 more
+        # (__fdividef is within 2 of them); then one of the product and one of the weight
+        slack = lrs[i] * ((size / (1 - b1 ** step) / denom) * 8 + update.abs() * 16) * 2.0 ** -23
+        bound = slack + (w.abs() * lrs[i] * decays[i] + want.abs()) * 2.0 ** -23
+        if master:
+            assert bool(((t["masters"][i].double() - want).abs() <= bound).all())
+            assert torch.equal(t["params"][i], t["masters"][i].to(dtype))
+        else:
+            tiny = torch.finfo(dtype).smallest_normal * HALF[dtype]
+            half = HALF[dtype] if dtype != torch.float32 else 0.0
+            assert bool(((t["params"][i].double() - want).abs()
+                         <= bound * 2 + want.abs() * half * (1 + 2.0 ** -8) + tiny).all())
+        if bits == 32:
+            assert bool(((t["exp_avgs"][i].double() - m).abs() <= size * 5 * 2.0 ** -24).all())
+            assert bool(((t["exp_avg_sqs"][i].double() - v).abs() <= v * 6 * 2.0 ** -24).all())
+        assert torch.equal(t["grads"][i], old["grads"][i])
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_8bit_moments_are_those_of_the_plain_form(dtype, offset):
+    """Products and sums are rounded one by one on both sides: the same numbers, to the bit, over steps."""
+    t = _tensors(SIZES, dtype, 8, False, offset, seed=5)
+    r = _copy(t)
+    gs = torch.full((1,), 0.7, device="cuda")
+    for step in range(1, 4):
+        multi_tensor_adamw(**t, lr=1e-3, step=step, grad_scale=gs)
+        for i in range(len(SIZES)):
+            _reference_step(r["params"][i], r["grads"][i], None, r["exp_avgs"][i], r["exp_avg_sqs"][i],
+                            r["exp_avg_scales"][i], r["exp_avg_sq_scales"][i], 1e-3, 0.01, (0.9, 0.999),
+                            1e-8, step, gs)
+            for name in ("exp_avgs", "exp_avg_sqs"):
+                assert torch.equal(t[name][i].view(torch.uint8), r[name][i].view(torch.uint8)), name
+                scales = name[:-1] + "_scales"
+                assert torch.equal(t[scales][i], r[scales][i])
+
+
+def test_8bit_extremes():
+    """Blocks of zeros, of very small and of very large values, and a NaN that stays in its place."""
+    n = 256 * 6
+    g = torch.zeros(n, device="cuda")
+    g[256:512] = 1e-25
+    g[512:768] = 1e15 * torch.linspace(-1, 1, 256, device="cuda")
+    g[768:1024] = torch.logspace(-30, 3, 256, device="cuda")
+    g[1030] = float("nan")
+    w = torch.zeros(n, device="cuda")
+    m, ms = quantize_moment(torch.zeros(n, device="cuda"))
+    v, vs = quantize_moment(torch.zeros(n, device="cuda"), second=True)
+    m2, ms2, v2, vs2, w2 = m.clone(), ms.clone(), v.clone(), vs.clone(), w.clone()
+    multi_tensor_adamw([w], [g], [m], [v], lr=1e-3, step=1, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    ok = torch.arange(n, device="cuda") // 256 != 4
+    _reference_step(w2, torch.where(ok, g, torch.zeros_like(g)), None, m2, v2, ms2, vs2, 1e-3, 0.01,
+                    (0.9, 0.999), 1e-8, 1, None)
+    assert torch.equal(m.view(torch.uint8)[ok], m2.view(torch.uint8)[ok])
+    assert torch.equal(v.view(torch.uint8)[ok], v2.view(torch.uint8)[ok])
+    assert bool((dequantize_moment(v, vs, True)[768:1024][g[768:1024].square() > 0] >= 0).all())
+    assert bool(torch.isnan(w[1030])) and int(torch.isnan(w).sum()) == 1
+    assert bool(torch.isnan(m.float()[1030])) and int(torch.isnan(m.float()).sum()) == 1
+
+
+@pytest.mark.parametrize("count", [1, 48, 49, 360, 361, 800])
+def test_number_of_tensors(count):
+    sizes = [(i * 37) % 301 for i in range(count)]
+    t = _tensors(sizes, torch.bfloat16, 8, True)
+    r = _copy(t)
+    before = native.launch_count()
+    multi_tensor_adamw(**t, lr=1e-3, step=2)
+    assert native.launch_count() - before <= -(-count // 360)
+    for i in range(count):
+        _reference_step(r["params"][i], r["grads"][i], r["masters"][i], r["exp_avgs"][i], r["exp_avg_sqs"][i],
+                        r["exp_avg_scales"][i], r["exp_avg_sq_scales"][i], 1e-3, 0.01, (0.9, 0.999), 1e-8,
+                        2, None)
+        assert torch.equal(t["exp_avgs"][i].view(torch.uint8), r["exp_avgs"][i].view(torch.uint8))
+        # (an update is at most some lr, off by a few 2^-23 of it)
+        torch.testing.assert_close(t["masters"][i], r["masters"][i], rtol=2.0 ** -22,
+                                   atol=1e-3 * 32 * 2.0 ** -23)
+
+
+def test_neighbours_are_left_alone():
+    """Memory before and behind each tensor, and factors of other tensors, keep their values."""
+    for bits in (8, 32):
+        t = _tensors([300, 1000], torch.bfloat16, bits, True)
+        guarded = {}
+        for k, v in t.items():
+            guarded[k] = []
+            for x in v:
+                whole = torch.full((x.numel() + 64,), 3.0, device="cuda").to(x.dtype)
+                whole[32:-32].copy_(x)
+                guarded[k].append(whole)
+        multi_tensor_adamw(**{k: [x[32:-32] for x in v] for k, v in guarded.items()}, lr=1e-3, step=1)
+        multi_tensor_adamw(**t, lr=1e-3, step=1)
+        for k, v in guarded.items():
+            for whole, x in zip(v, t[k]):
+                assert torch.equal(whole[32:-32].float(), x.float()), k
+                assert bool((whole[:32].float() == 3).all()) and bool((whole[-32:].float() == 3).all()), k
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_steps_go_on_counting(bits):
+    torch.manual_seed(0)
+    a = torch.nn.Linear(40, 30, device="cuda").to(torch.bfloat16)
+    b = copy.deepcopy(a)
+    one = FusedAdamW(a.parameters(), lr=1e-2, state_bits=bits, capturable=True)
+    two = FusedAdamW(b.parameters(), lr=1e-2, state_bits=bits)
+    for m in (a, b):
+        for p in m.parameters():
+            p.grad = torch.zeros_like(p)
+
+    def grads(seed):
+        for m in (a, b):
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            for p in m.parameters():
+                p.grad.normal_(generator=g)
+
+    fresh = FusedAdamW(copy.deepcopy(a).parameters(), lr=1e-2, capturable=True)
+    grads(0)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        one.step()
+    torch.cuda.current_stream().wait_stream(stream)
+    two.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one.step()
+    for step in range(1, 5):
+        grads(step)
+        graph.replay()
+        two.step()
+        for p, q in zip(a.parameters(), b.parameters()):
+            # (1 - beta^t is formed in 64 bits on both sides and rounded)
+            assert torch.equal(p, q)
+            assert int(one.state[p]["step"]) == two.state[q]["step"] == step + 1
+    one.load_state_dict(copy.deepcopy(two.state_dict()))
+    grads(9)
+    one.step()
+    two.step()
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q)
+    a.bias.grad = None
+    with pytest.raises(RuntimeError, match="together"):
+        one.step()
+    for p in fresh.param_groups[0]["params"]:
+        p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fresh.step()
+    torch.cuda.synchronize()
+
+
+def test_saved_parameters_are_noticed():
+    w = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = FusedAdamW([w], lr=1e-2)
+    loss = (w * w).sum()
+    w.grad = torch.ones_like(w)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+def test_refusals():
+    def call(**kw):
+        t = _tensors([300, 40], torch.bfloat16, 32, True)
+        t.update(lr=1e-3, step=1)
+        t.update({k: v(t) if callable(v) else v for k, v in kw.items()})
+        multi_tensor_adamw(**t)
+
+    call()
+    bad = [("entry", dict(masters=lambda t: t["masters"][:1])),
+           ("values required", dict(grads=lambda t: t["grads"][::-1])),
+           ("contiguous", dict(grads=lambda t: [torch.zeros(600, device="cuda", dtype=torch.bfloat16)[::2],
+                                                t["grads"][1]])),
+           ("must be", dict(grads=lambda t: [g.float() for g in t["grads"]])),
+           ("must be", dict(exp_avgs=lambda t: [x.half() for x in t["exp_avgs"]])),
+           ("CUDA tensors", dict(masters=lambda t: [x.cpu() for x in t["masters"]])),
+           ("share memory", dict(params=lambda t: [t["params"][0], t["params"][0][:40]])),
+           ("share memory", dict(exp_avgs=lambda t: [t["exp_avgs"][0], t["exp_avgs"][0][260:]])),
+           ("count from 1", dict(step=0)), ("betas", dict(betas=(0.9, 1.0))),
+           ("must be", dict(step=torch.ones(1, device="cuda"))),
+           ("values required", dict(grad_scale=torch.ones(2, device="cuda"))),
+           ("must be", dict(params=lambda t: [p.double() for p in t["params"]],
+                            grads=lambda t: [p.double() for p in t["grads"]]))]
+    for message, kw in bad[:-1]:
+        with pytest.raises((RuntimeError, ValueError), match=message):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="bf16, fp16 or fp32"):
+        call(**bad[-1][1])
+    t = _tensors([300], torch.bfloat16, 8, True)
+    t["exp_avg_scales"][0] = torch.ones(state_blocks(300) + 1, device="cuda")
+    with pytest.raises(RuntimeError, match="factors"):
+        multi_tensor_adamw(**t, lr=1e-3, step=1)
