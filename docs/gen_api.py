@@ -26,6 +26,7 @@ SECTIONS = [
     ("Ops", "slapo_b200.op", None),
     ("Functional kernels", "slapo_b200.ops.functional", ["linear", "linear_t", "gemm", "bias_act",
                                                          "dropout_add_layer_norm", "flash_attention",
+                                                         "embedding",
                                                          "effective_dropout_p"]),
     ("Tensor-parallel fused ops", "slapo_b200.parallel.fused_tp",
      ["ag_linear", "rs_linear", "ar_linear", "ag_gemm", "ag_gemm_pushed", "gemm_rs", "gemm_ar",

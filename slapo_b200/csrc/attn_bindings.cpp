@@ -29,10 +29,22 @@ const float* opt_f32(const optional<Tensor>& t, const char* name) {
   return t->data_ptr<float>();
 }
 
+// `window` keys up to a query's own and the first `sinks`; window 0: no such limit
+std::pair<int, int> check_window(int64_t window, int64_t sinks, bool causal, const optional<Tensor>& rel) {
+  TORCH_CHECK(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0),
+              "a window of one key and more, and no negative number of sinks required");
+  TORCH_CHECK(window == 0 || (causal && !(rel.has_value() && rel->defined())),
+              "a window needs causal attention without a relative bias");
+  // (a number that no length reaches, so that sums with positions fit)
+  const int64_t most = int64_t(1) << 30;
+  return {static_cast<int>(std::min(window, most)), static_cast<int>(std::min(sinks, most))};
+}
+
 std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                           const optional<Tensor>& kbias,
                                           const optional<Tensor>& rel, bool causal, double scale,
-                                          double p_drop, const optional<Tensor>& rng) {
+                                          double p_drop, const optional<Tensor>& rng, int64_t window_in,
+                                          int64_t sinks_in) {
   check_bshd(q, "q"); check_bshd(k, "k"); check_bshd(v, "v");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "bf16/fp16 only");
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
@@ -41,13 +53,14 @@ std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, cons
   TORCH_CHECK(k.size(0) == B && k.size(2) == H && k.size(3) == D && v.sizes() == k.sizes());
   if (kbias.has_value() && kbias->defined()) TORCH_CHECK(kbias->numel() == (int64_t)B * Sk);
   if (rel.has_value() && rel->defined()) TORCH_CHECK(rel->numel() == (int64_t)H * (Sq + Sk - 1));
+  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel);
   Tensor o = at::empty({B, Sq, H, D}, q.options());
   Tensor lse = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
   const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)};
   const int64_t ks[3] = {k.stride(0), k.stride(1), k.stride(2)};
   const int64_t vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
   // few row tiles: the keys are split over work items, whose shares a second kernel combines
-  const int64_t splits = slapo::flash_fwd_splits(B, H, Sq, Sk, D);
+  const int64_t splits = slapo::flash_fwd_splits(B, H, Sq, Sk, D, window, sinks);
   Tensor scratch;
   if (splits > 1)
     scratch = at::empty({splits * B * H * Sq * (D + 2)}, q.options().dtype(at::kFloat));
@@ -55,7 +68,7 @@ std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, cons
       q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
       splits > 1 ? scratch.data_ptr<float>() : nullptr,
       opt_f32(kbias, "key bias"), opt_f32(rel, "relative bias"), B, H, Sq, Sk, D, qs, ks, vs,
-      static_cast<float>(scale), causal ? 1 : 0, static_cast<float>(p_drop), unpack_rng(rng),
+      static_cast<float>(scale), causal ? 1 : 0, window, sinks, static_cast<float>(p_drop), unpack_rng(rng),
       q.scalar_type() == at::kBFloat16, slapo_status_ptr(q.get_device()),
       at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "flash_attn_fwd: launch refused (code ", rc, ")");
@@ -66,7 +79,8 @@ std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, cons
 std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
     const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
     const Tensor& lse, const optional<Tensor>& kbias, const optional<Tensor>& rel, bool causal,
-    double scale, double p_drop, const optional<Tensor>& rng, bool packed_qkv, int64_t keep_words) {
+    double scale, double p_drop, const optional<Tensor>& rng, bool packed_qkv, int64_t keep_words, int64_t window_in,
+    int64_t sinks_in) {
   check_bshd(q, "q"); check_bshd(k, "k"); check_bshd(v, "v");
   TORCH_CHECK(dout.is_contiguous() && o.is_contiguous(), "dout and out must be contiguous");
   c10::cuda::CUDAGuard guard(q.device());
@@ -90,8 +104,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
   }
   const bool has_bias = kbias.has_value() && kbias->defined();
   const bool has_rel = rel.has_value() && rel->defined();
-  const slapo::FlashBwdPlan plan = slapo::flash_bwd_plan(
-      B, H, Sq, Sk, D, packed_qkv, causal, has_bias, has_rel, static_cast<float>(p_drop), keep_words);
+  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel);
+  const slapo::FlashBwdPlan plan =
+      slapo::flash_bwd_plan(B, H, Sq, Sk, D, packed_qkv, causal, window, sinks, has_bias, has_rel,
+                            static_cast<float>(p_drop), keep_words);
   Tensor scratch = at::empty({plan.total()}, q.options().dtype(at::kFloat));
   Tensor drel;
   if (has_rel) drel = at::zeros_like(*rel);
@@ -105,7 +121,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
       dv.data_ptr(), row_stride, row_stride, opt_f32(kbias, "key bias"),
       opt_f32(rel, "relative bias"),
       has_rel ? drel.data_ptr<float>() : nullptr, B, H, Sq, Sk, D, qs, ks, vs,
-      static_cast<float>(scale), causal ? 1 : 0, static_cast<float>(p_drop), unpack_rng(rng),
+      static_cast<float>(scale), causal ? 1 : 0, window, sinks, static_cast<float>(p_drop), unpack_rng(rng),
       q.scalar_type() == at::kBFloat16, slapo_status_ptr(q.get_device()),
       at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "flash_attn_bwd: launch refused (code ", rc, ")");
@@ -242,9 +258,9 @@ Tensor rel_bias_bwd(const Tensor& grad, const Tensor& buckets, const Tensor& tab
 }  // namespace
 
 void register_attn_ops(torch::Library& m) {
-  m.def("flash_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng) -> (Tensor, Tensor)",
+  m.def("flash_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, int window=0, int sinks=0) -> (Tensor, Tensor)",
         &flash_attn_fwd);
-  m.def("flash_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, bool packed_qkv, int keep_words=0) -> (Tensor, Tensor, Tensor, Tensor)",
+  m.def("flash_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, bool packed_qkv, int keep_words=0, int window=0, int sinks=0) -> (Tensor, Tensor, Tensor, Tensor)",
         &flash_attn_bwd);
   m.def("append_kv(Tensor past_k, Tensor past_v, Tensor k, Tensor v) -> (Tensor, Tensor)", &append_kv);
   m.def("rel_buckets(Tensor table, int sq, int sk, bool bidirectional, float inv_exact, float inv_log) -> Tensor",

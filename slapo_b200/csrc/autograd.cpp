@@ -317,28 +317,31 @@ struct DropoutAddNormFn : public Function<DropoutAddNormFn> {
 // ------------------------------------------------------------------------ //
 using FlashFwd = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&,
                                             const optional<Tensor>&, const optional<Tensor>&, bool,
-                                            double, double, const optional<Tensor>&);
+                                            double, double, const optional<Tensor>&, int64_t, int64_t);
 using FlashBwd = std::tuple<Tensor, Tensor, Tensor, Tensor>(
     const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
     const optional<Tensor>&, const optional<Tensor>&, bool, double, double, const optional<Tensor>&,
-    bool, int64_t);
+    bool, int64_t, int64_t, int64_t);
 
 // Attention on separate q, k, v [B, S, H, D] (q only given: the packed [B, S, H, 3, D], read in
 // place through strided views and its gradient written into one tensor of that layout).
 struct FlashFn : public Function<FlashFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_or_qkv, const optional<Tensor>& k,
                         const optional<Tensor>& v, const optional<Tensor>& key_bias,
-                        const optional<Tensor>& rel, bool causal, double scale, double p) {
+                        const optional<Tensor>& rel, bool causal, double scale, double p, int64_t window,
+                        int64_t sinks) {
     const bool packed = !k.has_value();
     const Tensor q = packed ? q_or_qkv.select(3, 0) : q_or_qkv;
     const Tensor kk = packed ? q_or_qkv.select(3, 1) : *k, vv = packed ? q_or_qkv.select(3, 2) : *v;
     optional<Tensor> rng;
     if (p > 0.0) rng = philox_reserve(q.size(0) * q.size(2) * q.size(1) * kk.size(1));
     static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
-    auto [out, lse] = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng);
+    auto [out, lse] = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
     ctx->save_for_backward({q_or_qkv, or_undefined(k), or_undefined(v), out, lse,
                             or_undefined(key_bias), or_undefined(rel)});
     ctx->saved_data["causal"] = causal;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["p"] = p;
     if (rng.has_value()) ctx->saved_data["rng"] = *rng;
@@ -355,8 +358,9 @@ struct FlashFn : public Function<FlashFn> {
     static auto f = op<FlashBwd>("slapo_b200::flash_attn_bwd");
     auto [dq, dk, dv, drel] =
         f.call(grads[0].contiguous(), q, k, v, s[3], s[4], opt(s[5]), opt(s[6]),
-               ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), p, rng, packed, /*keep_words=*/0);
-    tensor_list out(8);
+               ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), p, rng, packed, /*keep_words=*/0,
+               ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt());
+    tensor_list out(10);
     out[0] = dq;
     if (!packed) {
       out[1] = dk;
@@ -462,8 +466,8 @@ std::tuple<Tensor, Tensor> dropout_add_norm(const Tensor& x, const optional<Tens
 }
 Tensor flash(const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v,
              const optional<Tensor>& key_bias, const optional<Tensor>& rel, bool causal, double scale,
-             double p) {
-  return FlashFn::apply(q, k, v, key_bias, rel, causal, scale, p);
+             double p, int64_t window, int64_t sinks) {
+  return FlashFn::apply(q, k, v, key_bias, rel, causal, scale, p, window, sinks);
 }
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, int64_t start, const optional<int64_t>& padding,
@@ -486,6 +490,6 @@ void register_autograd_ops(torch::Library& m) {
         &dropout_add_norm);
   m.def("rel_bias(Tensor table, Tensor buckets) -> Tensor", &rel_bias);
   m.def("embedding(Tensor ids, Tensor weight, int start, int? padding, float scale) -> Tensor", &embedding);
-  m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p) -> Tensor",
+  m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p, int window=0, int sinks=0) -> Tensor",
         &flash);
 }

@@ -37,13 +37,14 @@ void launch_ln_bwd(const void* gy, const void* gz, const void* zin, const void* 
 namespace slapo {
 // Flash attention on [B, S, H, D] tensors (D contiguous, a multiple of 8 up to 128);
 // *_strides = element strides of (B, S, H).  Return 0 on success.
-int flash_fwd_splits(int B, int H, int Sq, int Sk, int D);
+// window > 0, with causal: a query sees that many keys up to its own, and the first `sinks`
+int flash_fwd_splits(int B, int H, int Sq, int Sk, int D, int window, int sinks);
 int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                      float* scratch,
                      const float* kbias, const float* rel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                     float scale, int causal, float p_drop, PhiloxArgs rng, bool bf16, int* status,
-                     cudaStream_t stream);
+                     float scale, int causal, int window, int sinks, float p_drop, PhiloxArgs rng, bool bf16,
+                     int* status, cudaStream_t stream);
 // How the backward runs, and its scratch in floats: row statistics, padded key bias, keep bits
 // (dropout in two launches) and shares of dQ (keys split over work items).
 struct FlashBwdPlan {
@@ -55,7 +56,7 @@ struct FlashBwdPlan {
 };
 // keep_words: 32-bit words of keep bits at a time (one pair's at least); 0: 1 GB of them, and whether
 // the passes run in one launch, without keep bits, is left to the plan.
-FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal,
+FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal, int window, int sinks,
                             bool key_bias, bool rel, float p_drop, int64_t keep_words);
 // dq_row_stride / dkv_row_stride: elements between consecutive (b, s, head) rows of the outputs
 int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
@@ -63,8 +64,8 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
                      void* dv, int64_t dq_row_stride, int64_t dkv_row_stride, const float* kbias,
                      const float* rel, float* drel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                     float scale, int causal, float p_drop, PhiloxArgs rng, bool bf16, int* status,
-                     cudaStream_t stream);
+                     float scale, int causal, int window, int sinks, float p_drop, PhiloxArgs rng, bool bf16,
+                     int* status, cudaStream_t stream);
 void launch_flash_dropout_mask(uint8_t* mask, int B, int H, int Sq, int Sk, float p_drop,
                                PhiloxArgs rng, cudaStream_t stream);
 }  // namespace slapo

@@ -89,6 +89,7 @@ struct FlashFwdParams {
   const float* rel;    // [H, Sq + Sk - 1] additive bias by (key - query) + Sq - 1, or nullptr
   float scale_log2;    // softmax scale * log2(e)
   int causal;
+  int window, sinks;   // kWin: a query sees `window` keys up to its own and the first `sinks` (see KeyWindow)
   float p_drop;        // effective probability thr7 / 128
   uint32_t thr7;
   PhiloxArgs rng;
@@ -122,11 +123,13 @@ __device__ __forceinline__ void fwd_fetch_bias(const FlashFwdParams& p, float* d
 }
 
 // They have arrived, are visible to the warp, and the readers of its other buffer are done.
+template <bool kWin>
 __device__ __forceinline__ void fwd_land_bias(const FlashFwdParams& p, float* bias, int lane) {
   cp_async_wait();
   if (p.kbias != nullptr) {
 #pragma unroll
-    for (int i = lane; i < 128; i += 32) bias[i] *= kLog2e;      // (the elements that this lane copied)
+    for (int i = lane; i < 128; i += 32)      // (the elements that this lane copied)
+      bias[i] = kWin ? window_bias(bias[i]) : bias[i] * kLog2e;
   }
   __syncwarp();
 }
@@ -165,7 +168,7 @@ __device__ __forceinline__ void fwd_add_bias(const FlashFwdParams& p, uint32_t (
 }
 
 // -inf for keys that a row does not see, of the tile from k0 on; row0: the warp's first row
-template <int kSets>
+template <bool kWin, int kSets>
 __device__ __forceinline__ void fwd_mask(const FlashFwdParams& p, uint32_t (&raw)[kSets][32], int k0, int row0,
                                          int lane) {
   const int diag = p.Sk - p.Sq;         // key j visible to query i iff j <= i + diag (causal)
@@ -178,6 +181,19 @@ __device__ __forceinline__ void fwd_mask(const FlashFwdParams& p, uint32_t (&raw
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (!(seen & (1u << i))) raw[c][i] = 0xff800000u;   // -inf
+    }
+  }
+  if constexpr (kWin) {
+    // (the warp's last row has the latest window)
+    if (k0 < row0 + 31 + diag + 1 - p.window && k0 + kSets * 32 > p.sinks) {
+      const int before = row0 + lane + diag + 1 - p.window - k0;
+#pragma unroll
+      for (int c = 0; c < kSets; ++c) {
+        const uint32_t hidden = low_bits(before - c * 32) & ~low_bits(p.sinks - k0 - c * 32);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (hidden & (1u << i)) raw[c][i] = 0xff800000u;
+      }
     }
   }
 }
@@ -211,7 +227,8 @@ struct FwdSmem {
 // kGeneral: key bias, relative bias, causal mask, a ragged last key tile or a scale <= 0;
 // without any of them the kernel takes row maxima on the raw scores and every probability is
 // one fused multiply-add plus one exp2.
-template <int D, bool kGeneral, bool kDrop, typename T>
+// kWin (with kGeneral): a window and sinks.
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 __global__ void __launch_bounds__(192, D == 64 ? 2 : 1)
 flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const FlashFwdParams p) {
@@ -270,6 +287,9 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   tc::fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const int items = p.walk.items() * p.splits;
+  const KeyWindow keys{diag, p.window, p.sinks};
+  // key tile j of a row tile's
+  auto key_tile = [&](int tile, int j) { return kWin ? keys.at<kBlockN>(tile * kBlockM, j) : j; };
   // row tile, (batch, head) and key tiles [j0, j0 + n) of a work item
   auto item_at = [&](int item, int& tile, int& bh, int& j0) {
     const int unit = p.splits == 1 ? item : item / p.splits;
@@ -279,6 +299,7 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const int last_key = min(p.Sk, tile * kBlockM + kBlockM + diag);
       n = max(1, min(n, (last_key + kBlockN - 1) / kBlockN));
     }
+    if constexpr (kWin) n -= keys.skip<kBlockN>(tile * kBlockM);
     j0 = 0;
     if (p.splits > 1) {     // (one row tile per head: every split has at least one key tile)
       j0 = (item - unit * p.splits) * p.tiles_per_split;
@@ -311,13 +332,13 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
           for (int d = 0; d < kDBlocks; ++d)
             tc::tma_load_4d(s_k + st * kTileBytes + d * kBlkBytes, &tm_k, &k_full[st], d * 64, head,
-                            (j0 + j) * kBlockN, batch);
+                            key_tile(tile, j0 + j) * kBlockN, batch);
           if (!tc::mbar_wait(&v_empty[st], ph ^ 1, abort_flag)) { ok = false; break; }
           tc::mbar_arrive_expect_tx(&v_full[st], kTileBytes);
 #pragma unroll
           for (int d = 0; d < kDBlocks; ++d)
             tc::tma_load_4d(s_v + st * kTileBytes + d * kBlkBytes, &tm_v, &v_full[st], d * 64, head,
-                            (j0 + j) * kBlockN, batch);
+                            key_tile(tile, j0 + j) * kBlockN, batch);
         }
       }
     }
@@ -403,8 +424,8 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     // to them (or the scale would turn the maximum around)
     const bool biased = kGeneral && (p.kbias != nullptr || p.rel != nullptr || !(p.scale_log2 > 0.f));
     const float sc = biased ? 1.f : p.scale_log2;
-    auto fetch_bias = [&](int tile, int bh, int jt, int buf) {
-      fwd_fetch_bias(p, bias_buf + buf * kBiasFloats, tile, quarter, lane, bh, jt);
+    auto fetch_bias = [&](int tile, int bh, int j, int buf) {
+      fwd_fetch_bias(p, bias_buf + buf * kBiasFloats, tile, quarter, lane, bh, key_tile(tile, j));
     };
     bool ok = true;
     int t = 0;
@@ -423,10 +444,10 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       float m_ref = -INFINITY;
       uint64_t l2 = 0;      // two fp32 partial row sums
       for (int j = 0; j < n; ++j, ++t) {
-        const int k0 = (j0 + j) * kBlockN;
+        const int k0 = key_tile(tile, j0 + j) * kBlockN;
         const float* bias = bias_buf + (t & 1) * kBiasFloats;
         if (kGeneral && biased) {
-          fwd_land_bias(p, bias_buf + (t & 1) * kBiasFloats, lane);
+          fwd_land_bias<kWin>(p, bias_buf + (t & 1) * kBiasFloats, lane);
           if (j + 1 < n) {
             fetch_bias(tile, bh, j0 + j + 1, (t + 1) & 1);
           } else if (item + static_cast<int>(gridDim.x) < items) {
@@ -446,7 +467,7 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (lane == 0) tc::mbar_arrive(s_free);
         if constexpr (kGeneral) {
           if (biased) fwd_add_bias(p, raw, bias, lane);
-          fwd_mask(p, raw, k0, tile * kBlockM + quarter * 32, lane);
+          fwd_mask<kWin>(p, raw, k0, tile * kBlockM + quarter * 32, lane);
         }
         const float m_tile = fwd_max(raw) * sc;
         // P of the tile before has been read (and O includes it)
@@ -617,7 +638,7 @@ struct GroupsSmem {
 // 9.4; 4 x 2048 x 16 x 128 causal: 111 -> 91, all keys 154 -> 128; 4 x 1000 x 32 x 80 causal with key bias: 70 -> 60;
 // 4 x 1024 x 16 x 128, p 0.1: 61 -> 49.  With a single row tile there are too few tiles to share out: 2 x 60 x 60 x
 // 8 x 128: 6.5 -> 8.0 (which calls come here: fwd_in_groups).
-template <int D, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 __global__ void __launch_bounds__(512, 1)
 flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashFwdParams p) {
@@ -693,6 +714,9 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   tc::fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const int items = p.walk.items();       // (several row tiles: keys are not split)
+  const KeyWindow keys{diag, p.window, p.sinks};
+  // key tile j of a row tile's
+  auto key_tile = [&](int tile, int j) { return kWin ? keys.at<kBlockN>(tile * kBlockM, j) : j; };
   // row tile, (batch, head) and number of key tiles of a work item
   auto item_at = [&](int item, int& tile, int& bh) {
     p.walk.at(item, tile, bh);
@@ -701,6 +725,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const int last_key = min(p.Sk, min(tile * kBlockM + kBlockM, p.Sq) + diag);
       n = max(1, min(n, (last_key + kBlockN - 1) / kBlockN));
     }
+    if constexpr (kWin) n -= keys.skip<kBlockN>(tile * kBlockM);
     return n;
   };
 
@@ -730,7 +755,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
                             tile * kBlockM, batch);
           for (int j = 0; j < n; ++j, r.step()) {
             ok = false;
-            const int k0 = j * kBlockN;
+            const int k0 = key_tile(tile, j) * kBlockN;
             if (!tc::mbar_wait(&k_empty[r.slot], r.phase ^ 1, abort_flag)) break;
             tc::mbar_arrive_expect_tx(&k_full[r.slot], kTileBytes);
 #pragma unroll
@@ -948,8 +973,8 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const bool biased = kGeneral && (p.kbias != nullptr || p.rel != nullptr || !(p.scale_log2 > 0.f));
     const float sc = biased ? 1.f : p.scale_log2;
     const uint64_t sc2 = f2_pack(sc, sc);
-    auto fetch_bias = [&](int tile, int bh, int jt, int buf) {
-      fwd_fetch_bias(p, bias_buf + buf * kBiasFloats, tile, quarter, lane, bh, jt);
+    auto fetch_bias = [&](int tile, int bh, int j, int buf) {
+      fwd_fetch_bias(p, bias_buf + buf * kBiasFloats, tile, quarter, lane, bh, key_tile(tile, j));
     };
     // a tile of the sequence: key tile j of a work item (j < n), u0 is the item's first
     struct Pos {
@@ -979,7 +1004,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       Pos next = pos;
       for (; pos.j < pos.n; pos.j += 2, ++k) {
         const uint32_t ph = k & 1;
-        const int k0 = pos.j * kBlockN;
+        const int k0 = key_tile(pos.tile, pos.j) * kBlockN;
         const float* bias = bias_buf + ph * kBiasFloats;
         if (pos.j + 2 >= pos.n) {
           next.u0 += pos.n;
@@ -989,7 +1014,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           next.j = pos.j + 2;
         }
         if (kGeneral && biased) {
-          fwd_land_bias(p, bias_buf + ph * kBiasFloats, lane);
+          fwd_land_bias<kWin>(p, bias_buf + ph * kBiasFloats, lane);
           if (next.item < items) fetch_bias(next.tile, next.bh, next.j, ph ^ 1);
         }
         if (!tc::mbar_wait_warp(&s_full[g], ph, abort_flag)) { ok = false; break; }
@@ -1006,7 +1031,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           tc::tmem_ld_wait();
           if constexpr (kGeneral) {
             if (biased) fwd_add_bias(p, raw, bias + c, lane);
-            fwd_mask(p, raw, k0 + c, pos.tile * kBlockM + quarter * 32, lane);
+            fwd_mask<kWin>(p, raw, k0 + c, pos.tile * kBlockM + quarter * 32, lane);
 #pragma unroll
             for (int b = 0; b < 2; ++b) tc::tmem_st_x32(tmem_s + c + b * 32, raw[b]);
           }
@@ -1154,12 +1179,12 @@ void launch_flash_dropout_mask(uint8_t* mask, int B, int H, int Sq, int Sk, floa
   flash_dropout_mask_kernel<<<sm_count() * 4, 256, 0, stream>>>(mask, B, H, Sq, Sk, p_drop, rng);
 }
 
-template <int D, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 static int launch_fwd_groups(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                              const FlashFwdParams& p, int64_t items, cudaStream_t stream) {
   constexpr int kSmem = GroupsSmem<D>::kTotal;
   static_assert(kSmem <= 227 * 1024, "flash forward: shared memory over the per-CTA limit");
-  auto kernel = flash_fwd_groups_kernel<D, kGeneral, kDrop, T>;
+  auto kernel = flash_fwd_groups_kernel<D, kGeneral, kDrop, kWin, T>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
@@ -1170,6 +1195,19 @@ static int launch_fwd_groups(const CUtensorMap& tq, const CUtensorMap& tk, const
   count_launch();
   kernel<<<static_cast<int>(items < sm_count() ? items : sm_count()), 512, kSmem, stream>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+// Key tiles that a row tile streams with a window, of the first row tile and of most
+static int fwd_window_tiles(int Sq, int Sk, int window, int sinks) {
+  const int64_t first = static_cast<int64_t>(Sk) - Sq + 1 - window;
+  const int begin = static_cast<int>(first > 0 ? first : 0) / kBlockN;
+  const int sink_tiles = ((sinks < Sk ? sinks : Sk) + kBlockN - 1) / kBlockN;
+  return (Sk + kBlockN - 1) / kBlockN - (begin > sink_tiles ? begin - sink_tiles : 0);
+}
+static int window_tiles(int window, int sinks, int Sk) {
+  const int n = (window + kBlockN - 1) / kBlockN + 1 + (sinks + kBlockN - 1) / kBlockN;
+  const int all = (Sk + kBlockN - 1) / kBlockN;
+  return n < all ? n : all;
 }
 
 // Whether a call without split keys goes to the two softmax groups.  At D = 64 they have one CTA per SM where the other
@@ -1187,16 +1225,16 @@ template <int D, bool kGeneral, bool kDrop>
 static bool fwd_in_groups(const FlashFwdParams& p, int64_t items) {
   if (p.walk.row_tiles == 1) return false;
   if (D != 64 || items > 2 * sm_count()) return true;
-  const int key_tiles = (p.Sk + kBlockN - 1) / kBlockN;
+  const int key_tiles = p.window > 0 ? window_tiles(p.window, p.sinks, p.Sk) : (p.Sk + kBlockN - 1) / kBlockN;
   return key_tiles > 3 || (key_tiles > 1 && (items <= sm_count() || (kDrop && !kGeneral)));
 }
 
-template <int D, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 static int launch_fwd_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                         const FlashFwdParams& p, cudaStream_t stream) {
   constexpr int kSmem = FwdSmem<D>::kTotal;
   static_assert(FwdSmem<D>::kCtas * (kSmem + 1024) <= 228 * 1024, "flash forward: shared memory");
-  auto kernel = flash_fwd_kernel<D, kGeneral, kDrop, T>;
+  auto kernel = flash_fwd_kernel<D, kGeneral, kDrop, kWin, T>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
@@ -1206,7 +1244,7 @@ static int launch_fwd_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   }
   const int64_t items = static_cast<int64_t>(p.walk.row_tiles) * p.walk.nbh * p.splits;
   if (fwd_in_groups<D, kGeneral, kDrop>(p, items))
-    return launch_fwd_groups<D, kGeneral, kDrop, T>(tq, tk, tv, p, items, stream);
+    return launch_fwd_groups<D, kGeneral, kDrop, kWin, T>(tq, tk, tv, p, items, stream);
   const int64_t cap = FwdSmem<D>::kCtas * sm_count();
   count_launch();
   kernel<<<static_cast<int>(items < cap ? items : cap), 192, kSmem, stream>>>(tq, tk, tv, p);
@@ -1222,8 +1260,8 @@ static int launch_fwd_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
 // 12.7 -> 8.9, 48 x 2000 x 128: 21.9 -> 14.3, 74 x 4000 x 128: 42 -> 30, 48 x 450 x 128: 8.0 -> 8.3.  For one query with
 // D <= 64 the line lies too low: seven tiles and one item per SM would be right (12 x 600 x 64: 6.5 -> 7.6, 48 x
 // 1000 x 64: 8.5 -> 11.0, 96 x 2000 x 64: 13.0 -> 16.4).
-int flash_fwd_splits(int B, int H, int Sq, int Sk, int D) {
-  const int tiles = (Sk + kBlockN - 1) / kBlockN;
+int flash_fwd_splits(int B, int H, int Sq, int Sk, int D, int window, int sinks) {
+  const int tiles = window > 0 ? fwd_window_tiles(Sq, Sk, window, sinks) : (Sk + kBlockN - 1) / kBlockN;
   const int64_t bh = static_cast<int64_t>(B) * H;
   const int64_t cap = (D <= 64 ? FwdSmem<64>::kCtas : FwdSmem<128>::kCtas) * sm_count();
   if (Sq > kBlockM || bh <= 0) return 1;
@@ -1235,23 +1273,30 @@ int flash_fwd_splits(int B, int H, int Sq, int Sk, int D) {
   return (tiles + per - 1) / per;     // no empty split
 }
 
+// `window` > 0 (with `causal`): a query sees that many keys up to its own and the first `sinks`.
 // `scratch`: flash_fwd_splits() * B * H * Sq * (D + 2) floats, or null with a single split
 int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                      float* scratch,
                      const float* kbias, const float* rel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                     float scale, int causal, float p_drop, PhiloxArgs rng, bool bf16, int* status,
-                     cudaStream_t stream) {
+                     float scale, int causal, int window, int sinks, float p_drop, PhiloxArgs rng, bool bf16,
+                     int* status, cudaStream_t stream) {
   // any head dimension up to 128 that is a multiple of 8 (16-byte rows for TMA): the kernels
   // work on 64- or 128-wide tiles whose columns beyond D are zero-filled by the tile loads
   if (D < 8 || D > 128 || D % 8 != 0) return 1;
   if (B <= 0 || H <= 0 || Sq <= 0 || Sk <= 0) return 1;     // (no tensor map without an address)
+  if (window < 0 || sinks < 0 || (window > 0 ? (!causal || rel != nullptr) : sinks > 0)) return 1;
   FlashFwdParams p;
+  if (window > Sk) window = Sk;      // (they see no more)
+  if (sinks > Sk) sinks = Sk;
+  p.window = window;
+  p.sinks = sinks;
   p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.Dr = D; p.O = o; p.lse = lse; p.kbias = kbias; p.rel = rel;
   p.k_steps = (D + 15) / 16;
-  p.walk.set((Sq + kBlockM - 1) / kBlockM, 0, B * H, causal ? 2 : 0);
-  p.splits = scratch != nullptr ? flash_fwd_splits(B, H, Sq, Sk, D) : 1;
-  const int key_tiles = (Sk + kBlockN - 1) / kBlockN;
+  // (row tiles of a window differ little)
+  p.walk.set((Sq + kBlockM - 1) / kBlockM, 0, B * H, causal && window == 0 ? 2 : 0);
+  p.splits = scratch != nullptr ? flash_fwd_splits(B, H, Sq, Sk, D, window, sinks) : 1;
+  const int key_tiles = window > 0 ? fwd_window_tiles(Sq, Sk, window, sinks) : (Sk + kBlockN - 1) / kBlockN;
   p.tiles_per_split = (key_tiles + p.splits - 1) / p.splits;
   const int64_t rows = static_cast<int64_t>(B) * H * Sq;
   p.part_o = scratch;
@@ -1267,20 +1312,22 @@ int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float
   const bool general = kbias != nullptr || rel != nullptr || causal || Sk % kBlockN != 0 || !(scale > 0.f);
   int rc;
   if (Sq == 1 && p.thr7 == 0 && rel == nullptr) {
-    // a single query sees all keys, causal or not; its kernel needs no tensor maps
+    // a single query sees all keys of its window, causal or not; its kernel needs no tensor maps
     rc = launch_flash_decode(q, k, v, o, lse, p.part_o, p.part_ml, kbias, B, H, Sk, D, q_strides, k_strides,
-                             v_strides, scale, p.splits, p.tiles_per_split * kBlockN, bf16, stream);
+                             v_strides, scale, p.window, p.sinks, p.splits, p.tiles_per_split * kBlockN, bf16, stream);
   } else {
     CUtensorMap tq, tk, tv;
     if (!make_tmap_bshd(&tq, q, B, Sq, H, D, q_strides[0], q_strides[1], q_strides[2], 128, bf16) ||
         !make_tmap_bshd(&tk, k, B, Sk, H, D, k_strides[0], k_strides[1], k_strides[2], 128, bf16) ||
         !make_tmap_bshd(&tv, v, B, Sk, H, D, v_strides[0], v_strides[1], v_strides[2], 128, bf16))
       return 2;
-#define FLASH_FWD_CASE(D_, T_)                                            \
-  rc = p.thr7 != 0 ? (general ? launch_fwd_d<D_, true, true, T_>(tq, tk, tv, p, stream)          \
-                              : launch_fwd_d<D_, false, true, T_>(tq, tk, tv, p, stream))        \
-                   : (general ? launch_fwd_d<D_, true, false, T_>(tq, tk, tv, p, stream)         \
-                              : launch_fwd_d<D_, false, false, T_>(tq, tk, tv, p, stream))
+#define FLASH_FWD_CASE(D_, T_)                                                                         \
+  rc = p.thr7 != 0 ? (window > 0 ? launch_fwd_d<D_, true, true, true, T_>(tq, tk, tv, p, stream)       \
+                      : general  ? launch_fwd_d<D_, true, true, false, T_>(tq, tk, tv, p, stream)      \
+                                 : launch_fwd_d<D_, false, true, false, T_>(tq, tk, tv, p, stream))    \
+                   : (window > 0 ? launch_fwd_d<D_, true, false, true, T_>(tq, tk, tv, p, stream)      \
+                      : general  ? launch_fwd_d<D_, true, false, false, T_>(tq, tk, tv, p, stream)     \
+                                 : launch_fwd_d<D_, false, false, false, T_>(tq, tk, tv, p, stream))
     if (D <= 64) {
       if (bf16) FLASH_FWD_CASE(64, __nv_bfloat16);
       else FLASH_FWD_CASE(64, __half);

@@ -82,6 +82,7 @@ struct FlashBwdParams {
   int64_t row_stride1, row_stride2;
   float scale, scale_log2, inv_keep;
   int causal;
+  int window, sinks;      // kWin: a query sees `window` keys up to its own and the first `sinks` (see KeyWindow)
   uint32_t thr7;          // dropout: keep a draw >= thr7 of 128 ; 0 = no dropout
   PhiloxArgs rng;
   uint32_t idesc_s, idesc_acc;
@@ -112,14 +113,15 @@ __global__ void __launch_bounds__(256) flash_bwd_stats_kernel(
     const T* __restrict__ dout, const T* __restrict__ out, const float* __restrict__ lse,
     float* __restrict__ nlse, float* __restrict__ ndelta, const float* __restrict__ kbias,
     float* __restrict__ kb2, int H, int Sq, int Rq, int Sk, int Rk, int Dr, int lanes,
-    float keep_prob) {
+    float keep_prob, int windowed) {
   __shared__ float sums[8][33];
   pdl_launch();
   const int i0 = blockIdx.x * 32, h0 = blockIdx.y * 8, b = blockIdx.z;
   if (kbias != nullptr && blockIdx.y == 0)
-    for (int key = blockIdx.x * 256 + threadIdx.x; key < Rk; key += gridDim.x * 256)
-      kb2[static_cast<int64_t>(b) * Rk + key] =
-          key < Sk ? kbias[static_cast<int64_t>(b) * Sk + key] * kLog2e : 0.f;
+    for (int key = blockIdx.x * 256 + threadIdx.x; key < Rk; key += gridDim.x * 256) {
+      const float bias = key < Sk ? kbias[static_cast<int64_t>(b) * Sk + key] : 0.f;
+      kb2[static_cast<int64_t>(b) * Rk + key] = windowed ? window_bias(bias) : bias * kLog2e;
+    }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // `lanes` (8 or 16) threads share a row of Dr; a warp's rows four at a time, all of their loads first (one at
   // a time the kernel ran at half of the memory's rate: 4 x 2048 x 16 x 128: 18.5 -> 13.3 us, 4 x 1000 x 32 x 80: 17 -> 12)
@@ -198,9 +200,9 @@ struct BwdSmem {
 // groups (warps 4 - 11 and 12 - 19), a row and half of a half tile's columns per thread, which take the half
 // tiles in turn; and the warps that read the accumulators out (20 - 23).
 // kKeys: the dK / dV pass.  kGeneral: key bias, relative bias, causal mask or ragged lengths.
-// kDrop: with dropout.  kDraw: the dK / dV pass then draws the keep decisions itself, and the dQ pass leaves none.
+// kWin (with kGeneral): a window and sinks.  kDrop: with dropout.  kDraw: the dK / dV pass then draws the keep decisions itself, and the dQ pass leaves none.
 // CTA `cta` of `ctas` that run the pass.
-template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kDraw, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kDraw, bool kWin, typename T>
 __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtensorMap& tm_x2,
                                          const CUtensorMap& tm_y1, const CUtensorMap& tm_y2,
                                          const FlashBwdParams& p, const int cta, const int ctas) {
@@ -246,6 +248,12 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
   constexpr int kAcc = kKeys && D == 128 ? 1 : 2;
   const int items = p.walk.items() * (kKeys ? 1 : p.splits);
   constexpr bool drop = kDrop;
+  const KeyWindow keys{diag, p.window, p.sinks};
+  // The j-th half tile that a work item streams, `first` of item_at.  With a window the dQ pass goes through the
+  // sinks' half tiles first, and `first` is the gap behind them.
+  auto half_at = [&](int first, int j) {
+    return kWin && !kKeys && j < ((p.sinks + 63) >> 6) ? j : first + j;
+  };
 
   // row tile and (batch, head) of a work item, its first streamed half tile and how many (at least
   // one: a row tile or a split that nothing reaches still has its zeros written)
@@ -257,10 +265,19 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
     if constexpr (kKeys) {
       n = (p.Sq + 63) >> 6;
       if (p.causal) first = min(max(0, tile * 128 - diag) >> 6, n - 1);
+      if constexpr (kWin) {     // the last query that sees any of the tile's keys (sinks: all do)
+        const int last = tile * 128 + 127 - diag + p.window - 1;
+        if (tile * 128 >= p.sinks) n = min(n, max(last, 0) / 64 + 1);
+        n = max(n, first + 1);
+      }
       n -= first;
     } else {
       n = (p.Sk + 63) >> 6;
       if (p.causal) n = min(n, (min(tile * 128 + 128, p.Sq) + diag + 63) >> 6);
+      if constexpr (kWin) {
+        first = keys.skip<64>(tile * 128);
+        n -= first;
+      }
       if (p.splits > 1) {
         first = (item - unit * p.splits) * p.tiles_per_split * 2;
         n = min(p.tiles_per_split * 2, n - first);
@@ -379,7 +396,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
           if (!load_x(&tm_x1, x1_full, x1_empty, 0)) break;
           for (int j = 0; j < n; ++j, r1.step(), r2.step()) {
             ok = false;
-            const int s0 = (first + j) * 64;
+            const int s0 = half_at(first, j) * 64;
             // (the slot's column vectors were read before ds_ready, which y1_empty follows)
             if (!tc::mbar_wait(&y1_empty[r1.slot], r1.phase ^ 1, abort_flag)) break;
             uint64_t* full = &y1_full[r1.slot];
@@ -678,7 +695,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
     auto fetch_rel = [&](const Pos& pos, int buf) {
       const int head = (p.walk.bh0 + pos.bhl) % p.H;
       const float* src = p.rel + static_cast<int64_t>(head) * (p.Sq + p.Sk - 1) + p.Sq - 1;
-      const int r0 = pos.tile * 128 + quarter * 32, c0 = (pos.first + pos.j) * 64 + half * 32;
+      const int r0 = pos.tile * 128 + quarter * 32, c0 = half_at(pos.first, pos.j) * 64 + half * 32;
       const int d0 = kKeys ? r0 - (c0 + 31) : c0 - (r0 + 31);
 #pragma unroll
       for (int i = lane; i < L::kRelFloats; i += 32)
@@ -703,7 +720,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
       const uint64_t drop_row = (static_cast<uint64_t>(bh) * p.Sq + min(row, p.Sq - 1)) * sk16;
       Pos next = pos;
       for (; pos.j < pos.n; pos.j += 2) {
-        const int col0 = (pos.first + pos.j) * 64 + half * 32;       // this warp's first column
+        const int col0 = half_at(pos.first, pos.j) * 64 + half * 32;       // this warp's first column
         const uint8_t* vec = s_vec + slot * L::kVec;
         if (pos.j + 2 >= pos.n) {       // the item's last: the next one's rows, under its work
           next.u0 += pos.n;
@@ -809,6 +826,17 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
               for (int i = 0; i < 32; ++i)
                 if (hidden & (1u << i)) pr[i] = -INFINITY;
             }
+            if constexpr (kWin) {
+              // ... and, unless it is a sink, by queries < row - diag + window
+              const int end = row - diag + p.window - col0;
+              if (pos.tile * 128 + quarter * 32 - diag + p.window < col0 + 32 &&
+                  pos.tile * 128 + quarter * 32 + 31 >= p.sinks) {
+                const uint32_t hidden = row < p.sinks ? 0u : ~low_bits(end);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (hidden & (1u << i)) pr[i] = -INFINITY;
+              }
+            }
           } else {
             const int first_limit = p.causal ? min(p.Sk, pos.tile * 128 + quarter * 32 + diag + 1) : p.Sk;
             if (col0 + 32 > first_limit) {
@@ -816,6 +844,14 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (!(seen & (1u << i))) pr[i] = -INFINITY;
+            }
+            if constexpr (kWin) {
+              if (col0 < pos.tile * 128 + quarter * 32 + 31 + diag + 1 - p.window && col0 + 32 > p.sinks) {
+                const uint32_t hidden = low_bits(row + diag + 1 - p.window - col0) & ~low_bits(p.sinks - col0);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (hidden & (1u << i)) pr[i] = -INFINITY;
+              }
             }
           }
         }
@@ -946,16 +982,16 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
 }
 
 // One pass.
-template <int D, bool kKeys, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kWin, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 flash_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__ CUtensorMap tm_x2,
                  const __grid_constant__ CUtensorMap tm_y1, const __grid_constant__ CUtensorMap tm_y2,
                  const __grid_constant__ FlashBwdParams p) {
-  bwd_pass<D, kKeys, kGeneral, kDrop, false, T>(tm_x1, tm_x2, tm_y1, tm_y2, p, blockIdx.x, gridDim.x);
+  bwd_pass<D, kKeys, kGeneral, kDrop, false, kWin, T>(tm_x1, tm_x2, tm_y1, tm_y2, p, blockIdx.x, gridDim.x);
 }
 
 // Both passes side by side, the dQ pass on the first `q_ctas` CTAs.
-template <int D, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 flash_bwd_both_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -963,10 +999,10 @@ flash_bwd_both_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                       const __grid_constant__ FlashBwdParams pk, const int q_ctas) {
   const int cta = blockIdx.x;
   if (cta < q_ctas)
-    bwd_pass<D, false, kGeneral, kDrop, true, T>(tm_q, tm_do, tm_k, tm_v, pq, cta, q_ctas);
+    bwd_pass<D, false, kGeneral, kDrop, true, kWin, T>(tm_q, tm_do, tm_k, tm_v, pq, cta, q_ctas);
   else
-    bwd_pass<D, true, kGeneral, kDrop, true, T>(tm_k, tm_v, tm_q, tm_do, pk, cta - q_ctas,
-                                         gridDim.x - q_ctas);
+    bwd_pass<D, true, kGeneral, kDrop, true, kWin, T>(tm_k, tm_v, tm_q, tm_do, pk, cta - q_ctas,
+                                                     gridDim.x - q_ctas);
 }
 
 // dQ of rows whose keys were split over work items: the shares added in their order
@@ -1022,12 +1058,12 @@ static int launch_bwd(void (*kernel)(P...), int ctas, int smem, bool early, cuda
   return 4;
 }
 
-template <int D, bool kKeys, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kWin, typename T>
 static int launch_pass(const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
                        const CUtensorMap& y2, const FlashBwdParams& p, cudaStream_t stream) {
   constexpr int kSmem = BwdSmem<D, kKeys>::kTotal;
   static_assert(kSmem <= 227 * 1024, "flash backward: shared memory over the per-CTA limit");
-  auto kernel = flash_bwd_kernel<D, kKeys, kGeneral, kDrop, T>;
+  auto kernel = flash_bwd_kernel<D, kKeys, kGeneral, kDrop, kWin, T>;
   static bool configured = false;
   if (!allow_smem(kernel, kSmem, configured)) return 3;
   const int64_t items = static_cast<int64_t>(p.walk.row_tiles) * p.walk.nbh * p.splits;
@@ -1037,18 +1073,18 @@ static int launch_pass(const CUtensorMap& x1, const CUtensorMap& x2, const CUten
 }
 
 // The passes of `pq` (dQ) and `pk` (dK / dV), side by side or one after the other
-template <int D, bool kGeneral, bool kDrop, typename T>
+template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
 static int launch_passes(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                          const CUtensorMap& dout, const FlashBwdParams& pq, const FlashBwdParams& pk,
                          int q_ctas, cudaStream_t stream) {
   if (q_ctas == 0) {
     // dQ first: with dropout it leaves the keep bits that the dK / dV pass reads
-    const int rc = launch_pass<D, false, kGeneral, kDrop, T>(q, dout, k, v, pq, stream);
-    return rc != 0 ? rc : launch_pass<D, true, kGeneral, kDrop, T>(k, v, q, dout, pk, stream);
+    const int rc = launch_pass<D, false, kGeneral, kDrop, kWin, T>(q, dout, k, v, pq, stream);
+    return rc != 0 ? rc : launch_pass<D, true, kGeneral, kDrop, kWin, T>(k, v, q, dout, pk, stream);
   }
   constexpr int kSmemQ = BwdSmem<D, false>::kTotal, kSmemK = BwdSmem<D, true>::kTotal;
   constexpr int kSmem = kSmemQ > kSmemK ? kSmemQ : kSmemK;
-  auto kernel = flash_bwd_both_kernel<D, kGeneral, kDrop, T>;
+  auto kernel = flash_bwd_both_kernel<D, kGeneral, kDrop, kWin, T>;
   static bool configured = false;
   if (!allow_smem(kernel, kSmem, configured)) return 3;
   const int64_t items = static_cast<int64_t>(pk.walk.row_tiles) * pk.walk.nbh;
@@ -1063,11 +1099,13 @@ template <bool kDrop, typename T>
 static int launch_typed(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                         const CUtensorMap& dout, const FlashBwdParams& pq, const FlashBwdParams& pk,
                         int q_ctas, bool general, cudaStream_t stream) {
-  if (pq.Dr <= 64)
-    return general ? launch_passes<64, true, kDrop, T>(q, k, v, dout, pq, pk, q_ctas, stream)
-                   : launch_passes<64, false, kDrop, T>(q, k, v, dout, pq, pk, q_ctas, stream);
-  return general ? launch_passes<128, true, kDrop, T>(q, k, v, dout, pq, pk, q_ctas, stream)
-                 : launch_passes<128, false, kDrop, T>(q, k, v, dout, pq, pk, q_ctas, stream);
+#define FLASH_BWD_PASSES(D_)                                                                                \
+  pq.window > 0 ? launch_passes<D_, true, kDrop, true, T>(q, k, v, dout, pq, pk, q_ctas, stream)            \
+  : general     ? launch_passes<D_, true, kDrop, false, T>(q, k, v, dout, pq, pk, q_ctas, stream)           \
+                : launch_passes<D_, false, kDrop, false, T>(q, k, v, dout, pq, pk, q_ctas, stream)
+  if (pq.Dr <= 64) return FLASH_BWD_PASSES(64);
+  return FLASH_BWD_PASSES(128);
+#undef FLASH_BWD_PASSES
 }
 
 static int round128(int n) { return (n + 127) / 128 * 128; }
@@ -1110,7 +1148,7 @@ static int both_q_ctas(int64_t q_items, int64_t k_items, int64_t q_item_tiles, i
   return best_n;
 }
 
-FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal,
+FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal, int window, int sinks,
                             bool key_bias, bool rel, float p_drop, int64_t keep_words) {
   FlashBwdPlan s;
   const int64_t rq = round128(Sq), rk = round128(Sk), bh = static_cast<int64_t>(B) * H;
@@ -1120,7 +1158,7 @@ FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bo
   // chain of tiles, where that takes four tiles off its own.  (2 x 60 queries x 2000 keys x 8 x 128:
   // 72 -> 48 us for the whole backward.)
   s.splits = 1;
-  if (!packed && bh > 0 && q_tiles > 0 && k_tiles > q_tiles) {
+  if (!packed && window == 0 && bh > 0 && q_tiles > 0 && k_tiles > q_tiles) {
     int64_t n = sm_count() / (q_tiles * bh);
     const int64_t most = (k_tiles + q_tiles - 1) / q_tiles;
     if (n > most) n = most;
@@ -1129,9 +1167,16 @@ FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bo
       if (k_tiles - per >= 4) s.splits = static_cast<int>((k_tiles + per - 1) / per);
     }
   }
+  int64_t q_item_tiles = (k_tiles + s.splits - 1) / s.splits, k_item_tiles = q_tiles;
+  if (window > 0) {      // what most items of either pass stream; they differ little
+    const int64_t near = (static_cast<int64_t>(window) + 127) / 128 + 1;
+    const int64_t far = near + (static_cast<int64_t>(sinks) + 127) / 128;
+    if (far < q_item_tiles) q_item_tiles = far;
+    if (near < k_item_tiles) k_item_tiles = near;
+  }
   s.q_ctas = bh == 0 || keep_words > 0 ? 0
-                     : both_q_ctas(q_tiles * bh * s.splits, k_tiles * bh,
-                                   (k_tiles + s.splits - 1) / s.splits, q_tiles, D, causal, rel, drop);
+                     : both_q_ctas(q_tiles * bh * s.splits, k_tiles * bh, q_item_tiles, k_item_tiles, D,
+                                   causal && window == 0, rel, drop);
   s.stats = 2 * bh * rq;
   s.bias = key_bias ? B * rk : 0;
   const bool keep = drop && s.q_ctas == 0;
@@ -1151,10 +1196,13 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
                      void* dv, int64_t dq_row_stride, int64_t dkv_row_stride, const float* kbias,
                      const float* rel, float* drel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                     float scale, int causal, float p_drop, PhiloxArgs rng, bool bf16, int* status,
-                     cudaStream_t stream) {
+                     float scale, int causal, int window, int sinks, float p_drop, PhiloxArgs rng, bool bf16,
+                     int* status, cudaStream_t stream) {
   if (D < 8 || D > 128 || D % 8 != 0 || B > 65535) return 1;
   if (B <= 0 || H <= 0 || Sq <= 0 || Sk <= 0) return 1;
+  if (window < 0 || sinks < 0 || (window > 0 ? (!causal || rel != nullptr) : sinks > 0)) return 1;
+  if (window > Sk) window = Sk;      // (they see no more)
+  if (sinks > Sk) sinks = Sk;
   CUtensorMap tq, tk, tv, tdo;
   const int64_t do_strides[3] = {static_cast<int64_t>(Sq) * H * D, static_cast<int64_t>(H) * D, D};
   if (!make_tmap_bshd(&tq, q, B, Sq, H, D, q_strides[0], q_strides[1], q_strides[2], 64, bf16) ||
@@ -1181,6 +1229,7 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
   p.rel = rel; p.drel = drel;
   p.scale = scale; p.scale_log2 = scale * kLog2e; p.inv_keep = 1.f / keep_prob;
   p.causal = causal; p.rng = rng; p.status = status;
+  p.window = window; p.sinks = sinks;
   p.idesc_s = tc::instr_desc_f16(128, 64, bf16 ? 1 : 0, false, false);
   p.idesc_acc = tc::instr_desc_f16(128, p.k_steps * 16, bf16 ? 1 : 0, false, true);
   {
@@ -1190,11 +1239,11 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
     if (bf16)
       flash_bwd_stats_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(
           static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(o), lse, nlse,
-          ndelta, kbias, kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob);
+          ndelta, kbias, kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob, window > 0);
     else
       flash_bwd_stats_kernel<__half><<<grid, 256, 0, stream>>>(
           static_cast<const __half*>(dout), static_cast<const __half*>(o), lse, nlse, ndelta, kbias,
-          kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob);
+          kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob, window > 0);
     if (cudaGetLastError() != cudaSuccess) return 4;
   }
   const bool general = kbias != nullptr || rel != nullptr || causal || Sk % 128 != 0;
@@ -1210,8 +1259,9 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
   pk.out2 = dv; pk.row_stride2 = dkv_row_stride;
   for (int at = 0; at < bh; at += plan.pairs) {
     const int pairs = bh - at < plan.pairs ? bh - at : plan.pairs;
-    pq.walk.set(p.Rq / 128, at, pairs, causal ? 2 : 0);
-    pk.walk.set(p.Rk / 128, at, pairs, causal ? 1 : 0);
+    // (with a window row tiles differ little, but for the keys of sinks, which all queries see)
+    pq.walk.set(p.Rq / 128, at, pairs, causal && window == 0 ? 2 : 0);
+    pk.walk.set(p.Rk / 128, at, pairs, causal && (window == 0 || sinks > 0) ? 1 : 0);
 #define FLASH_BWD_CASE(T_)                                                                          \
   p.thr7 != 0 ? launch_typed<true, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)       \
               : launch_typed<false, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)

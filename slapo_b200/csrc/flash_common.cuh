@@ -145,6 +145,28 @@ __device__ __forceinline__ uint4 philox_keep16(const PhiloxUniform& s, uint64_t 
   return c;
 }
 
+// Which keys queries see with a window and sinks: key j a query at position i (its index + diag) if j <= i and
+// (j > i - window or j < sinks).  A tile of queries whose first has index row0 then streams the tiles of kTile keys
+// that the sinks lie in and, after a gap, those from its first window on.
+struct KeyWindow {
+  int diag, window, sinks;
+  // tiles in the gap
+  template <int kTile>
+  __device__ __forceinline__ int skip(int row0) const {
+    const int sink_tiles = (sinks + kTile - 1) / kTile;
+    return max(0, max(0, row0 + diag + 1 - window) / kTile - sink_tiles);
+  }
+  // the j-th tile that is streamed
+  template <int kTile>
+  __device__ __forceinline__ int at(int row0, int j) const {
+    return j < (sinks + kTile - 1) / kTile ? j : j + skip<kTile>(row0);
+  }
+};
+
+// A key's bias in the log2 domain.  With a window, keys masked by a type's lowest value are not seen at all, like
+// those masked by -inf: an additive bias of 1e30 and more leaves nothing of the scores.
+__device__ __forceinline__ float window_bias(float b) { return b < -1e30f ? -INFINITY : b * kLog2e; }
+
 // Position in a ring of N slots
 template <int N>
 struct Ring {

@@ -27,11 +27,21 @@ struct FlashDecodeParams {
   const float* kbias;   // [B, Sk] or nullptr
   float scale_log2;
   int rows;             // B H
+  int bias_row;         // kWin: Sk counts the keys that the query sees, kbias has this many for each batch entry;
+  int head, skip;       // from the head-th on the keys lie `skip` further
 };
 
 constexpr int kDecodeUnroll = 4;
 
-template <int L, int kWarps, typename T>
+// where a key lies among all
+template <bool kWin>
+__device__ __forceinline__ int decode_place(const FlashDecodeParams& p, int key) {
+  if constexpr (kWin) return key < p.head ? key : key + p.skip;
+  else return key;
+}
+
+// kWin: the first keys (sinks) and those of the window before the query, taken as one row of keys
+template <int L, int kWarps, bool kWin, typename T>
 __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) flash_decode_kernel(const FlashDecodeParams p) {
   constexpr int kRows = 32 / L;                 // key rows of a warp's load
   __shared__ float s_o[kWarps][L * 8];
@@ -58,8 +68,8 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) flash_decode_kernel(
       const int key = at + u * kRows + lane / L;
       const bool ok = key < end && d_ok;
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      r.k[u] = ok ? *reinterpret_cast<const uint4*>(k + key * p.ks) : zero;
-      r.v[u] = ok ? *reinterpret_cast<const uint4*>(v + key * p.vs) : zero;
+      r.k[u] = ok ? *reinterpret_cast<const uint4*>(k + decode_place<kWin>(p, key) * p.ks) : zero;
+      r.v[u] = ok ? *reinterpret_cast<const uint4*>(v + decode_place<kWin>(p, key) * p.vs) : zero;
     }
   };
   float m = -INFINITY, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -78,7 +88,12 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) flash_decode_kernel(
       for (int i = 0; i < 8; ++i) x = fmaf(kk[i], q[i], x);
 #pragma unroll
       for (int w = L / 2; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      if (p.kbias != nullptr && key < end) x = fmaf(p.kbias[static_cast<int64_t>(b) * p.Sk + key], kLog2e, x);
+      if constexpr (kWin) {
+        if (p.kbias != nullptr && key < end)
+          x += window_bias(p.kbias[static_cast<int64_t>(b) * p.bias_row + decode_place<kWin>(p, key)]);
+      } else {
+        if (p.kbias != nullptr && key < end) x = fmaf(p.kbias[static_cast<int64_t>(b) * p.Sk + key], kLog2e, x);
+      }
       s[u] = key < end ? x : -INFINITY;
       top = fmaxf(top, s[u]);
     }
@@ -138,11 +153,13 @@ __global__ void __launch_bounds__(32 * kWarps, 16 / kWarps) flash_decode_kernel(
   if (d == 0) p.lse[bh] = sum > 0.f ? use * 0.6931471805599453f + logf(sum) : -INFINITY;
 }
 
-// One query, no dropout and no relative bias (the caller has looked).  part_o, part_ml: with splits > 1.
+// One query, no dropout and no relative bias (the caller has looked); window 0: all keys, else keys_per_split counts
+// those that it sees.  part_o, part_ml: with splits > 1.
 int launch_flash_decode(const void* q, const void* k, const void* v, void* o, float* lse, float* part_o,
                         float2* part_ml, const float* kbias, int B, int H, int Sk, int D,
                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                        float scale, int splits, int keys_per_split, bool bf16, cudaStream_t stream) {
+                        float scale, int window, int sinks, int splits, int keys_per_split, bool bf16,
+                        cudaStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
     return 1;
   for (int i = 0; i < 3; ++i)
@@ -154,6 +171,14 @@ int launch_flash_decode(const void* q, const void* k, const void* v, void* o, fl
   p.vb = v_strides[0]; p.vs = v_strides[1]; p.vh = v_strides[2];
   p.H = H; p.Sk = Sk; p.D = D; p.splits = splits; p.keys_per_split = keys_per_split;
   p.kbias = kbias; p.scale_log2 = scale * kLog2e; p.rows = B * H;
+  // (window and sinks are at most Sk)
+  p.head = sinks < Sk - window ? sinks : Sk - window;
+  p.bias_row = Sk;
+  p.skip = Sk - window - p.head;
+  if (window > 0) {
+    p.Sk = window + p.head;
+    p.keys_per_split = keys_per_split = (p.Sk + splits - 1) / splits;
+  }
   const int64_t ctas = static_cast<int64_t>(p.rows) * splits;
   if (ctas > 0x7fffffff) return 1;
   const unsigned grid = static_cast<unsigned>(ctas);
@@ -168,8 +193,10 @@ int launch_flash_decode(const void* q, const void* k, const void* v, void* o, fl
   const bool few = 2 * keys_per_split <= step || (2 * ctas >= 3 * sm_count() && keys_per_split <= 2 * step) ||
                    ctas >= 6 * sm_count();
 #define FLASH_DECODE_CASE(L_, W_)                                                                     \
-  if (bf16) flash_decode_kernel<L_, W_, __nv_bfloat16><<<grid, 32 * W_, 0, stream>>>(p);              \
-  else flash_decode_kernel<L_, W_, __half><<<grid, 32 * W_, 0, stream>>>(p)
+  if (window > 0 && bf16) flash_decode_kernel<L_, W_, true, __nv_bfloat16><<<grid, 32 * W_, 0, stream>>>(p);  \
+  else if (window > 0) flash_decode_kernel<L_, W_, true, __half><<<grid, 32 * W_, 0, stream>>>(p);    \
+  else if (bf16) flash_decode_kernel<L_, W_, false, __nv_bfloat16><<<grid, 32 * W_, 0, stream>>>(p);  \
+  else flash_decode_kernel<L_, W_, false, __half><<<grid, 32 * W_, 0, stream>>>(p)
   if (D <= 64) {
     if (few) { FLASH_DECODE_CASE(8, 4); }
     else { FLASH_DECODE_CASE(8, 16); }

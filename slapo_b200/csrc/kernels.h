@@ -112,11 +112,12 @@ int launch_gemm_rows(const void* A, const void* W, void* C, const void* bias, in
 bool gemm_rows_takes(int M, int N, int K);
 
 // Attention of one query per (batch, head), no dropout, no relative bias (flash_decode.cu); strides of
-// batch, token and head in elements; part_o / part_ml with splits > 1 (see flash_fwd_splits)
+// batch, token and head in elements; window 0: all keys; part_o / part_ml with splits > 1 (see flash_fwd_splits)
 int launch_flash_decode(const void* q, const void* k, const void* v, void* o, float* lse, float* part_o,
                         float2* part_ml, const float* kbias, int B, int H, int Sk, int D,
                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                        float scale, int splits, int keys_per_split, bool bf16, cudaStream_t stream);
+                        float scale, int window, int sinks, int splits, int keys_per_split, bool bf16,
+                        cudaStream_t stream);
 
 // out[i] = cache past[i] ([B, past_len, H, head_bytes] contiguous) followed along the tokens by
 // fresh[i] ([B, new_len, H, head_bytes], strides of B / token / head in bytes), i = k, v.

@@ -2,6 +2,10 @@
 GPT-2 (``Conv1D`` projections, fused ``c_attn``) and GPT-Neo (separate
 bias-free q/k/v projections, no 1/sqrt(d) scaling).  Free of data-dependent
 control flow, so every level traces with ``torch.fx``.
+
+GPT-Neo's attention is global in every layer unless the configuration names the layers
+(``attention_layers=("global", "local", ...)``): a local layer's token sees the ``window_size`` tokens up
+to itself.
 """
 from __future__ import annotations
 
@@ -46,6 +50,8 @@ class GPTConfig:
     layer_norm_epsilon: float = 1e-5
     initializer_range: float = 0.02
     model_type: str = "gpt2"
+    attention_layers: tuple = None     # GPT-Neo: "global" or "local" for each layer (None: all global)
+    window_size: int = 256             # tokens that a local layer's token sees
 
     def __post_init__(self):
         if self.intermediate_size is None:
@@ -102,13 +108,15 @@ def _act(name):
     raise ValueError(f"unsupported activation {name}")
 
 
-def _causal_attention(q, k, v, attention_mask, dropout, scale):
-    """q, k, v: [B, H, S, D]; additive mask [B, 1, 1, S] or None."""
+def _causal_attention(q, k, v, attention_mask, dropout, scale, window=None):
+    """q, k, v: [B, H, S, D]; additive mask [B, 1, 1, S] or None; ``window``: keys that a query sees."""
     s = q.size(-2)
     scores = torch.matmul(q, k.transpose(-1, -2))
     if scale is not None:
         scores = scores * scale
     causal = torch.ones(s, s, dtype=torch.bool, device=q.device).tril()
+    if window is not None:
+        causal = causal.triu(1 - window)
     scores = scores.masked_fill(~causal, torch.finfo(scores.dtype).min)
     if attention_mask is not None:
         scores = scores + attention_mask
@@ -167,6 +175,8 @@ class GPT2Block(nn.Module):
 
 # ---------------------------------------------------------------------- #
 class GPTNeoSelfAttention(nn.Module):
+    window = None       # keys that a query sees in a local layer
+
     def __init__(self, config):
         super().__init__()
         h = config.hidden_size
@@ -186,7 +196,7 @@ class GPTNeoSelfAttention(nn.Module):
         q = self._heads(self.q_proj(hidden_states))
         k = self._heads(self.k_proj(hidden_states))
         v = self._heads(self.v_proj(hidden_states))
-        ctx = _causal_attention(q, k, v, attention_mask, self.attn_dropout, None)
+        ctx = _causal_attention(q, k, v, attention_mask, self.attn_dropout, None, self.window)
         ctx = ctx.permute(0, 2, 1, 3).contiguous()
         ctx = ctx.view(ctx.size()[:-2] + (-1,))
         return (self.resid_dropout(self.out_proj(ctx)), None)
@@ -255,9 +265,22 @@ class GPTTransformer(_GPTBase):
         self.wpe = nn.Embedding(config.n_positions, config.hidden_size)
         self.drop = nn.Dropout(config.embed_dropout)
         self.h = nn.ModuleList([block_cls(config) for _ in range(config.num_layers)])
+        if config.attention_layers is not None:
+            self._localise(config)
         self.ln_f = nn.LayerNorm(config.hidden_size, eps=config.layer_norm_epsilon)
         self.register_buffer("position_ids", torch.arange(config.n_positions).unsqueeze(0),
                              persistent=False)
+
+    def _localise(self, config):
+        kinds = tuple(config.attention_layers)
+        if len(kinds) != config.num_layers or set(kinds) - {"global", "local"}:
+            raise ValueError(f"attention_layers: 'global' or 'local' for each of {config.num_layers} layers "
+                             f"required, not {kinds}")
+        for block, kind in zip(self.h, kinds):
+            if kind == "local":
+                if not isinstance(block, GPTNeoBlock):
+                    raise ValueError("only GPT-Neo has local layers")
+                block.attn.attention.window = config.window_size
 
     def forward(self, input_ids, attention_mask=None, position_ids=None):
         if position_ids is None:

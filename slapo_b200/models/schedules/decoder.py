@@ -6,7 +6,9 @@ MLP, embeddings and head live in each model).  Options (``sch_config``):
 ``attn_op_name``, ``disable_flash_attn``, ``fuse`` (FusedMLP / fused
 LayerNorm), ``sequence_parallel`` (+ ``sequence_parallel_axis``),
 ``ckpt_ratio``, ``checkpoint_method`` (``uniform`` | ``head``), ``bcast_input``,
-``pipeline_cuts``, ``trace_config`` (the example shapes - ``batch_size``, ``seq_len`` or
+``pipeline_cuts``, ``local_attention`` (the local layers of an unmodified Hugging Face GPT-Neo stay local;
+default: all layers are global, as the reference replaces them; this library's GPT-Neo is followed in any
+case), ``trace_config`` (the example shapes - ``batch_size``, ``seq_len`` or
 ``input_shapes`` - that the graphs of an unmodified Hugging Face model are specialised on when
 pipeline cuts make the recipe trace it).
 
@@ -114,7 +116,15 @@ def _extract_qkv(old, kind, hidden):
     return ws, bs, (old.out_proj.weight.data, old.out_proj.bias.data)
 
 
-def replace_attention(sch, config, lay, prefix, attn_op_name):
+def _window(old, config, local_attention):
+    """The window of the attention module that is replaced, or None."""
+    window = getattr(old, "window", None)
+    if window is None and local_attention and getattr(old, "attention_type", None) == "local":
+        window = int(config.window_size)
+    return window
+
+
+def replace_attention(sch, config, lay, prefix, attn_op_name, local_attention=False):
     count = 0
     hidden = config.hidden_size
     heads = _cfg(config, lay["heads"])
@@ -131,7 +141,7 @@ def replace_attention(sch, config, lay, prefix, attn_op_name):
                               attn_op_name=attn_op_name, bias=has_bias, output_proj=True,
                               fused_qkv=True, causal=True, scale=lay["scale"],
                               device="meta" if is_meta else probe.weight.device,
-                              dtype=probe.weight.dtype)
+                              dtype=probe.weight.dtype, window=_window(old, config, local_attention))
         if not is_meta:
             ws, bs, (ow, ob) = _extract_qkv(old, lay["kind"], hidden)
             attn.qkv.weight = nn.Parameter(
@@ -269,7 +279,7 @@ def schedule_decoder(model, family, model_config=None, prefix=None, fp16=False, 
                      group=None, attn_op_name="auto", disable_flash_attn=False, fuse=True,
                      sequence_parallel=False, sequence_parallel_axis=1, ckpt_ratio=0.0,
                      checkpoint_method="uniform", bcast_input=False, pipeline_cuts=None,
-                     trace_config=None,
+                     trace_config=None, local_attention=False,
                      shard_vocab=True, **_unused):
     lay = LAYOUTS[family]
     config = model_config if model_config is not None else getattr(model, "config", None)
@@ -280,7 +290,8 @@ def schedule_decoder(model, family, model_config=None, prefix=None, fp16=False, 
     prefix = lay["prefix"] if prefix is None else prefix
     if prefix not in sch:  # the trunk itself was passed in
         prefix = prefix.split(".", 1)[1] if "." in prefix and prefix.split(".", 1)[1] in sch else ""
-    n_attn = 0 if disable_flash_attn else replace_attention(sch, config, lay, prefix, attn_op_name)
+    n_attn = 0 if disable_flash_attn else replace_attention(sch, config, lay, prefix, attn_op_name,
+                                                            local_attention)
     n_mlp = replace_mlp(sch, config, lay, prefix) if fuse else 0
     n_ln = replace_layernorm(sch) if fuse else 0
     if shard_vocab:

@@ -45,8 +45,13 @@ class FlashAttentionOp(nn.Module):
     traceable = False
 
     def __init__(self, attn_op_name="auto", apply_causal_mask=False, scale=None,
-                 rel_bias_table=None, rel_bidirectional=True, rel_max_distance=128):
+                 rel_bias_table=None, rel_bidirectional=True, rel_max_distance=128, window=None,
+                 sinks=0):
+        """``window``, ``sinks``: every query sees so many keys up to its own and the first ``sinks`` keys
+        (:func:`slapo_b200.ops.functional.flash_attention`)."""
         super().__init__()
+        NF.check_window(window, sinks, apply_causal_mask, rel_bias_table)
+        self.window, self.sinks = window, sinks
         self.attn_op_name = attn_op_name
         self.apply_causal_mask = apply_causal_mask
         self.scale = scale
@@ -68,14 +73,14 @@ class FlashAttentionOp(nn.Module):
             return NF.attention_reference(
                 query_layer, key_layer, value_layer, None, self.apply_causal_mask, self.scale, p,
                 self.training, table, self.rel_bidirectional, self.rel_max_distance,
-                attn_bias=attention_mask)
+                attn_bias=attention_mask, window=self.window, sinks=self.sinks)
         key_bias = self._key_bias(attention_mask, key_layer.shape[0], key_layer.shape[1])
         args = (query_layer, key_layer, value_layer, key_bias, self.apply_causal_mask,
                 self.scale, p, self.training, table, self.rel_bidirectional,
                 self.rel_max_distance)
         if self.attn_op_name in _REFERENCE_NAMES:
-            return NF.attention_reference(*args)
-        return NF.flash_attention(*args)
+            return NF.attention_reference(*args, window=self.window, sinks=self.sinks)
+        return NF.flash_attention(*args, window=self.window, sinks=self.sinks)
 
     def _is_general_bias(self, attention_mask):
         """True for a 4-D bias that is not a key-padding mask (nor, for causal attention, the
@@ -117,10 +122,11 @@ class FlashAttentionOp(nn.Module):
         key_bias = self._key_bias(attention_mask, qkv.shape[0], qkv.shape[1])
         return flash_attention_qkvpacked(
             qkv, key_bias, self.apply_causal_mask, self.scale, p if self.training else 0.0,
-            self.rel_bias_table, self.rel_bidirectional, self.rel_max_distance)
+            self.rel_bias_table, self.rel_bidirectional, self.rel_max_distance, self.window, self.sinks)
 
     def extra_repr(self):
-        return f"op={self.attn_op_name}, causal={self.apply_causal_mask}, scale={self.scale}"
+        window = "" if self.window is None else f", window={self.window}, sinks={self.sinks}"
+        return f"op={self.attn_op_name}, causal={self.apply_causal_mask}, scale={self.scale}" + window
 
 
 class FlashAttention(nn.Module):
@@ -128,11 +134,12 @@ class FlashAttention(nn.Module):
 
     ``causal=None`` keeps the reference's convention (causal iff the block has
     an output projection, slapo/op/attention.py:428); pass it explicitly for
-    anything else."""
+    anything else.  ``window`` and ``sinks`` limit what a token sees (``FlashAttentionOp``), in generation
+    over a cache as in training."""
 
     def __init__(self, hidden_size, num_attention_heads, attn_pdrop=0.0, resid_pdrop=0.0,
                  attn_op_name="auto", bias=True, output_proj=True, fused_qkv=False,
-                 causal=None, scale=None, device=None, dtype=None):
+                 causal=None, scale=None, device=None, dtype=None, window=None, sinks=0):
         super().__init__()
         if hidden_size % num_attention_heads != 0:
             raise ValueError(f"hidden size {hidden_size} is not a multiple of "
@@ -154,7 +161,7 @@ class FlashAttention(nn.Module):
             self.resid_dropout = nn.Dropout(resid_pdrop)
         self.attn_pdrop = attn_pdrop
         causal = output_proj if causal is None else causal
-        self.attn_op = FlashAttentionOp(attn_op_name, causal, scale)
+        self.attn_op = FlashAttentionOp(attn_op_name, causal, scale, window=window, sinks=sinks)
 
     @staticmethod
     def layout_qkv_from_separate(q, k, v, num_heads):

@@ -65,26 +65,33 @@ def relative_bias_by_distance(table, sq, sk, bidirectional, max_distance):
     return table.float()[buckets].t().contiguous()
 
 
-def flash_attention_native(q, k, v, key_bias, causal, scale, p, rel_table, rel_bidir, rel_maxd):
+def flash_attention_native(q, k, v, key_bias, causal, scale, p, rel_table, rel_bidir, rel_maxd,
+                           window=None, sinks=0):
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if key_bias is not None:
         key_bias = key_bias.float().contiguous()
     rel = None
     if rel_table is not None:
         rel = relative_bias_by_distance(rel_table, q.shape[1], k.shape[1], rel_bidir, rel_maxd)
-    return native.ops().flash(q, k, v, key_bias, rel, bool(causal), float(scale), float(p))
+    return native.ops().flash(q, k, v, key_bias, rel, bool(causal), float(scale), float(p),
+                              window or 0, sinks)
 
 
 def flash_attention_qkvpacked(qkv, key_bias=None, causal=False, scale=None, p=0.0,
-                              rel_table=None, rel_bidir=True, rel_maxd=128):
-    """Attention on a packed ``[B, S, H, 3, D]`` projection output."""
+                              rel_table=None, rel_bidir=True, rel_maxd=128, window=None, sinks=0):
+    """Attention on a packed ``[B, S, H, 3, D]`` projection output (``window``, ``sinks``: see
+    :func:`slapo_b200.ops.functional.flash_attention`)."""
+    from .functional import check_window
+
+    check_window(window, sinks, causal, rel_table)
     scale = 1.0 / math.sqrt(qkv.shape[-1]) if scale is None else scale
     if key_bias is not None:
         key_bias = key_bias.float().contiguous()
     rel = None
     if rel_table is not None:
         rel = relative_bias_by_distance(rel_table, qkv.shape[1], qkv.shape[1], rel_bidir, rel_maxd)
-    return native.ops().flash(qkv, None, None, key_bias, rel, bool(causal), float(scale), float(p))
+    return native.ops().flash(qkv, None, None, key_bias, rel, bool(causal), float(scale), float(p),
+                              window or 0, sinks)
 
 
 def packed_supported(qkv) -> bool:

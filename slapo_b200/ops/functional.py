@@ -249,15 +249,33 @@ def t5_relative_position_bucket(relative_position, bidirectional=True, num_bucke
     return ret + torch.where(is_small, rp, large)
 
 
+def check_window(window, sinks, causal, rel_bias_table=None):
+    """Refuse what attention with a window does not take: see :func:`flash_attention`."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks are the keys that stay visible outside of a window: give one")
+        return
+    if isinstance(window, bool) or not isinstance(window, int) or window < 1:
+        raise ValueError(f"a window is a number of keys, 1 and more, not {window!r}")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError(f"sinks is a number of keys, not {sinks!r}")
+    if not causal:
+        raise ValueError("a window needs causal attention")
+    if rel_bias_table is not None:
+        raise ValueError("a window and a relative-position table are not supported together")
+
+
 def attention_reference(q, k, v, key_padding_bias=None, causal=False, scale=None,
                         dropout_p=0.0, training=False, rel_bias_table=None,
                         rel_bidirectional=True, rel_max_distance=128, dropout_mask=None,
-                        attn_bias=None):
+                        attn_bias=None, window=None, sinks=0):
     """Plain-PyTorch attention on ``[B, S, H, D]`` tensors (the oracle).
 
     ``key_padding_bias`` is an additive ``[B, Sk]`` bias (0 / large negative);
     ``rel_bias_table`` a ``[num_buckets, H]`` T5 relative-position table; ``attn_bias`` any
-    additive bias that broadcasts to ``[B, H, Sq, Sk]`` (only this function takes one)."""
+    additive bias that broadcasts to ``[B, H, Sq, Sk]`` (only this function takes one);
+    ``window`` and ``sinks`` as in :func:`flash_attention`."""
+    check_window(window, sinks, causal, rel_bias_table)
     b, sq, h, d = q.shape
     sk = k.shape[1]
     scale = (1.0 / math.sqrt(d)) if scale is None else scale
@@ -276,13 +294,30 @@ def attention_reference(q, k, v, key_padding_bias=None, causal=False, scale=None
     if causal:
         keep = torch.ones(sq, sk, dtype=torch.bool, device=q.device).tril(diagonal=sk - sq)
         scores = scores.masked_fill(~keep, float("-inf"))
-    probs = torch.softmax(scores, dim=-1)
+    if window is not None:
+        hidden = _outside_window(sq, sk, window, sinks, q.device)
+        for bias in (None if key_padding_bias is None else key_padding_bias.view(b, 1, 1, sk), attn_bias):
+            if bias is not None:
+                hidden = hidden | (bias.float() < -1e30)
+        scores = scores.masked_fill(hidden, float("-inf"))
+        # (a row without a key: probabilities and gradients of 0)
+        empty = (scores == float("-inf")).all(-1, keepdim=True)
+        probs = torch.softmax(scores.masked_fill(empty, 0.0), dim=-1).masked_fill(empty, 0.0)
+    else:
+        probs = torch.softmax(scores, dim=-1)
     if dropout_mask is not None:
         probs = probs * dropout_mask / (1.0 - dropout_p)
     elif dropout_p > 0.0 and training:
         probs = F.dropout(probs, dropout_p, True)
     out = torch.matmul(probs, vf)
     return out.transpose(1, 2).to(q.dtype)
+
+
+def _outside_window(sq, sk, window, sinks, device):
+    """``[Sq, Sk]``: keys before a query's window that are not sinks."""
+    pos = torch.arange(sq, device=device)[:, None] + (sk - sq)
+    key = torch.arange(sk, device=device)[None, :]
+    return (key <= pos - window) & (key >= sinks)
 
 
 def _transformed(tensors):
@@ -332,17 +367,25 @@ def _warn_attention_fallback(q, k):
 
 def flash_attention(q, k, v, key_padding_bias=None, causal=False, scale=None, dropout_p=0.0,
                     training=True, rel_bias_table=None, rel_bidirectional=True,
-                    rel_max_distance=128):
+                    rel_max_distance=128, window=None, sinks=0):
     """Attention on ``[B, S, H, D]`` tensors (any strides on B/S/H, D
-    contiguous).  CUDA bf16/fp16 inputs run the tcgen05 flash kernels."""
+    contiguous).  CUDA bf16/fp16 inputs run the tcgen05 flash kernels.
+
+    ``window``, with ``causal``: a query sees the ``window`` keys up to its own and the first ``sinks`` keys;
+    tiles of keys that no query of a tile sees are not touched.  Queries are the last ``Sq`` of ``Sk``
+    positions, as without.  A key with a bias below -1e30 (-inf, a mask of the type's lowest value) is then
+    not seen at all, and a query that sees no key has an output and gradients of 0.  Keys and values must be
+    finite, hidden ones too."""
+    check_window(window, sinks, causal, rel_bias_table)
     from .flash_attn import flash_attention_native, native_supported
 
     if torch.is_tensor(q) and q.is_cuda and native_supported(q, k, v):
         _native_ok(q)
         return flash_attention_native(q, k, v, key_padding_bias, causal, scale,
                                       dropout_p if training else 0.0, rel_bias_table,
-                                      rel_bidirectional, rel_max_distance)
+                                      rel_bidirectional, rel_max_distance, window, sinks)
     if torch.is_tensor(q) and q.is_cuda:
         _warn_attention_fallback(q, k)
     return attention_reference(q, k, v, key_padding_bias, causal, scale, dropout_p, training,
-                               rel_bias_table, rel_bidirectional, rel_max_distance)
+                               rel_bias_table, rel_bidirectional, rel_max_distance, window=window,
+                               sinks=sinks)
