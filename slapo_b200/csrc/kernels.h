@@ -37,11 +37,11 @@ int launch_embedding_fwd(const void* ids, bool ids64, const void* w, void* out, 
                          int64_t cols, int64_t row_stride, int64_t start, float scale, int dtype,
                          cudaStream_t stream);
 // Its gradient: dw [rows, cols] contiguous, every row written; tokens with id `padding` have none.
-// Scratch in 32-bit words: ids and places twice (`sorted` each), the rows' ranges, shares of frequent rows.
+// Scratch in 32-bit words: ids and places twice (`sorted` each), where the rows' tokens end, sums of rows whose tokens go
+// over several of the stretches that the sorted tokens are dealt out in.
 struct EmbedGradPlan {
-  int64_t sorted, range, shares, part;
-  int share;          // sorted tokens to a share
-  int64_t words() const { return 4 * sorted + range + part; }
+  int64_t sorted, ends, stretches, part;
+  int64_t words() const { return 4 * sorted + ends + part; }
 };
 EmbedGradPlan embedding_bwd_plan(int64_t tokens, int64_t rows, int64_t cols);
 int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, int32_t* scratch,
