@@ -50,7 +50,7 @@ int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, 
 
 // AdamW over many tensors (adamw_multi.cu).  Pointers of one tensor of n values in row order; master: fp32 weights
 // or null (then `param` is what is updated); m, v: moments, fp32 or with m_scale and v_scale 8 bits in blocks of 256;
-// aligned: all on 16 bytes (8-bit moments on 8), so that vectors of eight can be read
+// aligned: all on 32 bytes, so that vectors can be read
 struct AdamwTensor {
   void* param;
   const void* grad;

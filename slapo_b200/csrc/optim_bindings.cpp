@@ -71,6 +71,7 @@ void multi_adamw(List params, List grads, List masters, List exp_avgs, List exp_
               "multi_adamw: betas in [0, 1) and eps >= 0 required");
   TORCH_CHECK(n <= INT_MAX, "multi_adamw: too many tensors");
   const Tensor& p0 = params[0];
+  TORCH_CHECK(masters.empty() || p0.scalar_type() != at::kFloat, "multi_adamw: fp32 parameters are their own masters");
   TORCH_CHECK(p0.is_cuda(), "multi_adamw: parameters must be CUDA tensors");
   const at::ScalarType type = p0.scalar_type(), moments = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
   slapo::AdamwScalars s{};
@@ -118,8 +119,7 @@ void multi_adamw(List params, List grads, List masters, List exp_avgs, List exp_
     t.n = count;
     t.lr = static_cast<float>(lrs[i]);
     t.weight_decay = static_cast<float>(weight_decays[i]);
-    t.aligned = on(t.param, 16) && on(t.grad, 16) && on(t.master, 16) && on(t.m, bits8 ? 8 : 16) &&
-                on(t.v, bits8 ? 8 : 16);
+    t.aligned = on(t.param, 32) && on(t.grad, 32) && on(t.master, 32) && on(t.m, 32) && on(t.v, 32);
     if (count > 0) table.push_back(t);
   }
   for (auto& [list, name] : {std::make_pair(params, "parameters"), std::make_pair(masters, "masters"),

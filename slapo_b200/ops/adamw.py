@@ -71,13 +71,13 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
         w -= lr * ((m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps) + weight_decay * w)
 
     All lists have one entry per parameter: contiguous tensors of the parameter's length on one device,
-    parameters and gradients of one type (bf16, fp16 or fp32).  ``masters``: fp32 weights that are updated
-    and rounded to the parameters (without them the parameters themselves are).  ``exp_avgs`` and
-    ``exp_avg_sqs`` are fp32, or with ``exp_avg_scales`` and ``exp_avg_sq_scales`` 8-bit moments as
-    :func:`quantize_moment` makes them.  ``lr`` and ``weight_decay``: a number, or one per tensor.  ``step``
-    counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step goes on
-    counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in its
-    place)."""
+    parameters and gradients of one type (bf16, fp16 or fp32).  ``masters``, for 16-bit parameters: fp32
+    weights that are updated and rounded to the parameters (without them the parameters themselves are).
+    ``exp_avgs`` and ``exp_avg_sqs`` are fp32, or with ``exp_avg_scales`` and ``exp_avg_sq_scales`` 8-bit
+    moments as :func:`quantize_moment` makes them.  ``lr`` and ``weight_decay``: a number, or one per tensor.
+    ``step`` counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step goes
+    on counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in its
+    place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits."""
     params, grads = list(params), list(grads)
     n = len(params)
     lrs, decays = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")
@@ -101,6 +101,8 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
     for name, got in (("masters", masters), ("factors", m_scales), ("factors", v_scales)):
         if len(got) not in (0, n):
             raise ValueError(f"{name}: {n} tensors required, not {len(got)}")
+    if masters and params[0].dtype == torch.float32:
+        raise ValueError("fp32 parameters are their own masters")
     t = int(step)
     if t < 1:
         raise ValueError(f"steps count from 1, not {t}")

@@ -171,5 +171,7 @@ def test_refusals():
         multi_tensor_adamw(z(), z(), z(), z(), lr=[1.0, 2.0], step=1)
     with pytest.raises(ValueError, match="gradients"):
         multi_tensor_adamw(z(), [], z(), z(), lr=1.0, step=1)
+    with pytest.raises(ValueError, match="own masters"):
+        multi_tensor_adamw(z(), z(), z(), z(), lr=1.0, step=1, masters=z())
     multi_tensor_adamw([], [], [], [], lr=1.0, step=1)
     assert math.isfinite(float(w.sum()))
