@@ -46,11 +46,14 @@ int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float
                      float scale, int causal, int window, int sinks, float p_drop, PhiloxArgs rng, bool bf16,
                      int* status, cudaStream_t stream);
 // How the backward runs, and its scratch in floats: row statistics, padded key bias, keep bits
-// (dropout in two launches) and shares of dQ (keys split over work items).
+// (dropout in two launches) and shares of dQ (keys split over work items)
+// or of the sinks' dK and dV (queries split).
 struct FlashBwdPlan {
   int pairs;         // (batch, head) pairs per launch: the keep bits of all would grow with B H Sq Sk
   int splits;        // work items per query tile in the dQ pass
   int q_ctas;        // both passes in one launch, this many CTAs for dQ; 0: one launch each
+  int sink_splits;   // with a window and no dropout: work items for each key tile with sinks in the dK / dV pass, and
+  int sink_each;     // the half tiles of queries to each but the last
   int64_t stats, bias, keep, part;
   int64_t total() const { return stats + bias + keep + part; }
 };

@@ -59,6 +59,8 @@
 #include "flash_common.cuh"
 #include "kernels.h"
 
+#include <algorithm>
+
 namespace slapo {
 
 struct FlashBwdParams {
@@ -69,8 +71,9 @@ struct FlashBwdParams {
   TileWalk walk;
   int splits;             // dQ pass: work items per row tile, each takes tiles_per_split key tiles
   int tiles_per_split;
-  float* part;            // splits > 1: [splits][B Sq H][Dr] fp32 shares of dQ
-  int64_t part_rows;      // B Sq H
+  float* part;            // splits > 1: [splits][B Sq H][Dr] fp32 shares of dQ, or [splits][dK, dV][B H][rows of the
+                          // sinks' tiles][Dr]
+  int64_t part_rows;      // B Sq H, or B H rows
   const float* nlse;      // [B H][Rq]  -log2(e) * lse ; -inf for rows without any key (and padding)
   const float* ndelta;    // [B H][Rq]  -rowsum(dO O) * keep probability ; 0 in the padding
   const float* kb2;       // [B][Rk] log2(e) * key bias, 0 in the padding, or nullptr
@@ -83,6 +86,10 @@ struct FlashBwdParams {
   float scale, scale_log2, inv_keep;
   int causal;
   int window, sinks;      // kWin: a query sees `window` keys up to its own and the first `sinks` (see KeyWindow)
+  // ... dK / dV pass: row tiles that the sinks lie in, each `splits` work items (see sink_splits) of sink_each half tiles,
+  // the last of what is left
+  int sink_tiles, sink_each;
+  FastDiv sink_div;       // by splits
   uint32_t thr7;          // dropout: keep a draw >= thr7 of 128 ; 0 = no dropout
   PhiloxArgs rng;
   uint32_t idesc_s, idesc_acc;
@@ -200,9 +207,11 @@ struct BwdSmem {
 // groups (warps 4 - 11 and 12 - 19), a row and half of a half tile's columns per thread, which take the half
 // tiles in turn; and the warps that read the accumulators out (20 - 23).
 // kKeys: the dK / dV pass.  kGeneral: key bias, relative bias, causal mask or ragged lengths.
-// kWin (with kGeneral): a window and sinks.  kDrop: with dropout.  kDraw: the dK / dV pass then draws the keep decisions itself, and the dQ pass leaves none.
+// kWindow (with kGeneral): 1 = a window and sinks, 2 = the queries of the sinks' tiles dealt out too (in a dK / dV pass of
+// its own form: as a run-time choice it cost every other call, 4 x 2048 x 16 x 128 with a window of 256: 115 -> 140 us).
+// kDrop: with dropout.  kDraw: the dK / dV pass then draws the keep decisions itself, and the dQ pass leaves none.
 // CTA `cta` of `ctas` that run the pass.
-template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kDraw, bool kWin, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kDraw, int kWindow, typename T>
 __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtensorMap& tm_x2,
                                          const CUtensorMap& tm_y1, const CUtensorMap& tm_y2,
                                          const FlashBwdParams& p, const int cta, const int ctas) {
@@ -247,7 +256,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
   constexpr uint32_t kAccCols = kKeys ? 2 * D : D;        // from one set to the next
   constexpr int kAcc = kKeys && D == 128 ? 1 : 2;
   const int items = p.walk.items() * (kKeys ? 1 : p.splits);
-  constexpr bool drop = kDrop;
+  constexpr bool drop = kDrop, kWin = kWindow != 0, kShares = kWindow == 2 && kKeys;
   const KeyWindow keys{diag, p.window, p.sinks};
   // The j-th half tile that a work item streams, `first` of item_at.  With a window the dQ pass goes through the
   // sinks' half tiles first, and `first` is the gap behind them.
@@ -255,6 +264,18 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
     return kWin && !kKeys && j < ((p.sinks + 63) >> 6) ? j : first + j;
   };
 
+  // With a window, dK / dV pass: the queries of a row tile with sinks are dealt out to p.splits work items.  Which
+  // share a work item has, given its place `tile` in the order of work items, and its row tile; -1 if it has all.
+  auto sink_share = [&](int& tile) {
+    if (!kShares) return -1;
+    if (tile >= p.sink_tiles * p.splits) {
+      tile -= p.sink_tiles * (p.splits - 1);
+      return -1;
+    }
+    const int place = tile;
+    tile = p.sink_div(place);
+    return place - tile * p.splits;
+  };
   // row tile and (batch, head) of a work item, its first streamed half tile and how many (at least
   // one: a row tile or a split that nothing reaches still has its zeros written)
   auto item_at = [&](int item, int& tile, int& bhl, int& first) {
@@ -263,6 +284,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
     int n;
     first = 0;
     if constexpr (kKeys) {
+      const int share = sink_share(tile);
       n = (p.Sq + 63) >> 6;
       if (p.causal) first = min(max(0, tile * 128 - diag) >> 6, n - 1);
       if constexpr (kWin) {     // the last query that sees any of the tile's keys (sinks: all do)
@@ -271,6 +293,10 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
         n = max(n, first + 1);
       }
       n -= first;
+      if (kShares && share >= 0) {
+        first += share * p.sink_each;
+        n = share + 1 < p.splits ? p.sink_each : n - share * p.sink_each;
+      }
     } else {
       n = (p.Sk + 63) >> 6;
       if (p.causal) n = min(n, (min(tile * 128 + 128, p.Sq) + diag + 63) >> 6);
@@ -616,6 +642,20 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
         }
       }
     };
+    // ... of a share of the sinks' dK and dV, as they are (apart, so that the other stays as short as it is)
+    auto read_share = [&](uint32_t col, float* share, bool row_ok) {
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t r[16];
+        tc::tmem_ld_x16(tmem_row + col + c, r);
+        tc::tmem_ld_wait();
+        if (!row_ok) continue;
+#pragma unroll
+        for (int g = 0; g < 16; g += 4)
+          if (c + g < p.Dr)
+            *reinterpret_cast<uint4*>(share + c + g) = make_uint4(r[g], r[g + 1], r[g + 2], r[g + 3]);
+      }
+    };
     Ring<kAcc> acc;
     for (int item = cta; item < items; item += ctas, acc.step()) {
       int tile, bhl, first;
@@ -628,19 +668,32 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
       float* share = nullptr;
       if (!kKeys && p.splits > 1)
         share = p.part + (static_cast<int64_t>(item % p.splits) * p.part_rows + at) * p.Dr;
+      if constexpr (kShares) {
+        int place, pair;
+        p.walk.at(item, place, pair);
+        const int which = sink_share(place);
+        if (which >= 0)
+          share = p.part + (2 * which * p.part_rows + static_cast<int64_t>(bh) * p.sink_tiles * 128 + row) * p.Dr;
+      }
       if constexpr (kKeys) {      // (dV's last product is a step before dK's)
         if (!tc::mbar_wait_warp(&acc2_full[acc.slot], acc.phase, abort_flag)) break;
         tc::fence_after_sync();
-        read_out(kColA2 + acc.slot * kAccCols, p.inv_keep, static_cast<T*>(p.out2) + at * p.row_stride2, nullptr,
-                 row < rows);
+        if (kShares && share != nullptr)
+          read_share(kColA2 + acc.slot * kAccCols, share + p.part_rows * p.Dr, row < rows);
+        else
+          read_out(kColA2 + acc.slot * kAccCols, p.inv_keep, static_cast<T*>(p.out2) + at * p.row_stride2, nullptr,
+                   row < rows);
         tc::fence_before_sync();
         __syncwarp();
         tc::mbar_arrive_if(&acc2_free[acc.slot], lane == 0);
       }
       if (!tc::mbar_wait_warp(&acc1_full[acc.slot], acc.phase, abort_flag)) break;
       tc::fence_after_sync();
-      read_out(kColA1 + acc.slot * kAccCols, out_scale, static_cast<T*>(p.out1) + at * p.row_stride1, share,
-               row < rows);
+      if (kShares && share != nullptr)
+        read_share(kColA1 + acc.slot * kAccCols, share, row < rows);
+      else
+        read_out(kColA1 + acc.slot * kAccCols, out_scale, static_cast<T*>(p.out1) + at * p.row_stride1, share,
+                 row < rows);
       tc::fence_before_sync();
       __syncwarp();
       tc::mbar_arrive_if(&acc1_free[acc.slot], lane == 0);
@@ -982,16 +1035,16 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_x1, const CUtenso
 }
 
 // One pass.
-template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, int kWindow, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 flash_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__ CUtensorMap tm_x2,
                  const __grid_constant__ CUtensorMap tm_y1, const __grid_constant__ CUtensorMap tm_y2,
                  const __grid_constant__ FlashBwdParams p) {
-  bwd_pass<D, kKeys, kGeneral, kDrop, false, kWin, T>(tm_x1, tm_x2, tm_y1, tm_y2, p, blockIdx.x, gridDim.x);
+  bwd_pass<D, kKeys, kGeneral, kDrop, false, kWindow, T>(tm_x1, tm_x2, tm_y1, tm_y2, p, blockIdx.x, gridDim.x);
 }
 
 // Both passes side by side, the dQ pass on the first `q_ctas` CTAs.
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 flash_bwd_both_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -999,9 +1052,9 @@ flash_bwd_both_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
                       const __grid_constant__ FlashBwdParams pk, const int q_ctas) {
   const int cta = blockIdx.x;
   if (cta < q_ctas)
-    bwd_pass<D, false, kGeneral, kDrop, true, kWin, T>(tm_q, tm_do, tm_k, tm_v, pq, cta, q_ctas);
+    bwd_pass<D, false, kGeneral, kDrop, true, kWindow, T>(tm_q, tm_do, tm_k, tm_v, pq, cta, q_ctas);
   else
-    bwd_pass<D, true, kGeneral, kDrop, true, kWin, T>(tm_k, tm_v, tm_q, tm_do, pk, cta - q_ctas,
+    bwd_pass<D, true, kGeneral, kDrop, true, kWindow, T>(tm_k, tm_v, tm_q, tm_do, pk, cta - q_ctas,
                                                      gridDim.x - q_ctas);
 }
 
@@ -1022,6 +1075,33 @@ __global__ void __launch_bounds__(256) flash_dq_combine_kernel(const float* __re
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] *= scale;
   Vec8<T>::store(dq + at, v);
+}
+
+// dK and dV of the sinks' tiles: their shares added in their order, eight values to a thread
+template <typename T>
+__global__ void __launch_bounds__(256) flash_sink_combine_kernel(const FlashBwdParams p, int pairs_rows, int sink_rows,
+                                                                 float dk_scale) {
+  const int64_t vecs = static_cast<int64_t>(pairs_rows) * (p.Dr / 8);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= 2 * vecs) return;
+  const int which = i >= vecs ? 1 : 0;         // dV
+  const int64_t v = i - which * vecs, at = v / (p.Dr / 8);
+  const int d = static_cast<int>(v - at * (p.Dr / 8)) * 8;
+  const int bh = static_cast<int>(at / sink_rows), row = static_cast<int>(at - static_cast<int64_t>(bh) * sink_rows);
+  const int batch = bh / p.H, head = bh - batch * p.H;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float* part = p.part + (which * p.part_rows + static_cast<int64_t>(bh) * p.sink_tiles * 128 + row) * p.Dr + d;
+  for (int s = 0; s < p.splits; ++s) {
+    float x[8];
+    Vec8<float>::load(part + 2 * s * p.part_rows * p.Dr, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum[k] += x[k];
+  }
+  const float f = which == 0 ? dk_scale : p.inv_keep;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[k] *= f;
+  const int64_t to = (static_cast<int64_t>(batch) * p.Sk + row) * p.H + head;
+  Vec8<T>::store(static_cast<T*>(which == 0 ? p.out1 : p.out2) + to * (which == 0 ? p.row_stride1 : p.row_stride2) + d, sum);
 }
 
 // A kernel's shared memory, allowed once per kernel
@@ -1058,33 +1138,33 @@ static int launch_bwd(void (*kernel)(P...), int ctas, int smem, bool early, cuda
   return 4;
 }
 
-template <int D, bool kKeys, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kKeys, bool kGeneral, bool kDrop, int kWindow, typename T>
 static int launch_pass(const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
                        const CUtensorMap& y2, const FlashBwdParams& p, cudaStream_t stream) {
   constexpr int kSmem = BwdSmem<D, kKeys>::kTotal;
   static_assert(kSmem <= 227 * 1024, "flash backward: shared memory over the per-CTA limit");
-  auto kernel = flash_bwd_kernel<D, kKeys, kGeneral, kDrop, kWin, T>;
+  auto kernel = flash_bwd_kernel<D, kKeys, kGeneral, kDrop, kWindow, T>;
   static bool configured = false;
   if (!allow_smem(kernel, kSmem, configured)) return 3;
-  const int64_t items = static_cast<int64_t>(p.walk.row_tiles) * p.walk.nbh * p.splits;
+  const int64_t items = static_cast<int64_t>(p.walk.row_tiles) * p.walk.nbh * (kKeys ? 1 : p.splits);
   const int64_t cap = sm_count();
   return launch_bwd(kernel, static_cast<int>(items < cap ? items : cap), kSmem, items <= 3 * cap, stream,
                     x1, x2, y1, y2, p);
 }
 
 // The passes of `pq` (dQ) and `pk` (dK / dV), side by side or one after the other
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 static int launch_passes(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                          const CUtensorMap& dout, const FlashBwdParams& pq, const FlashBwdParams& pk,
                          int q_ctas, cudaStream_t stream) {
   if (q_ctas == 0) {
     // dQ first: with dropout it leaves the keep bits that the dK / dV pass reads
-    const int rc = launch_pass<D, false, kGeneral, kDrop, kWin, T>(q, dout, k, v, pq, stream);
-    return rc != 0 ? rc : launch_pass<D, true, kGeneral, kDrop, kWin, T>(k, v, q, dout, pk, stream);
+    const int rc = launch_pass<D, false, kGeneral, kDrop, (kWindow > 0 ? 1 : 0), T>(q, dout, k, v, pq, stream);
+    return rc != 0 ? rc : launch_pass<D, true, kGeneral, kDrop, kWindow, T>(k, v, q, dout, pk, stream);
   }
   constexpr int kSmemQ = BwdSmem<D, false>::kTotal, kSmemK = BwdSmem<D, true>::kTotal;
   constexpr int kSmem = kSmemQ > kSmemK ? kSmemQ : kSmemK;
-  auto kernel = flash_bwd_both_kernel<D, kGeneral, kDrop, kWin, T>;
+  auto kernel = flash_bwd_both_kernel<D, kGeneral, kDrop, kWindow, T>;
   static bool configured = false;
   if (!allow_smem(kernel, kSmem, configured)) return 3;
   const int64_t items = static_cast<int64_t>(pk.walk.row_tiles) * pk.walk.nbh;
@@ -1099,10 +1179,12 @@ template <bool kDrop, typename T>
 static int launch_typed(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                         const CUtensorMap& dout, const FlashBwdParams& pq, const FlashBwdParams& pk,
                         int q_ctas, bool general, cudaStream_t stream) {
-#define FLASH_BWD_PASSES(D_)                                                                                \
-  pq.window > 0 ? launch_passes<D_, true, kDrop, true, T>(q, k, v, dout, pq, pk, q_ctas, stream)            \
-  : general     ? launch_passes<D_, true, kDrop, false, T>(q, k, v, dout, pq, pk, q_ctas, stream)           \
-                : launch_passes<D_, false, kDrop, false, T>(q, k, v, dout, pq, pk, q_ctas, stream)
+  // (with dropout the sinks' tiles are not dealt out)
+#define FLASH_BWD_PASSES(D_)                                                                                       \
+  !kDrop && pk.splits > 1 ? launch_passes<D_, true, kDrop, kDrop ? 1 : 2, T>(q, k, v, dout, pq, pk, q_ctas, stream) \
+  : pq.window > 0         ? launch_passes<D_, true, kDrop, 1, T>(q, k, v, dout, pq, pk, q_ctas, stream)            \
+  : general               ? launch_passes<D_, true, kDrop, 0, T>(q, k, v, dout, pq, pk, q_ctas, stream)            \
+                          : launch_passes<D_, false, kDrop, 0, T>(q, k, v, dout, pq, pk, q_ctas, stream)
   if (pq.Dr <= 64) return FLASH_BWD_PASSES(64);
   return FLASH_BWD_PASSES(128);
 #undef FLASH_BWD_PASSES
@@ -1148,6 +1230,28 @@ static int both_q_ctas(int64_t q_items, int64_t k_items, int64_t q_item_tiles, i
   return best_n;
 }
 
+// Work items for each row tile of keys with sinks, which all later queries see: about as long as those of other tiles, or
+// half of what a CTA has to do in all (the sinks' come first), with at most 64 MB of shares.
+static int sink_splits(int64_t bh, int Sq, int Sk, int D, int window, int sinks, int* each) {
+  *each = 0;
+  const int64_t half_tiles = (static_cast<int64_t>(Sq) + 63) / 64, k_tiles = round128(Sk) / 128;
+  const int64_t sink_tiles = (static_cast<int64_t>(sinks < Sk ? sinks : Sk) + 127) / 128;
+  const int64_t near = (static_cast<int64_t>(window < Sk ? window : Sk) + 127 + 63) / 64;
+  if (sink_tiles == 0 || bh == 0 || half_tiles <= near) return 1;
+  const int64_t all = bh * (sink_tiles * half_tiles + (k_tiles - sink_tiles) * near), cta = all / sm_count();
+  const int64_t target = near > cta / 2 ? near : cta / 2;
+  int64_t n = (half_tiles + target - 1) / target;
+  // (no share without a half tile: the last of these tiles has the fewest)
+  const int64_t before = (sink_tiles - 1) * 128 - (static_cast<int64_t>(Sk) - Sq);
+  const int64_t fewest = half_tiles - (before > 0 ? before / 64 : 0);
+  if (n > fewest) n = fewest;
+  const int64_t most = (int64_t(64) << 20) / (2 * bh * sink_tiles * 128 * D * 4);
+  if (n > most) n = most;
+  if (n < 2) return 1;
+  *each = static_cast<int>(fewest / n);
+  return static_cast<int>(n);
+}
+
 FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal, int window, int sinks,
                             bool key_bias, bool rel, float p_drop, int64_t keep_words) {
   FlashBwdPlan s;
@@ -1174,8 +1278,10 @@ FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bo
     if (far < q_item_tiles) q_item_tiles = far;
     if (near < k_item_tiles) k_item_tiles = near;
   }
+  s.sink_splits = window > 0 && !drop ? sink_splits(bh, Sq, Sk, D, window, sinks, &s.sink_each) : 1;
+  const int64_t sink_tiles = (std::min(sinks, Sk) + 127) / 128;
   s.q_ctas = bh == 0 || keep_words > 0 ? 0
-                     : both_q_ctas(q_tiles * bh * s.splits, k_tiles * bh, q_item_tiles, k_item_tiles, D,
+                     : both_q_ctas(q_tiles * bh * s.splits, (k_tiles + sink_tiles * (s.sink_splits - 1)) * bh, q_item_tiles, k_item_tiles, D,
                                    causal && window == 0, rel, drop);
   s.stats = 2 * bh * rq;
   s.bias = key_bias ? B * rk : 0;
@@ -1188,6 +1294,7 @@ FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bo
   s.pairs = static_cast<int>(pairs);
   s.keep = keep ? s.pairs * words : 0;
   s.part = s.splits > 1 ? s.splits * bh * Sq * D : 0;
+  if (s.sink_splits > 1) s.part = s.sink_splits * 2 * bh * sink_tiles * 128 * D;
   return s;
 }
 
@@ -1253,7 +1360,11 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
   pq.tiles_per_split = (p.Rk / 128 + plan.splits - 1) / plan.splits;
   pq.out1 = dq; pq.row_stride1 = dq_row_stride;
   pq.out2 = nullptr; pq.row_stride2 = 0;
-  pk.splits = 1;
+  pk.splits = plan.sink_splits;
+  pk.sink_tiles = (sinks + 127) / 128;
+  pk.sink_each = plan.sink_each;
+  pk.sink_div.set(pk.splits);
+  if (pk.splits > 1) pk.part_rows = static_cast<int64_t>(B) * H * pk.sink_tiles * 128;
   pk.tiles_per_split = p.Rq / 128;
   pk.out1 = dk; pk.row_stride1 = dkv_row_stride;
   pk.out2 = dv; pk.row_stride2 = dkv_row_stride;
@@ -1261,13 +1372,26 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
     const int pairs = bh - at < plan.pairs ? bh - at : plan.pairs;
     // (with a window row tiles differ little, but for the keys of sinks, which all queries see)
     pq.walk.set(p.Rq / 128, at, pairs, causal && window == 0 ? 2 : 0);
-    pk.walk.set(p.Rk / 128, at, pairs, causal && (window == 0 || sinks > 0) ? 1 : 0);
+    pk.walk.set(p.Rk / 128 + (pk.splits > 1 ? pk.sink_tiles * (pk.splits - 1) : 0), at, pairs,
+                causal && (window == 0 || sinks > 0) ? 1 : 0);
 #define FLASH_BWD_CASE(T_)                                                                          \
   p.thr7 != 0 ? launch_typed<true, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)       \
               : launch_typed<false, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)
     const int rc = bf16 ? (FLASH_BWD_CASE(__nv_bfloat16)) : (FLASH_BWD_CASE(__half));
 #undef FLASH_BWD_CASE
     if (rc != 0) return rc;
+  }
+  if (pk.splits > 1) {
+    const int sink_rows = pk.sink_tiles * 128 < Sk ? pk.sink_tiles * 128 : Sk;
+    const int64_t rows = static_cast<int64_t>(bh) * sink_rows;
+    const unsigned blocks = static_cast<unsigned>((2 * rows * (D / 8) + 255) / 256);
+    const float f = p.scale * p.inv_keep;
+    count_launch();
+    if (bf16)
+      flash_sink_combine_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(pk, static_cast<int>(rows), sink_rows, f);
+    else
+      flash_sink_combine_kernel<__half><<<blocks, 256, 0, stream>>>(pk, static_cast<int>(rows), sink_rows, f);
+    if (cudaGetLastError() != cudaSuccess) return 4;
   }
   if (plan.splits > 1) {
     const int64_t n = p.part_rows * D;

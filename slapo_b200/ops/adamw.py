@@ -75,9 +75,9 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
     weights that are updated and rounded to the parameters (without them the parameters themselves are).
     ``exp_avgs`` and ``exp_avg_sqs`` are fp32, or with ``exp_avg_scales`` and ``exp_avg_sq_scales`` 8-bit
     moments as :func:`quantize_moment` makes them.  ``lr`` and ``weight_decay``: a number, or one per tensor.
-    ``step`` counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step goes
-    on counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in its
-    place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits."""
+    ``step`` counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step
+    goes on counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in
+    its place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits."""
     params, grads = list(params), list(grads)
     n = len(params)
     lrs, decays = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")
