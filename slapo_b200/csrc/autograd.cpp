@@ -9,6 +9,7 @@
 //
 // The kernels are reached through their registered operators, so that each keeps its checks.
 #include <ATen/ATen.h>
+#include <ATen/FuncTorchTLS.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -340,8 +341,7 @@ struct FlashFn : public Function<FlashFn> {
     ctx->save_for_backward({q_or_qkv, or_undefined(k), or_undefined(v), out, lse,
                             or_undefined(key_bias), or_undefined(rel)});
     ctx->saved_data["causal"] = causal;
-    ctx->saved_data["window"] = window;
-    ctx->saved_data["sinks"] = sinks;
+    if (window > 0) ctx->saved_data["window"] = std::vector<int64_t>{window, sinks};
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["p"] = p;
     if (rng.has_value()) ctx->saved_data["rng"] = *rng;
@@ -355,11 +355,13 @@ struct FlashFn : public Function<FlashFn> {
     optional<Tensor> rng;
     const double p = ctx->saved_data["p"].toDouble();
     if (p > 0.0) rng = ctx->saved_data["rng"].toTensor();
+    std::vector<int64_t> window{0, 0};
+    if (const auto at = ctx->saved_data.find("window"); at != ctx->saved_data.end()) window = at->second.toIntVector();
     static auto f = op<FlashBwd>("slapo_b200::flash_attn_bwd");
     auto [dq, dk, dv, drel] =
         f.call(grads[0].contiguous(), q, k, v, s[3], s[4], opt(s[5]), opt(s[6]),
                ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), p, rng, packed, /*keep_words=*/0,
-               ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt());
+               window[0], window[1]);
     tensor_list out(10);
     out[0] = dq;
     if (!packed) {
@@ -420,6 +422,15 @@ struct EmbeddingFn : public Function<EmbeddingFn> {
   }
 };
 
+// Whether a node has to be around what is computed of these: something is differentiated or transformed (which the
+// node reports that it does not take)
+bool wants_node(std::initializer_list<const Tensor*> inputs) {
+  if (at::functorch::functorchTLSAccessor() != nullptr) return true;
+  const bool grad = at::GradMode::is_enabled();
+  for (const Tensor* t : inputs)
+    if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
+  return false;
+}
 // ------------------------------------------------------------------------ //
 // A bias that starts anywhere, as the kernels read it: 16 bytes at a time.  (A copy that is differentiated.)
 Tensor aligned(const Tensor& bias) {
@@ -467,11 +478,21 @@ std::tuple<Tensor, Tensor> dropout_add_norm(const Tensor& x, const optional<Tens
 Tensor flash(const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v,
              const optional<Tensor>& key_bias, const optional<Tensor>& rel, bool causal, double scale,
              double p, int64_t window, int64_t sinks) {
+  const Tensor bias = or_undefined(key_bias), distances = or_undefined(rel);
+  if (k.has_value() && v.has_value() && p == 0.0 && !wants_node({&q, &*k, &*v, &bias, &distances})) {
+    // (a token of generation is a launch: no node around it)
+    static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
+    return std::get<0>(f.call(q, *k, *v, key_bias, rel, causal, scale, p, c10::nullopt, window, sinks));
+  }
   return FlashFn::apply(q, k, v, key_bias, rel, causal, scale, p, window, sinks);
 }
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, int64_t start, const optional<int64_t>& padding,
                  double scale) {
+  if (!wants_node({&weight})) {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, double)>("slapo_b200::embedding_fwd");
+    return f.call(ids, weight, start, scale);
+  }
   return EmbeddingFn::apply(weight, ids, start, padding, scale);
 }
 

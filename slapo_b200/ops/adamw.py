@@ -209,7 +209,7 @@ class FusedAdamW(torch.optim.Optimizer):
                     raise RuntimeError("FusedAdamW takes dense gradients")
                 s = self.state[p] or self._init_state(p, self._new_counter(p, fresh))
                 count = s["step"]
-                key = (p.device, p.dtype, group["betas"], group["eps"],
+                key = (p.device, p.dtype, tuple(group["betas"]), group["eps"],
                        id(count) if torch.is_tensor(count) else count)
                 run = runs.get(key)
                 if run is None:

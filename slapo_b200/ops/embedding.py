@@ -38,6 +38,8 @@ class FusedEmbedding(nn.Embedding):
     Ids outside of the table give zeros (see :func:`slapo_b200.ops.functional.embedding`).  ``max_norm``,
     ``scale_grad_by_freq`` and ``sparse`` are not supported."""
 
+    traceable = False
+
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
         super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
         self.scale = float(scale)

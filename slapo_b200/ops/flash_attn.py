@@ -27,8 +27,13 @@ def native_supported(q, k, v) -> bool:
     if q.dim() != 4 or not head_dim_supported(q.shape[-1]):
         return False
     for t in (q, k, v):
-        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        # (one look at each: this is a good part of a token's attention on the host)
+        *outer, last = t.stride()
+        if last != 1 or t.data_ptr() % 16:
             return False
+        for s in outer:
+            if s % 8:
+                return False
     return native.available()
 
 

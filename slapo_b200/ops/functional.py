@@ -380,7 +380,6 @@ def flash_attention(q, k, v, key_padding_bias=None, causal=False, scale=None, dr
     from .flash_attn import flash_attention_native, native_supported
 
     if torch.is_tensor(q) and q.is_cuda and native_supported(q, k, v):
-        _native_ok(q)
         return flash_attention_native(q, k, v, key_padding_bias, causal, scale,
                                       dropout_p if training else 0.0, rel_bias_table,
                                       rel_bidirectional, rel_max_distance, window, sinks)

@@ -56,6 +56,8 @@ def _lower_vocab_embedding(sub, ctx) -> bool:
         return False
     if mod.weight.dtype not in (torch.bfloat16, torch.float16) or mod.embedding_dim % 8:
         return False
+    if getattr(mod, "scale", 1.0) != 1.0:       # (FusedEmbedding's factor)
+        return False
     for table in (mod._forward_pre_hooks, mod._forward_hooks):
         for key, fn in list(table.items()):
             if getattr(fn, "__self__", None) is hooks:
