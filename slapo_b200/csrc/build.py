@@ -7,19 +7,23 @@
 (the kernel sources include no torch header, so each takes seconds), the
 ``.cpp`` binding files with the host compiler against the installed torch,
 and links them into one shared object next to the package, which is what
-``slapo_b200.ops.native`` loads.  Objects are rebuilt only when their source
-or a header changed.  No GPU is needed.
+``slapo_b200.ops.native`` loads; ``py_entry.cpp`` alone becomes the CPython
+module ``slapo_b200/_py.so``.  Objects are rebuilt only when their source or
+a header changed.  No GPU is needed.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 OUT = os.path.join(PKG, "_C.so")
+PY_OUT = os.path.join(PKG, "_py.so")     # a CPython module: hosts without an interpreter load the other
+PY_SRCS = {"py_entry.cpp"}
 OBJ_DIR = os.path.join(HERE, "build")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -72,7 +76,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     # report through the device status word (code 7) instead of touching a bad peer address
     debug = ["-DSLAPO_B200_DEBUG"] if os.environ.get("SLAPO_B200_DEBUG", "0") == "1" else []
     cxx = os.environ.get("CXX", "g++")
-    log, jobs, objs = [], [], []
+    log, jobs, objs, py_objs = [], [], [], []
     for src in cu_srcs:
         obj = os.path.join(OBJ_DIR, src + ".o")
         objs.append(obj)
@@ -82,10 +86,10 @@ def build(verbose: bool = False, force: bool = False) -> str:
     cxx_flags = [f.replace("ABI=1", f"ABI={abi}") for f in CXX_FLAGS]
     for src in cpp_srcs:
         obj = os.path.join(OBJ_DIR, src + ".o")
-        objs.append(obj)
+        (py_objs if src in PY_SRCS else objs).append(obj)
         if force or _newer([os.path.join(HERE, src)] + headers, obj):
             cmd = [cxx] + cxx_flags + ["-I", HERE, "-I", os.path.join(_cuda_home(), "include")]
-            for path in inc:
+            for path in inc + ([sysconfig.get_paths()["include"]] if src in PY_SRCS else []):
                 cmd += ["-isystem", path]
             jobs.append(cmd + ["-c", os.path.join(HERE, src), "-o", obj])
     if jobs:
@@ -113,6 +117,12 @@ def build(verbose: bool = False, force: bool = False) -> str:
             f"-Wl,-rpath,{torch_lib}"]
         _run(link, log)
         os.replace(tmp, OUT)
+    if jobs or force or _newer(py_objs, PY_OUT):
+        tmp = PY_OUT + ".tmp"
+        _run([cxx, "-shared", "-o", tmp] + py_objs + [
+            "-l:libstdc++.so.6", "-L", torch_lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+            f"-Wl,-rpath,{torch_lib}"], log)
+        os.replace(tmp, PY_OUT)
     return OUT
 
 

@@ -1,0 +1,25 @@
+// What AdamW over many tensors takes, as lists of tensors that live elsewhere.
+#pragma once
+#include <ATen/ATen.h>
+
+namespace slapo {
+
+struct AdamwLists {
+  struct List {
+    const at::Tensor* const* at;
+    size_t size;
+    const at::Tensor& operator[](size_t i) const { return *at[i]; }
+  };
+  List params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales;
+  const double* lrs;
+  size_t n_lrs;
+  const double* weight_decays;
+  size_t n_weight_decays;
+  double beta1, beta2, eps;
+  int64_t step;
+  const at::Tensor* step_tensor;       // or null
+  const at::Tensor* grad_scale;        // or null
+};
+using AdamwEntry = void (*)(const AdamwLists&);
+
+}  // namespace slapo

@@ -5,6 +5,7 @@ directory and registers its entry points as ``torch.ops.slapo_b200.*``.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 
 import torch
@@ -40,6 +41,17 @@ def ops():
     if not available():
         raise RuntimeError(f"slapo_b200 native extension unavailable: {_STATE['error']}")
     return torch.ops.slapo_b200
+
+
+def py_module():
+    """The CPython module beside the extension (``csrc/py_entry.cpp``)."""
+    if "py" not in _STATE:
+        path = os.path.join(os.path.dirname(_LIB), "_py.so")
+        spec = importlib.util.spec_from_file_location("slapo_b200._py", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _STATE["py"] = module
+    return _STATE["py"]
 
 
 def reset():

@@ -290,3 +290,43 @@ def test_refusals():
     t["exp_avg_scales"][0] = torch.ones(state_blocks(300) + 1, device="cuda")
     with pytest.raises(RuntimeError, match="factors"):
         multi_tensor_adamw(**t, lr=1e-3, step=1)
+    t = _tensors([300, 40], torch.bfloat16, 32, False)
+    t["grads"][1].untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="no memory"):
+        multi_tensor_adamw(**t, lr=1e-3, step=1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_operator_and_the_lists_agree(bits):
+    """The registered operator, and the entry that reads Python lists in place; the latter leaves tensors that
+    the dispatcher has to see to the former, which has no form for tensors without values."""
+    a = _tensors([300, 4100, 40], torch.bfloat16, bits, True)
+    b = _copy(a)
+    multi_tensor_adamw(**a, lr=[1e-3, 2e-3, 3e-3], weight_decay=0.1, step=3)
+    native.ops().multi_adamw(b["params"], b["grads"], b["masters"], b["exp_avgs"], b["exp_avg_sqs"],
+                             b.get("exp_avg_scales", []), b.get("exp_avg_sq_scales", []), [1e-3, 2e-3, 3e-3],
+                             [0.1] * 3, 0.9, 0.999, 1e-8, 3, None, None)
+    for name in a:
+        for x, y in zip(a[name], b[name]):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        fake = [torch.zeros(8, device="cuda") for _ in range(4)]
+    before = native.launch_count()
+    with pytest.raises(Exception):
+        multi_tensor_adamw([fake[0]], [fake[1]], [fake[2]], [fake[3]], lr=1e-3, step=1)
+    assert native.launch_count() == before
+
+
+def test_another_stream():
+    a = _tensors([70001, 300], torch.bfloat16, 8, True)
+    b = _copy(a)
+    multi_tensor_adamw(**a, lr=1e-3, step=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        multi_tensor_adamw(**b, lr=1e-3, step=1)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in a:
+        for x, y in zip(a[name], b[name]):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
