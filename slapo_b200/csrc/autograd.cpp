@@ -400,28 +400,6 @@ tensor_list RelBiasFn::backward(AutogradContext* ctx, tensor_list grads) {
   return {RelBiasSumFn::apply(grads[0], s[1], s[0].detach()), Tensor()};
 }
 
-// Rows of a table by token ids; the ids are what the backward needs.
-struct EmbeddingFn : public Function<EmbeddingFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, int64_t start,
-                        const optional<int64_t>& padding, double scale) {
-    ctx->save_for_backward({ids});
-    ctx->saved_data["rows"] = weight.size(0);
-    ctx->saved_data["start"] = start;
-    ctx->saved_data["padding"] = padding;
-    ctx->saved_data["scale"] = scale;
-    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, double)>("slapo_b200::embedding_fwd");
-    return f.call(ids, weight, start, scale);
-  }
-  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, int64_t, const optional<int64_t>&, double)>(
-        "slapo_b200::embedding_bwd");
-    return {f.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
-                   ctx->saved_data["start"].toInt(), ctx->saved_data["padding"].toOptional<int64_t>(),
-                   ctx->saved_data["scale"].toDouble()),
-            Tensor(), Tensor(), Tensor(), Tensor()};
-  }
-};
-
 // Whether a node has to be around what is computed of these: something is differentiated or transformed (which the
 // node reports that it does not take)
 bool wants_node(std::initializer_list<const Tensor*> inputs) {
@@ -431,6 +409,61 @@ bool wants_node(std::initializer_list<const Tensor*> inputs) {
     if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
   return false;
 }
+
+// Rows of a table by token ids, and the sum over the tokens of each id: linear maps, each the other's derivative (of
+// any order), but for the padding id, whose tokens have a row and give none.
+struct TokenRows {
+  int64_t rows, start;
+  optional<int64_t> padding;
+  double scale;
+  void save(AutogradContext* ctx) const {
+    ctx->saved_data["rows"] = rows;
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["scale"] = scale;
+  }
+  static TokenRows saved(AutogradContext* ctx) {
+    return {ctx->saved_data["rows"].toInt(), ctx->saved_data["start"].toInt(),
+            ctx->saved_data["padding"].toOptional<int64_t>(), ctx->saved_data["scale"].toDouble()};
+  }
+  Tensor lookup(const Tensor& ids, const Tensor& weight) const {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, double)>("slapo_b200::embedding_fwd");
+    return f.call(ids, weight, start, scale);
+  }
+  Tensor sum(const Tensor& ids, const Tensor& dy) const {
+    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, int64_t, const optional<int64_t>&, double)>(
+        "slapo_b200::embedding_bwd");
+    return f.call(dy, ids, rows, start, padding, scale);
+  }
+};
+struct EmbeddingFn : public Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, const TokenRows& at) {
+    ctx->save_for_backward({ids});
+    at.save(ctx);
+    return at.lookup(ids, weight);
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads);
+};
+struct EmbeddingSumFn : public Function<EmbeddingSumFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dy, const Tensor& ids, const TokenRows& at) {
+    ctx->save_for_backward({ids});
+    at.save(ctx);
+    return at.sum(ids, dy);
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const Tensor ids = ctx->get_saved_variables()[0];
+    const TokenRows at = TokenRows::saved(ctx);
+    Tensor out = EmbeddingFn::apply(grads[0].contiguous(), ids, at);
+    if (at.padding.has_value()) out = out.masked_fill(ids.eq(*at.padding).unsqueeze(-1), 0.0);
+    return {out, Tensor(), Tensor()};
+  }
+};
+tensor_list EmbeddingFn::backward(AutogradContext* ctx, tensor_list grads) {
+  const Tensor ids = ctx->get_saved_variables()[0];
+  const TokenRows at = TokenRows::saved(ctx);
+  return {wants_node({&grads[0]}) ? EmbeddingSumFn::apply(grads[0], ids, at) : at.sum(ids, grads[0]), Tensor(), Tensor()};
+}
+
 // ------------------------------------------------------------------------ //
 // A bias that starts anywhere, as the kernels read it: 16 bytes at a time.  (A copy that is differentiated.)
 Tensor aligned(const Tensor& bias) {
@@ -489,11 +522,9 @@ Tensor flash(const Tensor& q, const optional<Tensor>& k, const optional<Tensor>&
 
 Tensor embedding(const Tensor& ids, const Tensor& weight, int64_t start, const optional<int64_t>& padding,
                  double scale) {
-  if (!wants_node({&weight})) {
-    static auto f = op<Tensor(const Tensor&, const Tensor&, int64_t, double)>("slapo_b200::embedding_fwd");
-    return f.call(ids, weight, start, scale);
-  }
-  return EmbeddingFn::apply(weight, ids, start, padding, scale);
+  const TokenRows at{weight.size(0), start, padding, scale};
+  if (!wants_node({&weight})) return at.lookup(ids, weight);
+  return EmbeddingFn::apply(weight, ids, at);
 }
 
 Tensor rel_bias(const Tensor& table, const Tensor& buckets) { return RelBiasFn::apply(table, buckets); }

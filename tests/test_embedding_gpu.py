@@ -161,3 +161,55 @@ def test_refusals():
         native.ops().embedding_bwd(torch.randn(3, 8, device="cuda"), ids, 10, 0, None, 1.0)
     with pytest.raises(RuntimeError, match="int64 or int32"):
         native.ops().embedding_fwd(ids.short(), w, 0, 1.0)
+
+
+@pytest.mark.parametrize("padding", [None, 3])
+def test_second_derivatives(padding):
+    """Lookup and gradient are each other's derivative: as indexing the table in 64 bits, to the roundings of
+    the chain (2^-24 each, sums of fewer than 64 terms)."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn(9, 8, device="cuda", generator=g).requires_grad_()
+    x = torch.randn(40, 8, device="cuda", generator=g).requires_grad_()
+    ids = torch.randint(-1, 10, (40,), device="cuda", generator=g)      # (two of them outside of the table)
+
+    def third(w, x, lookup):
+        out = lookup(w)
+        (dw,) = torch.autograd.grad((out ** 3 * x).sum(), w, create_graph=True)
+        dw2, dx2 = torch.autograd.grad((dw ** 2).sum(), (w, x), create_graph=True)
+        return [dw, dw2, dx2, *torch.autograd.grad((dw2 * dw).sum() + (dx2 ** 2).sum(), (w, x))]
+
+    def plain(w):
+        own = (ids >= 0) & (ids < 9)
+        rows = w[ids.clamp(0, 8)]
+        if padding is not None:
+            rows = torch.where((ids != padding)[:, None], rows, rows.detach())
+        return torch.where(own[:, None], rows, 0.0) * 1.5
+
+    got = third(w, x, lambda w: NF.embedding(ids, w, padding_idx=padding, scale=1.5))
+    w64, x64 = (t.detach().double().requires_grad_() for t in (w, x))
+    want = third(w64, x64, plain)
+    for a, b in zip(got, want):
+        assert bool(((a.double() - b).abs() <= 256 * 2.0 ** -24 * b.abs().max()).all())
+
+
+def test_offsets_beyond_32_bits():
+    """A table and a gradient of more than 2^31 elements, each row by one token."""
+    rows, cols = 270_000, 8192
+    g = torch.Generator(device="cuda").manual_seed(2)
+    ids = torch.randperm(rows, device="cuda", generator=g)
+    w = torch.randn(rows, 1, device="cuda", generator=g).to(torch.bfloat16)
+    w = (w * torch.linspace(1, 2, cols, device="cuda", dtype=torch.bfloat16)).requires_grad_()
+    out = NF.embedding(ids, w)
+    assert torch.equal(out.detach(), w.detach()[ids])
+    (dw,) = torch.autograd.grad(out, w, out.detach())
+    assert torch.equal(dw, w.detach())
+
+
+def test_the_same_row_as_parameter_of_two_lookups():
+    """A table that is looked up twice in a step: gradients add up."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = torch.randn(50, 16, device="cuda", generator=g).requires_grad_()
+    a, b = (torch.randint(0, 50, (n,), device="cuda", generator=g) for n in (30, 70))
+    (NF.embedding(a, w).sum() + NF.embedding(b, w, scale=2.0).sum()).backward()
+    want = torch.bincount(a, minlength=50) + 2 * torch.bincount(b, minlength=50)
+    assert torch.equal(w.grad, want[:, None].float().expand(50, 16))
