@@ -162,9 +162,10 @@ class FusedAdamW(torch.optim.Optimizer):
     ``state_bits``: 32, or 8 for moments of one byte each (rounded by at most 1 / 16 of themselves).
     ``master_weights``: keep fp32 copies of 16-bit parameters, which are what is updated (default); without
     them an update below half a step of the parameter's type is lost.  ``capturable``: steps are counted on
-    the device, so that a captured ``step()`` can be replayed; parameters that were first updated together
-    then have to go on together.  ``step(grad_scale=...)`` takes a one-element fp32
-    tensor that multiplies every gradient (clipping, loss scaling).  Parameter groups may differ in ``lr``,
+    the device, so that a captured ``step()`` can be replayed (with the ``lr`` and ``weight_decay`` of its
+    capture); parameters that were first updated together then have to go on together.
+    ``step(grad_scale=...)`` takes a one-element fp32 tensor that multiplies every gradient (clipping, loss
+    scaling).  Parameter groups may differ in ``lr``,
     ``weight_decay``, ``betas`` and ``eps``.  Parameters must be contiguous and their gradients dense."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
@@ -275,7 +276,11 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``; states keep their own types, whatever the
-        parameters' is."""
+        parameters' is.  Saved moments of another number of bits are refused; masters that are wanted and were
+        not saved are made of the parameters, and saved ones that are not wanted are left out."""
+        for old in state_dict["state"].values():
+            if ("exp_avg_scale" in old) != (self.state_bits == 8):
+                raise ValueError("the saved moments have another number of bits")
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
@@ -284,9 +289,11 @@ class FusedAdamW(torch.optim.Optimizer):
             old = state_dict["state"].get(index)
             if old is None:
                 continue
-            if ("exp_avg_scale" in old) != (self.state_bits == 8):
-                raise ValueError("the saved moments have another number of bits")
             s = self.state[p]
+            s.pop("master", None)
+            keeps = self.master_weights and p.dtype != torch.float32
+            if keeps and "master" not in old:
+                s["master"] = p.detach().float()
             for name, value in old.items():
                 if name == "step":
                     step = int(value)
@@ -297,5 +304,5 @@ class FusedAdamW(torch.optim.Optimizer):
                         s["step"] = counters[p.device, step]
                     else:
                         s["step"] = step
-                elif torch.is_tensor(value):
+                elif torch.is_tensor(value) and (keeps or name != "master"):
                     s[name] = value.detach().to(device=p.device, copy=True)

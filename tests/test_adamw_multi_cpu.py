@@ -102,6 +102,29 @@ def test_state_dict_round_trip(bits, dtype):
         FusedAdamW(b.parameters(), state_bits=40 - bits).load_state_dict(opt.state_dict())
 
 
+@pytest.mark.parametrize("saved,wanted", [(True, False), (False, True)])
+def test_state_of_an_optimizer_with_other_masters(saved, wanted):
+    """Masters that were not saved begin at the parameters; those that are not wanted are left out.  Refused
+    states leave the optimizer as it was."""
+    a = _model().to(torch.bfloat16)
+    opt = FusedAdamW(a.parameters(), lr=1e-2, master_weights=saved)
+    _grads(a, 0)
+    opt.step()
+    b = copy.deepcopy(a)
+    other = FusedAdamW(b.parameters(), lr=1e-2, master_weights=wanted)
+    other.load_state_dict(opt.state_dict())
+    for p in b.parameters():
+        assert ("master" in other.state[p]) == wanted
+        if wanted:
+            assert torch.equal(other.state[p]["master"], p.float())
+    _grads(b, 1)
+    other.step()
+    fresh = FusedAdamW(_model().parameters(), state_bits=8)
+    with pytest.raises(ValueError, match="bits"):
+        fresh.load_state_dict(opt.state_dict())
+    assert not fresh.state
+
+
 def test_parameters_without_a_gradient_are_left_alone():
     m = _model()
     opt = FusedAdamW(m.parameters(), lr=1e-2)
@@ -186,7 +209,8 @@ def test_the_entry_for_lists_refuses_other_things():
     rest = (p, p, [], p, p, [], [], [0.1], [0.1], 0.9, 0.99, 1e-8, 1, None, None)
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         call(entry, *rest)
-    for at, value in ((0, tuple(p)), (1, [None]), (7, [1]), (7, ["x"]), (9, "x"), (12, 1.5), (13, 3), (14, [])):
+    for at, value in ((0, tuple(p)), (1, [None]), (7, [1]), (7, ["x"]), (9, "x"), (12, 1.5), (13, 3),
+                      (14, [])):
         bad = list(rest)
         bad[at] = value
         with pytest.raises((TypeError, RuntimeError)):

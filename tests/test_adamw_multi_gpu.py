@@ -330,3 +330,25 @@ def test_another_stream():
     for name in a:
         for x, y in zip(a[name], b[name]):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_beyond_32_bits(bits):
+    """A parameter of more than 2^31 elements: its end as that part alone, and zeros stay zeros."""
+    n, tail = 2 ** 31 + 812, 812
+    small = _tensors([tail], torch.bfloat16, bits, False)
+    large = {k: [torch.zeros(n if "scale" not in k else state_blocks(n), device="cuda",
+                             dtype=torch.uint8 if v[0].dtype == torch.float8_e4m3fn else v[0].dtype)]
+             for k, v in small.items()}
+    for name, (x,) in large.items():
+        if "scale" in name:
+            x.fill_(2.0 ** -126)
+        if x.dtype == torch.uint8:
+            large[name][0] = x.view(torch.float8_e4m3fn)
+        x[-small[name][0].numel():].copy_(small[name][0].view(x.dtype))
+    for t in (small, large):
+        multi_tensor_adamw(**t, lr=1e-3, step=2)
+    for name, (x,) in large.items():
+        end = small[name][0].numel()
+        assert torch.equal(x[-end:].view(torch.uint8), small[name][0].view(torch.uint8)), name
+    assert int(torch.count_nonzero(large["params"][0][:-tail])) == 0

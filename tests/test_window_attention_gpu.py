@@ -298,3 +298,41 @@ def test_refusals():
         NF.flash_attention(q, q, q, causal=True, window=0)
     huge = NF.flash_attention(q, q, q, causal=True, window=2 ** 40, sinks=2 ** 40)
     assert torch.equal(huge, NF.flash_attention(q, q, q, causal=True))
+
+
+@pytest.mark.parametrize("sq,window,sinks", [(1, 500, 4), (40, 300, 0), (40, 300, 130)])
+def test_offsets_beyond_32_bits(sq, window, sinks):
+    """A cache of more than 2^31 elements: as over the keys alone that any query sees."""
+    b, sk, n, d = 2, 600_000, 16, 128
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(b, sq, n, d, generator=g, device="cuda").to(torch.bfloat16)
+    do = torch.randn(b, sq, n, d, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.empty(b, sk, n, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g) for _ in "kv")
+    kept = torch.cat((torch.arange(sinks), torch.arange(sk - window - sq + 1, sk))).cuda()
+    if sq == 1:
+        _check([NF.flash_attention(q, k, v, causal=True, window=window, sinks=sinks)], q, k[:, kept],
+               v[:, kept], None, window, sinks)
+        return
+    out, dq, dk, dv = _run(*(t.requires_grad_() for t in (q, k, v)), do, window, sinks)
+    _check([out, dq, dk[:, kept], dv[:, kept]], q, k[:, kept], v[:, kept], do, window, sinks)
+    rest = torch.ones(sk, dtype=torch.bool, device="cuda")
+    rest[kept] = False
+    for t in (dk, dv):
+        assert int(t.ne(0).view(b, sk, -1).any(-1)[:, rest].sum()) == 0
+
+
+def test_two_streams_at_once():
+    """Calls in flight together share nothing."""
+    q, k, v, do = _tensors(2, 700, 700, 4, 64, torch.bfloat16)
+    want = _run(q, k, v, do, 200, 130)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(_run(q, k, v, do, 200, 130))
+    torch.cuda.synchronize()
+    for one in got:
+        for a, b in zip(one, want):
+            assert torch.equal(a, b)
