@@ -48,6 +48,7 @@ std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, cons
   check_bshd(q, "q"); check_bshd(k, "k"); check_bshd(v, "v");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "bf16/fp16 only");
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "q, k and v must be on one device");
   c10::cuda::CUDAGuard guard(q.device());
   const int B = q.size(0), Sq = q.size(1), H = q.size(2), D = q.size(3), Sk = k.size(1);
   TORCH_CHECK(k.size(0) == B && k.size(2) == H && k.size(3) == D && v.sizes() == k.sizes());

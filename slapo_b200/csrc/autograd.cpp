@@ -14,6 +14,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include "py_entry.h"
+
 namespace {
 
 using at::Tensor;
@@ -541,6 +543,11 @@ void register_autograd_ops(torch::Library& m) {
   m.def("dropout_add_norm(Tensor x, Tensor? bias, Tensor residual, Tensor weight, Tensor? ln_bias, float p, float eps) -> (Tensor, Tensor)",
         &dropout_add_norm);
   m.def("rel_bias(Tensor table, Tensor buckets) -> Tensor", &rel_bias);
+  // for py_entry.cpp: where these functions are
+  m.def("flash_entry() -> int",
+        []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::FlashEntry>(&flash)); });
+  m.def("embedding_entry() -> int",
+        []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::EmbeddingEntry>(&embedding)); });
   m.def("embedding(Tensor ids, Tensor weight, int start, int? padding, float scale) -> Tensor", &embedding);
   m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p, int window=0, int sinks=0) -> Tensor",
         &flash);

@@ -9,7 +9,7 @@
 #include <vector>
 
 #include "kernels.h"
-#include "optim_entry.h"
+#include "py_entry.h"
 
 namespace {
 

@@ -61,9 +61,6 @@ def _per_tensor(value, n, name):
     return [float(value)] * n
 
 
-_ENTRY = []       # the address of the extension's function
-
-
 @torch.no_grad()
 def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 0.999), eps=1e-8,
                        weight_decay=0.01, step, masters=None, exp_avg_scales=None, exp_avg_sq_scales=None,
@@ -94,11 +91,9 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
         return
     if params[0].is_cuda and native_adamw():
         on_device = torch.is_tensor(step)
-        if not _ENTRY:
-            _ENTRY.append(native.ops().multi_adamw_entry())
         args = (params, grads, masters, exp_avgs, exp_avg_sqs, m_scales, v_scales, lrs, decays, betas[0],
                 betas[1], eps, 0 if on_device else step, step if on_device else None, grad_scale)
-        if not native.py_module().multi_adamw(_ENTRY[0], *args):   # a tensor that the dispatcher has to see
+        if not native.direct("multi_adamw")(*args):      # (something that the dispatcher has to see)
             native.ops().multi_adamw(*args)
         return
     for name, got in (("gradients", grads), ("first moments", exp_avgs), ("second moments", exp_avg_sqs)):

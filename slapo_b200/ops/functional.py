@@ -156,6 +156,11 @@ def embedding(ids, weight, padding_idx=None, scale: float = 1.0, vocab_start: in
     Ids outside of ``[vocab_start, vocab_start + rows)`` give zeros and no gradient, so that a shard of a
     table takes the ids of all (no id is an error).  Tokens with id ``padding_idx`` have no gradient.  The
     gradient of a row is summed in fp32 in the order of its tokens and rounded once, the same every time."""
+    if torch.is_tensor(weight) and weight.is_cuda:
+        fn = native.direct("embedding")
+        out = None if fn is None else fn(ids, weight, vocab_start, padding_idx, scale)
+        if out is not None:
+            return out
     if weight.dim() != 2:
         raise ValueError(f"a 2-D table is required, not {tuple(weight.shape)}")
     if ids.dtype not in (torch.int64, torch.int32):
@@ -377,6 +382,11 @@ def flash_attention(q, k, v, key_padding_bias=None, causal=False, scale=None, dr
     not seen at all, and a query that sees no key has an output and gradients of 0.  Keys and values must be
     finite, hidden ones too."""
     check_window(window, sinks, causal, rel_bias_table)
+    if torch.is_tensor(q) and q.is_cuda and rel_bias_table is None and not (training and dropout_p > 0.0):
+        fn = native.direct("flash")
+        out = None if fn is None else fn(q, k, v, key_padding_bias, causal, scale, window, sinks)
+        if out is not None:
+            return out
     from .flash_attn import flash_attention_native, native_supported
 
     if torch.is_tensor(q) and q.is_cuda and native_supported(q, k, v):

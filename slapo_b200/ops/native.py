@@ -5,6 +5,7 @@ directory and registers its entry points as ``torch.ops.slapo_b200.*``.
 """
 from __future__ import annotations
 
+import functools
 import importlib.util
 import os
 
@@ -12,6 +13,7 @@ import torch
 
 _LIB = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_C.so")
 _STATE = {"tried": False, "ok": False, "error": None}
+_DIRECT = {}
 
 
 def lib_path() -> str:
@@ -43,15 +45,19 @@ def ops():
     return torch.ops.slapo_b200
 
 
-def py_module():
-    """The CPython module beside the extension (``csrc/py_entry.cpp``)."""
-    if "py" not in _STATE:
-        path = os.path.join(os.path.dirname(_LIB), "_py.so")
-        spec = importlib.util.spec_from_file_location("slapo_b200._py", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        _STATE["py"] = module
-    return _STATE["py"]
+def direct(name):
+    """The function ``name`` of the CPython module beside the extension (``csrc/py_entry.cpp``), without its
+    first argument; None without the extension."""
+    fn = _DIRECT.get(name)
+    if fn is None and available():
+        if "module" not in _DIRECT:
+            path = os.path.join(os.path.dirname(_LIB), "_py.so")
+            spec = importlib.util.spec_from_file_location("slapo_b200._py", path)
+            _DIRECT["module"] = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(_DIRECT["module"])
+        entry = int(getattr(ops(), name + "_entry")())
+        fn = _DIRECT[name] = functools.partial(getattr(_DIRECT["module"], name), entry)
+    return fn
 
 
 def reset():

@@ -204,16 +204,16 @@ def test_the_entry_for_lists_refuses_other_things():
     from slapo_b200.ops import native
     if not native.available():
         pytest.skip("extension not built")
-    call, entry = native.py_module().multi_adamw, native.ops().multi_adamw_entry()
+    call = native.direct("multi_adamw")
     p = [torch.zeros(3)]
     rest = (p, p, [], p, p, [], [], [0.1], [0.1], 0.9, 0.99, 1e-8, 1, None, None)
     with pytest.raises(RuntimeError, match="CUDA tensors"):
-        call(entry, *rest)
+        call(*rest)
     for at, value in ((0, tuple(p)), (1, [None]), (7, [1]), (7, ["x"]), (9, "x"), (12, 1.5), (13, 3),
                       (14, [])):
         bad = list(rest)
         bad[at] = value
         with pytest.raises((TypeError, RuntimeError)):
-            call(entry, *bad)
+            call(*bad)
     with pytest.raises(TypeError):
-        call(entry, *rest[:-1])
+        call(*rest[:-1])

@@ -336,3 +336,57 @@ def test_two_streams_at_once():
     for one in got:
         for a, b in zip(one, want):
             assert torch.equal(a, b)
+
+
+def test_modes_see_the_operators():
+    """Calls go past the dispatcher only where nobody watches it, with the same results."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class WatchFunctions(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    q, k, v, _ = (t.detach() for t in _tensors(2, 1, 300, 4, 64, torch.bfloat16))
+    ids = torch.arange(5, device="cuda")
+    bias = torch.zeros(2, 300, device="cuda")
+    for b in (None, bias, bias.to(torch.bfloat16)):       # (the last is converted in Python)
+        plain = NF.flash_attention(q, k, v, b, causal=True, window=200, sinks=3)
+        for mode in (Watch, WatchFunctions):
+            seen.clear()
+            with mode():
+                watched = NF.flash_attention(q, k, v, b, causal=True, window=200, sinks=3)
+            # (a dispatch mode sees what the operator allocates, as of every operator of the extension)
+            assert any(("flash" if mode is WatchFunctions else "empty") in name for name in seen)
+            assert torch.equal(plain, watched)
+    table = q.reshape(8, 64)
+    plain = NF.embedding(ids, table, scale=2.0)
+    seen.clear()
+    with WatchFunctions():
+        watched = NF.embedding(ids, table, scale=2.0)
+    assert any("embedding" in name for name in seen) and torch.equal(plain, watched)
+
+
+def test_tensors_that_calls_do_not_take_as_they_are():
+    """Subclasses, odd strides, parameters, another default for the scale: the same as contiguous tensors."""
+    class Sub(torch.Tensor):
+        pass
+
+    q, k, v, do = _tensors(2, 130, 130, 4, 64, torch.bfloat16)
+    want = _run(q, k, v, do, 100, 3)
+    got = _run(*(torch.nn.Parameter(t.detach()) for t in (q, k, v)), do, 100, 3, scale=0.125)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    out = NF.flash_attention(*(t.detach().as_subclass(Sub) for t in (q, k, v)), causal=True, window=100,
+                             sinks=3)
+    assert torch.equal(out.as_subclass(torch.Tensor), want[0].detach())
+    with pytest.raises(Exception, match="Expected|sizes|size"):
+        NF.flash_attention(q, k.detach()[:, :, :2], v, causal=True, window=100)
