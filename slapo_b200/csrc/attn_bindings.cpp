@@ -40,11 +40,13 @@ std::pair<int, int> check_window(int64_t window, int64_t sinks, bool causal, con
   return {static_cast<int>(std::min(window, most)), static_cast<int>(std::min(sinks, most))};
 }
 
-std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
+// Output, log-sum-exp and, where `keep_rest` asks for it and the kernels leave it, what the output has lost by rounding
+// (else empty)
+std::tuple<Tensor, Tensor, Tensor> run_flash_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                           const optional<Tensor>& kbias,
                                           const optional<Tensor>& rel, bool causal, double scale,
                                           double p_drop, const optional<Tensor>& rng, int64_t window_in,
-                                          int64_t sinks_in) {
+                                          int64_t sinks_in, bool keep_rest) {
   check_bshd(q, "q"); check_bshd(k, "k"); check_bshd(v, "v");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "bf16/fp16 only");
   TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
@@ -65,15 +67,43 @@ std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, cons
   Tensor scratch;
   if (splits > 1)
     scratch = at::empty({splits * B * H * Sq * (D + 2)}, q.options().dtype(at::kFloat));
+  // Rows that see few keys: those of small windows, the first ones of short sequences, those in a padding.  Where such rows
+  // count, what the output loses by rounding is kept for the backward's row terms.  Error of dQ over that of its rounding
+  // alone, fp16, without / with it (sqrt 2 is the least, dS being rounded too): window 4: 1.78 / 1.49, 16: 1.53 / 1.45,
+  // 64 queries: 1.56 / 1.44, 256: 1.55 / 1.44; 1000 with a third of padding 1.60 / 1.45.  Else there is little to gain for
+  // a byte per value and 2 - 5 % of the time: 2048 queries, window 256: 1.46 / 1.43, 183 / 194 us (B 4, H 16, D 128).
+  // (A window over all keys is causal attention, with its results to the bit.  Split keys are joined by a kernel that
+  // leaves none, and one query's kernel neither: rows that see many keys.)
+  const bool few_keys = (kbias.has_value() && kbias->defined()) || window < 128 || Sk < 1024;
+  Tensor rest;
+  if (keep_rest)
+    rest = at::empty(few_keys && window > 0 && window < Sk && splits == 1 && Sq > 1 ? at::IntArrayRef({B, Sq, H, D}) : at::IntArrayRef({0}),
+                     q.options().dtype(at::kByte));
   int rc = slapo::launch_flash_fwd(
-      q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
+      q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+      keep_rest && rest.numel() > 0 ? rest.data_ptr<uint8_t>() : nullptr, lse.data_ptr<float>(),
       splits > 1 ? scratch.data_ptr<float>() : nullptr,
       opt_f32(kbias, "key bias"), opt_f32(rel, "relative bias"), B, H, Sq, Sk, D, qs, ks, vs,
       static_cast<float>(scale), causal ? 1 : 0, window, sinks, static_cast<float>(p_drop), unpack_rng(rng),
       q.scalar_type() == at::kBFloat16, slapo_status_ptr(q.get_device()),
       at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "flash_attn_fwd: launch refused (code ", rc, ")");
+  return {o, lse, rest};
+}
+
+std::tuple<Tensor, Tensor> flash_attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                          const optional<Tensor>& kbias,
+                                          const optional<Tensor>& rel, bool causal, double scale,
+                                          double p_drop, const optional<Tensor>& rng, int64_t window,
+                                          int64_t sinks) {
+  auto [o, lse, rest] = run_flash_fwd(q, k, v, kbias, rel, causal, scale, p_drop, rng, window, sinks, false);
   return {o, lse};
+}
+std::tuple<Tensor, Tensor, Tensor> flash_attn_fwd_rest(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                       const optional<Tensor>& kbias, const optional<Tensor>& rel,
+                                                       bool causal, double scale, double p_drop,
+                                                       const optional<Tensor>& rng, int64_t window, int64_t sinks) {
+  return run_flash_fwd(q, k, v, kbias, rel, causal, scale, p_drop, rng, window, sinks, true);
 }
 
 // keep_words: see flash_bwd_plan (0: its default)
@@ -81,7 +111,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
     const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o,
     const Tensor& lse, const optional<Tensor>& kbias, const optional<Tensor>& rel, bool causal,
     double scale, double p_drop, const optional<Tensor>& rng, bool packed_qkv, int64_t keep_words, int64_t window_in,
-    int64_t sinks_in) {
+    int64_t sinks_in, const optional<Tensor>& rest) {
   check_bshd(q, "q"); check_bshd(k, "k"); check_bshd(v, "v");
   TORCH_CHECK(dout.is_contiguous() && o.is_contiguous(), "dout and out must be contiguous");
   c10::cuda::CUDAGuard guard(q.device());
@@ -116,8 +146,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
   const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)};
   const int64_t ks[3] = {k.stride(0), k.stride(1), k.stride(2)};
   const int64_t vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
+  const bool has_rest = rest.has_value() && rest->defined() && rest->numel() > 0;
+  if (has_rest)
+    TORCH_CHECK(rest->device() == q.device() && rest->scalar_type() == at::kByte && rest->is_contiguous() &&
+                    rest->numel() == o.numel(), "flash_attn_bwd: one byte for each value of the output required");
   int rc = slapo::launch_flash_bwd(
-      q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dout.data_ptr(),
+      q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+      has_rest ? rest->const_data_ptr<uint8_t>() : nullptr, dout.data_ptr(),
       lse.data_ptr<float>(), plan, scratch.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
       dv.data_ptr(), row_stride, row_stride, opt_f32(kbias, "key bias"),
       opt_f32(rel, "relative bias"),
@@ -261,7 +296,9 @@ Tensor rel_bias_bwd(const Tensor& grad, const Tensor& buckets, const Tensor& tab
 void register_attn_ops(torch::Library& m) {
   m.def("flash_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, int window=0, int sinks=0) -> (Tensor, Tensor)",
         &flash_attn_fwd);
-  m.def("flash_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, bool packed_qkv, int keep_words=0, int window=0, int sinks=0) -> (Tensor, Tensor, Tensor, Tensor)",
+  m.def("flash_attn_fwd_rest(Tensor q, Tensor k, Tensor v, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, int window=0, int sinks=0) -> (Tensor, Tensor, Tensor)",
+        &flash_attn_fwd_rest);
+  m.def("flash_attn_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor? kbias, Tensor? rel, bool causal, float scale, float p_drop, Tensor? rng, bool packed_qkv, int keep_words=0, int window=0, int sinks=0, Tensor? rest=None) -> (Tensor, Tensor, Tensor, Tensor)",
         &flash_attn_bwd);
   m.def("append_kv(Tensor past_k, Tensor past_v, Tensor k, Tensor v) -> (Tensor, Tensor)", &append_kv);
   m.def("rel_buckets(Tensor table, int sq, int sk, bool bidirectional, float inv_exact, float inv_log) -> Tensor",

@@ -321,10 +321,13 @@ struct DropoutAddNormFn : public Function<DropoutAddNormFn> {
 using FlashFwd = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&,
                                             const optional<Tensor>&, const optional<Tensor>&, bool,
                                             double, double, const optional<Tensor>&, int64_t, int64_t);
+using FlashFwdRest = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&,
+                                                        const optional<Tensor>&, const optional<Tensor>&, bool,
+                                                        double, double, const optional<Tensor>&, int64_t, int64_t);
 using FlashBwd = std::tuple<Tensor, Tensor, Tensor, Tensor>(
     const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
     const optional<Tensor>&, const optional<Tensor>&, bool, double, double, const optional<Tensor>&,
-    bool, int64_t, int64_t, int64_t);
+    bool, int64_t, int64_t, int64_t, const optional<Tensor>&);
 
 // Attention on separate q, k, v [B, S, H, D] (q only given: the packed [B, S, H, 3, D], read in
 // place through strided views and its gradient written into one tensor of that layout).
@@ -338,10 +341,16 @@ struct FlashFn : public Function<FlashFn> {
     const Tensor kk = packed ? q_or_qkv.select(3, 1) : *k, vv = packed ? q_or_qkv.select(3, 2) : *v;
     optional<Tensor> rng;
     if (p > 0.0) rng = philox_reserve(q.size(0) * q.size(2) * q.size(1) * kk.size(1));
-    static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
-    auto [out, lse] = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
+    Tensor out, lse, rest;
+    if (window > 0) {
+      static auto f = op<FlashFwdRest>("slapo_b200::flash_attn_fwd_rest");
+      std::tie(out, lse, rest) = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
+    } else {
+      static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
+      std::tie(out, lse) = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
+    }
     ctx->save_for_backward({q_or_qkv, or_undefined(k), or_undefined(v), out, lse,
-                            or_undefined(key_bias), or_undefined(rel)});
+                            or_undefined(key_bias), or_undefined(rel), rest});
     ctx->saved_data["causal"] = causal;
     if (window > 0) ctx->saved_data["window"] = std::vector<int64_t>{window, sinks};
     ctx->saved_data["scale"] = scale;
@@ -363,7 +372,7 @@ struct FlashFn : public Function<FlashFn> {
     auto [dq, dk, dv, drel] =
         f.call(grads[0].contiguous(), q, k, v, s[3], s[4], opt(s[5]), opt(s[6]),
                ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), p, rng, packed, /*keep_words=*/0,
-               window[0], window[1]);
+               window[0], window[1], opt(s[7]));
     tensor_list out(10);
     out[0] = dq;
     if (!packed) {

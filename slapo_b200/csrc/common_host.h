@@ -39,7 +39,7 @@ namespace slapo {
 // *_strides = element strides of (B, S, H).  Return 0 on success.
 // window > 0, with causal: a query sees that many keys up to its own, and the first `sinks`
 int flash_fwd_splits(int B, int H, int Sq, int Sk, int D, int window, int sinks);
-int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, uint8_t* rest, float* lse,
                      float* scratch,
                      const float* kbias, const float* rel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -62,7 +62,8 @@ struct FlashBwdPlan {
 FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal, int window, int sinks,
                             bool key_bias, bool rel, float p_drop, int64_t keep_words);
 // dq_row_stride / dkv_row_stride: elements between consecutive (b, s, head) rows of the outputs
-int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+// rest: what launch_flash_fwd left of it, or null
+int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o, const uint8_t* rest, const void* dout,
                      const float* lse, const FlashBwdPlan& plan, float* scratch, void* dq, void* dk,
                      void* dv, int64_t dq_row_stride, int64_t dkv_row_stride, const float* kbias,
                      const float* rel, float* drel, int B, int H, int Sq, int Sk, int D,

@@ -84,6 +84,7 @@ struct FlashFwdParams {
   float* part_o;       // splits > 1: [splits][B H Sq][Dr] unnormalised outputs and
   float2* part_ml;     // [splits][B H Sq] (maximum in the log2 domain, sum), see combine kernel
   void* O;             // [B, Sq, H, Dr] contiguous
+  uint8_t* rest;       // kWindow == 2: what O loses by rounding (rest_word), in its layout
   float* lse;          // [B, H, Sq] natural-log sum-exp of the scaled scores
   const float* kbias;  // [B, Sk] additive key bias or nullptr
   const float* rel;    // [H, Sq + Sk - 1] additive bias by (key - query) + Sq - 1, or nullptr
@@ -227,11 +228,13 @@ struct FwdSmem {
 // kGeneral: key bias, relative bias, causal mask, a ragged last key tile or a scale <= 0;
 // without any of them the kernel takes row maxima on the raw scores and every probability is
 // one fused multiply-add plus one exp2.
-// kWin (with kGeneral): a window and sinks.
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+// kWindow (with kGeneral): 1 = a window and sinks, 2 = and what O loses by rounding is kept (in a form of its own: as a
+// run-time choice it cost the calls without 4 us of 48, 4 x 2048 x 16 x 128 with a window of 256).
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 __global__ void __launch_bounds__(192, D == 64 ? 2 : 1)
 flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const FlashFwdParams p) {
+  constexpr bool kWin = kWindow != 0, kRest = kWindow == 2;
   using L = FwdSmem<D>;
   constexpr int kTileBytes = L::kTile;
   constexpr int kStages = L::kStages;
@@ -573,11 +576,15 @@ flash_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           for (int g = 0; g < 4; ++g) {
             if (c * 32 + g * 8 < p.Dr) {     // padded columns are not part of the output
               uint32_t v[4];
+              float f[8];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[i] = pack16<T>(__uint_as_float(o[g * 8 + 2 * i]) * inv,
-                                 __uint_as_float(o[g * 8 + 2 * i + 1]) * inv);
+              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[g * 8 + i]) * inv;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] = pack16<T>(f[2 * i], f[2 * i + 1]);
               *reinterpret_cast<uint4*>(dst + (c * 32 + g * 8) * 2) = make_uint4(v[0], v[1], v[2], v[3]);
+              if constexpr (kRest)
+                *reinterpret_cast<uint2*>(p.rest + (dst - static_cast<uint8_t*>(p.O)) / 2 + c * 32 + g * 8) =
+                    make_uint2(rest_word<T>(f[0], f[1], f[2], f[3]), rest_word<T>(f[4], f[5], f[6], f[7]));
             }
           }
         }
@@ -638,10 +645,11 @@ struct GroupsSmem {
 // 9.4; 4 x 2048 x 16 x 128 causal: 111 -> 91, all keys 154 -> 128; 4 x 1000 x 32 x 80 causal with key bias: 70 -> 60;
 // 4 x 1024 x 16 x 128, p 0.1: 61 -> 49.  With a single row tile there are too few tiles to share out: 2 x 60 x 60 x
 // 8 x 128: 6.5 -> 8.0 (which calls come here: fwd_in_groups).
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 __global__ void __launch_bounds__(512, 1)
 flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FlashFwdParams p) {
+  constexpr bool kWin = kWindow != 0, kRest = kWindow == 2;
   using L = GroupsSmem<D>;
   constexpr int kTileBytes = L::kTile;
   constexpr int kStages = L::kStages, kQ = L::kQ;
@@ -934,6 +942,7 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         p.lse[static_cast<int64_t>(bh) * p.Sq + row] =
             l > 0.f ? (m == -INFINITY ? 0.f : m) * 0.6931471805599453f + logf(l) : -INFINITY;
       }
+      uint32_t lost[8];         // (of 32 columns)
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
         uint32_t x[16], y[16];
@@ -948,8 +957,17 @@ flash_fwd_groups_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           for (int e = 0; e < 2; ++e) {
             v[e] = __uint_as_float(x[2 * i + e]) * fa;
             if (two) v[e] = fmaf(__uint_as_float(y[2 * i + e]), fb, v[e]);
+            if constexpr (kRest) x[2 * i + e] = __float_as_uint(v[e]);
           }
           w[i] = pack16<T>(v[0], v[1]);
+        }
+        if constexpr (kRest) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            lost[(c & 1) * 4 + i / 4] = rest_word<T>(__uint_as_float(x[i]), __uint_as_float(x[i + 1]),
+                                                     __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+          if ((c & 1) != 0 && row < p.Sq)
+            store_cols8(p.rest + (done_at - static_cast<T*>(p.O)), (c - 1) * 16, p.Dr, lost);
         }
         if (!kHold && row < p.Sq) store_cols16(done_at, c * 16, p.Dr, w);
       }
@@ -1179,12 +1197,12 @@ void launch_flash_dropout_mask(uint8_t* mask, int B, int H, int Sq, int Sk, floa
   flash_dropout_mask_kernel<<<sm_count() * 4, 256, 0, stream>>>(mask, B, H, Sq, Sk, p_drop, rng);
 }
 
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 static int launch_fwd_groups(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                              const FlashFwdParams& p, int64_t items, cudaStream_t stream) {
   constexpr int kSmem = GroupsSmem<D>::kTotal;
   static_assert(kSmem <= 227 * 1024, "flash forward: shared memory over the per-CTA limit");
-  auto kernel = flash_fwd_groups_kernel<D, kGeneral, kDrop, kWin, T>;
+  auto kernel = flash_fwd_groups_kernel<D, kGeneral, kDrop, kWindow, T>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
@@ -1229,12 +1247,12 @@ static bool fwd_in_groups(const FlashFwdParams& p, int64_t items) {
   return key_tiles > 3 || (key_tiles > 1 && (items <= sm_count() || (kDrop && !kGeneral)));
 }
 
-template <int D, bool kGeneral, bool kDrop, bool kWin, typename T>
+template <int D, bool kGeneral, bool kDrop, int kWindow, typename T>
 static int launch_fwd_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                         const FlashFwdParams& p, cudaStream_t stream) {
   constexpr int kSmem = FwdSmem<D>::kTotal;
   static_assert(FwdSmem<D>::kCtas * (kSmem + 1024) <= 228 * 1024, "flash forward: shared memory");
-  auto kernel = flash_fwd_kernel<D, kGeneral, kDrop, kWin, T>;
+  auto kernel = flash_fwd_kernel<D, kGeneral, kDrop, kWindow, T>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
@@ -1244,7 +1262,7 @@ static int launch_fwd_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   }
   const int64_t items = static_cast<int64_t>(p.walk.row_tiles) * p.walk.nbh * p.splits;
   if (fwd_in_groups<D, kGeneral, kDrop>(p, items))
-    return launch_fwd_groups<D, kGeneral, kDrop, kWin, T>(tq, tk, tv, p, items, stream);
+    return launch_fwd_groups<D, kGeneral, kDrop, kWindow, T>(tq, tk, tv, p, items, stream);
   const int64_t cap = FwdSmem<D>::kCtas * sm_count();
   count_launch();
   kernel<<<static_cast<int>(items < cap ? items : cap), 192, kSmem, stream>>>(tq, tk, tv, p);
@@ -1275,7 +1293,9 @@ int flash_fwd_splits(int B, int H, int Sq, int Sk, int D, int window, int sinks)
 
 // `window` > 0 (with `causal`): a query sees that many keys up to its own and the first `sinks`.
 // `scratch`: flash_fwd_splits() * B * H * Sq * (D + 2) floats, or null with a single split
-int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+// (`rest`, with a window and without `scratch`, for several queries or with dropout: what O loses by rounding, a byte a value;
+// or null)
+int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, uint8_t* rest, float* lse,
                      float* scratch,
                      const float* kbias, const float* rel, int B, int H, int Sq, int Sk, int D,
                      const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
@@ -1291,6 +1311,7 @@ int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float
   if (sinks > Sk) sinks = Sk;
   p.window = window;
   p.sinks = sinks;
+  p.rest = window > 0 ? rest : nullptr;
   p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.Dr = D; p.O = o; p.lse = lse; p.kbias = kbias; p.rel = rel;
   p.k_steps = (D + 15) / 16;
   // (row tiles of a window differ little)
@@ -1321,13 +1342,16 @@ int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, float
         !make_tmap_bshd(&tk, k, B, Sk, H, D, k_strides[0], k_strides[1], k_strides[2], 128, bf16) ||
         !make_tmap_bshd(&tv, v, B, Sk, H, D, v_strides[0], v_strides[1], v_strides[2], 128, bf16))
       return 2;
-#define FLASH_FWD_CASE(D_, T_)                                                                         \
-  rc = p.thr7 != 0 ? (window > 0 ? launch_fwd_d<D_, true, true, true, T_>(tq, tk, tv, p, stream)       \
-                      : general  ? launch_fwd_d<D_, true, true, false, T_>(tq, tk, tv, p, stream)      \
-                                 : launch_fwd_d<D_, false, true, false, T_>(tq, tk, tv, p, stream))    \
-                   : (window > 0 ? launch_fwd_d<D_, true, false, true, T_>(tq, tk, tv, p, stream)      \
-                      : general  ? launch_fwd_d<D_, true, false, false, T_>(tq, tk, tv, p, stream)     \
-                                 : launch_fwd_d<D_, false, false, false, T_>(tq, tk, tv, p, stream))
+    const int form = window == 0 ? 0 : p.rest != nullptr ? 2 : 1;
+#define FLASH_FWD_CASE(D_, T_)                                                                   \
+  rc = p.thr7 != 0 ? (form == 2  ? launch_fwd_d<D_, true, true, 2, T_>(tq, tk, tv, p, stream)    \
+                      : form == 1 ? launch_fwd_d<D_, true, true, 1, T_>(tq, tk, tv, p, stream)   \
+                      : general   ? launch_fwd_d<D_, true, true, 0, T_>(tq, tk, tv, p, stream)   \
+                                  : launch_fwd_d<D_, false, true, 0, T_>(tq, tk, tv, p, stream)) \
+                   : (form == 2   ? launch_fwd_d<D_, true, false, 2, T_>(tq, tk, tv, p, stream)  \
+                      : form == 1 ? launch_fwd_d<D_, true, false, 1, T_>(tq, tk, tv, p, stream)  \
+                      : general   ? launch_fwd_d<D_, true, false, 0, T_>(tq, tk, tv, p, stream)  \
+                                  : launch_fwd_d<D_, false, false, 0, T_>(tq, tk, tv, p, stream))
     if (D <= 64) {
       if (bf16) FLASH_FWD_CASE(64, __nv_bfloat16);
       else FLASH_FWD_CASE(64, __half);

@@ -115,9 +115,10 @@ template <> __device__ __forceinline__ float dot_pair<__half>(uint32_t a, uint32
 // 8 heads: lanes along d while reading (16-byte loads), then the sums pass through shared
 // memory so that the stores run along the rows.  The blocks of the first heads also write
 //   kb2    [B][Rk]    log2(e) * key bias, 0 in the padding
-template <typename T>
+// kRest: with what O has lost by rounding.
+template <bool kRest, typename T>
 __global__ void __launch_bounds__(256) flash_bwd_stats_kernel(
-    const T* __restrict__ dout, const T* __restrict__ out, const float* __restrict__ lse,
+    const T* __restrict__ dout, const T* __restrict__ out, const uint8_t* __restrict__ rest, const float* __restrict__ lse,
     float* __restrict__ nlse, float* __restrict__ ndelta, const float* __restrict__ kbias,
     float* __restrict__ kb2, int H, int Sq, int Rq, int Sk, int Rk, int Dr, int lanes,
     float keep_prob, int windowed) {
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(256) flash_bwd_stats_kernel(
   constexpr int kAhead = 4;                    // (256 rows are 8 or 16 rounds)
   for (int r0 = warp * rows_per_warp + lane / lanes; r0 < 256; r0 += kAhead * 8 * rows_per_warp) {
     uint4 x[kAhead], y[kAhead];
+    uint2 z[kRest ? kAhead : 1];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int r = r0 + u * 8 * rows_per_warp, i = i0 + (r >> 3), h = h0 + (r & 7);    // neighbouring heads are contiguous
@@ -145,14 +147,25 @@ __global__ void __launch_bounds__(256) flash_bwd_stats_kernel(
         const int64_t at = ((static_cast<int64_t>(b) * Sq + i) * H + h) * Dr + d;
         x[u] = __ldg(reinterpret_cast<const uint4*>(dout + at));
         y[u] = __ldg(reinterpret_cast<const uint4*>(out + at));
+        if constexpr (kRest) z[u] = __ldg(reinterpret_cast<const uint2*>(rest + at));
+      } else if constexpr (kRest) {
+        z[u] = make_uint2(0u, 0u);
       }
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      float s = dot_pair<T>(x[u].x, y[u].x, 0.f);
-      s = dot_pair<T>(x[u].y, y[u].y, s);
-      s = dot_pair<T>(x[u].z, y[u].z, s);
-      s = dot_pair<T>(x[u].w, y[u].w, s);
+      float s;
+      if constexpr (kRest) {
+        s = rest_dot<0>(x[u].x, y[u].x, z[u].x, 0.f, T());
+        s = rest_dot<1>(x[u].y, y[u].y, z[u].x, s, T());
+        s = rest_dot<0>(x[u].z, y[u].z, z[u].y, s, T());
+        s = rest_dot<1>(x[u].w, y[u].w, z[u].y, s, T());
+      } else {
+        s = dot_pair<T>(x[u].x, y[u].x, 0.f);
+        s = dot_pair<T>(x[u].y, y[u].y, s);
+        s = dot_pair<T>(x[u].z, y[u].z, s);
+        s = dot_pair<T>(x[u].w, y[u].w, s);
+      }
       for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       const int r = r0 + u * 8 * rows_per_warp;
       if (lane % lanes == 0) sums[r & 7][r >> 3] = s;
@@ -1298,7 +1311,7 @@ FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bo
   return s;
 }
 
-int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o, const uint8_t* rest, const void* dout,
                      const float* lse, const FlashBwdPlan& plan, float* scratch, void* dq, void* dk,
                      void* dv, int64_t dq_row_stride, int64_t dkv_row_stride, const float* kbias,
                      const float* rel, float* drel, int B, int H, int Sq, int Sk, int D,
@@ -1343,14 +1356,18 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
     const int lanes = D <= 64 ? 8 : 16;
     const dim3 grid((p.Rq + 31) / 32, (H + 7) / 8, B);
     count_launch();
-    if (bf16)
-      flash_bwd_stats_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(
-          static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(o), lse, nlse,
-          ndelta, kbias, kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob, window > 0);
-    else
-      flash_bwd_stats_kernel<__half><<<grid, 256, 0, stream>>>(
-          static_cast<const __half*>(dout), static_cast<const __half*>(o), lse, nlse, ndelta, kbias,
-          kb2, H, Sq, p.Rq, Sk, p.Rk, D, lanes, keep_prob, window > 0);
+#define FLASH_BWD_STATS(REST_, T_)                                                                                    \
+  flash_bwd_stats_kernel<REST_, T_><<<grid, 256, 0, stream>>>(static_cast<const T_*>(dout), static_cast<const T_*>(o), \
+                                                              rest, lse, nlse, ndelta, kbias, kb2, H, Sq, p.Rq, Sk,   \
+                                                              p.Rk, D, lanes, keep_prob, window > 0)
+    if (rest != nullptr) {
+      if (bf16) FLASH_BWD_STATS(true, __nv_bfloat16);
+      else FLASH_BWD_STATS(true, __half);
+    } else {
+      if (bf16) FLASH_BWD_STATS(false, __nv_bfloat16);
+      else FLASH_BWD_STATS(false, __half);
+    }
+#undef FLASH_BWD_STATS
     if (cudaGetLastError() != cudaSuccess) return 4;
   }
   const bool general = kbias != nullptr || rel != nullptr || causal || Sk % 128 != 0;

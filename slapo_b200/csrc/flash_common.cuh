@@ -1,6 +1,8 @@
 // Device helpers shared by the flash-attention forward and backward kernels: packed fp32
 // arithmetic, 16-bit packing by type, exp2 on the special-function unit.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "tc05.cuh"
 
@@ -91,6 +93,17 @@ __device__ __forceinline__ void store_cols16(void* row, int col, int cols, const
   }
 }
 
+// Bytes col .. col + 31 of a row of `cols` (a multiple of 8), likewise
+__device__ __forceinline__ void store_cols8(uint8_t* row, int col, int cols, const uint32_t (&v)[8]) {
+  if ((cols & 15) == 0) {
+    store_cols16(row, col / 2, cols / 2, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + 8 * i < cols) *reinterpret_cast<uint2*>(row + col + 8 * i) = make_uint2(v[2 * i], v[2 * i + 1]);
+  }
+}
+
 // Overlap of a kernel's prologue with the kernel before it in the stream: a kernel that the next
 // one may start under says so, and one that was launched that way waits until all work before it
 // is complete and visible (at once, when it was launched the ordinary way).
@@ -176,6 +189,41 @@ struct Ring {
     if (++slot == N) { slot = 0; phase ^= 1; }
   }
 };
+
+// What the forward's output loses by rounding, for the backward's row term sum_d dO O, a byte for each value: the first
+// eight bits of the fp32 number behind those that the type keeps.  Read as signed they are what the number is above or
+// below the rounded one in size, in steps of 2^8 (bf16) or 2^5 (fp16) of fp32's.  (A tie, -128, went up or down to the even
+// neighbour: it counts as nothing.)  Rows that see few keys, of which attention with a window has many more among those
+// that count, otherwise carry that rounding into dQ and dK next to those of dS and of the result:
+// 4 x 1000 x 32 x 80, fp16, window 201, padded: error 0.00033 -> 0.00030 (the other two alone: 0.00029).
+// (As an e5m2 number of the difference itself the bytes held the forward up: 4 x 2048 x 16 x 128, window 256: 48 -> 57 us.)
+template <typename T> __device__ __forceinline__ uint32_t rest_word(float a, float b, float c, float d) {
+  constexpr int kUp = std::is_same<T, __half>::value ? 3 : 0;       // to bits 8 .. 15
+  const uint32_t lo = __byte_perm(__float_as_uint(a) << kUp, __float_as_uint(b) << kUp, 0x0051);
+  const uint32_t hi = __byte_perm(__float_as_uint(c) << kUp, __float_as_uint(d) << kUp, 0x0051);
+  const uint32_t word = __byte_perm(lo, hi, 0x5410);
+  return word & (((word & 0x7f7f7f7fu) + 0x7f7f7f7fu) | 0x7f7f7f7fu);      // (bytes of 0x80 become 0)
+}
+// s + sum of a pair of O, with bytes 2 kPair and 2 kPair + 1 of such a word, times a pair of dO.  bf16: the byte, with its
+// sign, goes to bits 8 .. 31 and is added to the number.
+template <int kPair> __device__ __forceinline__ float rest_dot(uint32_t x, uint32_t y, uint32_t word, float s, __nv_bfloat16) {
+  int a, b;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(a) : "r"(word), "n"(kPair == 0 ? 0x8804 : 0xaa24));
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(b) : "r"(word), "n"(kPair == 0 ? 0x9914 : 0xbb34));
+  const float2 f = pair_floats(x, __nv_bfloat16());
+  s = fmaf(f.x, __int_as_float(static_cast<int>(y << 16) + a), s);
+  return fmaf(f.y, __int_as_float(static_cast<int>(y & 0xffff0000u) + b), s);
+}
+// fp16: the byte over 256, from the half of 1024 + 128 + byte, times the number's power of two (nothing for zeros and
+// denormals): 2^10 times what is missing.
+template <int kPair> __device__ __forceinline__ float rest_dot(uint32_t x, uint32_t y, uint32_t word, float s, __half) {
+  const uint32_t magic = __byte_perm(word ^ 0x80808080u, 0x64646464u, kPair == 0 ? 0x4140 : 0x4342), power = y & 0xfc00fc00u;
+  const __half2 part = __hfma2(*reinterpret_cast<const __half2*>(&magic), __float2half2_rn(0.00390625f), __float2half2_rn(-4.5f));
+  const float2 lost = __half22float2(__hmul2(part, *reinterpret_cast<const __half2*>(&power)));
+  const float2 f = pair_floats(x, __half()), o = pair_floats(y, __half());
+  s = fmaf(f.x, fmaf(lost.x, 0.0009765625f, o.x), s);
+  return fmaf(f.y, fmaf(lost.y, 0.0009765625f, o.y), s);
+}
 
 // Division of 0 .. 2^31 - 1 by a number that is fixed for a launch: a product and a shift, for d <= 2^s with
 // mul = ceil(2^(31 + s) / d) = (2^(31 + s) + e) / d, e < d: n mul / 2^(31 + s) exceeds n / d by n e / (d 2^(31 + s)) < 1 / d.

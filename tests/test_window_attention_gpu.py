@@ -390,3 +390,57 @@ def test_tensors_that_calls_do_not_take_as_they_are():
     assert torch.equal(out.as_subclass(torch.Tensor), want[0].detach())
     with pytest.raises(Exception, match="Expected|sizes|size"):
         NF.flash_attention(q, k.detach()[:, :, :2], v, causal=True, window=100)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("s,d", [(3, 64), (100, 40), (128, 128), (300, 64), (300, 80), (777, 128)])
+def test_what_the_output_loses_by_rounding(s, d, dtype):
+    """With q = 0 and a window of two keys the output is the mean of two values, exact in fp32: a byte holds
+    the next eight bits, so that less than one of their last (2^8 or 2^5 of fp32's 2^-23 of the value) stays
+    lost.  Nothing is held of ties and what begins like one, nor of fp16's denormals."""
+    _, _, v, do = _tensors(2, s, s, 3, d, dtype)
+    v = v.detach()
+    q = torch.zeros_like(v)
+    ops = native.ops()
+    out, lse, rest = ops.flash_attn_fwd_rest(q, v, v, None, None, True, 1.0, 0.0, None, 2, 0)
+    x = v.double()
+    x[:, 1:] = (x[:, 1:] + x[:, :-1]) / 2
+    assert torch.equal(out, x.to(dtype))
+    byte = rest.view(torch.int8).int()
+    lost = out.float().view(torch.int32) + byte * (32 if dtype == torch.float16 else 256)
+    left_out = byte == 0
+    if dtype == torch.float16:
+        left_out |= out.abs() < 2.0 ** -14
+    assert int((byte == -128).sum()) == 0
+    got = torch.where(left_out, out.float(), lost.view(torch.float32)).double()
+    step = 2.0 ** (-18 if dtype == torch.float16 else -15)
+    room = torch.where(left_out, HALF[dtype], step) * x.abs() * (1 + HALF[dtype])
+    assert bool(((got - x).abs() <= room.clamp(min=2.0 ** -25)).all())
+    args = (do, q, v, v, out, lse, None, None, True, 1.0, 0.0, None, False, 0, 2, 0)
+    for given in (rest, rest[:0], None):
+        assert all(bool(t.isfinite().all()) for t in ops.flash_attn_bwd(*args, given)[:3])
+    for bad in (rest[:, :, :1], rest.view(torch.int8), rest.cpu(), rest.flatten()[1:]):
+        with pytest.raises(RuntimeError, match="byte"):
+            ops.flash_attn_bwd(*args, bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_carry_two_roundings(dtype):
+    """dQ and dK: dS and the result are rounded to the type, each an independent error of the same size (a
+    factor of sqrt 2 over the result's alone).  The output in the row term comes without its rounding; that of
+    the probabilities in it, with many rows that see few keys, measured in 64 bits, adds 0.3 of one: 1.45."""
+    b, s, n, d, window, sinks = 4, 1000, 4, 80, 201, 5
+    q, k, v, do = _tensors(b, s, s, n, d, dtype)
+    bias = torch.zeros(b, s, device="cuda")
+    for i in range(b):
+        bias[i, 500 + 100 * i:] = -10000.0
+    got = _run(q, k, v, do, window, sinks, bias)
+    q64, k64, v64 = (t.detach().double().transpose(1, 2) for t in (q, k, v))
+    p = q64 @ k64.transpose(-1, -2) / math.sqrt(d) + bias.double()[:, None, None]
+    p = torch.softmax(p.masked_fill(~_seen(s, s, window, sinks, bias), -math.inf), -1)
+    dp = do.double().transpose(1, 2) @ v64.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) / math.sqrt(d)
+    for x, want in ((got[1], ds @ k64), (got[2], ds.transpose(-1, -2) @ q64)):
+        want = want.transpose(1, 2)
+        rounding = (want.to(dtype).double() - want).norm()
+        assert float((x.double() - want).norm() / rounding) < 1.5
