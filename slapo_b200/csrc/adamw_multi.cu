@@ -17,8 +17,8 @@
 // Bound by memory: 28 bytes per element with 16-bit weights, 32-bit masters and moments, 16 with 8-bit moments,
 // 10 without masters; with 8-bit moments by instructions too, some 45 per element (a scheduler's slots are three
 // quarters full at 10 bytes).
-// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 819 us (96 % of the copy rate), 8-bit
-// moments 554 us (81 %); 304 M elements, 8-bit, no masters: 585 us (80 %).
+// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 820 us (96 % of the copy
+// rate), 8-bit moments 540 - 562 us (80 - 83 %); 304 M elements, 8-bit, no masters: 560 - 588 us (80 - 84 %), from box to box.
 #include <cuda_fp8.h>
 
 #include <type_traits>
