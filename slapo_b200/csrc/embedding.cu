@@ -17,7 +17,7 @@
 //
 // Measured (us; lookup, sort and zeros, sums, joins): 16384 tokens, 30528 x 1024 bf16: 9, 20, 10, 5; 8192 tokens, 50304 x 2048:
 // 9 (scaled), 35 (the zeros: 5.9 TB/s), 10, 5; both lookups and sums move their bytes at 6 - 7 TB/s, the sort alone is
-// latency: its passes' counting, exchange over the cluster and placing take some 6 us each.
+// latency.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
