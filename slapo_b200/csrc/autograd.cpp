@@ -537,6 +537,12 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, int64_t start, const o
   if (!wants_node({&weight})) return at.lookup(ids, weight);
   return EmbeddingFn::apply(weight, ids, at);
 }
+// The lookup's gradient by itself, for backward passes written in Python.
+Tensor embedding_sum(const Tensor& dy, const Tensor& ids, int64_t rows, int64_t start, const optional<int64_t>& padding,
+                     double scale) {
+  const TokenRows at{rows, start, padding, scale};
+  return wants_node({&dy}) ? EmbeddingSumFn::apply(dy, ids, at) : at.sum(ids, dy);
+}
 
 Tensor rel_bias(const Tensor& table, const Tensor& buckets) { return RelBiasFn::apply(table, buckets); }
 
@@ -558,6 +564,7 @@ void register_autograd_ops(torch::Library& m) {
   m.def("embedding_entry() -> int",
         []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::EmbeddingEntry>(&embedding)); });
   m.def("embedding(Tensor ids, Tensor weight, int start, int? padding, float scale) -> Tensor", &embedding);
+  m.def("embedding_sum(Tensor dy, Tensor ids, int rows, int start, int? padding, float scale) -> Tensor", &embedding_sum);
   m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p, int window=0, int sinks=0) -> Tensor",
         &flash);
 }

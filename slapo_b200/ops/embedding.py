@@ -105,7 +105,7 @@ class _VocabEmbedFn(torch.autograd.Function):
                 full = full.view(world, b, s // world, -1).permute(1, 0, 2, 3)
             grad = full.reshape(flat.numel(), -1)
         g = grad.reshape(flat.numel(), -1)
-        grad_w = native.ops().embedding_bwd(g, flat, ctx.rows, ctx.lo, None, 1.0)
+        grad_w = native.ops().embedding_sum(g, flat, ctx.rows, ctx.lo, None, 1.0)
         return None, grad_w.to(ctx.dtype), None
 
 

@@ -295,3 +295,26 @@ def test_vocab_parallel_embedding_scatter_form_emulated_ranks(world, sp_axis):
     for r in range(world):
         got = ctx.rank_view("vocab_embed_out_0", r, torch.bfloat16, tuple(want[r].shape))
         assert torch.equal(got, want[r]), f"rank {r}"
+
+
+def test_vocab_parallel_embedding_second_derivative():
+    """The backward is differentiated in its turn: what a rank's gradient depends on is the gradient of
+    the rows that it owns, linearly."""
+    from slapo_b200.ops.embedding import FusedVocabParallelEmbedding
+    from slapo_b200.parallel.symm import LocalSymmContext
+
+    torch.manual_seed(6)
+    world, vocab, hidden = 2, 40, 64
+    ctx = LocalSymmContext(world)
+    weight = torch.nn.Parameter(torch.randn(vocab // world, hidden, device="cuda").bfloat16())
+    mod = FusedVocabParallelEmbedding(weight, vocab // world, ctx.as_rank(1))
+    ctx.epoch = 0
+    mod.flag_buf.view(torch.int32, (8,)).fill_(1)
+    ids = torch.randint(0, vocab, (3, 30), device="cuda")
+    dy = torch.randn(3, 30, hidden, device="cuda").bfloat16().requires_grad_()
+    x = torch.randn(vocab // world, hidden, device="cuda").bfloat16()
+    (dw,) = torch.autograd.grad(mod(ids), weight, dy, create_graph=True)
+    (got,) = torch.autograd.grad(dw, dy, x)
+    local = ids - vocab // world
+    want = torch.where((local >= 0)[..., None], x[local.clamp(min=0)], 0.0)
+    assert torch.equal(got, want)       # (a copy of rows)
