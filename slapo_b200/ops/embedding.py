@@ -88,6 +88,8 @@ class _VocabEmbedFn(torch.autograd.Function):
         ctx.save_for_backward(flat)
         ctx.lo, ctx.rows, ctx.dtype = mod.vocab_start_index, weight.shape[0], weight.dtype
         ctx.sctx, ctx.sp_axis, ctx.ids_shape = sctx, mod.sp_axis, tuple(ids.shape)
+        # (the module's is a row of its shard, ids are those of the whole table)
+        ctx.padding = None if mod.padding_idx is None else mod.vocab_start_index + mod.padding_idx
         return out.view(out_shape)
 
     @staticmethod
@@ -105,7 +107,7 @@ class _VocabEmbedFn(torch.autograd.Function):
                 full = full.view(world, b, s // world, -1).permute(1, 0, 2, 3)
             grad = full.reshape(flat.numel(), -1)
         g = grad.reshape(flat.numel(), -1)
-        grad_w = native.ops().embedding_sum(g, flat, ctx.rows, ctx.lo, None, 1.0)
+        grad_w = native.ops().embedding_sum(g, flat, ctx.rows, ctx.lo, ctx.padding, 1.0)
         return None, grad_w.to(ctx.dtype), None
 
 
@@ -117,7 +119,8 @@ class FusedVocabParallelEmbedding(nn.Module):
 
     def __init__(self, weight, vocab_start_index, symm_ctx, padding_idx=None, sp_axis=None):
         """``sp_axis``: None = every rank gets every token's row; 0 / 1 = sequence parallel,
-        this rank keeps its chunk of the batch / of every sequence."""
+        this rank keeps its chunk of the batch / of every sequence.  ``padding_idx``: the row of this
+        shard whose tokens have no gradient, as a sharded ``nn.Embedding`` has it."""
         super().__init__()
         self.sp_axis = sp_axis
         self.weight = weight

@@ -318,3 +318,30 @@ def test_vocab_parallel_embedding_second_derivative():
     local = ids - vocab // world
     want = torch.where((local >= 0)[..., None], x[local.clamp(min=0)], 0.0)
     assert torch.equal(got, want)       # (a copy of rows)
+
+
+def test_vocab_parallel_embedding_padding_has_no_gradient():
+    """The padding row keeps out of the gradient on the rank that owns it, as in the sharded nn.Embedding
+    that the module is made from; other ranks have no such row."""
+    from slapo_b200.ops.embedding import FusedVocabParallelEmbedding
+    from slapo_b200.parallel.symm import LocalSymmContext
+
+    torch.manual_seed(7)
+    world, vocab, hidden, padding = 2, 40, 64, 23
+    rows = vocab // world
+    table = torch.randn(vocab, hidden, device="cuda").bfloat16()
+    ids = torch.randint(0, vocab, (4, 25), device="cuda")
+    ids[:, 20:] = padding
+    dy = torch.ones(4, 25, hidden, device="cuda").bfloat16()
+    want = torch.bincount(ids[ids != padding], minlength=vocab)[:, None].expand(-1, hidden)
+    ctx = LocalSymmContext(world)
+    for r in range(world):
+        # (what sharding leaves on the module)
+        emb = torch.nn.Embedding(rows, hidden, padding_idx=padding - r * rows if r == 1 else None)
+        emb.weight = torch.nn.Parameter(table.chunk(world)[r].clone())
+        emb.vocab_start_index = r * rows
+        mod = FusedVocabParallelEmbedding.from_sharded(emb, r, ctx.as_rank(r))
+        ctx.epoch = 0
+        mod.flag_buf.view(torch.int32, (8,)).fill_(1)
+        mod(ids).backward(dy)
+        assert torch.equal(mod.weight.grad.float(), want[r * rows:(r + 1) * rows].float())
