@@ -186,17 +186,21 @@ __device__ __noinline__ void gather_unit(const AdamwTensor& t, int unit, AdamSta
     to.scale[lane / kAdamUnit][lane % kAdamUnit] = (lane < kAdamUnit ? t.m_scale : t.v_scale)[block];
 }
 
-// (of what is neither denormal nor that large)
-__device__ __forceinline__ float reciprocal(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// (0 for a denormal)
-__device__ __forceinline__ float square_root(float x) {
+// The divisions and roots of the two kernels.  With 32-bit moments the arithmetic has time under the bytes: rounded
+// correctly, denormals and all, so that eps may be as small as one likes, 0 included.  With 8-bit moments instructions
+// count: the special-function unit's, for which a second moment below 2^-126 is zero and the divisor never
+// that small (the caller has looked at eps).
+template <bool k8> __device__ __forceinline__ float square_root(float x) {
+  if constexpr (!k8) return __fsqrt_rn(x);
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+template <bool k8> __device__ __forceinline__ float quotient(float x, float y) {
+  if constexpr (!k8) return __fdiv_rn(x, y);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return x * r;
 }
 
 // What does not change over a launch
@@ -221,13 +225,14 @@ __device__ __forceinline__ AdamStepScalars adam_scalars(const AdamwScalars& s) {
 }
 
 // One element: its moments m and v brought up to date, u = sqrt(v), and the new weight
+template <bool k8>
 __device__ __forceinline__ float adam_value(float g, float w, float& m, float& v, float& u, const AdamwTensor& t,
                                             const AdamStepScalars& c) {
   const float x = __fmul_rn(g, c.grad_scale);
   m = __fadd_rn(__fmul_rn(m, c.beta1), __fmul_rn(x, c.one_beta1));
   v = __fadd_rn(__fmul_rn(v, c.beta2), __fmul_rn(__fmul_rn(x, x), c.one_beta2));
-  u = square_root(v);
-  const float step = m * c.inv_bc1 * reciprocal(fmaf(u, c.inv_sqrt_bc2, c.eps));
+  u = square_root<k8>(v);
+  const float step = quotient<k8>(m * c.inv_bc1, fmaf(u, c.inv_sqrt_bc2, c.eps));
   return fmaf(-t.lr, fmaf(t.weight_decay, w, step), w);
 }
 
@@ -260,7 +265,7 @@ __device__ __forceinline__ void adam_block(const AdamwTensor& t, const AdamStepS
       m[e] = __fmul_rn(m[e], m_scale);
       u[e] = __fmul_rn(u[e], v_scale);
       float v = __fmul_rn(u[e], u[e]);
-      y[k] = adam_value(x[k], y[k], m[e], v, u[e], t, c);
+      y[k] = adam_value<true>(x[k], y[k], m[e], v, u[e], t, c);
     }
     if constexpr (kMaster) w_new.set(i, y[0], y[1]);
     p_new.set(i, y[0], y[1]);
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float u;
-        w[i] = adam_value(g[i], w[i], m[i], v[i], u, t, c);
+        w[i] = adam_value<false>(g[i], w[i], m[i], v[i], u, t, c);
       }
       if constexpr (kMaster) store_once(t.master + at, w);
       store_once(param + at, w);
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw32_kernel(const __grid_cons
       for (int64_t at = begin + threadIdx.x; at < end; at += kAdamThreads) {
         float m = exp_avg[at], v = exp_avg_sq[at], u;
         float w = kMaster ? t.master[at] : static_cast<float>(param[at]);
-        w = adam_value(static_cast<float>(grad[at]), w, m, v, u, t, c);
+        w = adam_value<false>(static_cast<float>(grad[at]), w, m, v, u, t, c);
         if constexpr (kMaster) t.master[at] = w;
         param[at] = static_cast<T>(w);
         exp_avg[at] = m;

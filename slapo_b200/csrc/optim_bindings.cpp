@@ -86,6 +86,10 @@ void run(const AdamwLists& x) {
               "multi_adamw: one entry for each of the ", n, " parameters required in every list");
   TORCH_CHECK(x.beta1 >= 0.0 && x.beta1 < 1.0 && x.beta2 >= 0.0 && x.beta2 < 1.0 && x.eps >= 0.0,
               "multi_adamw: betas in [0, 1) and eps >= 0 required");
+  // (8 bits: a second moment below 2^-126 counts as zero.  The root of its corrected value is below 2^-63 / sqrt(1 - beta2)
+  // then; where eps is no less, leaving it out of the divisor makes a step at most twice as long.)
+  TORCH_CHECK(!bits8 || x.eps * std::sqrt(1.0 - x.beta2) >= std::ldexp(1.0, -63),
+              "multi_adamw: 8-bit moments need eps of at least 2^-63 / sqrt(1 - beta2), not ", x.eps);
   TORCH_CHECK(n <= INT_MAX, "multi_adamw: too many tensors");
   const Tensor& p0 = x.params[0];
   TORCH_CHECK(p0.is_cuda(), "multi_adamw: parameters must be CUDA tensors");

@@ -77,7 +77,8 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
     moments as :func:`quantize_moment` makes them.  ``lr`` and ``weight_decay``: a number, or one per tensor.
     ``step`` counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step
     goes on counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in
-    its place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits."""
+    its place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits, and ``eps`` must be at least
+    2^-63 / sqrt(1 - b2) with them (3.4e-18 for 0.999); with 32 bits it may be 0."""
     params, grads = list(params), list(grads)
     n = len(params)
     lrs, decays = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")
@@ -154,7 +155,8 @@ def _reference_step(param, grad, master, exp_avg, exp_avg_sq, m_scale, v_scale, 
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW whose step is one kernel for all tensors of a type: ``FusedAdamW(model.parameters(), lr=...)``.
 
-    ``state_bits``: 32, or 8 for moments of one byte each (rounded by at most 1 / 16 of themselves).
+    ``state_bits``: 32, or 8 for moments of one byte each (rounded by at most 1 / 16 of themselves; ``eps`` as
+    :func:`multi_tensor_adamw` says).
     ``master_weights``: keep fp32 copies of 16-bit parameters, which are what is updated (default); without
     them an update below half a step of the parameter's type is lost.  ``capturable``: steps are counted on
     the device, so that a captured ``step()`` can be replayed (with the ``lr`` and ``weight_decay`` of its

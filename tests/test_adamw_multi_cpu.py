@@ -217,3 +217,28 @@ def test_the_entry_for_lists_refuses_other_things():
             call(*bad)
     with pytest.raises(TypeError):
         call(*rest[:-1])
+
+
+def test_the_kernel_refuses_an_eps_that_8bit_moments_do_not_bear():
+    """What counts as zero in 8 bits has a corrected root of up to 2^-63 / sqrt(1 - beta2): eps must not be
+    less.  (The check comes before the one that CPU tensors do not pass.)"""
+    from slapo_b200.ops import native
+    if not native.available():
+        pytest.skip("extension not built")
+    p = [torch.zeros(3)]
+    codes, scale = quantize_moment(p[0])
+
+    def call(eps, bits, b2=0.999):
+        factors = [scale] if bits == 8 else []
+        m = [codes] if bits == 8 else p
+        native.direct("multi_adamw")(p, p, [], m, m, factors, factors, [0.1], [0.1], 0.9, b2, eps, 1, None, None)
+
+    least = 2.0 ** -63 / math.sqrt(1 - 0.999)
+    for eps in (0.0, 1e-30, least * 0.999):
+        with pytest.raises(RuntimeError, match="8-bit moments need eps"):
+            call(eps, 8)
+    for eps, bits in ((least * 1.001, 8), (1e-8, 8), (0.0, 32)):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call(eps, bits)
+    with pytest.raises(RuntimeError, match="8-bit moments need eps"):
+        call(least * 1.001, 8, 0.9999)

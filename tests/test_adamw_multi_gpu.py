@@ -352,3 +352,24 @@ def test_offsets_beyond_32_bits(bits):
         end = small[name][0].numel()
         assert torch.equal(x[-end:].view(torch.uint8), small[name][0].view(torch.uint8)), name
     assert int(torch.count_nonzero(large["params"][0][:-tail])) == 0
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30])
+def test_32bit_moments_with_hardly_any_eps(eps, offset):
+    """Second moments and divisors below the smallest normal number count: the first step moves each weight by
+    lr g / (|g| + eps), whatever the gradient's size."""
+    n = 5000
+    g = torch.logspace(-20.5, 3, n, device="cuda") * (1 - 2 * (torch.arange(n, device="cuda") % 2))
+    t = [torch.zeros(n + offset, device="cuda")[offset:] for _ in range(4)]
+    t[1].copy_(g)
+    lr, b1, b2 = 1e-3, 0.9, 0.999
+    multi_tensor_adamw([t[0]], [t[1]], [t[2]], [t[3]], lr=lr, betas=(b1, b2), eps=eps, weight_decay=0.0, step=1)
+    # v = g^2 (1 - b2) in fp32: below 2^-126 steps are 2^-149, so that the product is off by half of one and
+    # by (1 - b2) of the square's half: 2^-150 * 1.001 = e v in all, e < 0.08.  The root is off by
+    # 1 - sqrt(1 - e) < 0.52 e, its inverse by less than 0.57 e
+    v = g.double().square() * (1 - b2)
+    off = 2.0 ** -150 / v + 32 * 2.0 ** -24
+    assert float(off.max()) < 0.2
+    want = -lr * g.double() / (g.double().abs() + torch.tensor(eps, dtype=torch.float32).double().item())
+    assert bool(((t[0].double() - want).abs() <= want.abs() * off).all())
