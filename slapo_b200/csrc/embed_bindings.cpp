@@ -55,6 +55,8 @@ Tensor embedding_bwd(const Tensor& dy_in, const Tensor& ids_in, int64_t rows, in
   const int64_t cols = dy_in.size(-1), tokens = ids_in.numel();
   TORCH_CHECK(dy_in.numel() == tokens * cols, "embedding: one row of the gradient for each of the ", tokens,
               " ids required");
+  TORCH_CHECK(tokens <= slapo::kEmbedGradTokens, "embedding: the gradient takes at most ", slapo::kEmbedGradTokens,
+              " ids at a time, not ", tokens);
   c10::cuda::CUDAGuard guard(dy_in.device());
   const Tensor dy = dy_in.contiguous(), ids = ids_in.contiguous();
   Tensor dw = at::empty({rows, cols}, dy.options().memory_format(at::MemoryFormat::Contiguous));

@@ -475,7 +475,7 @@ int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, 
                          const EmbedGradPlan& plan, int64_t tokens, int64_t rows, int64_t cols, int64_t start,
                          int64_t padding, float scale, int dtype, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return 0;
-  if (tokens > 0x7fffff00 || rows > 0x7ffffff0 || cols > 0x7fffffff) return 1;
+  if (tokens > kEmbedGradTokens || rows > 0x7ffffff0 || cols > 0x7fffffff) return 1;
   const size_t element = dtype == 2 ? 4 : 2;
   const bool wide = cols * element % 16 == 0 && on16(dy, dw);
   const int64_t vecs = wide ? cols * element / 16 : cols, chunks = (vecs + 31) / 32;

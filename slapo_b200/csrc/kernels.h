@@ -43,6 +43,8 @@ struct EmbedGradPlan {
   int64_t sorted, ends, stretches, part;
   int64_t words() const { return 4 * sorted + ends + part; }
 };
+// As many ids as their places, rounded up to 32 tokens for each of the sort's 256 warps, have numbers of 32 bits
+constexpr int64_t kEmbedGradTokens = 0x7fffe000;
 EmbedGradPlan embedding_bwd_plan(int64_t tokens, int64_t rows, int64_t cols);
 int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, int32_t* scratch,
                          const EmbedGradPlan& plan, int64_t tokens, int64_t rows, int64_t cols, int64_t start,

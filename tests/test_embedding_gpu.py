@@ -213,3 +213,14 @@ def test_the_same_row_as_parameter_of_two_lookups():
     (NF.embedding(a, w).sum() + NF.embedding(b, w, scale=2.0).sum()).backward()
     want = torch.bincount(a, minlength=50) + 2 * torch.bincount(b, minlength=50)
     assert torch.equal(w.grad, want[:, None].float().expand(50, 16))
+
+
+def test_more_tokens_than_the_sort_numbers():
+    """Refused before anything is allocated or copied (ids and gradient are one element each, seen many times)."""
+    ids = torch.zeros(1, device="cuda", dtype=torch.int32)
+    dy = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16)
+    held, launches = torch.cuda.memory_allocated(), native.launch_count()
+    for n in (2 ** 31 - 8191, 2 ** 31 - 256, 2 ** 31, 2 ** 33):
+        with pytest.raises(RuntimeError, match="at most 2147475456 ids"):
+            native.ops().embedding_bwd(dy.expand(n, 1), ids.expand(n), 4, 0, None, 1.0)
+    assert torch.cuda.memory_allocated() == held and native.launch_count() == launches
