@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const Id* __restrict
 
 // ------------------------------------------------------------------------ //
 constexpr int kSortWarps = 32, kSortThreads = 32 * kSortWarps, kDigits = 256, kSortCtas = 8;
-// shared memory for a CTA's slice beside 40 KB of counters: the most, and what needs no permission
-constexpr int kSortSlices = 184 * 1024, kSortPlain = 8 * 1024;
+// shared memory for a CTA's slice beside 40 KB of counters, at most
+constexpr int kSortSlices = 184 * 1024;
 
 struct SortParams {
   const void* ids;
@@ -522,8 +522,7 @@ int launch_embedding_bwd(const void* ids, bool ids64, const void* dy, void* dw, 
   if (shared) {
     cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
     // (of the current device; cheap beside a launch)
-    if (bytes > kSortPlain &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSlices) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSlices) != cudaSuccess)
       return 3;
   }
   count_launch();
