@@ -224,3 +224,35 @@ def test_more_tokens_than_the_sort_numbers():
         with pytest.raises(RuntimeError, match="at most 2147475456 ids"):
             native.ops().embedding_bwd(dy.expand(n, 1), ids.expand(n), 4, 0, None, 1.0)
     assert torch.cuda.memory_allocated() == held and native.launch_count() == launches
+
+
+# (94208 tokens are the last whose sort stays in shared memory: eight CTAs' slices of 11776)
+@pytest.mark.parametrize("n", [94208, 94209, 150001])
+@pytest.mark.parametrize("kind", ["zipf", "one"])
+def test_sort_through_global_memory(n, kind):
+    """Repeated ids, rows over many stretches, a padding id and ids of other shards, in one and two passes."""
+    for vocab in (200, 3001):
+        ids = _ids(n, vocab + 20, kind)
+        ids[n // 2:n // 2 + 1000] = 40
+        got = _check(ids, torch.randn(vocab, 24, device="cuda", dtype=torch.bfloat16),
+                     torch.randn(n, 24, device="cuda", dtype=torch.bfloat16), 0.5, padding=40, start=10)
+        assert bool((got[30] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [30, 300, 12500, 20000])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_tokens_of_a_row_stay_in_their_order(rows, dtype):
+    """Eight tokens to each row: a warp adds up one row's, so that the result has the order of the tokens, to
+    the bit.  (The sort goes through shared memory for the first two, through global memory for the others.)"""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ids = torch.arange(8 * rows, device="cuda")[torch.randperm(8 * rows, device="cuda", generator=g)] % rows
+    dy = torch.randn(8 * rows, 12, device="cuda", generator=g)
+    got = native.ops().embedding_bwd(dy, ids.to(dtype), rows, 0, None, 1.0)
+    of_row = dy[torch.argsort(ids, stable=True)].view(rows, 8, 12)
+    want = torch.zeros(rows, 12, device="cuda")
+    for i in range(8):
+        want = want + of_row[:, i]
+    other = torch.zeros(rows, 12, device="cuda")
+    for i in reversed(range(8)):
+        other = other + of_row[:, i]
+    assert torch.equal(got, want) and not torch.equal(got, other)
