@@ -9,7 +9,6 @@
 //
 // The kernels are reached through their registered operators, so that each keeps its checks.
 #include <ATen/ATen.h>
-#include <ATen/FuncTorchTLS.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -414,7 +413,7 @@ tensor_list RelBiasFn::backward(AutogradContext* ctx, tensor_list grads) {
 // Whether a node has to be around what is computed of these: something is differentiated or transformed (which the
 // node reports that it does not take)
 bool wants_node(std::initializer_list<const Tensor*> inputs) {
-  if (at::functorch::functorchTLSAccessor() != nullptr) return true;
+  if (slapo::transforming()) return true;
   const bool grad = at::GradMode::is_enabled();
   for (const Tensor* t : inputs)
     if (t->defined() && ((grad && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;

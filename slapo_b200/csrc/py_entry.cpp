@@ -11,7 +11,6 @@
 //
 // What the dispatcher has to see goes to the operators: each function here says so by its result, with nothing done.
 #include <Python.h>
-#include <ATen/FuncTorchTLS.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -30,7 +29,7 @@ using slapo::AdamwLists;
 // Whether something watches calls that pass through the dispatcher: modes, function transforms, a tracer
 bool watched() {
   return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() ||
-         at::functorch::functorchTLSAccessor() != nullptr ||
+         slapo::transforming() ||
          c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer);
 }
 

@@ -1,10 +1,18 @@
 // Functions of this extension that py_entry.cpp calls without the dispatcher in between.
 #pragma once
 #include <ATen/ATen.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 
 #include <optional>
 
 namespace slapo {
+
+// Whether a function transform is at work: calls pass through its layer then.  (Whether the thread has a record of
+// transforms says less: it stays behind once one was made.)
+inline bool transforming() {
+  return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode);
+}
 
 // What AdamW over many tensors takes, as lists of tensors that live elsewhere.
 struct AdamwLists {

@@ -242,3 +242,23 @@ def test_the_kernel_refuses_an_eps_that_8bit_moments_do_not_bear():
             call(eps, bits)
     with pytest.raises(RuntimeError, match="8-bit moments need eps"):
         call(least * 1.001, 8, 0.9999)
+
+
+def test_the_entry_for_lists_after_a_function_transform():
+    """A transform that is at work has to see the call (False, nothing done); one that is over is none."""
+    from slapo_b200.ops import native
+    if not native.available():
+        pytest.skip("extension not built")
+    p = [torch.zeros(3)]
+
+    def call():
+        return native.direct("multi_adamw")(p, p, [], p, p, [], [], [0.1], [0.1], 0.9, 0.99, 1e-8, 1, None, None)
+
+    def inside(x):
+        assert call() is False
+        return x + 1
+
+    torch.func.vmap(inside)(torch.zeros(2))
+    torch.func.grad(lambda x: inside(x).sum())(torch.zeros(2))
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        call()

@@ -256,3 +256,22 @@ def test_tokens_of_a_row_stay_in_their_order(rows, dtype):
     for i in reversed(range(8)):
         other = other + of_row[:, i]
     assert torch.equal(got, want) and not torch.equal(got, other)
+
+
+def test_after_a_function_transform():
+    """A transform that is over does not keep calls from the entry without the dispatcher, nor makes a node."""
+    torch.func.vmap(lambda x: x + 1)(torch.zeros(2, device="cuda"))
+    w = torch.randn(10, 8, device="cuda")
+    ids = torch.tensor([1, 2], device="cuda")
+    assert torch.equal(native.direct("embedding")(ids, w, 0, None, 1.0), w[ids])
+    q = torch.randn(1, 1, 2, 64, device="cuda", dtype=torch.bfloat16)
+    assert native.direct("flash")(q, q, q, None, True, None, 4, 0) is not None
+
+    def inside(x):
+        assert native.direct("embedding")(ids, w, 0, None, 1.0) is None
+        return x + 1
+
+    torch.func.vmap(inside)(torch.zeros(2, device="cuda"))
+    # (inside, the operator's node says that it does not take transforms)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: NF.embedding(ids, t).sum())(w)
