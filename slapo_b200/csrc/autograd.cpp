@@ -328,6 +328,21 @@ using FlashBwd = std::tuple<Tensor, Tensor, Tensor, Tensor>(
     const optional<Tensor>&, const optional<Tensor>&, bool, double, double, const optional<Tensor>&,
     bool, int64_t, int64_t, int64_t, const optional<Tensor>&);
 
+// q, k and v of a call: three tensors, or views of the packed one
+struct FlashInputs {
+  bool packed;
+  Tensor q, k, v;
+  FlashInputs(const Tensor& q_or_qkv, const Tensor& k_in, const Tensor& v_in)
+      : packed(!k_in.defined()),
+        q(packed ? q_or_qkv.select(3, 0) : q_or_qkv),
+        k(packed ? q_or_qkv.select(3, 1) : k_in),
+        v(packed ? q_or_qkv.select(3, 2) : v_in) {}
+  optional<Tensor> rng(double p) const {
+    if (p > 0.0) return philox_reserve(q.size(0) * q.size(2) * q.size(1) * k.size(1));
+    return c10::nullopt;
+  }
+};
+
 // Attention on separate q, k, v [B, S, H, D] (q only given: the packed [B, S, H, 3, D], read in
 // place through strided views and its gradient written into one tensor of that layout).
 struct FlashFn : public Function<FlashFn> {
@@ -335,18 +350,15 @@ struct FlashFn : public Function<FlashFn> {
                         const optional<Tensor>& v, const optional<Tensor>& key_bias,
                         const optional<Tensor>& rel, bool causal, double scale, double p, int64_t window,
                         int64_t sinks) {
-    const bool packed = !k.has_value();
-    const Tensor q = packed ? q_or_qkv.select(3, 0) : q_or_qkv;
-    const Tensor kk = packed ? q_or_qkv.select(3, 1) : *k, vv = packed ? q_or_qkv.select(3, 2) : *v;
-    optional<Tensor> rng;
-    if (p > 0.0) rng = philox_reserve(q.size(0) * q.size(2) * q.size(1) * kk.size(1));
+    const FlashInputs x(q_or_qkv, or_undefined(k), or_undefined(v));
+    const optional<Tensor> rng = x.rng(p);
     Tensor out, lse, rest;
     if (window > 0) {
       static auto f = op<FlashFwdRest>("slapo_b200::flash_attn_fwd_rest");
-      std::tie(out, lse, rest) = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
+      std::tie(out, lse, rest) = f.call(x.q, x.k, x.v, key_bias, rel, causal, scale, p, rng, window, sinks);
     } else {
       static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
-      std::tie(out, lse) = f.call(q, kk, vv, key_bias, rel, causal, scale, p, rng, window, sinks);
+      std::tie(out, lse) = f.call(x.q, x.k, x.v, key_bias, rel, causal, scale, p, rng, window, sinks);
     }
     ctx->save_for_backward({q_or_qkv, or_undefined(k), or_undefined(v), out, lse,
                             or_undefined(key_bias), or_undefined(rel), rest});
@@ -359,9 +371,7 @@ struct FlashFn : public Function<FlashFn> {
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    const bool packed = !s[1].defined();
-    const Tensor q = packed ? s[0].select(3, 0) : s[0];
-    const Tensor k = packed ? s[0].select(3, 1) : s[1], v = packed ? s[0].select(3, 2) : s[2];
+    const auto [packed, q, k, v] = FlashInputs(s[0], s[1], s[2]);
     optional<Tensor> rng;
     const double p = ctx->saved_data["p"].toDouble();
     if (p > 0.0) rng = ctx->saved_data["rng"].toTensor();
@@ -521,11 +531,12 @@ std::tuple<Tensor, Tensor> dropout_add_norm(const Tensor& x, const optional<Tens
 Tensor flash(const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& v,
              const optional<Tensor>& key_bias, const optional<Tensor>& rel, bool causal, double scale,
              double p, int64_t window, int64_t sinks) {
-  const Tensor bias = or_undefined(key_bias), distances = or_undefined(rel);
-  if (k.has_value() && v.has_value() && p == 0.0 && !wants_node({&q, &*k, &*v, &bias, &distances})) {
-    // (a token of generation is a launch: no node around it)
+  const Tensor kk = or_undefined(k), vv = or_undefined(v), bias = or_undefined(key_bias), distances = or_undefined(rel);
+  if (!wants_node({&q, &kk, &vv, &bias, &distances})) {
+    // (a token of generation is a launch: no node around it; nor is anything kept for a backward)
     static auto f = op<FlashFwd>("slapo_b200::flash_attn_fwd");
-    return std::get<0>(f.call(q, *k, *v, key_bias, rel, causal, scale, p, c10::nullopt, window, sinks));
+    const FlashInputs x(q, kk, vv);
+    return std::get<0>(f.call(x.q, x.k, x.v, key_bias, rel, causal, scale, p, x.rng(p), window, sinks));
   }
   return FlashFn::apply(q, k, v, key_bias, rel, causal, scale, p, window, sinks);
 }

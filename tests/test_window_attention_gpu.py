@@ -444,3 +444,35 @@ def test_gradients_carry_two_roundings(dtype):
         want = want.transpose(1, 2)
         rounding = (want.to(dtype).double() - want).norm()
         assert float((x.double() - want).norm() / rounding) < 1.5
+
+
+@pytest.mark.parametrize("p", [0.0, 0.25])
+@pytest.mark.parametrize("packed", [True, False])
+def test_nothing_is_kept_for_a_backward_that_will_not_be(packed, p):
+    """Without a gradient: the output (and row sums while the call runs), not a byte for each of its values
+    besides; the output is that of a call with a gradient."""
+    b, s, h, d = 2, 500, 4, 64
+    qkv = torch.randn(b, s, h, 3, d, device="cuda", dtype=torch.bfloat16)
+    bias = torch.zeros(b, s, device="cuda")
+    bias[:, 400:] = -10000.0
+
+    def call(qkv):
+        torch.manual_seed(3)
+        if packed:
+            return flash_attention_qkvpacked(qkv, bias, True, p=p, window=64, sinks=2)
+        return NF.flash_attention(*qkv.unbind(3), bias, True, dropout_p=p, window=64, sinks=2)
+
+    want = call(qkv.clone().requires_grad_())
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad):
+            got = call(qkv)             # (not a leaf that wants one)
+            assert torch.equal(got, want) and got.grad_fn is None
+            del got
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            held = torch.cuda.memory_allocated()
+            got = call(qkv)
+            kept = torch.cuda.max_memory_allocated() - held
+            # output, log sums, the generator's place; each rounded up to 512 bytes
+            assert kept <= b * s * h * (2 * d + 4) + 4 * 512, kept
+            del got
