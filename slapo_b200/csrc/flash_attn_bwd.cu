@@ -1261,13 +1261,16 @@ static int sink_splits(int64_t bh, int Sq, int Sk, int D, int window, int sinks,
   const int64_t most = (int64_t(64) << 20) / (2 * bh * sink_tiles * 128 * D * 4);
   if (n > most) n = most;
   if (n < 2) return 1;
-  *each = static_cast<int>(fewest / n);
-  return static_cast<int>(n);
+  // (rounded up, and as many shares as that fills: the last is the short one.  Rounded down it had all that was left over:
+  // 23 half tiles after 21 shares of 5, 8192 queries of one head with a window of 256: 54 us for 40.  Of several sinks'
+  // tiles the earlier ones have two half tiles more each, which go to their last share.)
+  *each = static_cast<int>((fewest + n - 1) / n);
+  return static_cast<int>((fewest + *each - 1) / *each);
 }
 
 FlashBwdPlan flash_bwd_plan(int B, int H, int Sq, int Sk, int D, bool packed, bool causal, int window, int sinks,
                             bool key_bias, bool rel, float p_drop, int64_t keep_words) {
-  FlashBwdPlan s;
+  FlashBwdPlan s{};
   const int64_t rq = round128(Sq), rk = round128(Sk), bh = static_cast<int64_t>(B) * H;
   const int64_t q_tiles = rq / 128, k_tiles = rk / 128;
   const bool drop = dropout_thr7(p_drop) != 0;

@@ -476,3 +476,11 @@ def test_nothing_is_kept_for_a_backward_that_will_not_be(packed, p):
             # output, log sums, the generator's place; each rounded up to 512 bytes
             assert kept <= b * s * h * (2 * d + 4) + 4 * 512, kept
             del got
+
+
+@pytest.mark.parametrize("s,n,window,sinks,d", [(8192, 1, 256, 4, 128), (8000, 1, 256, 4, 64), (4096, 3, 128, 1, 64),
+                                                (3001, 1, 65, 300, 32), (2600, 2, 1, 129, 128)])
+def test_shares_of_the_sinks_queries(s, n, window, sinks, d):
+    """Few heads and many queries: the sinks' are dealt out to many work items, some of one half tile more."""
+    q, k, v, do = _tensors(1, s, s, n, d, torch.bfloat16, seed=s)
+    _check(_run(q, k, v, do, window, sinks), q, k, v, do, window, sinks)
