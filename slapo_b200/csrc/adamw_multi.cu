@@ -18,7 +18,7 @@
 // 10 without masters; with 8-bit moments by instructions too, some 45 per element (a scheduler's slots are three
 // quarters full at 10 bytes).
 // Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 820 us (96 % of the copy
-// rate), 8-bit moments 540 - 562 us (80 - 83 %); 304 M elements, 8-bit, no masters: 560 - 588 us (80 - 84 %), from box to box.
+// rate), 8-bit moments 490 - 499 us (90 - 92 %); 304 M elements, 8-bit, no masters: 560 - 588 us (80 - 84 %), from box to box.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -31,7 +31,6 @@ namespace slapo {
 constexpr int kAdamBlock = 256;                       // values per factor: a warp's 32 x 8
 constexpr int kAdamUnit = 2, kAdamUnitSize = kAdamUnit * kAdamBlock;      // blocks that a warp takes at a time
 constexpr int kAdamThreads = 256, kAdamWarps = kAdamThreads / 32;
-constexpr int kAdamDepth = 3;                         // units of a warp in shared memory
 
 constexpr int kAdam32Unit = kAdamThreads * kVec;      // elements of a CTA's step in the other kernel
 
@@ -134,6 +133,20 @@ struct alignas(16) AdamStage {
   Weight w[kAdamUnitSize];
   uint8_t m[kAdamUnitSize], v[kAdamUnitSize];
   float scale[2][kAdamUnit];
+};
+
+// A CTA's ring, how many of them an SM holds, and how many launches' worth of resident CTAs the units are dealt out to.
+// 16-bit weights: three CTAs and one sweep (324 us for 183 M elements; two sweeps 332).  With masters two CTAs fit, and
+// four sweeps, each by CTAs that start as those before end, beat one: 490 for 545 us, 24 layers 900 for 1008, 4 layers of 2048
+// 820 for 936 (eight: 474, 875, 777, but 12 layers of 768 372 for 357).  fp32 weights: one CTA, and a unit more on its way:
+// 480 for 525 us with three in the ring, two CTAs of two each 568.
+template <bool kMaster, typename T>
+struct AdamRing {
+  using Stage = AdamStage<kMaster, T>;
+  static constexpr int kDepth = sizeof(T) == 4 ? 4 : 3;                   // units of a warp in shared memory
+  static constexpr int kSmem = kAdamWarps * kDepth * static_cast<int>(sizeof(Stage));
+  static constexpr int kCtas = sizeof(T) == 4 ? 1 : kMaster ? 2 : 3, kSweeps = kMaster ? 4 : 1;
+  static_assert(kCtas * (kSmem + 1024 + 16) <= 228 * 1024, "8-bit AdamW: shared memory of the CTAs on an SM");
 };
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
@@ -288,12 +301,14 @@ __device__ __forceinline__ void adam_block(const AdamwTensor& t, const AdamStepS
 // stretch of 16 blocks for each warp: 665 and 766 - thousands of places in memory at a time -, one sweep of all
 // warps: 583 and 660, two blocks at a time: 564 and 593.)
 template <bool kMaster, typename T, int N>
-__global__ void __launch_bounds__(kAdamThreads, 3) adamw8_kernel(const __grid_constant__ AdamBatch<N> b) {
+__global__ void __launch_bounds__(kAdamThreads, AdamRing<kMaster, T>::kCtas)
+adamw8_kernel(const __grid_constant__ AdamBatch<N> b) {
   extern __shared__ uint4 adam_smem[];
   using Stage = AdamStage<kMaster, T>;
+  constexpr int kAdamDepth = AdamRing<kMaster, T>::kDepth;
   Stage* ring = reinterpret_cast<Stage*>(adam_smem) + (threadIdx.x >> 5) * kAdamDepth;
   const AdamStepScalars c = adam_scalars(b.s);
-  // Neighbouring warps take neighbouring units, all of them one sweep over the tensors: memory is read page by page.
+  // Neighbouring warps take neighbouring units, the resident ones a sweep over the tensors: memory is read page by page.
   const int units = b.first[b.count], first = blockIdx.x * kAdamWarps + (threadIdx.x >> 5);
   const int stride = gridDim.x * kAdamWarps;
   auto seek = [&](int at, int tensor) {      // the tensor with first[tensor] <= at < first[tensor + 1], from there on
@@ -410,11 +425,13 @@ static int launch_batch(const AdamwTensor* t, int n, const AdamwScalars& s, cuda
   if (units == 0) return 0;
   count_launch();
   if constexpr (k8) {
-    constexpr int kSmem = kAdamWarps * kAdamDepth * static_cast<int>(sizeof(AdamStage<kMaster, T>));
+    using Ring = AdamRing<kMaster, T>;
+    constexpr int kSmem = Ring::kSmem;
     auto kernel = adamw8_kernel<kMaster, T, N>;
     // (of the current device; cheap beside a launch)
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return 3;
-    const int64_t ctas = (units + kAdamWarps - 1) / kAdamWarps, cap = static_cast<int64_t>(sm_count()) * 3;
+    const int64_t ctas = (units + kAdamWarps - 1) / kAdamWarps;
+    const int64_t cap = static_cast<int64_t>(sm_count()) * Ring::kCtas * Ring::kSweeps;
     kernel<<<static_cast<int>(ctas < cap ? ctas : cap), kAdamThreads, kSmem, stream>>>(b);
   } else {
     const int64_t cap = static_cast<int64_t>(sm_count()) * 16;
