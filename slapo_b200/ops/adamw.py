@@ -176,13 +176,12 @@ class FusedAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.capturable = state_bits, master_weights, capturable
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
-    def _init_state(self, p, counter):
+    def _new_state(self, p, counter):
         if not p.is_contiguous():
             raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")
         if p.dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise ValueError(f"parameters of bf16, fp16 or fp32 required, not {p.dtype}")
-        s = self.state[p]
-        s["step"] = counter if counter is not None else 0
+        s = {"step": counter if counter is not None else 0}
         if self.master_weights and p.dtype != torch.float32:
             s["master"] = p.detach().float()
         if self.state_bits == 8:
@@ -196,13 +195,15 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale=None):
-        """One update of every parameter that has a gradient."""
+        """One update of every parameter that has a gradient.  What a refused step has not updated keeps its
+        state and its number of steps."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         runs = {}       # one kernel for each device, type, betas, eps and number of steps
         fresh = {}      # the counters on the device of what is updated for the first time
+        new = []        # states that begin with this step
         for group in self.param_groups:
             lr, decay = float(group["lr"]), float(group["weight_decay"])
             for p in group["params"]:
@@ -211,7 +212,10 @@ class FusedAdamW(torch.optim.Optimizer):
                     continue
                 if grad.layout != torch.strided:
                     raise RuntimeError("FusedAdamW takes dense gradients")
-                s = self.state[p] or self._init_state(p, self._new_counter(p, fresh))
+                s = self.state.get(p)
+                if not s:
+                    s = self._new_state(p, self._new_counter(p, fresh))
+                    new.append(s)
                 count = s["step"]
                 key = (p.device, p.dtype, tuple(group["betas"]), group["eps"],
                        id(count) if torch.is_tensor(count) else count)
@@ -223,22 +227,32 @@ class FusedAdamW(torch.optim.Optimizer):
                 run[2].append(s)
                 run[3].append(lr)
                 run[4].append(decay)
-        self._count_on_device(runs.values())
-        for (_, _, betas, eps, _), (params, grads, states, lrs, decays) in runs.items():
-            step = states[0]["step"]
-            if not torch.is_tensor(step):
-                step += 1
-                for s in states:
-                    s["step"] = step
-            more = {}
-            if "master" in states[0]:
-                more["masters"] = [s["master"] for s in states]
-            if "exp_avg_scale" in states[0]:
-                more["exp_avg_scales"] = [s["exp_avg_scale"] for s in states]
-                more["exp_avg_sq_scales"] = [s["exp_avg_sq_scale"] for s in states]
-            multi_tensor_adamw(params, grads, [s["exp_avg"] for s in states],
-                               [s["exp_avg_sq"] for s in states], lr=lrs, betas=betas, eps=eps,
-                               weight_decay=decays, step=step, grad_scale=grad_scale, **more)
+        counters = self._count_on_device(runs.values(), new)
+        try:
+            for (_, _, betas, eps, _), (params, grads, states, lrs, decays) in runs.items():
+                step = states[0]["step"]
+                counted = torch.is_tensor(step)
+                more = {}
+                if "master" in states[0]:
+                    more["masters"] = [s["master"] for s in states]
+                if "exp_avg_scale" in states[0]:
+                    more["exp_avg_scales"] = [s["exp_avg_scale"] for s in states]
+                    more["exp_avg_sq_scales"] = [s["exp_avg_sq_scale"] for s in states]
+                multi_tensor_adamw(params, grads, [s["exp_avg"] for s in states],
+                                   [s["exp_avg_sq"] for s in states], lr=lrs, betas=betas, eps=eps,
+                                   weight_decay=decays, step=step if counted else step + 1,
+                                   grad_scale=grad_scale, **more)
+                if counted:
+                    counters.pop(id(step), None)
+                else:
+                    for s in states:
+                        s["step"] = step + 1
+                if new:
+                    self.state.update(zip(params, states))
+        except BaseException:
+            for counter in counters.values():       # (of what nothing was updated with)
+                counter.sub_(1)
+            raise
         return loss
 
     def _new_counter(self, p, fresh):
@@ -251,18 +265,19 @@ class FusedAdamW(torch.optim.Optimizer):
             fresh[p.device] = torch.zeros(1, dtype=torch.int64, device=p.device)
         return fresh[p.device]
 
-    def _count_on_device(self, runs):
-        """Advance the counters on the device, each once, by all of the parameters that share it."""
+    def _count_on_device(self, runs, new):
+        """Advance the counters on the device, each once, by all of the parameters that share it; by their
+        ``id``."""
         if not self.capturable:
-            return
+            return {}
         updated = {}
         for run in runs:
             for s in run[2]:
                 if torch.is_tensor(s["step"]):
                     updated.setdefault(id(s["step"]), [s["step"], 0])[1] += 1
         shared = {}
-        for s in self.state.values():
-            if torch.is_tensor(s["step"]):
+        for s in [*self.state.values(), *new]:
+            if torch.is_tensor(s.get("step")):
                 shared[id(s["step"])] = shared.get(id(s["step"]), 0) + 1
         for key, (counter, n) in updated.items():
             if n != shared[key]:
@@ -270,13 +285,14 @@ class FusedAdamW(torch.optim.Optimizer):
                                    f"their gradients together ({n} of {shared[key]} have one)")
         for counter, _ in updated.values():
             counter.add_(1)
+        return {key: counter for key, (counter, _) in updated.items()}
 
     def load_state_dict(self, state_dict):
         """As ``torch.optim.Optimizer.load_state_dict``; states keep their own types, whatever the
         parameters' is.  Saved moments of another number of bits are refused; masters that are wanted and were
         not saved are made of the parameters, and saved ones that are not wanted are left out."""
         for old in state_dict["state"].values():
-            if ("exp_avg_scale" in old) != (self.state_bits == 8):
+            if old and ("exp_avg_scale" in old) != (self.state_bits == 8):
                 raise ValueError("the saved moments have another number of bits")
         super().load_state_dict(state_dict)
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
@@ -284,7 +300,7 @@ class FusedAdamW(torch.optim.Optimizer):
         counters = {}
         for index, p in zip(saved, params):
             old = state_dict["state"].get(index)
-            if old is None:
+            if not old:
                 continue
             s = self.state[p]
             s.pop("master", None)

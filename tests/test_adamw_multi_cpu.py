@@ -262,3 +262,39 @@ def test_the_entry_for_lists_after_a_function_transform():
     torch.func.grad(lambda x: inside(x).sum())(torch.zeros(2))
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         call()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_step_changes_nothing(bits):
+    """Neither states nor their number of steps, for what is refused and for what comes before it."""
+    good, other = torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(4, 3).t())
+    opt = FusedAdamW([good, other], lr=1e-2, state_bits=bits, capturable=True)
+    good.grad, other.grad = torch.ones(5), torch.ones(4, 3).t()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    assert not opt.state and bool((good == 1).all())
+    other.grad = None
+    opt.step()
+    assert opt.state[good]["step"] == 1 and other not in opt.state
+    held = {k: v.clone() if torch.is_tensor(v) else v for k, v in opt.state[good].items()}
+    weights = good.detach().clone()
+    other.grad = torch.ones(4, 3).t()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    good.grad = torch.ones(5).to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        opt.step()
+    good.grad = torch.ones(5)
+    other.grad = None
+    with pytest.raises(AttributeError):
+        opt.step(grad_scale="not a tensor")
+    assert list(opt.state) == [good] and torch.equal(good, weights)
+    for name, value in opt.state[good].items():
+        assert torch.equal(value.float(), held[name].float()) if torch.is_tensor(value) else value == held[name]
+    # a state that something else has begun, without values, is none
+    assert opt.state[other] == {}
+    opt.step()
+    again = FusedAdamW([good, other], state_bits=bits)
+    again.load_state_dict(opt.state_dict())
+    assert again.state[good]["step"] == 2
+    again.step()

@@ -373,3 +373,59 @@ def test_32bit_moments_with_hardly_any_eps(eps, offset):
     assert float(off.max()) < 0.2
     want = -lr * g.double() / (g.double().abs() + torch.tensor(eps, dtype=torch.float32).double().item())
     assert bool(((t[0].double() - want).abs() <= want.abs() * off).all())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_does_not_count(capturable, bits):
+    """A gradient without memory is refused by the kernel's checks: weights, moments and the number of steps,
+    on the host or on the device, are as before; so after a first step under a capture."""
+    torch.manual_seed(1)
+    a = torch.nn.Linear(40, 30, device="cuda").to(torch.bfloat16)
+    b = copy.deepcopy(a)
+    one = FusedAdamW(a.parameters(), lr=1e-2, state_bits=bits, capturable=capturable)
+    two = FusedAdamW(b.parameters(), lr=1e-2, state_bits=bits, capturable=capturable)
+    grad = torch.randn(30, 40, device="cuda").to(torch.bfloat16)
+
+    def grads(m):
+        m.weight.grad, m.bias.grad = grad.clone(), torch.ones(30, device="cuda").to(torch.bfloat16)
+
+    def refused():
+        grads(a)
+        a.bias.grad.untyped_storage().resize_(0)
+        with pytest.raises(RuntimeError, match="no memory"):
+            one.step()
+
+    if capturable:
+        grads(a)
+        with pytest.raises(RuntimeError, match="before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                one.step()
+        torch.cuda.synchronize()
+    refused()
+    assert not one.state
+    for step in range(1, 4):
+        grads(a)
+        grads(b)
+        one.step()
+        two.step()
+        refused()
+        for p, q in zip(a.parameters(), b.parameters()):
+            assert torch.equal(p, q) and int(one.state[p]["step"]) == int(two.state[q]["step"]) == step
+            for name, value in one.state[p].items():
+                assert not torch.is_tensor(value) or torch.equal(value.float(), two.state[q][name].float())
+
+
+def test_what_was_updated_before_a_refusal_counts():
+    """Two types are two kernels: the first is through when the second is refused."""
+    a = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    b = torch.nn.Parameter(torch.ones(8, device="cuda", dtype=torch.bfloat16))
+    opt = FusedAdamW([a, b], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    b.grad.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="no memory"):
+        opt.step()
+    assert opt.state[a]["step"] == 1 and b not in opt.state and bool((a < 1).all())
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    assert opt.state[a]["step"] == 2 and opt.state[b]["step"] == 1
