@@ -176,6 +176,10 @@ class FusedAdamW(torch.optim.Optimizer):
         self.state_bits, self.master_weights, self.capturable = state_bits, master_weights, capturable
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        own = ("state_bits", "master_weights", "capturable")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in own}}
+
     def _new_state(self, p, counter):
         if not p.is_contiguous():
             raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous")

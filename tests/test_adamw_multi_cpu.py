@@ -298,3 +298,28 @@ def test_a_refused_step_changes_nothing(bits):
     again.load_state_dict(opt.state_dict())
     assert again.state[good]["step"] == 2
     again.step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("how", ["deepcopy", "save"])
+def test_a_copied_optimizer_goes_on(how, bits, tmp_path):
+    """A copy, and one that was saved whole, keep their options and states, and step as the original does."""
+    model = _model().to(torch.bfloat16)
+    opt = FusedAdamW(model.parameters(), lr=1e-2, state_bits=bits, master_weights=bits == 32)
+    _grads(model, 0)
+    opt.step()
+    if how == "deepcopy":
+        other = copy.deepcopy(opt)
+    else:
+        torch.save(opt, tmp_path / "opt.pt")
+        other = torch.load(tmp_path / "opt.pt", weights_only=False)
+    assert (other.state_bits, other.master_weights, other.capturable) == (bits, bits == 32, False)
+    copies = other.param_groups[0]["params"]
+    for i, p in enumerate(model.parameters()):
+        g = torch.full_like(p, 0.5 + i)
+        p.grad, copies[i].grad = g, g.clone()
+    opt.step()
+    other.step()
+    for p, q in zip(model.parameters(), copies):
+        assert p is not q and torch.equal(p, q)
+        assert other.state[q]["step"] == 2 and ("master" in other.state[q]) == (bits == 32)
