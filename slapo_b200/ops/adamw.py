@@ -160,7 +160,8 @@ class FusedAdamW(torch.optim.Optimizer):
     ``master_weights``: keep fp32 copies of 16-bit parameters, which are what is updated (default); without
     them an update below half a step of the parameter's type is lost.  ``capturable``: steps are counted on
     the device, so that a captured ``step()`` can be replayed (with the ``lr`` and ``weight_decay`` of its
-    capture); parameters that were first updated together then have to go on together.
+    capture; without, capturing a step is refused); parameters that were first updated together then have to
+    go on together.
     ``step(grad_scale=...)`` takes a one-element fp32 tensor that multiplies every gradient (clipping, loss
     scaling).  Parameter groups may differ in ``lr``,
     ``weight_decay``, ``betas`` and ``eps``.  Parameters must be contiguous and their gradients dense."""
@@ -225,6 +226,9 @@ class FusedAdamW(torch.optim.Optimizer):
                        id(count) if torch.is_tensor(count) else count)
                 run = runs.get(key)
                 if run is None:
+                    if not torch.is_tensor(count) and p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        # (every replay would be this step again, with its bias corrections)
+                        raise RuntimeError("FusedAdamW: a step that is captured needs capturable=True")
                     run = runs[key] = ([], [], [], [], [])
                 run[0].append(p)
                 run[1].append(grad if grad.is_contiguous() else grad.contiguous())

@@ -429,3 +429,22 @@ def test_what_was_updated_before_a_refusal_counts():
     a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
     opt.step()
     assert opt.state[a]["step"] == 2 and opt.state[b]["step"] == 1
+
+
+@pytest.mark.parametrize("steps", [0, 1])
+def test_a_step_that_counts_on_the_host_is_not_captured(steps):
+    """Its replays would keep the bias corrections of the one that was captured."""
+    w = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    w.grad = torch.ones_like(w)
+    opt = FusedAdamW([w], lr=1e-2)
+    for _ in range(steps):
+        opt.step()
+    torch.cuda.synchronize()
+    before = native.launch_count()
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert native.launch_count() == before and len(opt.state) == steps
+    opt.step()
+    assert opt.state[w]["step"] == steps + 1
