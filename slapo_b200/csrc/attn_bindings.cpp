@@ -22,10 +22,11 @@ void check_bshd(const Tensor& t, const char* name) {
   TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
 }
 
-const float* opt_f32(const optional<Tensor>& t, const char* name) {
+const float* opt_f32(const optional<Tensor>& t, const char* name, const Tensor& q) {
   if (!t.has_value() || !t->defined()) return nullptr;
   TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kFloat && t->is_contiguous(), name,
               " must be a contiguous fp32 CUDA tensor");
+  TORCH_CHECK(t->device() == q.device(), name, " must be on the device of the queries");
   return t->data_ptr<float>();
 }
 
@@ -83,7 +84,7 @@ std::tuple<Tensor, Tensor, Tensor> run_flash_fwd(const Tensor& q, const Tensor& 
       q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
       keep_rest && rest.numel() > 0 ? rest.data_ptr<uint8_t>() : nullptr, lse.data_ptr<float>(),
       splits > 1 ? scratch.data_ptr<float>() : nullptr,
-      opt_f32(kbias, "key bias"), opt_f32(rel, "relative bias"), B, H, Sq, Sk, D, qs, ks, vs,
+      opt_f32(kbias, "key bias", q), opt_f32(rel, "relative bias", q), B, H, Sq, Sk, D, qs, ks, vs,
       static_cast<float>(scale), causal ? 1 : 0, window, sinks, static_cast<float>(p_drop), unpack_rng(rng),
       q.scalar_type() == at::kBFloat16, slapo_status_ptr(q.get_device()),
       at::cuda::getCurrentCUDAStream().stream());
@@ -154,8 +155,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
       q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
       has_rest ? rest->const_data_ptr<uint8_t>() : nullptr, dout.data_ptr(),
       lse.data_ptr<float>(), plan, scratch.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(),
-      dv.data_ptr(), row_stride, row_stride, opt_f32(kbias, "key bias"),
-      opt_f32(rel, "relative bias"),
+      dv.data_ptr(), row_stride, row_stride, opt_f32(kbias, "key bias", q),
+      opt_f32(rel, "relative bias", q),
       has_rel ? drel.data_ptr<float>() : nullptr, B, H, Sq, Sk, D, qs, ks, vs,
       static_cast<float>(scale), causal ? 1 : 0, window, sinks, static_cast<float>(p_drop), unpack_rng(rng),
       q.scalar_type() == at::kBFloat16, slapo_status_ptr(q.get_device()),

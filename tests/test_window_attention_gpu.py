@@ -484,3 +484,18 @@ def test_shares_of_the_sinks_queries(s, n, window, sinks, d):
     """Few heads and many queries: the sinks' are dealt out to many work items, some of one half tile more."""
     q, k, v, do = _tensors(1, s, s, n, d, torch.bfloat16, seed=s)
     _check(_run(q, k, v, do, window, sinks), q, k, v, do, window, sinks)
+
+
+@pytest.mark.multigpu
+@pytest.mark.parametrize("sq", [1, 130])
+def test_a_bias_on_another_device_is_refused(sq):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    q = torch.randn(1, sq, 2, 64, device="cuda:0", dtype=torch.bfloat16)
+    k = torch.randn(1, 200, 2, 64, device="cuda:0", dtype=torch.bfloat16)
+    bias = torch.zeros(1, 200, device="cuda:1")
+    for window in (None, 64):
+        with pytest.raises(RuntimeError, match="device of the queries"):
+            NF.flash_attention(q, k, k, bias, causal=True, window=window)
+    with pytest.raises(RuntimeError, match="one device"):
+        NF.flash_attention(q, k.to("cuda:1"), k, None, causal=True, window=64)
