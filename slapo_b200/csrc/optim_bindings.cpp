@@ -153,9 +153,10 @@ void run(const AdamwLists& x) {
   const int rc = slapo::launch_adamw_multi(table.data(), static_cast<int>(table.size()), s, bits8, code,
                                            at::cuda::getCurrentCUDAStream().stream());
   TORCH_CHECK(rc == 0, "multi_adamw: launch refused (code ", rc, ")");
-  // (autograd notices that a saved parameter has changed)
-  for (size_t i = 0; i < n; ++i)
-    if (!x.params[i].is_inference()) x.params[i].unsafeGetTensorImpl()->bump_version();
+  // (autograd notices that what it has saved of these has changed)
+  for (const List* list : {&x.params, &x.masters, &x.exp_avgs, &x.exp_avg_sqs, &x.exp_avg_scales, &x.exp_avg_sq_scales})
+    for (size_t i = 0; i < list->size; ++i)
+      if (!(*list)[i].is_inference()) (*list)[i].unsafeGetTensorImpl()->bump_version();
 }
 
 using Ops = at::TensorList;
