@@ -96,7 +96,8 @@ class FlashAttentionOp(nn.Module):
         Accepted: ``[B, Sk]`` / ``[B, 1, 1, Sk]`` key-padding masks, and - for causal attention
         - the combined ``[B, 1, Sq, Sk]`` causal + padding mask that Hugging Face models build:
         its last query row is exactly the key-padding part (the triangular part is applied by
-        the kernel).  Boolean masks (``True`` = attend) become ``0 / -10000``."""
+        the kernel, and so is a window: not a mask that has the window's band in it).  Boolean masks
+        (``True`` = attend) become ``0 / -10000``."""
         if attention_mask is None:
             return None
         if attention_mask.dim() == 4:

@@ -72,9 +72,11 @@ def relative_bias_by_distance(table, sq, sk, bidirectional, max_distance):
 
 def flash_attention_native(q, k, v, key_bias, causal, scale, p, rel_table, rel_bidir, rel_maxd,
                            window=None, sinks=0):
+    from .functional import fp32_bias
+
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if key_bias is not None:
-        key_bias = key_bias.float().contiguous()
+        key_bias = fp32_bias(key_bias, window).contiguous()
     rel = None
     if rel_table is not None:
         rel = relative_bias_by_distance(rel_table, q.shape[1], k.shape[1], rel_bidir, rel_maxd)
@@ -86,12 +88,12 @@ def flash_attention_qkvpacked(qkv, key_bias=None, causal=False, scale=None, p=0.
                               rel_table=None, rel_bidir=True, rel_maxd=128, window=None, sinks=0):
     """Attention on a packed ``[B, S, H, 3, D]`` projection output (``window``, ``sinks``: see
     :func:`slapo_b200.ops.functional.flash_attention`)."""
-    from .functional import check_window
+    from .functional import check_window, fp32_bias
 
     check_window(window, sinks, causal, rel_table)
     scale = 1.0 / math.sqrt(qkv.shape[-1]) if scale is None else scale
     if key_bias is not None:
-        key_bias = key_bias.float().contiguous()
+        key_bias = fp32_bias(key_bias, window).contiguous()
     rel = None
     if rel_table is not None:
         rel = relative_bias_by_distance(rel_table, qkv.shape[1], qkv.shape[1], rel_bidir, rel_maxd)

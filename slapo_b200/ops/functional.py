@@ -293,18 +293,18 @@ def attention_reference(q, k, v, key_padding_bias=None, causal=False, scale=None
         buckets = t5_relative_position_bucket(
             mem_pos - ctx_pos, rel_bidirectional, rel_bias_table.shape[0], rel_max_distance)
         scores = scores + rel_bias_table.float()[buckets].permute(2, 0, 1)[None]
-    if key_padding_bias is not None:
-        scores = scores + key_padding_bias.float().view(b, 1, 1, sk)
+    biases = [] if key_padding_bias is None else [fp32_bias(key_padding_bias, window).view(b, 1, 1, sk)]
     if attn_bias is not None:
-        scores = scores + attn_bias.float()
+        biases.append(fp32_bias(attn_bias, window))
+    for bias in biases:
+        scores = scores + bias
     if causal:
         keep = torch.ones(sq, sk, dtype=torch.bool, device=q.device).tril(diagonal=sk - sq)
         scores = scores.masked_fill(~keep, float("-inf"))
     if window is not None:
         hidden = _outside_window(sq, sk, window, sinks, q.device)
-        for bias in (None if key_padding_bias is None else key_padding_bias.view(b, 1, 1, sk), attn_bias):
-            if bias is not None:
-                hidden = hidden | (bias.float() < -1e30)
+        for bias in biases:
+            hidden = hidden | (bias < -1e30)
         scores = scores.masked_fill(hidden, float("-inf"))
         # (a row without a key: probabilities and gradients of 0)
         empty = (scores == float("-inf")).all(-1, keepdim=True)
@@ -317,6 +317,14 @@ def attention_reference(q, k, v, key_padding_bias=None, causal=False, scale=None
         probs = F.dropout(probs, dropout_p, True)
     out = torch.matmul(probs, vf)
     return out.transpose(1, 2).to(q.dtype)
+
+
+def fp32_bias(bias, window):
+    """An additive bias in fp32.  With a window, fp16's lowest value stays what it is to a mask, "not seen at
+    all": as a number, -65504 is one that a row of nothing else would be averaged with."""
+    if window is None or bias.dtype != torch.float16:
+        return bias.float()
+    return bias.float().masked_fill(bias == torch.finfo(torch.float16).min, float("-inf"))
 
 
 def _outside_window(sq, sk, window, sinks, device):
@@ -379,8 +387,8 @@ def flash_attention(q, k, v, key_padding_bias=None, causal=False, scale=None, dr
 
     ``window``, with ``causal``: a query sees the ``window`` keys up to its own and the first ``sinks`` keys;
     tiles of keys that no query of a tile sees are not touched.  Queries are the last ``Sq`` of ``Sk``
-    positions, as without.  A key with a bias below -1e30 (-inf, a mask of the type's lowest value) is then
-    not seen at all, and a query that sees no key has an output and gradients of 0.  Keys and values must be
+    positions, as without.  A key with a bias below -1e30 (-inf, a mask of the type's lowest value, fp16's
+    too) is then not seen at all, and a query that sees no key has an output and gradients of 0.  Keys and values must be
     finite, hidden ones too."""
     check_window(window, sinks, causal, rel_bias_table)
     if torch.is_tensor(q) and q.is_cuda and rel_bias_table is None and not (training and dropout_p > 0.0):

@@ -154,3 +154,24 @@ def test_refusals():
         FlashAttention(32, 4, output_proj=False, window=2)
     with pytest.raises(ValueError):
         flash_attention_qkvpacked(torch.randn(1, 4, 2, 3, 8), causal=False, window=2)
+
+
+@pytest.mark.parametrize("general", [False, True])
+def test_the_lowest_value_of_a_16bit_mask(general):
+    """A mask in fp16 hides with -65504 as one in bf16 or fp32 with its lowest value: rows whose keys are all
+    masked are zeros, in the key-padding form and with a bias for each pair.  Without a window it is a number."""
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(2, 9, 2, 8, generator=g) for _ in range(3))
+    pad = torch.zeros(2, 1, 1, 9, dtype=torch.bool)
+    pad[0, ..., 6:] = True
+    pad[1, ..., :5] = True       # (the window of the first queries is all padding)
+    want = None
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        mask = torch.zeros(2, 1, 1, 9, dtype=dtype).masked_fill(pad, torch.finfo(dtype).min)
+        if general:
+            mask = mask.expand(2, 2, 9, 9)
+        got = FlashAttentionOp(apply_causal_mask=True, window=3)(q, k, v, mask)
+        want = got if want is None else want
+        assert torch.equal(got, want) and bool((got[1, :5] == 0).all()) and not bool((got[1, 5:] == 0).any())
+        plain = FlashAttentionOp(apply_causal_mask=True)(q, k, v, mask)
+        assert not bool((plain[1, :5] == 0).any())

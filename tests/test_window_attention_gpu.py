@@ -499,3 +499,21 @@ def test_a_bias_on_another_device_is_refused(sq):
             NF.flash_attention(q, k, k, bias, causal=True, window=window)
     with pytest.raises(RuntimeError, match="one device"):
         NF.flash_attention(q, k.to("cuda:1"), k, None, causal=True, window=64)
+
+
+@pytest.mark.parametrize("sq,sk", [(300, 300), (1, 300)])
+def test_the_lowest_value_of_a_16bit_mask(sq, sk):
+    """-65504 of an fp16 mask hides a key as -inf does, in all entries."""
+    q, k, v, do = _tensors(3, sq, sk, 2, 64, torch.float16, seed=4)
+    at = torch.arange(sk, device="cuda")
+    pad = torch.stack([at >= sk - 120, at < sk // 2, at >= 0])
+    low, inf = (torch.zeros(3, sk, device="cuda", dtype=t).masked_fill(pad, x)
+                for t, x in ((torch.float16, -65504.0), (torch.float32, -math.inf)))
+    got = _run(q, k, v, do, 33, 2, low)
+    for a, b in zip(got, _run(q, k, v, do, 33, 2, inf)):
+        assert torch.equal(a, b)
+    _check(got, q, k, v, do, 33, 2, inf)
+    assert bool((got[0][2] == 0).all())
+    if sq == sk:
+        qkv = torch.stack((q, k, v), 3).detach()
+        assert torch.equal(flash_attention_qkvpacked(qkv, low, True, window=33, sinks=2), got[0])
