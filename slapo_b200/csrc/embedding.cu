@@ -1,5 +1,5 @@
 // Token table: lookup with scaling, and its gradient by sorted tokens.
-//   out[t] = scale W[id_t]          dW[v] = scale sum of dY[t] over the tokens t with id_t = v, in their order
+//   out[t] = scale W[id_t]          dW[v] = scale sum of dY[t] over the tokens t with id_t = v
 // Ids outside of the table's rows [0, V) (of a shard: the other ranks' tokens) give rows of zeros and no gradient.
 //
 // The gradient of a table has few rows that anything is added to, some of them (frequent tokens, a padding id)
@@ -7,8 +7,8 @@
 // their order would change the result from run to run.  Here tokens are sorted by id (a stable radix sort, so that
 // a row's tokens stay in their order) and each warp adds up eight tokens in sorted order, all of their rows of dY on
 // their way at once whichever rows they belong to: a row of one token and one of thousands cost the same per token.
-// What belongs to one row is joined over a CTA's eight warps, and over CTAs by a second kernel, in order, so that the
-// result is the same every time.
+// What belongs to one row is joined over a CTA's eight warps, and over CTAs by a second kernel (an eighth of a row's
+// stretches to a warp), each time in order, so that the result is the same every time.
 //
 // Sorting is latency, not bytes: one cluster of up to eight CTAs does it, with digits of eight bits; per pass each
 // warp counts the digits of its stretch (match.any: equal digits of 32 tokens at a time), offsets are added up over

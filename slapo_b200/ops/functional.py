@@ -155,8 +155,8 @@ def embedding(ids, weight, padding_idx=None, scale: float = 1.0, vocab_start: in
 
     Ids outside of ``[vocab_start, vocab_start + rows)`` give zeros and no gradient, so that a shard of a
     table takes the ids of all (no id is an error).  Tokens with id ``padding_idx`` have no gradient.  The
-    gradient of a row is summed in fp32 in the order of its tokens and rounded once, the same every time
-    (of at most 2^31 - 8192 ids at a time)."""
+    gradient of a row is summed in fp32, its tokens eight at a time and those sums in order, and rounded once:
+    the same every time (of at most 2^31 - 8192 ids at a time)."""
     if torch.is_tensor(weight) and weight.is_cuda:
         fn = native.direct("embedding")
         out = None if fn is None else fn(ids, weight, vocab_start, padding_idx, scale)
