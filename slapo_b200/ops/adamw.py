@@ -78,7 +78,8 @@ def multi_tensor_adamw(params, grads, exp_avgs, exp_avg_sqs, *, lr, betas=(0.9, 
     ``step`` counts from 1; a one-element int64 CUDA tensor is read by the kernel, so that a captured step
     goes on counting.  ``grad_scale``: one fp32 value on the device.  Gradients must be finite (a NaN stays in
     its place).  On the GPU a second moment below 2^-126 counts as zero in 8 bits, and ``eps`` must be at least
-    2^-63 / sqrt(1 - b2) with them (3.4e-18 for 0.999); with 32 bits it may be 0."""
+    2^-63 / sqrt(1 - b2) with them (3.4e-18 for 0.999); with 32 bits it may be 0.  Autograd notices there that
+    parameters and masters have changed, not that moments have."""
     params, grads = list(params), list(grads)
     n = len(params)
     lrs, decays = _per_tensor(lr, n, "lr"), _per_tensor(weight_decay, n, "weight_decay")

@@ -450,19 +450,12 @@ def test_a_step_that_counts_on_the_host_is_not_captured(steps):
     assert opt.state[w]["step"] == steps + 1
 
 
-@pytest.mark.parametrize("which", ["params", "masters", "exp_avgs", "exp_avg_sqs", "exp_avg_scales",
-                                   "exp_avg_sq_scales", "grads"])
-def test_what_a_step_changes_is_noticed(which):
-    """Autograd refuses a backward that has saved what a step has written; gradients are only read."""
+@pytest.mark.parametrize("which", ["params", "masters", "grads"])
+def test_weights_that_a_step_changes_are_noticed(which):
+    """Autograd refuses a backward that has saved weights which a step has written; gradients are only read."""
     t = _tensors([300, 40], torch.bfloat16, 8, True)
     x = t[which][1]
-    a = torch.ones_like(x, dtype=torch.float32, requires_grad=True)
-    if x.dtype == torch.float8_e4m3fn:
-        version = x._version
-        multi_tensor_adamw(**t, lr=1e-3, step=1)
-        assert x._version > version
-        return
-    loss = (a * x).sum()
+    loss = (torch.ones_like(x, requires_grad=True) * x).sum()
     multi_tensor_adamw(**t, lr=1e-3, step=1)
     if which == "grads":
         loss.backward()
