@@ -1314,8 +1314,7 @@ int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, uint8
   p.rest = window > 0 ? rest : nullptr;
   p.B = B; p.H = H; p.Sq = Sq; p.Sk = Sk; p.Dr = D; p.O = o; p.lse = lse; p.kbias = kbias; p.rel = rel;
   p.k_steps = (D + 15) / 16;
-  // (row tiles of a window differ little)
-  p.walk.set((Sq + kBlockM - 1) / kBlockM, 0, B * H, causal && window == 0 ? 2 : 0);
+  p.walk.set((Sq + kBlockM - 1) / kBlockM, 0, B * H, causal ? 2 : 0);
   p.splits = scratch != nullptr ? flash_fwd_splits(B, H, Sq, Sk, D, window, sinks) : 1;
   const int key_tiles = window > 0 ? fwd_window_tiles(Sq, Sk, window, sinks) : (Sk + kBlockN - 1) / kBlockN;
   p.tiles_per_split = (key_tiles + p.splits - 1) / p.splits;

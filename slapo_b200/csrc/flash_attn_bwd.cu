@@ -1390,10 +1390,8 @@ int launch_flash_bwd(const void* q, const void* k, const void* v, const void* o,
   pk.out2 = dv; pk.row_stride2 = dkv_row_stride;
   for (int at = 0; at < bh; at += plan.pairs) {
     const int pairs = bh - at < plan.pairs ? bh - at : plan.pairs;
-    // (with a window row tiles differ little, but for the keys of sinks, which all queries see)
-    pq.walk.set(p.Rq / 128, at, pairs, causal && window == 0 ? 2 : 0);
-    pk.walk.set(p.Rk / 128 + (pk.splits > 1 ? pk.sink_tiles * (pk.splits - 1) : 0), at, pairs,
-                causal && (window == 0 || sinks > 0) ? 1 : 0);
+    pq.walk.set(p.Rq / 128, at, pairs, causal ? 2 : 0);
+    pk.walk.set(p.Rk / 128 + (pk.splits > 1 ? pk.sink_tiles * (pk.splits - 1) : 0), at, pairs, causal ? 1 : 0);
 #define FLASH_BWD_CASE(T_)                                                                          \
   p.thr7 != 0 ? launch_typed<true, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)       \
               : launch_typed<false, T_>(tq, tk, tv, tdo, pq, pk, plan.q_ctas, general, stream)
