@@ -30,14 +30,17 @@ const float* opt_f32(const optional<Tensor>& t, const char* name, const Tensor& 
   return t->data_ptr<float>();
 }
 
-// `window` keys up to a query's own and the first `sinks`; window 0: no such limit
-std::pair<int, int> check_window(int64_t window, int64_t sinks, bool causal, const optional<Tensor>& rel) {
+// `window` keys up to a query's own and the first `sinks`; window 0: no such limit, nor where both reach over all `keys`
+// and there is no key bias (one of less than -1e30 counts differently with a window)
+std::pair<int, int> check_window(int64_t window, int64_t sinks, bool causal, const optional<Tensor>& rel,
+                                 const optional<Tensor>& kbias, int64_t keys) {
   TORCH_CHECK(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0),
               "a window of one key and more, and no negative number of sinks required");
   TORCH_CHECK(window == 0 || (causal && !(rel.has_value() && rel->defined())),
               "a window needs causal attention without a relative bias");
   // (a number that no length reaches, so that sums with positions fit)
   const int64_t most = int64_t(1) << 30;
+  if (std::min(window, most) + std::min(sinks, most) >= keys && !(kbias.has_value() && kbias->defined())) return {0, 0};
   return {static_cast<int>(std::min(window, most)), static_cast<int>(std::min(sinks, most))};
 }
 
@@ -57,7 +60,7 @@ std::tuple<Tensor, Tensor, Tensor> run_flash_fwd(const Tensor& q, const Tensor& 
   TORCH_CHECK(k.size(0) == B && k.size(2) == H && k.size(3) == D && v.sizes() == k.sizes());
   if (kbias.has_value() && kbias->defined()) TORCH_CHECK(kbias->numel() == (int64_t)B * Sk);
   if (rel.has_value() && rel->defined()) TORCH_CHECK(rel->numel() == (int64_t)H * (Sq + Sk - 1));
-  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel);
+  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel, kbias, Sk);
   Tensor o = at::empty({B, Sq, H, D}, q.options());
   Tensor lse = at::empty({B, H, Sq}, q.options().dtype(at::kFloat));
   const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)};
@@ -136,7 +139,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> flash_attn_bwd(
   }
   const bool has_bias = kbias.has_value() && kbias->defined();
   const bool has_rel = rel.has_value() && rel->defined();
-  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel);
+  const auto [window, sinks] = check_window(window_in, sinks_in, causal, rel, kbias, Sk);
   const slapo::FlashBwdPlan plan =
       slapo::flash_bwd_plan(B, H, Sq, Sk, D, packed_qkv, causal, window, sinks, has_bias, has_rel,
                             static_cast<float>(p_drop), keep_words);

@@ -517,3 +517,22 @@ def test_the_lowest_value_of_a_16bit_mask(sq, sk):
     if sq == sk:
         qkv = torch.stack((q, k, v), 3).detach()
         assert torch.equal(flash_attention_qkvpacked(qkv, low, True, window=33, sinks=2), got[0])
+
+
+@pytest.mark.parametrize("sq,sk", [(1, 700), (60, 700), (700, 700), (300, 130), (200, 1)])
+@pytest.mark.parametrize("window,sinks", [(700, 0), (650, 50), (1, 699), (900, 900)])
+def test_what_reaches_over_all_keys_is_no_window(sq, sk, window, sinks):
+    """Output and gradients to the bit, queries before all keys (zeros) among them; and with a bias, whose
+    masked keys then count as with a window, rows of nothing but such keys are zeros."""
+    q, k, v, do = _tensors(2, sq, sk, 2, 64, torch.bfloat16, seed=sq)
+    out = NF.flash_attention(q, k, v, causal=True)
+    want = [out, *torch.autograd.grad(out, (q, k, v), do)]
+    got = _run(q, k, v, do, window, sinks)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    _check(got, q, k, v, do, window, sinks)
+    bias = torch.zeros(2, sk, device="cuda")
+    bias[1] = torch.finfo(torch.float32).min
+    got = _run(q, k, v, do, window, sinks, bias)
+    _check(got, q, k, v, do, window, sinks, bias)
+    assert bool((got[0][1] == 0).all()) and all(bool((g[1] == 0).all()) for g in got[1:])
