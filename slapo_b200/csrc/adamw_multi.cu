@@ -17,7 +17,7 @@
 // Bound by memory: 28 bytes per element with 16-bit weights, 32-bit masters and moments, 16 with 8-bit moments,
 // 10 without masters; with 8-bit moments by instructions too, some 45 per element (a scheduler's slots are three
 // quarters full at 10 bytes).
-// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 820 us (96 % of the copy
+// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 830 us (94 - 96 % of the copy
 // rate), 8-bit moments 490 - 499 us (90 - 92 %); 304 M elements, 8-bit, no masters: 560 - 588 us (80 - 84 %), from box to box.
 #include <cuda_fp8.h>
 
