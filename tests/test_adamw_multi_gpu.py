@@ -462,3 +462,23 @@ def test_weights_that_a_step_changes_are_noticed(which):
     else:
         with pytest.raises(RuntimeError, match="modified by an inplace"):
             loss.backward()
+
+
+@pytest.mark.parametrize("dtype,master", [(torch.bfloat16, True), (torch.float16, False), (torch.float32, False)])
+def test_8bit_moments_of_more_than_the_resident_warps_take(dtype, master):
+    """Every warp has several units, of several tensors, in one sweep and in more: first moments to the bit,
+    weights to some roundings of 2^-23 of an update, as the plain form; the rest of a tensor's memory is left."""
+    sizes = [3_000_001, 77, 2_500_000, 511, 4_000_003]
+    t = _tensors(sizes, dtype, 8, master, seed=7)
+    r = _copy(t)
+    multi_tensor_adamw(**t, lr=1e-3, step=2)
+    for i in range(len(sizes)):
+        _reference_step(r["params"][i], r["grads"][i], r["masters"][i] if master else None, r["exp_avgs"][i],
+                        r["exp_avg_sqs"][i], r["exp_avg_scales"][i], r["exp_avg_sq_scales"][i], 1e-3, 0.01,
+                        (0.9, 0.999), 1e-8, 2, None)
+        assert torch.equal(t["exp_avgs"][i].view(torch.uint8), r["exp_avgs"][i].view(torch.uint8))
+        assert torch.equal(t["exp_avg_scales"][i], r["exp_avg_scales"][i])
+        w, want = (x["masters" if master else "params"][i].float() for x in (t, r))
+        # (an update is at most some 30 lr, off by 2^-19 of it; what a type has in between goes up or down)
+        step = 0.0 if master or dtype == torch.float32 else 2 * HALF[dtype]
+        assert bool(((w - want).abs() <= want.abs() * (step + 2.0 ** -22) + 30e-3 * 2.0 ** -19).all())
