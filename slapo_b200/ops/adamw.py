@@ -202,7 +202,8 @@ class FusedAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, grad_scale=None):
         """One update of every parameter that has a gradient.  What a refused step has not updated keeps its
-        state and its number of steps."""
+        state, and its number of steps, unless that is counted on the device together with something that was
+        updated."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
