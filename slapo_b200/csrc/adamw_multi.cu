@@ -17,7 +17,7 @@
 // Bound by memory: 28 bytes per element with 16-bit weights, 32-bit masters and moments, 16 with 8-bit moments,
 // 10 without masters; with 8-bit moments by instructions too, some 45 per element (a scheduler's slots are three
 // quarters full at 10 bytes).
-// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 830 us (94 - 96 % of the copy
+// Measured: 183 M elements, 12 layers of 1024: 32-bit moments and masters 812 - 820 us (96 % of the copy
 // rate), 8-bit moments 490 - 499 us (90 - 92 %); 304 M elements, 8-bit, no masters: 560 - 588 us (80 - 84 %), from box to box.
 #include <cuda_fp8.h>
 
@@ -199,21 +199,25 @@ __device__ __noinline__ void gather_unit(const AdamwTensor& t, int unit, AdamSta
     to.scale[lane / kAdamUnit][lane % kAdamUnit] = (lane < kAdamUnit ? t.m_scale : t.v_scale)[block];
 }
 
-// The divisions and roots of the two kernels.  With 32-bit moments the arithmetic has time under the bytes: rounded
-// correctly, denormals and all, so that eps may be as small as one likes, 0 included.  With 8-bit moments instructions
-// count: the special-function unit's, for which a second moment below 2^-126 is zero and the divisor never
-// that small (the caller has looked at eps).
+// The quotients and roots of the two kernels.  With 32-bit moments denormals count, so that eps may be as small as one likes,
+// 0 included; both are within two units in the last place.  (Rounded correctly they cost 1 % of the time: 823 us for
+// 815.)  With 8-bit moments instructions count: a second moment below 2^-126 is zero and the divisor never that small (the
+// caller has looked at eps).
 template <bool k8> __device__ __forceinline__ float square_root(float x) {
-  if constexpr (!k8) return __fsqrt_rn(x);
   float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  if constexpr (k8) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 template <bool k8> __device__ __forceinline__ float quotient(float x, float y) {
-  if constexpr (!k8) return __fdiv_rn(x, y);
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
-  return x * r;
+  if constexpr (k8) {
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    r *= x;
+  } else {
+    asm("div.full.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  }
+  return r;
 }
 
 // What does not change over a launch
