@@ -1,6 +1,6 @@
 // Differentiable front ends of the kernels: the autograd nodes of linear, bias + activation,
-// bias + dropout + residual, the normalisations, flash attention, T5's relative bias and the token
-// table's lookup, as C++ functions.
+// bias + dropout + residual, the normalisations, flash attention, T5's relative bias, the token
+// table's lookup and the rotation by positions, as C++ functions.
 //
 // A layer of a small model is a few kernels of some microseconds each; a Python autograd function
 // costs about 30 us per direction on the host (argument packing, the interpreter, one operator
@@ -484,6 +484,46 @@ tensor_list EmbeddingFn::backward(AutogradContext* ctx, tensor_list grads) {
   return {wants_node({&grads[0]}) ? EmbeddingSumFn::apply(grads[0], ids, at) : at.sum(ids, grads[0]), Tensor(), Tensor()};
 }
 
+// Rotation by positions, and the transposed rotation: linear maps, each the other's derivative (of any order).
+struct RotaryFn : public Function<RotaryFn> {
+  static std::tuple<Tensor, Tensor> turn(const Tensor& q, const optional<Tensor>& k, const Tensor& table,
+                                         const optional<Tensor>& positions, int64_t start, bool interleaved, bool transposed) {
+    static auto f = op<std::tuple<Tensor, Tensor>(const Tensor&, const optional<Tensor>&, const Tensor&, const optional<Tensor>&,
+                                                  int64_t, bool, bool)>("slapo_b200::rotary_fwd");
+    return f.call(q, k, table, positions, start, interleaved, transposed);
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const optional<Tensor>& k, const Tensor& table,
+                               const optional<Tensor>& positions, int64_t start, bool interleaved, bool transposed) {
+    ctx->save_for_backward({table, or_undefined(positions)});
+    ctx->saved_data["start"] = start;
+    ctx->saved_data["flags"] = std::vector<int64_t>{interleaved, transposed, k.has_value()};
+    auto [a, b] = turn(q, k, table, positions, start, interleaved, transposed);
+    if (!k.has_value()) return {a};
+    return {a, b};
+  }
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor& table = saved[0];
+    const optional<Tensor> positions = opt(saved[1]);
+    const int64_t start = ctx->saved_data["start"].toInt();
+    const auto flags = ctx->saved_data["flags"].toIntVector();
+    const bool interleaved = flags[0] != 0, transposed = flags[1] == 0, pair = flags[2] != 0;
+    tensor_list out(7);
+    const Tensor &dq = grads[0];
+    const optional<Tensor> dk = pair ? optional<Tensor>(grads[1]) : c10::nullopt;
+    if (wants_node({&dq, pair ? &grads[1] : &dq})) {
+      const variable_list got = apply(dq, dk, table, positions, start, interleaved, transposed);
+      out[0] = got[0];
+      if (pair) out[1] = got[1];
+      return out;
+    }
+    auto [a, b] = turn(dq, dk, table, positions, start, interleaved, transposed);
+    out[0] = a;
+    if (pair) out[1] = b;
+    return out;
+  }
+};
+
 // ------------------------------------------------------------------------ //
 // A bias that starts anywhere, as the kernels read it: 16 bytes at a time.  (A copy that is differentiated.)
 Tensor aligned(const Tensor& bias) {
@@ -554,6 +594,15 @@ Tensor embedding_sum(const Tensor& dy, const Tensor& ids, int64_t rows, int64_t 
   return wants_node({&dy}) ? EmbeddingSumFn::apply(dy, ids, at) : at.sum(ids, dy);
 }
 
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const optional<Tensor>& k, const Tensor& table,
+                                  const optional<Tensor>& positions, int64_t start, bool interleaved) {
+  const Tensor kk = or_undefined(k);
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && table.requires_grad()), "rotary: the table has no gradient");
+  if (!wants_node({&q, &kk, &table})) return RotaryFn::turn(q, k, table, positions, start, interleaved, false);
+  const variable_list r = RotaryFn::apply(q, k, table, positions, start, interleaved, false);
+  return {r[0], k.has_value() ? r[1] : at::empty({0}, q.options())};
+}
+
 Tensor rel_bias(const Tensor& table, const Tensor& buckets) { return RelBiasFn::apply(table, buckets); }
 
 }  // namespace
@@ -573,6 +622,9 @@ void register_autograd_ops(torch::Library& m) {
         []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::FlashEntry>(&flash)); });
   m.def("embedding_entry() -> int",
         []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::EmbeddingEntry>(&embedding)); });
+  m.def("rotary(Tensor q, Tensor? k, Tensor table, Tensor? positions, int start, bool interleaved) -> (Tensor, Tensor)", &rotary);
+  m.def("rotary_entry() -> int",
+        []() -> int64_t { return reinterpret_cast<int64_t>(static_cast<slapo::RotaryEntry>(&rotary)); });
   m.def("embedding(Tensor ids, Tensor weight, int start, int? padding, float scale) -> Tensor", &embedding);
   m.def("embedding_sum(Tensor dy, Tensor ids, int rows, int start, int? padding, float scale) -> Tensor", &embedding_sum);
   m.def("flash(Tensor q, Tensor? k, Tensor? v, Tensor? key_bias, Tensor? rel, bool causal, float scale, float p, int window=0, int sinks=0) -> Tensor",

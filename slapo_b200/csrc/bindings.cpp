@@ -301,6 +301,7 @@ void register_comm_ops(torch::Library& m);
 void register_loss_ops(torch::Library& m);
 void register_optim_ops(torch::Library& m);
 void register_embed_ops(torch::Library& m);
+void register_generate_ops(torch::Library& m);
 void register_autograd_ops(torch::Library& m);
 
 TORCH_LIBRARY(slapo_b200, m) {
@@ -331,5 +332,6 @@ TORCH_LIBRARY(slapo_b200, m) {
   register_loss_ops(m);
   register_optim_ops(m);
   register_embed_ops(m);
+  register_generate_ops(m);
   register_autograd_ops(m);
 }

@@ -213,11 +213,163 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// A CUDA tensor that the kernels take as it is; None is none.  False: for the dispatcher.
+bool on_device(PyObject* item, std::optional<at::Tensor>& to) {
+  if (item == Py_None) return true;
+  const at::Tensor* t = plain(item);
+  if (t == nullptr || !t->is_cuda()) return false;
+  to = *t;
+  return true;
+}
+bool flag(PyObject* item, bool& to) {
+  const int v = PyObject_IsTrue(item);
+  to = v > 0;
+  return v >= 0;
+}
+
+// rotary(entry, q, k, table, positions, interleaved) -> (q, k) - the packed projection and None where k is None - or None
+// where the kernels do not take it as it is.  positions: None, a number or a tensor.
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 6) {
+    PyErr_SetString(PyExc_TypeError, "rotary takes 6 arguments");
+    return nullptr;
+  }
+  const at::Tensor *q = plain(args[1]), *table = plain(args[3]);
+  std::optional<at::Tensor> k, positions;
+  if (q == nullptr || !q->is_cuda() || table == nullptr || watched() || !on_device(args[2], k)) Py_RETURN_NONE;
+  int64_t start = 0;
+  bool interleaved;
+  if (PyLong_CheckExact(args[4])) {
+    if (!count(args[4], start)) return nullptr;
+  } else if (!on_device(args[4], positions)) {
+    Py_RETURN_NONE;
+  }
+  const auto entry = reinterpret_cast<slapo::RotaryEntry>(PyLong_AsVoidPtr(args[0]));
+  if (!flag(args[5], interleaved) || PyErr_Occurred()) return nullptr;
+  std::tuple<at::Tensor, at::Tensor> out;
+  {
+    WithoutGil released;
+    out = entry(*q, k, *table, positions, start, interleaved);
+  }
+  PyObject* first = THPVariable_Wrap(std::move(std::get<0>(out)));
+  if (first == nullptr || !k.has_value()) return first == nullptr ? nullptr : Py_BuildValue("(NO)", first, Py_None);
+  PyObject* second = THPVariable_Wrap(std::move(std::get<1>(out)));
+  if (second == nullptr) {
+    Py_DECREF(first);
+    return nullptr;
+  }
+  return Py_BuildValue("(NN)", first, second);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(entry, pages, scales, k, v, block_table, lengths, counts, q, rotary_table, interleaved) -> the queries (or a
+// tensor of nothing), or None where the kernels do not take it as it is.  counts, q, rotary_table: or None.
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 11) {
+    PyErr_SetString(PyExc_TypeError, "paged_append takes 11 arguments");
+    return nullptr;
+  }
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i) {
+    t[i] = plain(args[1 + i]);
+    if (t[i] == nullptr || !t[i]->is_cuda()) Py_RETURN_NONE;
+  }
+  std::optional<at::Tensor> counts, q, rot;
+  if (watched() || !on_device(args[7], counts) || !on_device(args[8], q) || !on_device(args[9], rot)) Py_RETURN_NONE;
+  bool interleaved;
+  const auto entry = reinterpret_cast<slapo::PagedAppendEntry>(PyLong_AsVoidPtr(args[0]));
+  if (!flag(args[10], interleaved) || PyErr_Occurred()) return nullptr;
+  at::Tensor out;
+  {
+    WithoutGil released;
+    out = entry(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], counts, q, rot, interleaved);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(entry, q, pages, scales, block_table, lengths, counts, scale, window) -> output, or None where the
+// kernels do not take it as it is.  counts, scale, window: or None.
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 9) {
+    PyErr_SetString(PyExc_TypeError, "paged_attention takes 9 arguments");
+    return nullptr;
+  }
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i) {
+    t[i] = plain(args[1 + i]);
+    if (t[i] == nullptr || !t[i]->is_cuda()) Py_RETURN_NONE;
+  }
+  const auto type = t[0]->scalar_type();
+  std::optional<at::Tensor> counts;
+  if ((type != at::kBFloat16 && type != at::kHalf) || watched() || !on_device(args[6], counts)) Py_RETURN_NONE;
+  std::optional<double> scale;
+  if (args[7] != Py_None) scale = PyFloat_AsDouble(args[7]);
+  int64_t window;
+  const auto entry = reinterpret_cast<slapo::PagedAttentionEntry>(PyLong_AsVoidPtr(args[0]));
+  if (!count(args[8], window) || PyErr_Occurred()) return nullptr;
+  at::Tensor out;
+  {
+    WithoutGil released;
+    out = entry(*t[0], *t[1], *t[2], *t[3], *t[4], counts, scale, window);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A number, or a tensor of one for each row.  0: an error is set, -1: for the dispatcher.
+int setting(PyObject* item, slapo::Setting<double>& to) {
+  if (THPVariable_Check(item)) return on_device(item, to.rows) ? 1 : -1;
+  to.value = PyFloat_AsDouble(item);
+  return to.value == -1.0 && PyErr_Occurred() ? 0 : 1;
+}
+int setting(PyObject* item, slapo::Setting<int64_t>& to) {
+  if (THPVariable_Check(item)) return on_device(item, to.rows) ? 1 : -1;
+  to.value = PyLong_AsLongLong(item);
+  return to.value == -1 && PyErr_Occurred() ? 0 : 1;
+}
+
+// sample(entry, logits, uniform, temperature, top_k, top_p, min_p) -> tokens, or None where the kernels do not take it as
+// it is
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 7) {
+    PyErr_SetString(PyExc_TypeError, "sample takes 7 arguments");
+    return nullptr;
+  }
+  const at::Tensor *logits = plain(args[1]), *uniform = plain(args[2]);
+  if (logits == nullptr || !logits->is_cuda() || uniform == nullptr || !uniform->is_cuda() || watched()) Py_RETURN_NONE;
+  slapo::Setting<double> temperature{}, top_p{}, min_p{};
+  slapo::Setting<int64_t> top_k{};
+  int got = setting(args[3], temperature);
+  if (got > 0) got = setting(args[4], top_k);
+  if (got > 0) got = setting(args[5], top_p);
+  if (got > 0) got = setting(args[6], min_p);
+  if (got == 0) return nullptr;
+  if (got < 0) Py_RETURN_NONE;
+  const auto entry = reinterpret_cast<slapo::SampleEntry>(PyLong_AsVoidPtr(args[0]));
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor out;
+  {
+    WithoutGil released;
+    out = entry(*logits, *uniform, temperature, top_k, top_p, min_p);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define SLAPO_METHOD(NAME_, DOC_) \
   {#NAME_, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&NAME_)), METH_FASTCALL, DOC_}
 PyMethodDef methods[] = {SLAPO_METHOD(multi_adamw, "One AdamW step on lists of tensors (see slapo_b200.ops.adamw)."),
                          SLAPO_METHOD(flash, "Attention (see slapo_b200.ops.functional.flash_attention)."),
                          SLAPO_METHOD(embedding, "Rows of a table (see slapo_b200.ops.functional.embedding)."),
+                         SLAPO_METHOD(rotary, "Heads by their positions (see slapo_b200.ops.rotary)."),
+                         SLAPO_METHOD(paged_append, "Tokens into a cache (see slapo_b200.ops.paged)."),
+                         SLAPO_METHOD(paged_attention, "Attention over a cache (see slapo_b200.ops.paged)."),
+                         SLAPO_METHOD(sample, "Tokens from logits (see slapo_b200.ops.sampling)."),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_py", "Entry points for calls whose host time counts.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

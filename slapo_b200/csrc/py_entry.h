@@ -4,6 +4,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 
 #include <optional>
+#include <tuple>
 
 namespace slapo {
 
@@ -39,5 +40,25 @@ using FlashEntry = at::Tensor (*)(const at::Tensor&, const std::optional<at::Ten
                                   int64_t, int64_t);
 // ids, table, first row, padding id, scale
 using EmbeddingEntry = at::Tensor (*)(const at::Tensor&, const at::Tensor&, int64_t, const std::optional<int64_t>&, double);
+
+// q (or the packed projection), k, table, positions (or the first one), interleaved
+using RotaryEntry = std::tuple<at::Tensor, at::Tensor> (*)(const at::Tensor&, const std::optional<at::Tensor>&,
+                                                           const at::Tensor&, const std::optional<at::Tensor>&, int64_t, bool);
+// pages, scales, k, v, block table, lengths, counts, q, rotation's table, interleaved
+using PagedAppendEntry = at::Tensor (*)(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                        const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                                        const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, bool);
+// q, pages, scales, block table, lengths, counts, scale, window
+using PagedAttentionEntry = at::Tensor (*)(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                           const at::Tensor&, const std::optional<at::Tensor>&, std::optional<double>, int64_t);
+// A setting: one number, or one for each row
+template <typename N>
+struct Setting {
+  N value;
+  std::optional<at::Tensor> rows;
+};
+// logits, random numbers, temperature, top_k, top_p, min_p
+using SampleEntry = at::Tensor (*)(const at::Tensor&, const at::Tensor&, const Setting<double>&, const Setting<int64_t>&,
+                                   const Setting<double>&, const Setting<double>&);
 
 }  // namespace slapo

@@ -8,4 +8,7 @@ from .cross_entropy import ParallelCrossEntropy  # noqa: F401
 from .embedding import FusedEmbedding  # noqa: F401
 from .mlp import FusedMLP  # noqa: F401
 from .norm import FusedDropoutAddLayerNorm, FusedLayerNorm, FusedRMSNorm  # noqa: F401
+from .paged import PagedKVCache  # noqa: F401
+from .rotary import RotaryEmbedding, rotary_table  # noqa: F401
+from .sampling import sample  # noqa: F401
 from .utils import Print  # noqa: F401

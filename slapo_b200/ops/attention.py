@@ -21,6 +21,7 @@ import torch
 from torch import nn
 
 from . import functional as NF
+from .paged import PagedLayer
 
 _REFERENCE_NAMES = ("reference", "native_xformers", "native_flash_attn", "eager")
 
@@ -136,11 +137,18 @@ class FlashAttention(nn.Module):
     ``causal=None`` keeps the reference's convention (causal iff the block has
     an output projection, slapo/op/attention.py:428); pass it explicitly for
     anything else.  ``window`` and ``sinks`` limit what a token sees (``FlashAttentionOp``), in generation
-    over a cache as in training."""
+    over a cache as in training.
+
+    ``rotary`` (:class:`slapo_b200.ops.rotary.RotaryEmbedding`): queries and keys are rotated by the tokens'
+    positions, those of ``position_ids`` or the ones that follow the cache.
+
+    A cache in generation is a pair of tensors, or a layer of a :class:`slapo_b200.ops.paged.PagedKVCache` that
+    has made room for the tokens: keys and values go into its pages in 8 bits, and tokens attend over these (a
+    prompt's first ones over the keys and values as they are)."""
 
     def __init__(self, hidden_size, num_attention_heads, attn_pdrop=0.0, resid_pdrop=0.0,
                  attn_op_name="auto", bias=True, output_proj=True, fused_qkv=False,
-                 causal=None, scale=None, device=None, dtype=None, window=None, sinks=0):
+                 causal=None, scale=None, device=None, dtype=None, window=None, sinks=0, rotary=None):
         super().__init__()
         if hidden_size % num_attention_heads != 0:
             raise ValueError(f"hidden size {hidden_size} is not a multiple of "
@@ -163,6 +171,9 @@ class FlashAttention(nn.Module):
         self.attn_pdrop = attn_pdrop
         causal = output_proj if causal is None else causal
         self.attn_op = FlashAttentionOp(attn_op_name, causal, scale, window=window, sinks=sinks)
+        if rotary is not None and rotary.rotary_dim > self.head_size:
+            raise ValueError(f"{rotary.rotary_dim} rotated values of heads of {self.head_size}")
+        self.rotary = rotary
 
     @staticmethod
     def layout_qkv_from_separate(q, k, v, num_heads):
@@ -177,16 +188,21 @@ class FlashAttention(nn.Module):
 
     def forward(self, hidden_states, attention_mask=None, layer_past=None, head_mask=None,
                 encoder_hidden_states=None, encoder_attention_mask=None, use_cache=False,
-                output_attentions=False, past_key_value=None, **_ignored):
+                output_attentions=False, past_key_value=None, position_ids=None, **_ignored):
         if encoder_hidden_states is not None:
             raise NotImplementedError("cross attention is not supported by FlashAttention")
         if head_mask is not None or output_attentions:
             raise NotImplementedError("head_mask / output_attentions are not supported")
         past = layer_past if layer_past is not None else past_key_value
+        paged = isinstance(past, PagedLayer)
+        if paged:
+            self._check_paged(attention_mask, position_ids)
         if self.fused_qkv:
             qkv = self.qkv(hidden_states)
             qkv = qkv.view(qkv.shape[:-1] + (-1, 3, self.head_size))
             if past is None and not use_cache:
+                if self.rotary is not None:
+                    qkv = self.rotary.forward_packed(qkv, position_ids)
                 packed = self.attn_op.forward_packed(
                     qkv, attention_mask, self.attn_pdrop if self.training else 0.0)
                 if packed is not None:
@@ -195,15 +211,43 @@ class FlashAttention(nn.Module):
                         ctx = self.resid_dropout(self.out_proj(ctx))
                     return ctx, None
             q, k, v = qkv[..., 0, :], qkv[..., 1, :], qkv[..., 2, :]
+            turned = past is None and not use_cache
         else:
+            turned = False
             q = self.reshape_for_scores(self.query(hidden_states))
             k = self.reshape_for_scores(self.key(hidden_states))
             v = self.reshape_for_scores(self.value(hidden_states))
-        if past is not None:
-            k, v = NF.append_kv(past[0], past[1], k, v)
-        present = (k, v) if use_cache else None
-        ctx = self.attn_op(q, k, v, attention_mask, self.attn_pdrop if self.training else 0.0)
+        if paged:
+            ctx, present = self._paged(past, q, k, v), past
+        else:
+            if self.rotary is not None and not turned:
+                at = position_ids if position_ids is not None or past is None else past[0].shape[1]
+                q, k = self.rotary(q, k, at)
+            if past is not None:
+                k, v = NF.append_kv(past[0], past[1], k, v)
+            present = (k, v) if use_cache else None
+            ctx = self.attn_op(q, k, v, attention_mask, self.attn_pdrop if self.training else 0.0)
         ctx = ctx.reshape(ctx.shape[:-2] + (-1,))
         if self.output_proj:
             ctx = self.resid_dropout(self.out_proj(ctx))
         return ctx, present
+
+    def _check_paged(self, attention_mask, position_ids):
+        op = self.attn_op
+        if attention_mask is not None or position_ids is not None:
+            raise NotImplementedError("a paged cache knows its tokens by their lengths: no mask, no position_ids")
+        if not op.apply_causal_mask or op.sinks or op.rel_bias_table is not None:
+            raise NotImplementedError("a paged cache needs causal attention without sinks or a relative-position table")
+        if self.training and self.attn_pdrop > 0.0:
+            raise NotImplementedError("no dropout of attention over a paged cache: call eval()")
+
+    def _paged(self, past, q, k, v):
+        table, interleaved = (None, False) if self.rotary is None else (self.rotary.table(q.device),
+                                                                         self.rotary.interleaved)
+        if past.fresh:
+            if self.rotary is not None:
+                q, k = self.rotary(q, k)
+            past.append(k, v)
+            return self.attn_op(q, k, v)
+        q = past.append(k, v, q, table, interleaved)
+        return past.attend(q, self.attn_op.scale, self.attn_op.window)

@@ -407,3 +407,10 @@ def flash_attention(q, k, v, key_padding_bias=None, causal=False, scale=None, dr
     return attention_reference(q, k, v, key_padding_bias, causal, scale, dropout_p, training,
                                rel_bias_table, rel_bidirectional, rel_max_distance, window=window,
                                sinks=sinks)
+
+
+# ---------------------------------------------------------------------- #
+# positions and generation
+from .paged import paged_append, paged_attention  # noqa: E402,F401
+from .rotary import rotary, rotary_qkvpacked, rotary_table  # noqa: E402,F401
+from .sampling import sample  # noqa: E402,F401
