@@ -6,12 +6,14 @@
 
 namespace slapo {
 
-// Positions of tokens: start + s, or from memory (32 or 64 bits wide) where `ids` is set
+// Positions of tokens: start + s, from memory (32 or 64 bits wide) where `ids` is set, or those of a cache's new tokens
+// where `lengths` is: the first counts[b] (or all) of S end at lengths[b], others have none
 struct RotaryPositions {
   const void* ids;
   bool ids64;
   int64_t batch_stride, token_stride;      // elements
   int64_t start;
+  const int32_t *lengths, *counts;
 };
 // Heads [B, S, heads, D] that are turned, or copied, from x to y; strides in elements, D contiguous
 struct RotaryPart {

@@ -48,6 +48,22 @@ struct Turn8 {
       if (d < half) cs[j].y = -cs[j].y;
     }
   }
+  // from a token's entries in shared memory, `stride` float4 between those of a place (modes 1 and 3)
+  __device__ __forceinline__ void take(const float4* token, int stride) {
+    if (mode == 0) return;
+    const int place = (mode == 3 || d0 < half ? d0 : d0 - half) / 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (mode == 3 && q >= 2) break;
+      const float4 e = token[q * stride + place];
+      cs[2 * q] = make_float2(e.x, e.y);
+      cs[2 * q + 1] = make_float2(e.z, e.w);
+    }
+    if (mode == 1 && d0 < half) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j].y = -cs[j].y;
+    }
+  }
   // v: the values at d0 of the head `x`
   template <typename T>
   __device__ __forceinline__ void apply(const T* x, float (&v)[8]) const {
@@ -119,14 +135,29 @@ __device__ __forceinline__ void new_tokens(const PagedCache& c, int b, int64_t& 
   start = static_cast<int64_t>(c.lengths[b]) - count;
 }
 
+// Eight values as they are in memory
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const { Vec8<T>::load(reinterpret_cast<const T*>(w), v); }
+};
+
+// The heads [h0, h1) of a side of a page.  More than one row to a thread: the rotation's rows of the page's tokens go
+// through shared memory, in the order in which lanes read them (16 bytes of each of the places of a token side by side).
 template <typename T, int kRows>
-__device__ __forceinline__ void append_page(const PagedAppend& a, int64_t tile) {
+__device__ __forceinline__ void append_page(const PagedAppend& a, int64_t tile, int per_cta) {
   const PagedCache& c = a.cache;
-  __shared__ float s_top[kThreads / 32];
+  extern __shared__ __align__(16) float4 s_rot[];
+  __shared__ float s_top[2][kThreads / 32];
   const int side = static_cast<int>(tile & 1);
   tile >>= 1;
-  const int h = static_cast<int>(tile % c.heads);
-  tile /= c.heads;
+  const int groups = (c.heads + per_cta - 1) / per_cta;
+  const int h0 = static_cast<int>(tile % groups) * per_cta, h1 = min(c.heads, h0 + per_cta);
+  tile /= groups;
   const int spans = (c.n + c.page - 2) / c.page + 1;
   const int b = static_cast<int>(tile / spans);
   int64_t start;
@@ -143,65 +174,86 @@ __device__ __forceinline__ void append_page(const PagedAppend& a, int64_t tile) 
   const int places = c.pitch / 8, rows = kThreads / places;
   const int place = threadIdx.x % places, row = threadIdx.x / places;
   const int d0 = place * 8;
-  const bool real = d0 < c.dim, mine = row < rows;
+  const bool mine = row < rows, real = mine && d0 < c.dim;
   const int64_t* stride = side ? a.v_stride : a.k_stride;
-  const T* x = static_cast<const T*>(side ? a.v : a.k) + b * stride[0] + h * stride[2];
-  uint8_t* codes = c.pages + ((id * 2 + side) * c.heads + h) * static_cast<int64_t>(c.page) * c.pitch + d0;
-  float* scale_at = c.scales + (id * 2 + side) * c.heads + h;
-  const float old = held > 0 ? *scale_at : 0.f;
-  Turn8 turn(d0, side == 0 && a.rot != nullptr ? a.rotary : 0, a.interleaved);
+  const T* x = static_cast<const T*>(side ? a.v : a.k) + b * stride[0] + (first - start) * stride[1] + d0;
+  const int64_t head_bytes = static_cast<int64_t>(c.page) * c.pitch;
+  uint8_t* codes = c.pages + (id * 2 + side) * c.heads * head_bytes + d0;
+  float* scales = c.scales + (id * 2 + side) * c.heads;
+  const bool turned = side == 0 && a.rot != nullptr;
+  Turn8 turn(d0, turned ? a.rotary : 0, a.interleaved);
+  const int half = a.rotary / 2, units = half / 2;                // float4 of a token's rotation
+  const int parts = a.interleaved ? 2 : 4;                        // ... of a place
+  const bool shared = kRows > 1 && turned && half % (2 * parts) == 0;
+  if (shared) {
+    for (int i = threadIdx.x; i < (last - held) * units; i += kThreads) {
+      const int t = i / units, u = i - t * units;
+      const int64_t pos = first + held + t;
+      s_rot[t * units + (u % parts) * (units / parts) + u / parts] =
+          pos < a.rot_rows ? reinterpret_cast<const float4*>(a.rot)[pos * units + u] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
+  }
+  auto slot_of = [&](int i) { return held + row + i * rows; };
 
-  float v[kRows][8];
-  float top = 0.f;
+  Raw8<T> next[kRows];
+  auto fetch = [&](int h) {
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < kRows; ++i)
+      if (real && slot_of(i) < last) next[i].load(x + h * stride[2] + slot_of(i) * stride[1]);
+  };
+  fetch(h0);
+  for (int h = h0; h < h1; ++h) {
+    const float old = held > 0 ? scales[h] : 0.f;
+    float v[kRows][8];
+    float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    const int slot = held + row + i * rows;
-    if (!mine || !real || slot >= last) continue;
-    const int64_t pos = first + slot;
-    const T* xt = x + (pos - start) * stride[1];
-    Vec8<T>::load(xt + d0, v[i]);
-    if (side == 0 && a.rot != nullptr) {
-      if (pos < a.rot_rows) {
-        turn.read(a.rot, pos);
-        turn.apply(xt, v[i]);
-      } else {
+    for (int i = 0; i < kRows; ++i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      const int slot = slot_of(i);
+      if (!real || slot >= last) continue;
+      next[i].values(v[i]);
+      if (turned) {
+        if (first + slot < a.rot_rows) {
+          if (shared) turn.take(s_rot + (slot - held) * units, units / parts);
+          else if (kRows > 1 || h == h0) turn.read(a.rot, first + slot);
+          turn.apply(x + h * stride[2] + slot * stride[1] - d0, v[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float size = fabsf(v[i][j]);
+        if (size <= 3.402823466e38f) top = fmaxf(top, size);
       }
     }
+    if (h + 1 < h1) fetch(h + 1);
+    top = warp_max(top);
+    float* tops = s_top[h & 1];
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();      // (every thread has read the old scale, and is done with the tops of two heads before)
+    top = tops[0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x_abs = fabsf(v[i][j]);
-      if (x_abs <= 3.402823466e38f) top = fmaxf(top, x_abs);
-    }
-  }
-  top = warp_max(top);
-  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-  __syncthreads();      // (and every thread has read the old scale)
-  top = s_top[0];
+    for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, tops[w]);
+    const int e = scale_exponent(top);
+    const float need = power_of_two(e), scale = fmaxf(old, need);
+    const float factor = scale == need ? power_of_two(-e) : 1.f / scale;
+    if (threadIdx.x == 0) scales[h] = scale;
+    uint8_t* to = codes + h * head_bytes;
 #pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, s_top[w]);
-  const int e = scale_exponent(top);
-  const float need = power_of_two(e);
-  const float scale = fmaxf(old, need);
-  const float factor = scale == need ? power_of_two(-e) : 1.f / scale;
-  if (threadIdx.x == 0) *scale_at = scale;
-  if (!mine) return;
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int slot = held + row + i * rows;
-    if (slot >= last) break;
-    *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(slot) * c.pitch) = to_codes(v[i], factor);
-  }
-  if (held > 0 && scale != old) {
-    const float ratio = old * factor;
-    for (int slot = row; slot < held; slot += rows) {
-      uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(slot) * c.pitch);
-      float w[8];
-      from_codes(*at, w);
-      *at = to_codes(w, ratio);
+    for (int i = 0; i < kRows; ++i)
+      if (mine && slot_of(i) < last) *reinterpret_cast<uint2*>(to + slot_of(i) * c.pitch) = to_codes(v[i], factor);
+    if (held > 0 && scale != old && mine) {
+      const float ratio = old * factor;
+      for (int slot = row; slot < held; slot += rows) {
+        uint2* at = reinterpret_cast<uint2*>(to + slot * c.pitch);
+        float w[8];
+        from_codes(*at, w);
+        *at = to_codes(w, ratio);
+      }
     }
   }
 }
@@ -236,29 +288,80 @@ __device__ __forceinline__ void append_query(const PagedAppend& a, int64_t token
 }
 
 template <typename T, int kRows>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppend a, int64_t tiles) {
-  if (blockIdx.x < tiles) append_page<T, kRows>(a, blockIdx.x);
+__global__ void __launch_bounds__(kThreads, kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta) {
+  if (blockIdx.x < tiles) append_page<T, kRows>(a, blockIdx.x, per_cta);
   else append_query<T>(a, blockIdx.x - tiles);
 }
 
+template <typename T, int kRows>
+int launch_rows(const PagedAppend& a, int64_t tiles, int per_cta, unsigned grid, cudaStream_t stream) {
+  auto kernel = paged_append_kernel<T, kRows>;
+  int bytes = 0;
+  if (kRows > 1 && a.rot != nullptr) {
+    bytes = (a.cache.n < a.cache.page ? a.cache.n : a.cache.page) * a.rotary * 4;
+    if (bytes > 48 * 1024) {
+      int device = 0;
+      if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 3;
+      static bool configured[64] = {};
+      if (!configured[device]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024) != cudaSuccess) return 3;
+        configured[device] = true;
+      }
+    }
+  }
+  count_launch();
+  kernel<<<grid, kThreads, bytes, stream>>>(a, tiles, per_cta);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
 template <typename T>
-int launch(const PagedAppend& a, cudaStream_t stream) {
+int launch(const PagedAppend& a_in, cudaStream_t stream) {
+  PagedAppend a = a_in;
   const PagedCache& c = a.cache;
-  const int64_t spans = (c.n + c.page - 2) / c.page + 1;
-  const int64_t tiles = static_cast<int64_t>(c.B) * spans * c.heads * 2;
+  const int64_t spans = (c.n + c.page - 2) / c.page + 1, pages = c.B * spans * 2;
+  // Many tokens: their queries by the rotation's own kernel, which has more bytes on their way.  (Few: one launch.)
+  if (a.q != nullptr && a.rot != nullptr && static_cast<int64_t>(c.B) * c.n >= 4 * sm_count()) {
+    RotaryCall r{};
+    RotaryPart& p = r.part[0];
+    p.x = a.q;
+    p.y = a.q_out;
+    for (int d = 0; d < 3; ++d) p.x_stride[d] = a.q_stride[d];
+    p.y_stride[2] = c.dim;
+    p.y_stride[1] = static_cast<int64_t>(a.q_heads) * c.dim;
+    p.y_stride[0] = p.y_stride[1] * c.n;
+    p.heads = a.q_heads;
+    p.turn = true;
+    r.parts = 1;
+    r.table = a.rot;
+    r.table_rows = a.rot_rows;
+    r.at.lengths = c.lengths;
+    r.at.counts = c.counts;
+    r.B = c.B;
+    r.S = c.n;
+    r.D = c.dim;
+    r.rotary = a.rotary;
+    r.interleaved = a.interleaved;
+    r.dtype = a.dtype;
+    const int rc = launch_rotary(r, stream);
+    if (rc != 0) return rc;
+    a.q = nullptr;
+  }
+  // as many heads to a CTA as leave each SM some CTAs: they share the rotation's rows
+  int per_cta = 8;
+  while (per_cta > 1 && pages * ((c.heads + per_cta - 1) / per_cta) < 6 * sm_count()) per_cta /= 2;
+  const int64_t tiles = pages * ((c.heads + per_cta - 1) / per_cta);
   const int64_t ctas = tiles + (a.q != nullptr ? static_cast<int64_t>(c.B) * c.n : 0);
   if (ctas > 0x7fffffff) return 5;
+  if (ctas == 0) return 0;
   const unsigned grid = static_cast<unsigned>(ctas);
   const int rows = kThreads / (c.pitch / 8);
   const int most = c.n < c.page ? c.n : c.page;           // new tokens of a page
   const int per = (most + rows - 1) / rows;
-  count_launch();
-  if (per <= 1) paged_append_kernel<T, 1><<<grid, kThreads, 0, stream>>>(a, tiles);
-  else if (per <= 2) paged_append_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a, tiles);
-  else if (per <= 4) paged_append_kernel<T, 4><<<grid, kThreads, 0, stream>>>(a, tiles);
-  else if (per <= 8) paged_append_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a, tiles);
-  else return 6;
-  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  if (per <= 1) return launch_rows<T, 1>(a, tiles, per_cta, grid, stream);
+  if (per <= 2) return launch_rows<T, 2>(a, tiles, per_cta, grid, stream);
+  if (per <= 4) return launch_rows<T, 4>(a, tiles, per_cta, grid, stream);
+  if (per <= 8) return launch_rows<T, 8>(a, tiles, per_cta, grid, stream);
+  return 6;
 }
 
 }  // namespace

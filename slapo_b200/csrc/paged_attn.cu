@@ -3,20 +3,20 @@
 // Row r of a cached head is query t = r / G of query head r % G of its G; it sees the keys up to its own position (and
 // not before its window).  With codes k, v and a page's scales ks, vs: s = ks (q k) scale, o = sum p vs v / sum p.
 //
-// Bound by reading the cache.  A warp works alone, on units of 16 keys of one head: S^T = K Q^T by m16n8k16 (16 keys,
-// 8 rows), O^T += V^T P^T (16 values of a head, 8 rows), codes converted to fp16 - exactly - on their way into the
-// registers of the products.  The tensor core's order of the contraction is free as long as both operands share it, so
-// that a lane's 16 bytes of a key are its operands of four products, and 16 bytes each of four values' rows, bytes
-// interleaved, those of eight.  Lanes copy what they themselves read later, by cp.async, into a ring in shared memory: no
-// barriers, and bytes enough on their way.  mma.sync and not tcgen05: a unit has one to eight rows of work, and the
-// operands pass through registers, since they are converted.
+// Bound by reading the cache.  A warp works alone, on units of 32 keys of one head: S^T = K Q^T by m16n8k32 of e4m3 numbers
+// (16 keys, 8 rows), the keys' codes as they are and the queries taken apart into two or three, and O^T += V^T P^T by
+// m16n8k16 of fp16 (16 values of a head, 8 rows), codes converted - exactly - on their way into the registers.  The
+// tensor core's order of the contraction is free as long as both operands share it, so that a lane's 16 bytes of a key are its
+// operands of two products, and 16 bytes each of four values' rows, bytes interleaved, those of eight.  Units come by
+// cp.async, 512 bytes of a page side by side at a time (lanes that copied what they read themselves, 64 bytes of each of
+// eight tokens at a time, took 1.3 times as long), into a ring in shared memory of the warp's own: no barriers.  mma.sync and
+// not tcgen05: a unit has one to eight rows of work, and the values pass through registers, since they are converted.
 //
 // Keys are dealt out over all warps evenly, whatever the sequences' lengths, which are in device memory: each warp counts
 // the units of all sequences and takes its share of their row, at least kLeastUnits; it writes an item (sequence, head,
 // rows) that lies wholly in its share, and leaves its part of the first and the last else, which a second kernel adds up.
 //
-// Roundings: q to fp16 by a power of two per row (exact for bf16 values within 2^-28 of the row's largest, and for fp16's),
-// probabilities to fp16 (2^-11), all else in fp32.
+// Roundings: queries to 2^-22 of their row's largest value, probabilities to fp16 (2^-11), all else in fp32.
 #include <cuda_fp8.h>
 
 #include "flash_common.cuh"
@@ -26,59 +26,48 @@
 namespace slapo {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kUnit = 16;          // keys
-constexpr int kLeastUnits = 4;     // of a warp's share
+// Warps of a CTA by the tiles of 8 rows that each has
+constexpr int warps_of(int tiles) { return tiles == 1 ? 12 : 8; }
+constexpr int kUnit = 32;          // keys: two blocks of 16
+constexpr int kLeastUnits = 2;     // of a warp's share
 
 // What is known of the work before lengths are: the same in both kernels
 struct Plan {
   PagedAttention a;
   int group, rows, tiles, tile_rows, warps, words;     // tiles of rows per head; words: of a row's part
-  int page_units;                                      // log2 of a page's units
+  int page_blocks;                                     // log2 of a page's blocks of 16 keys
   float scale_log2;
 };
 
-__device__ __forceinline__ void keys_of(const PagedCache& c, int window, int b, int& first_unit, int& units, int& len,
-                                        int& count) {
-  count = c.counts != nullptr ? min(max(c.counts[b], 0), c.n) : c.n;
-  const int64_t most = static_cast<int64_t>(c.table_pages) * c.page;
-  len = c.lengths[b];
-  const int seen = static_cast<int>(min(static_cast<int64_t>(max(len, 0)), most));
-  const int64_t first = window > 0 ? static_cast<int64_t>(len) - count - window + 1 : 0;
-  first_unit = first > 0 ? static_cast<int>(min(first, most)) / kUnit : 0;
-  units = count > 0 ? max((seen + kUnit - 1) / kUnit - first_unit, 0) : 0;
-}
-
-// Sum of the units of all sequences' items, and (for one thread each of the warps) the sequence with the `at`-th one
-struct Shares {
-  int64_t total;       // units
-  int64_t per;         // of a warp
-  __device__ __forceinline__ int64_t begin(int warp) const { return min(warp * per, total); }
+// A sequence's units: those with a key that one of its rows sees
+struct Keys {
+  int len, count, first_unit, units;
 };
-__device__ __forceinline__ Shares count_units(const Plan& p) {
-  const PagedCache& c = p.a.cache;
-  int64_t sum = 0;
-  for (int b = threadIdx.x & 31; b < c.B; b += 32) {
-    int first, units, len, count;
-    keys_of(c, p.a.window, b, first, units, len, count);
-    sum += units;
-  }
+__device__ __forceinline__ Keys keys_of(const PagedCache& c, int window, int b) {
+  Keys k;
+  k.count = c.counts != nullptr ? min(max(c.counts[b], 0), c.n) : c.n;
+  const int64_t most = static_cast<int64_t>(c.table_pages) * c.page;
+  k.len = c.lengths[b];
+  const int seen = static_cast<int>(min(static_cast<int64_t>(max(k.len, 0)), most));
+  const int64_t first = window > 0 ? static_cast<int64_t>(k.len) - k.count - window + 1 : 0;
+  k.first_unit = first > 0 ? static_cast<int>(min(first, most)) / kUnit : 0;
+  k.units = k.count > 0 ? max((seen + kUnit - 1) / kUnit - k.first_unit, 0) : 0;
+  return k;
+}
+__device__ __forceinline__ int64_t warp_sum_long(int64_t v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  Shares s;
-  s.total = sum * c.heads * p.tiles;
-  const int64_t even = (s.total + p.warps - 1) / p.warps;
-  s.per = max(even, static_cast<int64_t>(kLeastUnits));
-  return s;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Units of a warp's share, of `units` per item and all sequences
+__device__ __forceinline__ int64_t share_of(const Plan& p, int64_t units) {
+  const int64_t total = units * p.a.cache.heads * p.tiles;
+  return max((total + p.warps - 1) / p.warps, static_cast<int64_t>(kLeastUnits));
 }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
   const int n = ok ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t to, const void* from, bool ok) {
-  const int n = ok ? 8 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool ok) {
   const int n = ok ? 4 : 0;
@@ -87,6 +76,9 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool ok) {
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void clear16(uint32_t at) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+}
 __device__ __forceinline__ uint4 read16(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
@@ -97,9 +89,9 @@ __device__ __forceinline__ uint2 read8(uint32_t at) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
   return v;
 }
-__device__ __forceinline__ float read4(uint32_t at) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+__device__ __forceinline__ float2 read8f(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
   return v;
 }
 
@@ -116,150 +108,225 @@ __device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// 16 x 8 from 32 e4m3 numbers each
+__device__ __forceinline__ void product8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
+// Queries are taken apart into e4m3 numbers: x = x0 + 2^-5 x1 + 2^-10 x2, each the rest of those before, rounded.  Of a
+// row whose largest value is 2^7 to 2^8, two are bf16's eight bits, and three fp16's eleven, but for values below 2^-22
+// (three: 2^-27) of the largest, which are off by no more than that.
+template <typename T> constexpr int kPartsOf = 3;
+template <> constexpr int kPartsOf<__nv_bfloat16> = 2;
+
 // kWide: heads of 72 to 128, whose tokens are 80 to 128 bytes; else up to 64.  N: tiles of 8 rows.
 template <bool kWide, int N, typename T>
 struct Shape {
   static constexpr int kChunks = kWide ? 2 : 1;                   // of 64 values of a key
-  static constexpr int kKey = kChunks * 2 * 16;                   // a lane's bytes of a unit
-  static constexpr int kValue = 4 * (kWide ? 16 : 8);
-  static constexpr int kStage = 32 * (kKey + kValue + 8);
-  static constexpr int kStages = kWide ? 6 : 10;
-  static constexpr int kSmem = kWarps * kStages * kStage;
+  static constexpr int kPieces = 4 * kChunks;                     // of 16 bytes of a token
+  static constexpr int kBlock = 16 * 16 * kPieces;                // a block's bytes of keys, or of values, in a warp's ring
+  static constexpr int kCopies = kPieces / 2;                     // ... of a lane, 16 each
+  static constexpr int kScales = 4 * kBlock;                      // where a unit's four scales are
+  static constexpr int kStage = kScales + 16;
+  static constexpr int kParts = kPartsOf<T>;
+  static constexpr int kWarps = warps_of(N);
+  static constexpr int kStages = kWide ? (N == 2 ? 3 : 2) : (N == 1 ? 4 : 5);
   static constexpr int kTiles = kWide ? 8 : 4;                    // of 16 values of a head
   static constexpr int kValues = kWide ? 16 : 8;                  // consecutive ones that a lane has
+  // the queries' operands: in registers for one tile or two, beside the ring for more
+  static constexpr bool kSharedQ = N > 2;
+  static constexpr int kQuery = kSharedQ ? N * kChunks * kParts * 512 : 0;
+  static constexpr int kWarp = kStages * kStage + kQuery;
+  static constexpr int kSmem = kWarps * kWarp;
+  // where a piece of a token lies in a block
+  static __device__ __forceinline__ uint32_t place(int row, int piece) {
+    const int order = kWide ? (((row >> 1) & 3) << 1) ^ ((row & 1) << 2) : (row >> 1) & 3;
+    return (row * kPieces + (piece ^ order)) * 16;
+  }
 };
 
 // A place in the row of all units
 struct Cursor {
-  int b, item, unit, units, first_unit, len, count;
+  int b, item, unit;
+  Keys keys;
 };
-__device__ __forceinline__ void sequence(const Plan& p, Cursor& at) {
-  while (at.b < p.a.cache.B) {
-    keys_of(p.a.cache, p.a.window, at.b, at.first_unit, at.units, at.len, at.count);
-    if (at.units > 0) return;
-    ++at.b;
-  }
-}
-// the `target`-th unit
-__device__ __forceinline__ Cursor find(const Plan& p, int64_t target) {
-  const PagedCache& c = p.a.cache;
-  const int lane = threadIdx.x & 31;
-  const int64_t items = static_cast<int64_t>(c.heads) * p.tiles;
-  Cursor at{};
-  int64_t before = 0;
-  for (int b0 = 0; b0 < c.B; b0 += 32) {
-    int first, units = 0, len, count;
-    if (b0 + lane < c.B) keys_of(c, p.a.window, b0 + lane, first, units, len, count);
-    int64_t sum = units * items;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, before + sum > target);
-    if (past != 0) {
-      const int l = __ffs(past) - 1;
-      at.b = b0 + l;
-      const int64_t until = __shfl_sync(0xffffffffu, sum, l) + before;
-      at.units = __shfl_sync(0xffffffffu, units, l);
-      keys_of(c, p.a.window, at.b, at.first_unit, at.units, at.len, at.count);
-      const int64_t in = target - (until - at.units * items);
-      at.item = static_cast<int>(in / at.units);
-      at.unit = static_cast<int>(in - static_cast<int64_t>(at.item) * at.units);
-      return at;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  at.b = c.B;
-  return at;
-}
 
 // what a warp leaves of the item that it begins with (0) or ends with (1): a row of `words` floats for each row of the tile
 __device__ __forceinline__ float* part_of(const Plan& p, int warp, int which, int row) {
   return p.a.scratch + ((static_cast<int64_t>(warp) * 2 + which) * p.tile_rows + row) * p.words;
 }
 
-template <bool kWide, int N, typename T>
-__global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const Plan p) {
+// This warp's first unit and how many it has.  All lanes count the sequences' units together.
+__device__ __forceinline__ int begin_share(const Plan& p, int number, Cursor& at) {
+  const PagedCache& c = p.a.cache;
+  const int lane = threadIdx.x & 31;
+  Keys mine{};                     // of sequence `lane`, where there are at most 32
+  int64_t sum = 0;
+  for (int b = lane; b < c.B; b += 32) {
+    mine = keys_of(c, p.a.window, b);
+    sum += mine.units;
+  }
+  const int64_t all = warp_sum_long(sum), items = static_cast<int64_t>(c.heads) * p.tiles, per = share_of(p, all);
+  const int64_t target = number * per;
+  if (target >= all * items) return 0;
+  int64_t before = 0;
+  for (int b0 = 0;; b0 += 32) {        // (ends: the target is before the end)
+    if (c.B > 32) mine = b0 + lane < c.B ? keys_of(c, p.a.window, b0 + lane) : Keys{};
+    int64_t until = mine.units * items;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, until, o);
+      if (lane >= o) until += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + until > target);
+    if (past == 0) {
+      before += __shfl_sync(0xffffffffu, until, 31);
+      continue;
+    }
+    const int l = __ffs(past) - 1;
+    at.b = b0 + l;
+    at.keys.len = __shfl_sync(0xffffffffu, mine.len, l);
+    at.keys.count = __shfl_sync(0xffffffffu, mine.count, l);
+    at.keys.first_unit = __shfl_sync(0xffffffffu, mine.first_unit, l);
+    at.keys.units = __shfl_sync(0xffffffffu, mine.units, l);
+    const int64_t in = target - (before + __shfl_sync(0xffffffffu, until, l) - at.keys.units * items);
+    at.item = static_cast<int>(in / at.keys.units);
+    at.unit = static_cast<int>(in - static_cast<int64_t>(at.item) * at.keys.units);
+    return static_cast<int>(min(per, all * items - target));
+  }
+}
+
+template <bool kWide, int N, bool kSmallPages, typename T>
+__global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(const Plan p) {
   using S = Shape<kWide, N, T>;
   extern __shared__ __align__(128) uint8_t s_ring[];
   const PagedCache& c = p.a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int number = blockIdx.x * kWarps + warp;
+  const int number = warp * gridDim.x + blockIdx.x;        // (few shares: one to an SM)
   pdl_launch();
-  const Shares shares = count_units(p);
-  const int64_t begin = shares.begin(number), end = shares.begin(number + 1);
-  if (begin >= end) return;
-  int left = static_cast<int>(end - begin), to_issue = left;
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) + warp * S::kStages * S::kStage;
-  const int64_t head_bytes = static_cast<int64_t>(c.page) * c.pitch;
+  Cursor at;
+  int left = begin_share(p, number, at);
+  if (left == 0) return;
+  int to_issue = left;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) + warp * S::kWarp;
+  const int head_bytes = c.page * c.pitch;
+  const int items = c.heads * p.tiles;
 
-  Cursor in = find(p, begin), at = in;
-  auto page_of = [&](const Cursor& x) {        // of the unit's keys; -1: none
-    if (x.b >= c.B) return -1;
-    const int id = c.table[static_cast<int64_t>(x.b) * c.table_pages + ((x.first_unit + x.unit) >> p.page_units)];
+  Cursor in = at;
+  auto step = [&](Cursor& x) {
+    if (++x.unit < x.keys.units) return;
+    x.unit = 0;
+    if (++x.item < items) return;
+    x.item = 0;
+    while (++x.b < c.B) {
+      x.keys = keys_of(c, p.a.window, x.b);
+      if (x.keys.units > 0) return;
+    }
+  };
+  // the pages of a unit's two blocks of keys; -1: none
+  auto page_of = [&](const Cursor& x, int block) {
+    const int number = ((x.keys.first_unit + x.unit) * 2 + block) >> p.page_blocks;
+    if (kSmallPages && number >= c.table_pages) return -1;         // (of an odd number of blocks)
+    const int id = __ldg(c.table + static_cast<int64_t>(x.b) * c.table_pages + number);
     return id >= 0 && id < c.n_pages ? id : -1;
   };
-  auto step = [&](Cursor& x) {
-    if (++x.unit < x.units) return;
-    x.unit = 0;
-    if (++x.item < c.heads * p.tiles) return;
-    x.item = 0;
-    ++x.b;
-    sequence(p, x);
-  };
-  int page = page_of(in);
-  unsigned missing = 0;        // the stages whose unit has no page
-  // the unit's codes and scales on their way into a stage; the next unit's page is read ahead
+  constexpr int kPages = kSmallPages ? 2 : 1;
+  int page[kPages];
+#pragma unroll
+  for (int i = 0; i < kPages; ++i) page[i] = page_of(in, i);
+  unsigned missing = 0;        // two bits for a stage: its blocks that have no page
+  // A block's 16 tokens lie side by side in a page: lanes copy 16 bytes side by side, to a row of 128 (64) bytes for each
+  // token, whose pieces are in an order of its own, so that neither reading of them meets a bank twice (narrow: values twice).
+  const int pieces = c.pitch / 16;
+  uint32_t place[S::kCopies];
+  int row_of[S::kCopies];
+#pragma unroll
+  for (int i = 0; i < S::kCopies; ++i) {
+    const int piece = i * 32 + lane;
+    row_of[i] = piece / pieces;        // 16 and more: none
+    place[i] = S::place(row_of[i], piece - row_of[i] * pieces);
+  }
+  // (what lies behind a head's width is zeros from here on: the operands reach to 64 or 128 values)
+  if (pieces < S::kPieces) {
+    for (int i = lane; i < 4 * S::kStages * 16 * (S::kPieces - pieces); i += 32) {
+      const int block = i / (16 * (S::kPieces - pieces)), in_block = i - block * 16 * (S::kPieces - pieces);
+      const int row = in_block / (S::kPieces - pieces), piece = pieces + in_block - row * (S::kPieces - pieces);
+      clear16(ring + block / 4 * S::kStage + block % 4 * S::kBlock + S::place(row, piece));
+    }
+    __syncwarp();
+  }
+  // the unit's codes and scales on their way into a stage; the next unit's pages are read ahead
   auto issue = [&](int stage) {
     if (to_issue > 0) {
       --to_issue;
-      const int key0 = (in.first_unit + in.unit) * kUnit, h = in.item / p.tiles;
-      const bool known = page >= 0;
-      missing = (missing & ~(1u << stage)) | (known ? 0u : 1u << stage);
-      const int64_t side = (static_cast<int64_t>(known ? page : 0) * 2) * c.heads + h;
-      const uint8_t* k = c.pages + side * head_bytes + static_cast<int64_t>(key0 & (c.page - 1)) * c.pitch;
-      const uint8_t* v = k + c.heads * head_bytes;
-      const uint32_t to = ring + stage * S::kStage + lane * 16;
+      const int key0 = (in.keys.first_unit + in.unit) * kUnit, h = p.tiles == 1 ? in.item : in.item / p.tiles;
+      const uint32_t to = ring + stage * S::kStage;
+      missing &= ~(3u << (2 * stage));
       // keys that no row sees are zeros: a hidden code may be a NaN
-      const int until = in.len - key0;
-      const int from = p.a.window > 0 ? in.len - in.count - p.a.window + 1 - key0 : 0;
+      const int until = in.keys.len - key0;
+      const int from = p.a.window > 0 ? in.keys.len - in.keys.count - p.a.window + 1 - key0 : 0;
+      const int64_t side_bytes = c.heads * static_cast<int64_t>(head_bytes);
+      const bool every = page[0] >= 0 && page[kPages - 1] >= 0 && until >= kUnit && from <= 0;
 #pragma unroll
-      for (int j = 0; j < S::kChunks; ++j)
+      for (int block = 0; block < 2; ++block) {
+        const int id = page[kSmallPages ? block : 0];
+        // (a page without a key that is seen may never have been written, its scales neither)
+        const bool known = every || (id >= 0 && (!kSmallPages || (until > 16 * block && from < 16 * block + 16)));
+        if (!known) missing |= 1u << (2 * stage + block);
+        const int64_t side = (static_cast<int64_t>(known ? id : 0) * 2) * c.heads + h;
+        const uint8_t* k = c.pages + side * head_bytes + (((key0 + 16 * block) & (c.page - 1)) * c.pitch + lane * 16);
+        const uint8_t* v = k + side_bytes;
+        const uint32_t k_to = to + 2 * block * S::kBlock, v_to = k_to + S::kBlock;
+        if (every) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = g + 8 * r, d = 64 * j + 16 * t;
-          const bool ok = known && key < until && key >= from && d < c.pitch;
-          copy16(to + (j * 2 + r) * 512, ok ? k + key * c.pitch + d : c.pages, ok);
+          for (int i = 0; i < S::kCopies; ++i) {
+            if (row_of[i] < 16) {
+              copy16(k_to + place[i], k + i * 512, true);
+              copy16(v_to + place[i], v + i * 512, true);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::kCopies; ++i) {
+            if (row_of[i] < 16) {
+              const int key = 16 * block + row_of[i];
+              const bool ok = known && key < until && key >= from;
+              copy16(k_to + place[i], ok ? k + i * 512 : c.pages, ok);
+              copy16(v_to + place[i], ok ? v + i * 512 : c.pages, ok);
+            }
+          }
         }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = 2 * t + (r & 1) + 8 * (r >> 1), d = S::kValues * g;
-        const bool ok = known && key < until && key >= from && d < c.pitch;
-        const uint8_t* src = ok ? v + key * c.pitch + d : c.pages;
-        if constexpr (kWide) copy16(to + 32 * S::kKey + r * 512, src, ok);
-        else copy8(ring + stage * S::kStage + 32 * S::kKey + r * 256 + lane * 8, src, ok);
+        // keys' and values' scale by one lane each
+        if (lane < 2 && (kSmallPages || block == 0))
+          copy4(to + S::kScales + 8 * block + 4 * lane, c.scales + side + lane * c.heads, known);
       }
-      const uint32_t scales = ring + stage * S::kStage + 32 * (S::kKey + S::kValue) + lane * 8;
-      copy4(scales, c.scales + side, known);
-      copy4(scales + 4, c.scales + side + c.heads, known);
       step(in);
-      if (to_issue > 0) page = page_of(in);
+      if (to_issue > 0) {
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) page[i] = page_of(in, i);
+      }
     }
     commit_copies();
   };
 #pragma unroll 1
   for (int i = 0; i < S::kStages - 1; ++i) issue(i);
 
-  uint32_t q[N][S::kChunks][4][2];
+  const uint32_t q_at = ring + S::kStages * S::kStage + lane * 16;
+  uint32_t q[S::kSharedQ ? 1 : N][S::kChunks][S::kParts][4];
   float factor[N][2], m[N][2], l[N][2], o[N][S::kTiles][4];
-  int last[N][2];                      // the last key that a row sees (or less than 0), and with a window
+  int last[N][2];                      // the last key that a row sees, less than 0: none
+  // where this lane's operands are in a block: of keys g and g + 8, of values' rows 2 t, 2 t + 1 and eight further
+  const uint32_t key_at[2] = {S::place(g, t), S::place(g, kWide ? 4 + t : t)};
+  const uint32_t value_at[2] = {S::place(2 * t, kWide ? g : g / 2) + (kWide ? 0 : 8 * (g & 1)),
+                                S::place(2 * t + 1, kWide ? g : g / 2) + (kWide ? 0 : 8 * (g & 1))};
   bool fresh = true;                   // an item begins here
   int begun = 0;                       // ... at this unit of it
   int stage = 0;
@@ -291,25 +358,42 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest value in [2^13, 2^14); what is not finite stays so
-        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 13, -100), 115);
+        // the row's largest value in [2^7, 2^8); what is not finite stays so
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 7, -100), 121);
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-        for (int j = 0; j < S::kChunks; ++j)
+        for (int j = 0; j < S::kChunks; ++j) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < 16; ++k) x[j][k] *= down;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const __half2 w = __floats2half2_rn(x[j][4 * k + 2 * half] * down, x[j][4 * k + 2 * half + 1] * down);
-              q[i][j][k][half] = *reinterpret_cast<const uint32_t*>(&w);
+          for (int part = 0; part < S::kParts; ++part) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(x[j][k], x[j][k + 1]), __NV_SATFINITE, __NV_E4M3);
+              const float2 held = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3)));
+              x[j][k] = (x[j][k] - held.x) * 32.f;
+              x[j][k + 1] = (x[j][k + 1] - held.y) * 32.f;
+              w[k / 4] = k % 4 == 0 ? pair : w[k / 4] | pair << 16;
             }
+            if constexpr (S::kSharedQ) {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + ((i * S::kChunks + j) * S::kParts + part) * 512),
+                           "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) q[i][j][part][y] = w[y];
+            }
+          }
+        }
         // the two rows whose scores this lane has
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * p.scale_log2;
+        // (an infinite query's row: NaN)
+        const float up = top <= 3.402823466e38f ? __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * p.scale_log2
+                                                : __uint_as_float(0x7fffffffu);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           factor[i][k] = __shfl_sync(0xffffffffu, up, (2 * t + k) * 4);
           const int r = row0 + i * 8 + 2 * t + k, tok = r / p.group;
-          last[i][k] = r < p.rows && tok < at.count ? at.len - at.count + tok : -1;
+          last[i][k] = r < p.rows && tok < at.keys.count ? at.keys.len - at.keys.count + tok : -1;
           m[i][k] = -INFINITY;
           l[i][k] = 0.f;
         }
@@ -321,95 +405,173 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
     }
 
     wait_copies<S::kStages - 2>();
-    const uint32_t base = ring + stage * S::kStage + lane * 16;
-    float s[N][4];
+    __syncwarp();                      // (what a lane reads others have copied)
+    const uint32_t base = ring + stage * S::kStage;
+    const unsigned gone = (missing >> (2 * stage)) & 3u;
+    float s[N][2][4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < S::kChunks; ++j) {
-      const uint4 k0 = read16(base + (j * 2) * 512), k1 = read16(base + (j * 2 + 1) * 512);
-      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+      for (int block = 0; block < 2; ++block) s[i][block][0] = s[i][block][1] = s[i][block][2] = s[i][block][3] = 0.f;
+    uint4 keys[2][2][S::kChunks];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint2 a = halves(w0[k]), b = halves(w1[k]);
+    for (int block = 0; block < 2; ++block)
 #pragma unroll
-        for (int i = 0; i < N; ++i) product(s[i], a.x, b.x, a.y, b.y, q[i][j][k][0], q[i][j][k][1]);
+      for (int j = 0; j < S::kChunks; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          keys[block][r][j] = read16(base + 2 * block * S::kBlock + r * 8 * 16 * S::kPieces + (j == 0 ? key_at[0] : key_at[1]));
+    // the queries' least part first: the sum of each part is multiplied on its way to the next
+#pragma unroll
+    for (int part = S::kParts - 1; part >= 0; --part) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kChunks; ++j) {
+          uint32_t w[4];
+          if constexpr (S::kSharedQ) {
+            const uint4 x = read16(q_at + ((i * S::kChunks + j) * S::kParts + part) * 512);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+          } else {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) w[y] = q[i][j][part][y];
+          }
+#pragma unroll
+          for (int block = 0; block < 2; ++block) {
+            const uint4 &a = keys[block][0][j], &b = keys[block][1][j];
+            product8(s[i][block], a.x, b.x, a.y, b.y, w[0], w[1]);
+            product8(s[i][block], a.z, b.z, a.w, b.w, w[2], w[3]);
+          }
+        }
+      if (part > 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int block = 0; block < 2; ++block)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) s[i][block][y] *= 0.03125f;
       }
     }
-    const uint32_t scales = ring + stage * S::kStage + 32 * (S::kKey + S::kValue) + lane * 8;
-    const float k_scale = read4(scales), v_scale = read4(scales + 4);
-    uint32_t w[4][S::kValues / 4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (kWide) {
-        const uint4 x = read16(base + 32 * S::kKey + r * 512);
-        w[r][0] = x.x; w[r][1] = x.y; w[r][2] = x.z; w[r][3] = x.w;
-      } else {
-        const uint2 x = read8(ring + stage * S::kStage + 32 * S::kKey + r * 256 + lane * 8);
-        w[r][0] = x.x; w[r][1] = x.y;
+    float k_scale[2], v_scale[2];
+    {
+      const float2 x = read8f(base + S::kScales);
+      k_scale[0] = k_scale[1] = x.x;
+      v_scale[0] = v_scale[1] = x.y;
+      if constexpr (kSmallPages) {
+        const float2 y = read8f(base + S::kScales + 8);
+        k_scale[1] = y.x;
+        v_scale[1] = y.y;
       }
     }
-    const bool no_page = (missing >> stage) & 1;
-    // (what the stage before held is in registers and used)
-    issue(stage == 0 ? S::kStages - 1 : stage - 1);
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
-    const int key0 = (at.first_unit + at.unit) * kUnit;
-    uint32_t pb[N][2];
+    const int key0 = (at.keys.first_unit + at.unit) * kUnit;
+    // whether every row sees all of the unit's keys
+    const bool all = gone == 0 && key0 + kUnit <= at.keys.len - at.keys.count + 1 &&
+                     (p.a.window == 0 || key0 > at.keys.len - 1 - p.a.window);
+    uint32_t pb[N][2][2];
+    bool grown = false;
+    float shrink[N][2];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float shrink[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float f = factor[i][k] * k_scale;
-        const int from = p.a.window > 0 ? last[i][k] - p.a.window : -1;
-        float x[2], top = m[i][k];
+        float x[4], top = m[i][k];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int key = key0 + g + 8 * r;
-          x[r] = key <= last[i][k] && key > from && !no_page ? s[i][2 * r + k] * f : -INFINITY;
-          top = fmaxf(top, x[r]);
+        for (int block = 0; block < 2; ++block)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) x[2 * block + r] = s[i][block][2 * r + k] * (factor[i][k] * k_scale[block]);
+        if (!all) {
+          const int from = p.a.window > 0 ? last[i][k] - p.a.window : -1;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int key = key0 + g + 8 * y;
+            if (!(key <= last[i][k] && key > from) || ((gone >> (y >> 1)) & 1u) != 0) x[y] = -INFINITY;
+          }
         }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) top = fmaxf(top, x[y]);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const float use = top == -INFINITY ? 0.f : top;
-        shrink[k] = exp2f(m[i][k] - use);
+        grown |= top > m[i][k];
+        shrink[i][k] = exp2f(m[i][k] - use);
         m[i][k] = top;
-        const float p0 = exp2f(x[0] - use), p1 = exp2f(x[1] - use);
-        l[i][k] = l[i][k] * shrink[k] + p0 + p1;
-        s[i][k] = p0;
-        s[i][2 + k] = p1;
+        float sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float e = exp2f(x[y] - use);
+          sum += e;
+          s[i][y >> 1][2 * (y & 1) + k] = e;
+        }
+        l[i][k] = l[i][k] * shrink[i][k] + sum;
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const __half2 h2 = __floats2half2_rn(s[i][2 * r], s[i][2 * r + 1]);
-        pb[i][r] = transposed(*reinterpret_cast<const uint32_t*>(&h2));
-      }
+      for (int block = 0; block < 2; ++block)
 #pragma unroll
-      for (int j = 0; j < S::kTiles; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][j][k] *= shrink[k & 1];
+        for (int r = 0; r < 2; ++r) {
+          const __half2 h2 = __floats2half2_rn(s[i][block][2 * r], s[i][block][2 * r + 1]);
+          pb[i][block][r] = transposed(*reinterpret_cast<const uint32_t*>(&h2));
+        }
     }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kTiles; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][j][k] *= shrink[i][k & 1];
+    }
+    uint32_t w[2][4][S::kValues / 4];
+#pragma unroll
+    for (int block = 0; block < 2; ++block)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // (rows 2 t and 2 t + 1, and eight further)
+        const uint32_t v_from = base + (2 * block + 1) * S::kBlock + (r >> 1) * 8 * 16 * S::kPieces + value_at[r & 1];
+        if constexpr (kWide) {
+          const uint4 x = read16(v_from);
+          w[block][r][0] = x.x; w[block][r][1] = x.y; w[block][r][2] = x.z; w[block][r][3] = x.w;
+        } else {
+          const uint2 x = read8(v_from);
+          w[block][r][0] = x.x; w[block][r][1] = x.y;
+        }
+      }
+    __syncwarp();                      // (all lanes have read the stage before)
+    issue(stage == 0 ? S::kStages - 1 : stage - 1);
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
 #pragma unroll
     for (int j = 0; j < S::kTiles / 2; ++j) {
       // values 4 j .. 4 j + 3 of this lane's, of keys 2 t, 2 t + 1 and eight further
-      const uint2 a = halves(bytes(w[0][j], w[1][j], 0x5140)), b = halves(bytes(w[2][j], w[3][j], 0x5140));
-      const uint2 e = halves(bytes(w[0][j], w[1][j], 0x7362)), f = halves(bytes(w[2][j], w[3][j], 0x7362));
+      uint2 a[2], b[2], e[2], f[2];
+#pragma unroll
+      for (int block = 0; block < 2; ++block) {
+        const auto& x = w[block];
+        a[block] = halves(bytes(x[0][j], x[1][j], 0x5140));
+        b[block] = halves(bytes(x[2][j], x[3][j], 0x5140));
+        e[block] = halves(bytes(x[0][j], x[1][j], 0x7362));
+        f[block] = halves(bytes(x[2][j], x[3][j], 0x7362));
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-        product(x, a.x, a.y, b.x, b.y, pb[i][0], pb[i][1]);
-        product(y, e.x, e.y, f.x, f.y, pb[i][0], pb[i][1]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          o[i][2 * j][k] = fmaf(x[k], v_scale, o[i][2 * j][k]);
-          o[i][2 * j + 1][k] = fmaf(y[k], v_scale, o[i][2 * j + 1][k]);
+        for (int block = 0; block < 2; ++block) {
+          product(x, a[block].x, a[block].y, b[block].x, b[block].y, pb[i][block][0], pb[i][block][1]);
+          product(y, e[block].x, e[block].y, f[block].x, f[block].y, pb[i][block][0], pb[i][block][1]);
+          if (kSmallPages || block == 1) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              o[i][2 * j][k] = fmaf(x[k], v_scale[block], o[i][2 * j][k]);
+              o[i][2 * j + 1][k] = fmaf(y[k], v_scale[block], o[i][2 * j + 1][k]);
+              x[k] = y[k] = 0.f;
+            }
+          }
         }
       }
     }
 
     --left;
-    const bool complete = at.unit + 1 == at.units;
+    const bool complete = at.unit + 1 == at.keys.units;
     if (complete || left == 0) {
       const int h = at.item / p.tiles, row0 = (at.item - h * p.tiles) * 8 * N;
       const bool whole = complete && begun == 0;
@@ -422,7 +584,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
           for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
           const int in_tile = i * 8 + 2 * t + k, row = row0 + in_tile;
           if (row >= p.rows) continue;
-          const float scale = whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
+          const bool none = last[i][k] < 0;         // (masks are not applied where all rows see all keys)
+          const float scale = none ? 0.f : whole ? (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)) : 1.f;
           float* part = part_of(p, number, begun == 0 ? 1 : 0, in_tile);
           const int token = row / p.group;
           T* out = static_cast<T*>(p.a.out) +
@@ -432,14 +595,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
             const int d = S::kValues * g + 8 * j;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = o[i][4 * j + e / 2][2 * (e & 1) + k] * scale;
+            for (int e = 0; e < 8; ++e) x[e] = none ? 0.f : o[i][4 * j + e / 2][2 * (e & 1) + k] * scale;
             if (d >= c.dim) continue;
             if (whole) Vec8<T>::store(out + d, x);
             else Vec8<float>::store(part + d, x);
           }
           if (!whole && g == 0) {
-            part[c.dim] = m[i][k];
-            part[c.dim + 1] = sum;
+            part[c.dim] = none ? -INFINITY : m[i][k];
+            part[c.dim + 1] = none ? 0.f : sum;
           }
         }
       fresh = true;
@@ -448,76 +611,73 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
   }
 }
 
-// An item's parts added up, where more than one warp had it; zeros where none had
+// A row's parts added up, where more than one warp had its item; zeros where none had
 template <typename T>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const Plan p) {
+__global__ void __launch_bounds__(256) paged_combine_kernel(const Plan p, int tile_rows) {
   const PagedCache& c = p.a.cache;
   __shared__ float s_m[8], s_l[8], s_o[8][128];
   const int items = c.heads * p.tiles;
-  const int b = blockIdx.x / items, item = blockIdx.x - b * items;
+  const int r = blockIdx.x % tile_rows, at = blockIdx.x / tile_rows;
+  const int b = at / items, item = at - b * items;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Shares shares = count_units(p);
-  int64_t before = 0;
-  for (int x = lane; x < b; x += 32) {
-    int first, units, len, count;
-    keys_of(c, p.a.window, x, first, units, len, count);
-    before += units;
+  const int h = item / p.tiles, row = (item - h * p.tiles) * p.tile_rows + r;
+  int64_t before = 0, sum_all = 0;
+  Keys keys{};
+  for (int x = lane; x < c.B; x += 32) {
+    const Keys k = keys_of(c, p.a.window, x);
+    sum_all += k.units;
+    if (x < b) before += k.units;
+    if (x == b) keys = k;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  int first, units, len, count;
-  keys_of(c, p.a.window, b, first, units, len, count);
+  sum_all = warp_sum_long(sum_all);
+  before = warp_sum_long(before);
+  const int units = __shfl_sync(0xffffffffu, keys.units, b & 31);
+  const int64_t per = share_of(p, sum_all);
   const int64_t begin = before * items + static_cast<int64_t>(item) * units;
-  const int w0 = static_cast<int>(begin / shares.per), w1 = static_cast<int>((begin + units - 1) / shares.per);
+  const int w0 = static_cast<int>(begin / per), w1 = static_cast<int>((begin + units - 1) / per);
   pdl_wait();
-  if (units > 0 && w0 == w1) return;
-  const int h = item / p.tiles, row0 = (item - h * p.tiles) * p.tile_rows;
-  const int rows = min(p.tile_rows, p.rows - row0);
-  for (int r = 0; r < rows; ++r) {
-    const int row = row0 + r, token = row / p.group;
-    // each warp every eighth part, four values of a head to a lane
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    const int d = lane * 4;
-    if (units > 0) {
-      for (int w = w0 + warp; w <= w1; w += 8) {
-        const float* part = part_of(p, w, w == w0 ? 1 : 0, r);
-        const float pm = part[c.dim], pl = part[c.dim + 1];
-        const float top = fmaxf(m, pm), use = top == -INFINITY ? 0.f : top;
-        const float f0 = exp2f(m - use), f1 = exp2f(pm - use);
-        l = l * f0 + pl * f1;
-        if (d < c.dim) {
-          const float4 x = *reinterpret_cast<const float4*>(part + d);
-          o[0] = o[0] * f0 + x.x * f1;
-          o[1] = o[1] * f0 + x.y * f1;
-          o[2] = o[2] * f0 + x.z * f1;
-          o[3] = o[3] * f0 + x.w * f1;
-        }
-        m = top;
-      }
+  if (row >= p.rows || (units > 0 && w0 == w1)) return;
+  const int token = row / p.group;
+  // each warp every eighth part, four values of a head to a lane
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int d = lane * 4;
+  if (units > 0) {
+#pragma unroll 4
+    for (int w = w0 + warp; w <= w1; w += 8) {
+      const float* part = part_of(p, w, w == w0 ? 1 : 0, r);
+      const float2 ml = *reinterpret_cast<const float2*>(part + c.dim);
+      const float4 x = d < c.dim ? *reinterpret_cast<const float4*>(part + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float top = fmaxf(m, ml.x), use = top == -INFINITY ? 0.f : top;
+      const float f0 = exp2f(m - use), f1 = exp2f(ml.x - use);
+      l = l * f0 + ml.y * f1;
+      o[0] = o[0] * f0 + x.x * f1;
+      o[1] = o[1] * f0 + x.y * f1;
+      o[2] = o[2] * f0 + x.z * f1;
+      o[3] = o[3] * f0 + x.w * f1;
+      m = top;
     }
-    __syncthreads();
-    if (lane == 0) {
-      s_m[warp] = m;
-      s_l[warp] = l;
-    }
-    *reinterpret_cast<float4*>(&s_o[warp][d]) = make_float4(o[0], o[1], o[2], o[3]);
-    __syncthreads();
-    float top = -INFINITY;
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
+  *reinterpret_cast<float4*>(&s_o[warp][d]) = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, s_m[w]);
-    const float use = top == -INFINITY ? 0.f : top;
-    if (threadIdx.x < c.dim) {
-      float sum = 0.f, x = 0.f;
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_m[w]);
+  const float use = top == -INFINITY ? 0.f : top;
+  if (threadIdx.x < c.dim) {
+    float sum = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float f = exp2f(s_m[w] - use);
-        sum += s_l[w] * f;
-        x += s_o[w][threadIdx.x] * f;
-      }
-      T* out = static_cast<T*>(p.a.out) +
-               ((static_cast<int64_t>(b) * c.n + token) * p.a.q_heads + h * p.group + row - token * p.group) * c.dim;
-      out[threadIdx.x] = static_cast<T>(x * (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)));
+    for (int w = 0; w < 8; ++w) {
+      const float f = exp2f(s_m[w] - use);
+      sum += s_l[w] * f;
+      x += s_o[w][threadIdx.x] * f;
     }
+    T* out = static_cast<T*>(p.a.out) +
+             ((static_cast<int64_t>(b) * c.n + token) * p.a.q_heads + h * p.group + row - token * p.group) * c.dim;
+    out[threadIdx.x] = static_cast<T>(x * (sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum)));
   }
 }
 
@@ -529,21 +689,24 @@ Plan make_plan(const PagedAttention& a) {
   p.rows = p.group * c.n;
   p.tile_rows = p.rows <= 8 ? 8 : p.rows <= 16 ? 16 : 32;
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
-  p.page_units = 0;
-  while ((kUnit << p.page_units) < c.page) ++p.page_units;
+  p.page_blocks = 0;
+  while ((16 << p.page_blocks) < c.page) ++p.page_blocks;
   p.words = c.dim + 4;           // (rows on 16 bytes)
   p.scale_log2 = a.scale * kLog2e;
   // units if all sequences fill their rows of the table
-  const int64_t units = static_cast<int64_t>(c.B) * c.heads * p.tiles * ((static_cast<int64_t>(c.table_pages) * c.page) / kUnit);
-  const int64_t ctas = (units + kLeastUnits * kWarps - 1) / (kLeastUnits * kWarps);
-  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * kWarps;
+  const int64_t units = static_cast<int64_t>(c.B) * c.heads * p.tiles *
+                        ((static_cast<int64_t>(c.table_pages) * c.page + kUnit - 1) / kUnit);
+  const int warps = warps_of(p.tile_rows / 8);
+  const int64_t ctas = (units + kLeastUnits * warps - 1) / (kLeastUnits * warps);
+  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * warps;
   return p;
 }
 
-template <bool kWide, int N, typename T>
+template <bool kWide, int N, bool kSmallPages, typename T>
 int launch_tiles(const Plan& p, cudaStream_t stream) {
   using S = Shape<kWide, N, T>;
-  auto kernel = paged_attention_kernel<kWide, N, T>;
+  static_assert(S::kSmem <= 227 * 1024, "a CTA's shared memory");
+  auto kernel = paged_attention_kernel<kWide, N, kSmallPages, T>;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return 3;
   static bool configured[64] = {};
@@ -553,10 +716,11 @@ int launch_tiles(const Plan& p, cudaStream_t stream) {
     configured[device] = true;
   }
   count_launch();
-  kernel<<<p.warps / kWarps, kWarps * 32, S::kSmem, stream>>>(p);
+  kernel<<<p.warps / S::kWarps, S::kWarps * 32, S::kSmem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 4;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(p.a.cache.B * p.a.cache.heads * p.tiles));
+  const int tile_rows = p.rows < p.tile_rows ? p.rows : p.tile_rows;
+  config.gridDim = dim3(static_cast<unsigned>(p.a.cache.B) * p.a.cache.heads * p.tiles * tile_rows);
   config.blockDim = dim3(256);
   config.stream = stream;
   cudaLaunchAttribute attr{};
@@ -565,14 +729,21 @@ int launch_tiles(const Plan& p, cudaStream_t stream) {
   config.attrs = &attr;
   config.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&config, paged_combine_kernel<T>, p) == cudaSuccess ? 0 : 4;
+  return cudaLaunchKernelEx(&config, paged_combine_kernel<T>, p, tile_rows) == cudaSuccess ? 0 : 4;
 }
 
-template <bool kWide, typename T>
+template <bool kWide, bool kSmallPages, typename T>
 int launch_rows(const Plan& p, cudaStream_t stream) {
-  if (p.tile_rows == 8) return launch_tiles<kWide, 1, T>(p, stream);
-  if (p.tile_rows == 16) return launch_tiles<kWide, 2, T>(p, stream);
-  return launch_tiles<kWide, 4, T>(p, stream);
+  if (p.tile_rows == 8) return launch_tiles<kWide, 1, kSmallPages, T>(p, stream);
+  if (p.tile_rows == 16) return launch_tiles<kWide, 2, kSmallPages, T>(p, stream);
+  return launch_tiles<kWide, 4, kSmallPages, T>(p, stream);
+}
+
+template <typename T>
+int launch_heads(const Plan& p, cudaStream_t stream) {
+  const bool small = p.a.cache.page < kUnit;
+  if (p.a.cache.dim > 64) return small ? launch_rows<true, true, T>(p, stream) : launch_rows<true, false, T>(p, stream);
+  return small ? launch_rows<false, true, T>(p, stream) : launch_rows<false, false, T>(p, stream);
 }
 
 }  // namespace
@@ -588,9 +759,8 @@ int launch_paged_attention(const PagedAttention& a, cudaStream_t stream) {
   if (c.dim < 8 || c.dim > 128 || c.dim % 8 != 0 || c.pitch != (c.dim + 15) / 16 * 16) return 1;
   if (c.page != 16 && c.page != 32 && c.page != 64 && c.page != 128) return 2;
   const Plan p = make_plan(a);
-  if (static_cast<int64_t>(c.B) * c.heads * p.tiles > 0x7fffffff) return 5;
-  if (c.dim > 64) return a.bf16 ? launch_rows<true, __nv_bfloat16>(p, stream) : launch_rows<true, __half>(p, stream);
-  return a.bf16 ? launch_rows<false, __nv_bfloat16>(p, stream) : launch_rows<false, __half>(p, stream);
+  if (static_cast<int64_t>(c.B) * c.heads * p.tiles * p.tile_rows > 0x7fffffff) return 5;
+  return a.bf16 ? launch_heads<__nv_bfloat16>(p, stream) : launch_heads<__half>(p, stream);
 }
 
 }  // namespace slapo

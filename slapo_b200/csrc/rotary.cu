@@ -15,30 +15,23 @@
 namespace slapo {
 namespace {
 
+// V values as they are in memory: 16 bytes, or a single one
 template <typename T, int V>
-struct Values {
-  float v[V];
+struct __align__(V == 1 ? sizeof(T) : 16) Values {
+  T v[V];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (V == 1) {
-      v[0] = static_cast<float>(*p);
+      v[0] = *p;
     } else {
-      const uint4 raw = *reinterpret_cast<const uint4*>(p);
-      const T* x = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = static_cast<float>(x[i]);
+      *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(p));
     }
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (V == 1) {
-      *p = static_cast<T>(v[0]);
-    } else {
-      uint4 raw;
-      T* x = reinterpret_cast<T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = static_cast<T>(v[i]);
-      *reinterpret_cast<uint4*>(p) = raw;
-    }
+    if constexpr (V == 1) *p = v[0];
+    else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
   }
+  __device__ __forceinline__ float get(int i) const { return static_cast<float>(v[i]); }
+  __device__ __forceinline__ void set(int i, float x) { v[i] = static_cast<T>(x); }
 };
 
 // One place of a head for a thread: V values (16 bytes, or single ones) that are turned with V others, or copied.  Places
@@ -75,77 +68,77 @@ struct RotaryPlace {
       cs[j].y *= sign;
     }
   }
-  // x to y, as it is
-  __device__ __forceinline__ void move(const T* x, T* y) const {
-    Values<T, V> m;
+  __device__ __forceinline__ void load(const T* x, Values<T, V>& m, Values<T, V>& n) const {
     m.load(x + first);
-    m.store(y + first);
     if constexpr (!kNeighbours) {
-      if (!copy) {
-        m.load(x + second);
-        m.store(y + second);
-      }
+      if (!copy) n.load(x + second);
     }
   }
-  __device__ __forceinline__ void clear(T* y) const {
-    Values<T, V> m{};
+  __device__ __forceinline__ void store(T* y, const Values<T, V>& m, const Values<T, V>& n) const {
     m.store(y + first);
     if constexpr (!kNeighbours) {
-      if (!copy) m.store(y + second);
+      if (!copy) n.store(y + second);
     }
   }
-  __device__ __forceinline__ void turn(const T* x, T* y) const {
-    Values<T, V> m, n;
-    m.load(x + first);
-    if (copy) {
-      m.store(y + first);
-      return;
-    }
-    if constexpr (kNeighbours) {
+  __device__ __forceinline__ void turn(Values<T, V>& m, Values<T, V>& n) const {
+    if (copy) return;
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) {
-        n.v[2 * j] = turned_value(m.v[2 * j], cs[j].x, m.v[2 * j + 1], -cs[j].y);
-        n.v[2 * j + 1] = turned_value(m.v[2 * j + 1], cs[j].x, m.v[2 * j], cs[j].y);
-      }
-      n.store(y + first);
-    } else {
-      n.load(x + second);
-      Values<T, V> a, o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        a.v[j] = turned_value(m.v[j], cs[j].x, n.v[j], -cs[j].y);
-        o.v[j] = turned_value(n.v[j], cs[j].x, m.v[j], cs[j].y);
-      }
-      a.store(y + first);
-      o.store(y + second);
+    for (int j = 0; j < kCs; ++j) {
+      float a[2];
+      if constexpr (kNeighbours) { a[0] = m.get(2 * j); a[1] = m.get(2 * j + 1); }
+      else { a[0] = m.get(j); a[1] = n.get(j); }
+      const float x = turned_value(a[0], cs[j].x, a[1], -cs[j].y), y = turned_value(a[1], cs[j].x, a[0], cs[j].y);
+      if constexpr (kNeighbours) { m.set(2 * j, x); m.set(2 * j + 1, y); }
+      else { m.set(j, x); n.set(j, y); }
     }
   }
 };
 
+// Rows of heads that a thread has on their way at a time
+constexpr int kRowsAhead = 3;
+
 template <typename T, int V, bool kPairs>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall c) {
-  RotaryPlace<T, V, kPairs> place(threadIdx.x, c.rotary);
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall c, int rows) {
+  using Place = RotaryPlace<T, V, kPairs>;
+  Place place(threadIdx.x, c.rotary);
   for (int64_t token = blockIdx.x; token < c.B * c.S; token += gridDim.x) {
     const int64_t b = token / c.S, s = token - b * c.S;
     int64_t pos = c.at.start + s;
     if (c.at.ids != nullptr) {
       const int64_t at = b * c.at.batch_stride + s * c.at.token_stride;
       pos = c.at.ids64 ? static_cast<const int64_t*>(c.at.ids)[at] : static_cast<const int32_t*>(c.at.ids)[at];
+    } else if (c.at.lengths != nullptr) {
+      const int64_t count = c.at.counts != nullptr ? min(max(static_cast<int64_t>(c.at.counts[b]), int64_t{0}), c.S) : c.S;
+      pos = s < count ? c.at.lengths[b] - count + s : -1;
     }
     const bool known = pos >= 0 && pos < c.table_rows;
-    if (known) place.read(c.table, pos, c.rotary, c.transposed ? -1.f : 1.f);
+    for (int row0 = threadIdx.y; row0 < rows; row0 += kRowsAhead * blockDim.y) {
+      Values<T, V> m[kRowsAhead], n[kRowsAhead];
+      T* y[kRowsAhead];
+      bool turn[kRowsAhead];
 #pragma unroll
-    for (int p = 0; p < 3; ++p) {
-      if (p >= c.parts) break;
-      const RotaryPart& part = c.part[p];
-      const T* x = static_cast<const T*>(part.x) + b * part.x_stride[0] + s * part.x_stride[1];
-      T* y = static_cast<T*>(part.y) + b * part.y_stride[0] + s * part.y_stride[1];
-      for (int h = threadIdx.y; h < part.heads; h += blockDim.y) {
-        const T* xh = x + h * part.x_stride[2];
-        T* yh = y + h * part.y_stride[2];
-        if (!part.turn) place.move(xh, yh);
-        else if (known) place.turn(xh, yh);
-        else place.clear(yh);        // (a position outside of the table)
+      for (int u = 0; u < kRowsAhead; ++u) {
+        int h = row0 + u * blockDim.y;
+        y[u] = nullptr;
+        if (h >= rows) continue;
+        // the parts' heads are rows one after the other
+        int p = 0;
+        while (h >= c.part[p].heads) h -= c.part[p++].heads;
+        const RotaryPart& part = c.part[p];
+        turn[u] = part.turn;
+        y[u] = static_cast<T*>(part.y) + b * part.y_stride[0] + s * part.y_stride[1] + h * part.y_stride[2];
+        if (part.turn && !known) continue;
+        place.load(static_cast<const T*>(part.x) + b * part.x_stride[0] + s * part.x_stride[1] + h * part.x_stride[2], m[u], n[u]);
+      }
+      if (known && row0 == threadIdx.y) place.read(c.table, pos, c.rotary, c.transposed ? -1.f : 1.f);
+#pragma unroll
+      for (int u = 0; u < kRowsAhead; ++u) {
+        if (y[u] == nullptr) continue;
+        if (turn[u]) {
+          if (known) place.turn(m[u], n[u]);
+          else m[u] = n[u] = Values<T, V>{};        // (a position outside of the table)
+        }
+        place.store(y[u], m[u], n[u]);
       }
     }
   }
@@ -170,18 +163,20 @@ int launch(const RotaryCall& c, cudaStream_t stream) {
                                            : RotaryPlace<T, V, false>::places(c.D, c.rotary))
                           : RotaryPlace<T, 1, false>::places(c.D, c.rotary);
   int heads = 0;
-  for (int p = 0; p < c.parts; ++p) heads = c.part[p].heads > heads ? c.part[p].heads : heads;
+  for (int p = 0; p < c.parts; ++p) heads += c.part[p].heads;
   if (places > 256) return 2;
-  int rows = 256 / places;
-  if (rows > heads) rows = heads;
+  if (heads == 0) return 0;
+  // as few rounds over the heads as 256 threads take, with as few idle rows in the last one
+  const int most = 256 / places, rounds = (heads + most - 1) / most;
+  const int rows = (heads + rounds - 1) / rounds;
   const int64_t tokens = c.B * c.S;
   const unsigned grid = static_cast<unsigned>(tokens < 0x7fffffff ? tokens : 0x7fffffff);
   const dim3 block(places, rows);
   count_launch();
-  if (wide && c.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(c);
-  else if (wide) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(c);
-  else if (c.interleaved) rotary_kernel<T, 1, true><<<grid, block, 0, stream>>>(c);
-  else rotary_kernel<T, 1, false><<<grid, block, 0, stream>>>(c);
+  if (wide && c.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(c, heads);
+  else if (wide) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(c, heads);
+  else if (c.interleaved) rotary_kernel<T, 1, true><<<grid, block, 0, stream>>>(c, heads);
+  else rotary_kernel<T, 1, false><<<grid, block, 0, stream>>>(c, heads);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 

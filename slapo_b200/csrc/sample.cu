@@ -9,8 +9,10 @@
 //
 // Bound by latency for few rows and by the arithmetic of the weights for many; HBM is read once.  A cluster of CTAs has a
 // row, a slice each in shared memory.  Logits are counted in bins of (largest - x) / temperature, an eighth of a
-// factor 2 wide, with their weights where top_p asks for them; the bin in which a limit falls is narrowed by the bits of a key that orders
-// logits and indices until at most kList are left, and those are compared with one another.  No sort.
+// factor 2 wide, with their weights where top_p asks for them without a small top_k.  Where what lies before the end of the bin in
+// which the limit falls is at most kList tokens, the first CTA takes those, sorts them and finishes the row by itself.
+// Else that bin is narrowed by the bits of a key that orders logits and indices until at most kList are left, which
+// are compared with one another, and the cluster sums weights once more.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -31,17 +33,17 @@ static_assert(kSampleVocab == 1 << kIndexBits, "an index has as many bits");
 constexpr double kOne = 4398046511104.0;      // 2^42
 
 struct Shared {
-  unsigned long long mass[kBins];
+  unsigned mass[3][kBins];             // 14, 14 and 15 bits of the weights: of 2^15 elements, no overflow
   unsigned count[kBins];
-  unsigned long long list_key[kList], list_mass[kList];
+  unsigned long long list[kList], sorted[kList];       // places (see Slice::place)
   unsigned long long warp_mass[kWarps];
   unsigned warp_count[kWarps];
   // of the CTA, for the cluster to read
   unsigned long long cta_mass;
-  unsigned long long border;       // of the elements that a limit keeps, the last one's key
+  unsigned long long border;       // of the elements that a limit keeps, the last one's place
   unsigned cta_top, listed, cta_first;
   // of a decision in the CTA
-  unsigned long long above_mass;
+  unsigned long long above_mass, total_mass;
   unsigned above_count, in_bin;
   int bin;
 };
@@ -81,6 +83,21 @@ __device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
   return v;
 }
 
+// What a limit is: kept while the number of those before is less than `count`, or, by mass, their mass less than a
+// share of all
+struct Limit {
+  bool by_mass;
+  unsigned count;
+  double share;
+  unsigned long long mass;         // by mass: known, or 0: the share of all bins' masses
+};
+// less than the share of a mass: less than its ceiling, and the largest is kept
+__device__ __forceinline__ unsigned long long mass_limit(double share, unsigned long long mass) {
+  const double x = share * static_cast<double>(mass);
+  const unsigned long long limit = __double2ull_ru(x > 0.0 ? x : 0.0);
+  return limit == 0ull ? 1ull : limit;
+}
+
 // A row's slice in this CTA's shared memory, in a cluster of CTAs
 struct Slice {
   cg::cluster_group cluster;
@@ -94,10 +111,17 @@ struct Slice {
   __device__ __forceinline__ unsigned long long place(int i) const {
     return (static_cast<unsigned long long>(keys[i]) << kIndexBits) | static_cast<unsigned>(kSampleVocab - 1 - (first + i));
   }
+  static __device__ __forceinline__ unsigned key_at(unsigned long long place) {
+    return static_cast<unsigned>(place >> kIndexBits);
+  }
+  static __device__ __forceinline__ int index_at(unsigned long long place) {
+    return kSampleVocab - 1 - static_cast<int>(place & (kSampleVocab - 1));
+  }
 
   // Sums over the cluster of a value of each CTA
   __device__ __forceinline__ unsigned long long everywhere(unsigned long long mine) {
     const unsigned long long w = warp_total(mine);
+    __syncthreads();
     if ((threadIdx.x & 31) == 0) s.warp_mass[threadIdx.x >> 5] = w;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -112,98 +136,114 @@ struct Slice {
     return sum;
   }
 
+  // A warp's and the block's prefix sums (exclusive), and the block's total
+  template <typename V>
+  __device__ __forceinline__ V before(V mine, V* warps, V& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    V until = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const V x = __shfl_up_sync(0xffffffffu, until, o);
+      if (lane >= o) until += x;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = until;
+    __syncthreads();
+    V sum = until - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) sum += warps[w];
+      total += warps[w];
+    }
+    return sum;
+  }
+
   // Counts (and masses) of all CTAs' bins, and the bin in which a limit falls: the first whose beginning is below
-  // the limit and whose end is not.  by_mass: kept while the mass before is less than `limit`; else the count.
-  // `count0`, `mass0`: before the first bin.  Returns through s.bin (-1: the limit is not reached), s.above_*.
-  __device__ __forceinline__ void border_bin(bool by_mass, unsigned long long limit, unsigned count0,
-                                             unsigned long long mass0, int bins) {
+  // the limit and whose end is not.  `count0`, `mass0`: before the first bin.  Returns through s.bin (-1: the limit is not
+  // reached), s.above_*, s.in_bin.  The CTAs' bins can be written again after the cluster's next barrier.
+  __device__ __forceinline__ void border_bin(const Limit& limit, unsigned count0, unsigned long long mass0, int bins) {
     cluster.sync();
     const unsigned ranks = cluster.num_blocks();
     unsigned n = 0;
     unsigned long long m = 0;
     if (static_cast<int>(threadIdx.x) < bins) {
+      unsigned long long part[3] = {0ull, 0ull, 0ull};
       for (unsigned r = 0; r < ranks; ++r) {
         const Shared* o = cluster.map_shared_rank(&s, r);
         n += o->count[threadIdx.x];
-        m += o->mass[threadIdx.x];
-      }
-    }
-    unsigned n_end = n;
-    unsigned long long m_end = m;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (limit.by_mass) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned a = __shfl_up_sync(0xffffffffu, n_end, o);
-      const unsigned long long b = __shfl_up_sync(0xffffffffu, m_end, o);
-      if (lane >= o) {
-        n_end += a;
-        m_end += b;
+          for (int i = 0; i < 3; ++i) part[i] += o->mass[i][threadIdx.x];
+        }
       }
-    }
-    if (lane == 31) {
-      s.warp_count[warp] = n_end;
-      s.warp_mass[warp] = m_end;
+      m = part[0] + (part[1] << 14) + (part[2] << 28);
     }
     if (threadIdx.x == 0) s.bin = -1;
-    __syncthreads();
-    n_end += count0;
-    m_end += mass0;
-    for (int w = 0; w < warp; ++w) {
-      n_end += s.warp_count[w];
-      m_end += s.warp_mass[w];
-    }
-    const unsigned n_before = n_end - n;
-    const unsigned long long m_before = m_end - m;
-    const bool here = n > 0 && (by_mass ? m_before < limit && m_end >= limit : n_before < limit && n_end >= limit);
+    unsigned all;
+    unsigned long long mass;
+    const unsigned n_before = count0 + before(n, s.warp_count, all);
+    const unsigned long long m_before = mass0 + before(m, s.warp_mass, mass);
+    const unsigned long long most = limit.by_mass ? mass_limit(limit.share, limit.mass != 0ull ? limit.mass : mass) : 0ull;
+    const bool here = n > 0 && (limit.by_mass ? m_before < most && m_before + m >= most
+                                              : n_before < limit.count && n_before + n >= limit.count);
+    if (threadIdx.x == 0) s.total_mass = mass;
     if (here) {
       s.bin = threadIdx.x;
       s.above_count = n_before;
       s.above_mass = m_before;
       s.in_bin = n;
     }
-    cluster.sync();       // (all have read the others' bins)
-  }
-
-  __device__ __forceinline__ void clear_bins() {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-      s.count[i] = 0u;
-      s.mass[i] = 0ull;
-    }
     __syncthreads();
   }
 
-  // The key of the last element that a limit keeps (0: all): elements in order are kept while the mass (or number) of
-  // those before is less than the limit.
-  __device__ __forceinline__ unsigned long long border(bool by_mass, unsigned long long limit) {
-    clear_bins();
-    for (int i = threadIdx.x; i < size; i += kThreads) {
-      if (keys[i] == 0u) continue;
-      const int b = row.bin(keys[i]);
-      atomicAdd(&s.count[b], 1u);
-      const unsigned long long w = by_mass ? row.weight(keys[i]) : 0ull;
-      if (w != 0ull) atomicAdd(&s.mass[b], w);
+  __device__ __forceinline__ void clear_bins(bool masses) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      s.count[i] = 0u;
+      if (masses) s.mass[0][i] = s.mass[1][i] = s.mass[2][i] = 0u;
     }
-    border_bin(by_mass, limit, 0u, 0ull, kBins);
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add(int b, unsigned key, bool by_mass) {
+    atomicAdd(&s.count[b], 1u);
+    if (!by_mass) return;
+    const unsigned long long w = row.weight(key);
+    const unsigned part[3] = {static_cast<unsigned>(w) & 0x3fffu, static_cast<unsigned>(w >> 14) & 0x3fffu,
+                              static_cast<unsigned>(w >> 28)};
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (part[i] != 0u) atomicAdd(&s.mass[i][b], part[i]);
+  }
+  // All elements in bins, and the limit's one
+  __device__ __forceinline__ void count_bins(const Limit& limit) {
+    clear_bins(limit.by_mass);
+    for (int i = threadIdx.x; i < size; i += kThreads)
+      if (keys[i] != 0u) add(row.bin(keys[i]), keys[i], limit.by_mass);
+    border_bin(limit, 0u, 0ull, kBins);
+  }
+
+  // The place of the last element that a limit keeps (0: all), after count_bins
+  __device__ __forceinline__ unsigned long long border(const Limit& limit) {
     const int bin = s.bin;
     if (bin < 0) return 0ull;
     unsigned n0 = s.above_count, left = s.in_bin;
     unsigned long long m0 = s.above_mass;
+    Limit rest = limit;
+    if (limit.by_mass && limit.mass == 0ull) rest.mass = s.total_mass;
+    const unsigned long long most = limit.by_mass ? mass_limit(rest.share, rest.mass) : 0ull;
     // narrowed by the bits of the elements' places
     unsigned long long low = 0ull, mask = 0ull;
     for (int done = 0; left > kList && done < 32 + kIndexBits; done += 8) {
-      __syncthreads();
-      clear_bins();
+      cluster.sync();       // (all have read the bins)
+      clear_bins(limit.by_mass);
       const int by = max(32 + kIndexBits - 8 - done, 0), width = min(32 + kIndexBits - done, 8);
       for (int i = threadIdx.x; i < size; i += kThreads) {
         if (keys[i] == 0u || row.bin(keys[i]) != bin) continue;
         const unsigned long long p = place(i);
         if ((p & mask) != low) continue;
-        const int b = (1 << width) - 1 - static_cast<int>((p >> by) & ((1u << width) - 1));      // larger ones first
-        atomicAdd(&s.count[b], 1u);
-        const unsigned long long w = by_mass ? row.weight(keys[i]) : 0ull;
-        if (w != 0ull) atomicAdd(&s.mass[b], w);
+        add((1 << width) - 1 - static_cast<int>((p >> by) & ((1u << width) - 1)), keys[i], limit.by_mass);  // larger ones first
       }
-      border_bin(by_mass, limit, n0, m0, 256);
+      border_bin(rest, n0, m0, 256);
       n0 = s.above_count;
       m0 = s.above_mass;
       left = s.in_bin;
@@ -222,29 +262,127 @@ struct Slice {
       const unsigned long long p = place(i);
       if ((p & mask) != low) continue;
       const unsigned at = atomicAdd(&home->listed, 1u);
-      if (at < kList) {
-        home->list_key[at] = p;
-        home->list_mass[at] = row.weight(keys[i]);
-      }
+      if (at < kList) home->list[at] = p;
     }
     cluster.sync();
     if (cluster.block_rank() == 0) {
       const int n = static_cast<int>(min(s.listed, static_cast<unsigned>(kList)));
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned long long p = s.list_key[i];
-        unsigned before = n0;
-        unsigned long long sum = m0;
-        for (int j = 0; j < n; ++j) {
-          if (s.list_key[j] > p) {
-            ++before;
-            sum += s.list_mass[j];
-          }
-        }
-        if (by_mass ? sum < limit : before < limit) atomicMin(&s.border, p);
+      sort_list(n);
+      unsigned long long w[2], mine = 0ull, all;
+      const int i0 = 2 * threadIdx.x;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) mine += w[j] = limit.by_mass && i0 + j < n ? row.weight(key_at(s.sorted[i0 + j])) : 0ull;
+      unsigned long long sum = m0 + before(mine, s.warp_mass, all);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (i0 + j < n && (limit.by_mass ? sum < most : n0 + i0 + j < limit.count)) atomicMin(&s.border, s.sorted[i0 + j]);
+        sum += w[j];
       }
+      __syncthreads();
     }
     cluster.sync();
     return home->border;
+  }
+
+  // s.sorted: the list's n places, the largest first
+  __device__ __forceinline__ void sort_list(int n) {
+    int width = 2;
+    while (width < n) width *= 2;
+    for (int i = threadIdx.x; i < width; i += kThreads) s.sorted[i] = i < n ? s.list[i] : 0ull;
+    for (int k = 2; k <= width; k *= 2) {
+      for (int j = k / 2; j > 0; j /= 2) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < width / 2; i += kThreads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const unsigned long long x = s.sorted[a], y = s.sorted[b];
+          if ((x < y) == ((a & k) == 0)) {
+            s.sorted[a] = y;
+            s.sorted[b] = x;
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  // The row by the first CTA alone, from the elements of the bins up to `bin`, at most kList: the token (in all threads
+  // of the first CTA).  top_k: 0: all; mass: of all that top_k keeps, or 0: to be summed.
+  __device__ __forceinline__ int finish(int bin, unsigned top_k, double top_p, double min_p, unsigned long long mass, double u) {
+    // in the order of the indices: each warp a stretch of the slice
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stretch = (size + kWarps - 1) / kWarps, w0 = min(size, warp * stretch), w1 = min(size, w0 + stretch);
+    auto taken = [&](int i) { return i < w1 && keys[i] != 0u && row.bin(keys[i]) <= bin; };
+    unsigned found = 0;
+    for (int i0 = w0; i0 < w1; i0 += 32) found += __popc(__ballot_sync(0xffffffffu, taken(i0 + lane)));
+    __syncthreads();
+    if (lane == 0) s.warp_count[warp] = found;
+    __syncthreads();
+    unsigned at = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += s.warp_count[w];
+      all += s.warp_count[w];
+    }
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+      const bool mine = taken(i0 + lane);
+      const unsigned votes = __ballot_sync(0xffffffffu, mine);
+      const unsigned to = at + __popc(votes & ((1u << lane) - 1u));
+      if (mine && to < kList) s.list[to] = place(i0 + lane);
+      at += __popc(votes);
+    }
+    if (threadIdx.x == 0) s.listed = all;
+    cluster.sync();
+    if (cluster.block_rank() != 0) return -1;
+    unsigned n = s.listed;
+    __syncthreads();
+    for (unsigned r = 1; r < cluster.num_blocks(); ++r) {
+      const Shared* o = cluster.map_shared_rank(&s, r);
+      const unsigned more = o->listed;
+      for (unsigned i = threadIdx.x; i < more && n + i < kList; i += kThreads) s.list[n + i] = o->list[i];
+      n += more;
+    }
+    n = min(n, static_cast<unsigned>(kList));
+    __syncthreads();
+    sort_list(static_cast<int>(n));
+    // the kept ones begin the sorted row
+    const unsigned i0 = 2 * threadIdx.x;
+    const unsigned in_k = top_k > 0 ? min(top_k, n) : n;
+    unsigned long long w[2], sum[2], mine = 0ull, total;
+    double share[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      share[j] = i0 + j < in_k ? row.fraction(key_at(s.sorted[i0 + j])) : 0.0;
+      w[j] = i0 + j < in_k ? __double2ull_rn(share[j] * kOne) : 0ull;
+      mine += w[j];
+    }
+    sum[0] = before(mine, s.warp_mass, total);
+    sum[1] = sum[0] + w[0];
+    const unsigned long long most = mass_limit(top_p, mass != 0ull ? mass : total);
+    mine = 0ull;
+    unsigned kept = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (i0 + j < in_k && (i0 + j == 0 || ((sum[j] < most || !(top_p < 1.0)) && share[j] >= min_p))) {
+        mine += w[j];
+        ++kept;
+      }
+    }
+    unsigned kept_all;
+    before(kept, s.warp_count, kept_all);
+    before(mine, s.warp_mass, total);
+    const unsigned long long last = s.sorted[kept_all - 1];
+    const double share_u = u * static_cast<double>(total);
+    unsigned long long target = share_u > 0.0 ? __double2ull_rd(share_u) : 0ull;      // passed: more than it, more than its floor
+    if (target >= total) target = total - 1ull;
+    mine = 0ull;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) mine += w[j] = i0 + j < n && s.list[i0 + j] >= last ? row.weight(key_at(s.list[i0 + j])) : 0ull;
+    sum[0] = before(mine, s.warp_mass, total);
+    sum[1] = sum[0] + w[0];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (sum[j] <= target && target < sum[j] + w[j]) s.bin = index_at(s.list[i0 + j]);
+    __syncthreads();
+    return s.bin;
   }
 };
 
@@ -264,13 +402,29 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
   const float u = c.uniform[r];
 
   unsigned top = 0u;
-  for (int i = threadIdx.x; i < size; i += kThreads) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vectors = (reinterpret_cast<uintptr_t>(x + first) & 15) == 0;
+  const int whole = vectors ? size / V * V : 0;
+  for (int i = threadIdx.x * V; i < whole; i += kThreads * V) {
+    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + first + i));
+    const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      uint4 k;
+      k.x = key_of(static_cast<float>(v[j]));
+      k.y = key_of(static_cast<float>(v[j + 1]));
+      k.z = key_of(static_cast<float>(v[j + 2]));
+      k.w = key_of(static_cast<float>(v[j + 3]));
+      *reinterpret_cast<uint4*>(s_keys + i + j) = k;
+      top = max(max(top, max(k.x, k.y)), max(k.z, k.w));
+    }
+  }
+  for (int i = whole + threadIdx.x; i < size; i += kThreads) {
     const unsigned k = key_of(static_cast<float>(x[first + i]));
     s_keys[i] = k;
     top = max(top, k);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) s.warp_count[threadIdx.x >> 5] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -299,17 +453,36 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
 
   // the last place that is kept
   unsigned long long border = 0ull;
-  if (top_k > 0 && top_k < c.vocab) border = at.border(false, static_cast<unsigned long long>(top_k));
   const double least = static_cast<double>(min_p);
+  bool binned = false;
+  if (top_k > 0 && top_k < c.vocab) {
+    const Limit limit{false, static_cast<unsigned>(top_k), 0.0, 0ull};
+    at.count_bins(limit);
+    if (s.bin >= 0 && s.above_count + s.in_bin <= kList) {
+      const int token = at.finish(s.bin, static_cast<unsigned>(top_k), top_p, least, 0ull, u);
+      if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
+      cluster.sync();       // (the first CTA has read the others' lists)
+      return;
+    }
+    border = at.border(limit);
+    binned = true;
+  }
   if (top_p < 1.f) {
-    unsigned long long mine = 0ull;
-    for (int i = threadIdx.x; i < size; i += kThreads)
-      if (s_keys[i] != 0u && at.place(i) >= border) mine += row.weight(s_keys[i]);
-    const unsigned long long mass = at.everywhere(mine);
-    const double share = static_cast<double>(top_p) * static_cast<double>(mass);
-    unsigned long long limit = __double2ull_ru(share > 0.0 ? share : 0.0);      // less than the share: less than its ceiling
-    if (limit == 0ull) limit = 1ull;                                            // (the largest is kept)
-    border = max(border, at.border(true, limit));
+    Limit limit{true, 0u, static_cast<double>(top_p), 0ull};
+    if (binned) {
+      unsigned long long mine = 0ull;
+      for (int i = threadIdx.x; i < size; i += kThreads)
+        if (s_keys[i] != 0u && at.place(i) >= border) mine += row.weight(s_keys[i]);
+      limit.mass = at.everywhere(mine);
+    }
+    at.count_bins(limit);
+    if (!binned && s.bin >= 0 && s.above_count + s.in_bin <= kList) {
+      const int token = at.finish(s.bin, 0u, top_p, least, s.total_mass, u);
+      if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
+      cluster.sync();
+      return;
+    }
+    border = max(border, at.border(limit));
   }
   // each warp's stretch of the slice, in the order of the indices
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -339,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
     total += m;
   }
   const double share = static_cast<double>(u) * static_cast<double>(total);
-  unsigned long long target = share > 0.0 ? __double2ull_rd(share) : 0ull;       // passed: more than it, more than its floor
+  unsigned long long target = share > 0.0 ? __double2ull_rd(share) : 0ull;
   if (target >= total) target = total - 1ull;
   for (int w = 0; w < warp; ++w) before += s.warp_mass[w];
   if (before <= target && target < before + mine) {
@@ -367,9 +540,9 @@ int launch(const SampleCall& c, cudaStream_t stream) {
   auto kernel = sample_kernel<T>;
   // A slice of the row for each CTA of a cluster: many CTAs where rows are few, none of over 40 000 keys
   int ranks = 1;
-  while (ranks < 8 && (c.rows * ranks * 2 <= 2 * sm_count() || (c.vocab + ranks - 1) / ranks > 40000)) ranks *= 2;
+  while (ranks < 8 && (c.rows * ranks * 2 <= 2 * sm_count() || (c.vocab + ranks - 1) / ranks > 16384)) ranks *= 2;
   if (c.vocab < 2048) ranks = 1;
-  const int slice = (c.vocab + ranks - 1) / ranks;
+  const int slice = ((c.vocab + ranks - 1) / ranks + 7) / 8 * 8;        // (vectors)
   const int bytes = slice * 4;
   if (bytes > 190 * 1024) return 6;
   int device = 0;
