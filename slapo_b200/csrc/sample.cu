@@ -4,8 +4,8 @@
 // shortest beginning whose mass reaches that share of what top_k kept, min_p what weighs that much of the largest.  The
 // token is the first one kept, by index, at which the sum of weights passes the random number times their total.
 //
-// Weights are exp((x - largest) / temperature) in 64 bits, as multiples of 2^-42: sums of integers do not depend on their
-// order, so that the same call gives the same token, and what falls to rounding are 2^-43 of the largest weight.
+// Weights are exp((x - largest) / temperature) in 64 bits, to 2^-44 of themselves, as multiples of 2^-42: sums of integers
+// do not depend on their order, so that the same call gives the same token.
 //
 // Bound by latency for few rows and by the arithmetic of the weights for many; HBM is read once.  A cluster of CTAs has a
 // row, a slice each in shared memory.  Logits are counted in bins of (largest - x) / temperature, an eighth of a
@@ -14,6 +14,8 @@
 // Else that bin is narrowed by the bits of a key that orders logits and indices until at most kList are left, which
 // are compared with one another, and the cluster sums weights once more.
 #include <cooperative_groups.h>
+
+#include <cmath>
 
 #include "common.cuh"
 #include "generate.h"
@@ -35,13 +37,15 @@ constexpr double kOne = 4398046511104.0;      // 2^42
 struct Shared {
   unsigned mass[3][kBins];             // 14, 14 and 15 bits of the weights: of 2^15 elements, no overflow
   unsigned count[kBins];
+  double powers[64];
   unsigned long long list[kList], sorted[kList];       // places (see Slice::place)
   unsigned long long warp_mass[kWarps];
   unsigned warp_count[kWarps];
   // of the CTA, for the cluster to read
   unsigned long long cta_mass;
   unsigned long long border;       // of the elements that a limit keeps, the last one's place
-  unsigned cta_top, listed, cta_first;
+  unsigned cta_top, listed, cta_first, before_cta;
+  unsigned rank_of[256];
   // of a decision in the CTA
   unsigned long long above_mass, total_mass;
   unsigned above_count, in_bin;
@@ -59,17 +63,47 @@ __device__ __forceinline__ float logit_of(unsigned key) {
   return __uint_as_float((key & 0x80000000u) != 0 ? key ^ 0x80000000u : ~key);
 }
 
+// 2^(-i / 64)
+struct Powers {
+  double at[64];
+};
+
 struct Row {
   float top;
+  double top_wide;
   double slope;           // log2(e) / temperature
   float bins;             // eight times that
+  const double* powers;   // in shared memory
+  // A float as a double, by its bits: the conversion runs at a quarter of the products' rate.  (0 and what is below the
+  // normal numbers become some 2^-127.)
+  static __device__ __forceinline__ double wide(float x) {
+    const unsigned b = __float_as_uint(x);
+    return __hiloint2double(static_cast<int>((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)),
+                            static_cast<int>(b << 29));
+  }
+  // exp(-(top - x) / temperature) as 2^-n 2^(-i / 64) e^-g, |g| <= ln 2 / 128, by a table and the series of e^-g up to
+  // its fourth power (Tang, Table-driven implementation of the exponential function, ACM TOMS 15, 1989): off by 2^-44.  Eleven
+  // operations in 64 bits; exp2() and the conversions around it took twice the time.
   __device__ __forceinline__ double fraction(unsigned key) const {
     const float x = logit_of(key);
-    return x == top ? 1.0 : exp2((static_cast<double>(x) - static_cast<double>(top)) * slope);
+    if (x == top) return 1.0;
+    const double y = (top_wide - wide(x)) * slope;
+    if (!(y < 44.0)) return 0.0;
+    constexpr double kMagic = 6755399441055744.0;      // 1.5 2^52: what is added to it is rounded to an integer
+    const double t = fma(y, 64.0, kMagic);
+    const int n = __double2loint(t);
+    const double r = fma(y, 64.0, -(t - kMagic));
+    constexpr double kL = 0.010830424696249145;        // ln 2 / 64
+    double e = fma(r, kL * kL * kL * kL / 24.0, -kL * kL * kL / 6.0);
+    e = fma(r, e, kL * kL / 2.0);
+    e = fma(r, e, -kL);
+    e = fma(r, e, 1.0) * powers[n & 63];
+    return __hiloint2double(__double2hiint(e) - ((n >> 6) << 20), __double2loint(e));
   }
-  __device__ __forceinline__ unsigned long long weight(unsigned key) const {
-    return key == 0u ? 0ull : __double2ull_rn(fraction(key) * kOne);
+  static __device__ __forceinline__ unsigned long long held(double fraction) {
+    return static_cast<unsigned long long>(__double_as_longlong(fma(fraction, kOne, 4503599627370496.0))) & 0xfffffffffffffull;
   }
+  __device__ __forceinline__ unsigned long long weight(unsigned key) const { return key == 0u ? 0ull : held(fraction(key)); }
   // monotone in the key, as each of its steps is
   __device__ __forceinline__ int bin(unsigned key) const {
     const float y = (top - logit_of(key)) * bins;
@@ -106,6 +140,7 @@ struct Slice {
   int size, first;       // elements, and the index of the first one
   int vocab;
   Row row;
+  unsigned mine_before;      // of this thread's bin: elements of the CTAs before this one
 
   // larger logits first, then lower indices: unique
   __device__ __forceinline__ unsigned long long place(int i) const {
@@ -117,6 +152,10 @@ struct Slice {
   static __device__ __forceinline__ int index_at(unsigned long long place) {
     return kSampleVocab - 1 - static_cast<int>(place & (kSampleVocab - 1));
   }
+
+  // Elements of a thread that goes through the slice in the order of the indices: an odd number, so that a warp's meet
+  // every bank once
+  __device__ __forceinline__ int stretch() const { return ((size + kThreads - 1) / kThreads) | 1; }
 
   // Sums over the cluster of a value of each CTA
   __device__ __forceinline__ unsigned long long everywhere(unsigned long long mine) {
@@ -165,12 +204,13 @@ struct Slice {
   __device__ __forceinline__ void border_bin(const Limit& limit, unsigned count0, unsigned long long mass0, int bins) {
     cluster.sync();
     const unsigned ranks = cluster.num_blocks();
-    unsigned n = 0;
+    unsigned n = 0, lower = 0;           // of all CTAs, and of those before this one
     unsigned long long m = 0;
     if (static_cast<int>(threadIdx.x) < bins) {
       unsigned long long part[3] = {0ull, 0ull, 0ull};
       for (unsigned r = 0; r < ranks; ++r) {
         const Shared* o = cluster.map_shared_rank(&s, r);
+        if (r == cluster.block_rank()) lower = n;
         n += o->count[threadIdx.x];
         if (limit.by_mass) {
 #pragma unroll
@@ -187,7 +227,12 @@ struct Slice {
     const unsigned long long most = limit.by_mass ? mass_limit(limit.share, limit.mass != 0ull ? limit.mass : mass) : 0ull;
     const bool here = n > 0 && (limit.by_mass ? m_before < most && m_before + m >= most
                                               : n_before < limit.count && n_before + n >= limit.count);
-    if (threadIdx.x == 0) s.total_mass = mass;
+    if (threadIdx.x == 0) {
+      s.total_mass = mass;
+      s.listed = 0u;
+      s.before_cta = 0u;
+    }
+    mine_before = lower;
     if (here) {
       s.bin = threadIdx.x;
       s.above_count = n_before;
@@ -217,6 +262,7 @@ struct Slice {
   // All elements in bins, and the limit's one
   __device__ __forceinline__ void count_bins(const Limit& limit) {
     clear_bins(limit.by_mass);
+#pragma unroll 4
     for (int i = threadIdx.x; i < size; i += kThreads)
       if (keys[i] != 0u) add(row.bin(keys[i]), keys[i], limit.by_mass);
     border_bin(limit, 0u, 0ull, kBins);
@@ -284,10 +330,26 @@ struct Slice {
     return home->border;
   }
 
-  // s.sorted: the list's n places, the largest first
+  // s.sorted: the list's n places, the largest first.  Few of them are counted against one another, more sorted by
+  // exchanges (bitonic).
   __device__ __forceinline__ void sort_list(int n) {
     int width = 2;
     while (width < n) width *= 2;
+    if (width <= 256) {
+      const int i = threadIdx.x & (width - 1), parts = kThreads / width;
+      if (threadIdx.x < 256) s.rank_of[threadIdx.x] = 0u;
+      __syncthreads();
+      if (i < n) {
+        const unsigned long long p = s.list[i];
+        unsigned larger = 0;
+        for (int j = threadIdx.x / width; j < n; j += parts) larger += s.list[j] > p ? 1u : 0u;
+        atomicAdd(&s.rank_of[i], larger);
+      }
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < n) s.sorted[s.rank_of[threadIdx.x]] = s.list[threadIdx.x];
+      __syncthreads();
+      return;
+    }
     for (int i = threadIdx.x; i < width; i += kThreads) s.sorted[i] = i < n ? s.list[i] : 0ull;
     for (int k = 2; k <= width; k *= 2) {
       for (int j = k / 2; j > 0; j /= 2) {
@@ -305,43 +367,35 @@ struct Slice {
     __syncthreads();
   }
 
-  // The row by the first CTA alone, from the elements of the bins up to `bin`, at most kList: the token (in all threads
-  // of the first CTA).  top_k: 0: all; mass: of all that top_k keeps, or 0: to be summed.
-  __device__ __forceinline__ int finish(int bin, unsigned top_k, double top_p, double min_p, unsigned long long mass, double u) {
-    // in the order of the indices: each warp a stretch of the slice
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int stretch = (size + kWarps - 1) / kWarps, w0 = min(size, warp * stretch), w1 = min(size, w0 + stretch);
-    auto taken = [&](int i) { return i < w1 && keys[i] != 0u && row.bin(keys[i]) <= bin; };
-    unsigned found = 0;
-    for (int i0 = w0; i0 < w1; i0 += 32) found += __popc(__ballot_sync(0xffffffffu, taken(i0 + lane)));
-    __syncthreads();
-    if (lane == 0) s.warp_count[warp] = found;
-    __syncthreads();
-    unsigned at = 0, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += s.warp_count[w];
-      all += s.warp_count[w];
+  // The row by the first CTA alone, from the `number` elements of the bins up to `bin`, at most kList, after count_bins:
+  // the token (in all threads of the first CTA).  top_k: 0: all; mass: of all that top_k keeps, or 0: to be summed.
+  __device__ __forceinline__ int finish(int bin, unsigned number, unsigned top_k, double top_p, double min_p, unsigned long long mass, double u) {
+    // Each CTA's into the first one's list, in the order of the indices: behind those of the CTAs before it, each thread a
+    // stretch of the slice.  (Barriers: the others' bins are read; the list is whole.  CTAs that are done leave.)
+    cluster.barrier_arrive();
+    const int t0 = threadIdx.x * stretch(), t1 = min(size, t0 + stretch());
+    auto taken = [&](int i) { return keys[i] != 0u && row.bin(keys[i]) <= bin; };
+    const unsigned lower = static_cast<int>(threadIdx.x) <= bin ? mine_before : 0u;
+    const unsigned lower_warp = __reduce_add_sync(0xffffffffu, lower);
+    if ((threadIdx.x & 31) == 0 && lower_warp != 0u) atomicAdd(&s.before_cta, lower_warp);
+    unsigned found = 0, all;
+#pragma unroll 8
+    for (int i = t0; i < t1; ++i) found += taken(i) ? 1u : 0u;
+    unsigned to = before(found, s.warp_count, all);
+    Shared* home = cluster.map_shared_rank(&s, 0);
+    if (found != 0u) {
+      to += s.before_cta;
+      for (int i = t0; i < t1; ++i) {
+        if (!taken(i)) continue;
+        if (to < kList) home->list[to] = place(i);
+        ++to;
+      }
     }
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const bool mine = taken(i0 + lane);
-      const unsigned votes = __ballot_sync(0xffffffffu, mine);
-      const unsigned to = at + __popc(votes & ((1u << lane) - 1u));
-      if (mine && to < kList) s.list[to] = place(i0 + lane);
-      at += __popc(votes);
-    }
-    if (threadIdx.x == 0) s.listed = all;
-    cluster.sync();
+    cluster.barrier_wait();
+    cluster.barrier_arrive();
     if (cluster.block_rank() != 0) return -1;
-    unsigned n = s.listed;
-    __syncthreads();
-    for (unsigned r = 1; r < cluster.num_blocks(); ++r) {
-      const Shared* o = cluster.map_shared_rank(&s, r);
-      const unsigned more = o->listed;
-      for (unsigned i = threadIdx.x; i < more && n + i < kList; i += kThreads) s.list[n + i] = o->list[i];
-      n += more;
-    }
-    n = min(n, static_cast<unsigned>(kList));
-    __syncthreads();
+    cluster.barrier_wait();
+    const unsigned n = min(number, static_cast<unsigned>(kList));
     sort_list(static_cast<int>(n));
     // the kept ones begin the sorted row
     const unsigned i0 = 2 * threadIdx.x;
@@ -351,7 +405,7 @@ struct Slice {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       share[j] = i0 + j < in_k ? row.fraction(key_at(s.sorted[i0 + j])) : 0.0;
-      w[j] = i0 + j < in_k ? __double2ull_rn(share[j] * kOne) : 0ull;
+      w[j] = i0 + j < in_k ? Row::held(share[j]) : 0ull;
       mine += w[j];
     }
     sum[0] = before(mine, s.warp_mass, total);
@@ -387,7 +441,7 @@ struct Slice {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, int slice) {
+__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, int slice, const Powers powers) {
   extern __shared__ __align__(16) unsigned s_keys[];
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
@@ -405,18 +459,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
   constexpr int V = 16 / sizeof(T);
   const bool vectors = (reinterpret_cast<uintptr_t>(x + first) & 15) == 0;
   const int whole = vectors ? size / V * V : 0;
-  for (int i = threadIdx.x * V; i < whole; i += kThreads * V) {
-    const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + first + i));
-    const T* v = reinterpret_cast<const T*>(&raw);
+  if (threadIdx.x < 64) s.powers[threadIdx.x] = powers.at[threadIdx.x];
+  constexpr int kAhead = 4;
+  for (int i0 = threadIdx.x * V; i0 < whole; i0 += kThreads * V * kAhead) {
+    uint4 raw[kAhead];
 #pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      uint4 k;
-      k.x = key_of(static_cast<float>(v[j]));
-      k.y = key_of(static_cast<float>(v[j + 1]));
-      k.z = key_of(static_cast<float>(v[j + 2]));
-      k.w = key_of(static_cast<float>(v[j + 3]));
-      *reinterpret_cast<uint4*>(s_keys + i + j) = k;
-      top = max(max(top, max(k.x, k.y)), max(k.z, k.w));
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kThreads * V;
+      if (i < whole) raw[k] = __ldcs(reinterpret_cast<const uint4*>(x + first + i));
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kThreads * V;
+      if (i >= whole) break;
+      const T* v = reinterpret_cast<const T*>(&raw[k]);
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        uint4 w;
+        w.x = key_of(static_cast<float>(v[j]));
+        w.y = key_of(static_cast<float>(v[j + 1]));
+        w.z = key_of(static_cast<float>(v[j + 2]));
+        w.w = key_of(static_cast<float>(v[j + 3]));
+        *reinterpret_cast<uint4*>(s_keys + i + j) = w;
+        top = max(max(top, max(w.x, w.y)), max(w.z, w.w));
+      }
     }
   }
   for (int i = whole + threadIdx.x; i < size; i += kThreads) {
@@ -447,9 +513,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
   }
   Row row;
   row.top = logit_of(top);
+  row.top_wide = static_cast<double>(row.top);
+  row.powers = s.powers;
   row.slope = 1.4426950408889634 / static_cast<double>(temperature);
   row.bins = static_cast<float>(8.0 * row.slope);
-  Slice at{cluster, s, s_keys, size, first, c.vocab, row};
+  Slice at{cluster, s, s_keys, size, first, c.vocab, row, 0u};
 
   // the last place that is kept
   unsigned long long border = 0ull;
@@ -459,9 +527,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
     const Limit limit{false, static_cast<unsigned>(top_k), 0.0, 0ull};
     at.count_bins(limit);
     if (s.bin >= 0 && s.above_count + s.in_bin <= kList) {
-      const int token = at.finish(s.bin, static_cast<unsigned>(top_k), top_p, least, 0ull, u);
+      const int token = at.finish(s.bin, s.above_count + s.in_bin, static_cast<unsigned>(top_k), top_p, least, 0ull, u);
       if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
-      cluster.sync();       // (the first CTA has read the others' lists)
       return;
     }
     border = at.border(limit);
@@ -477,48 +544,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
     }
     at.count_bins(limit);
     if (!binned && s.bin >= 0 && s.above_count + s.in_bin <= kList) {
-      const int token = at.finish(s.bin, 0u, top_p, least, s.total_mass, u);
+      const int token = at.finish(s.bin, s.above_count + s.in_bin, 0u, top_p, least, s.total_mass, u);
       if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
-      cluster.sync();
       return;
     }
     border = max(border, at.border(limit));
   }
-  // each warp's stretch of the slice, in the order of the indices
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int stretch = (size + kWarps - 1) / kWarps, w0 = warp * stretch, w1 = min(size, w0 + stretch);
+  // each thread a stretch of the slice, in the order of the indices
+  const int stretch = at.stretch(), t0 = threadIdx.x * stretch, t1 = min(size, t0 + stretch);
   auto weight = [&](int i) -> unsigned long long {
     const unsigned k = s_keys[i];
     if (k == 0u || at.place(i) < border) return 0ull;
     const double f = row.fraction(k);
-    return f >= least || k == top ? __double2ull_rn(f * kOne) : 0ull;
+    return f >= least || k == top ? Row::held(f) : 0ull;
   };
-  unsigned long long mine = 0ull;
-  for (int i = w0 + lane; i < w1; i += 32) mine += weight(i);
-  mine = warp_total(mine);
-  __syncthreads();
-  if (lane == 0) s.warp_mass[warp] = mine;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned long long sum = 0;
-    for (int w = 0; w < kWarps; ++w) sum += s.warp_mass[w];
-    s.cta_mass = sum;
-  }
+  unsigned long long mine = 0ull, all;
+#pragma unroll 4
+  for (int i = t0; i < t1; ++i) mine += weight(i);
+  unsigned long long before = at.before(mine, s.warp_mass, all);
+  if (threadIdx.x == 0) s.cta_mass = all;
   cluster.sync();
-  unsigned long long before = 0ull, total = 0ull;
+  unsigned long long total = 0ull;
   for (int o = 0; o < ranks; ++o) {
     const unsigned long long m = cluster.map_shared_rank(&s, o)->cta_mass;
     if (o < rank) before += m;
     total += m;
   }
+  cluster.barrier_arrive();       // (this CTA reads the others' shared memory no more)
   const double share = static_cast<double>(u) * static_cast<double>(total);
   unsigned long long target = share > 0.0 ? __double2ull_rd(share) : 0ull;
   if (target >= total) target = total - 1ull;
-  for (int w = 0; w < warp; ++w) before += s.warp_mass[w];
-  if (before <= target && target < before + mine) {
-    for (int i0 = w0; i0 < w1; i0 += 32) {
+  // the thread in whose stretch it is passed; its warp goes through that together
+  const unsigned here = __ballot_sync(0xffffffffu, before <= target && target < before + mine);
+  if (here != 0u) {
+    const int lane = threadIdx.x & 31, owner = __ffs(here) - 1;
+    const int i1 = __shfl_sync(0xffffffffu, t1, owner);
+    before = __shfl_sync(0xffffffffu, before, owner);
+    for (int i0 = __shfl_sync(0xffffffffu, t0, owner); i0 < i1; i0 += 32) {
       const int i = i0 + lane;
-      unsigned long long sum = i < w1 ? weight(i) : 0ull;
+      unsigned long long sum = i < i1 ? weight(i) : 0ull;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long a = __shfl_up_sync(0xffffffffu, sum, o);
@@ -532,7 +596,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
   }
-  cluster.sync();       // (the others have read this CTA's shared memory)
+  cluster.barrier_wait();
 }
 
 template <typename T>
@@ -566,7 +630,12 @@ int launch(const SampleCall& c, cudaStream_t stream) {
   config.attrs = &attr;
   config.numAttrs = 1;
   count_launch();
-  return cudaLaunchKernelEx(&config, kernel, c, slice) == cudaSuccess ? 0 : 4;
+  static const Powers powers = [] {
+    Powers p;
+    for (int i = 0; i < 64; ++i) p.at[i] = std::exp2(-i / 64.0);
+    return p;
+  }();
+  return cudaLaunchKernelEx(&config, kernel, c, slice, powers) == cudaSuccess ? 0 : 4;
 }
 
 }  // namespace
