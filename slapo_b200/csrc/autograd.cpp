@@ -600,7 +600,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const optional<Tensor>& k, co
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && table.requires_grad()), "rotary: the table has no gradient");
   if (!wants_node({&q, &kk, &table})) return RotaryFn::turn(q, k, table, positions, start, interleaved, false);
   const variable_list r = RotaryFn::apply(q, k, table, positions, start, interleaved, false);
-  return {r[0], k.has_value() ? r[1] : at::empty({0}, q.options())};
+  return {r[0], k.has_value() ? r[1] : Tensor()};
 }
 
 Tensor rel_bias(const Tensor& table, const Tensor& buckets) { return RelBiasFn::apply(table, buckets); }

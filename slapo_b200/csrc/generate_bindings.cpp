@@ -49,10 +49,13 @@ void check_rotary_table(const Tensor& table, const Tensor& x) {
 
 Tensor heads_in_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
-slapo::RotaryPart part(const Tensor& x, const Tensor& y, bool turn) {
+// The heads of a tensor, or the `slice`-th ones of a packed projection.  (Views of it would take a microsecond each.)
+slapo::RotaryPart part(const Tensor& x, const Tensor& y, bool turn, int slice = 0) {
   slapo::RotaryPart p{};
-  p.x = x.const_data_ptr();
-  p.y = y.data_ptr();
+  const int64_t e = x.element_size();
+  const bool packed = x.dim() == 5;
+  p.x = static_cast<const char*>(x.const_data_ptr()) + (packed ? slice * x.stride(3) * e : 0);
+  p.y = static_cast<char*>(y.data_ptr()) + (packed ? slice * y.stride(3) * e : 0);
   for (int d = 0; d < 3; ++d) {
     p.x_stride[d] = x.stride(d);
     p.y_stride[d] = y.stride(d);
@@ -78,8 +81,7 @@ std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>
   slapo::RotaryCall c{};
   if (packed) {
     out_q = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
-    out_k = at::empty({0}, q.options());
-    for (int i = 0; i < 3; ++i) c.part[i] = part(q.select(3, i), out_q.select(3, i), i < 2);
+    for (int i = 0; i < 3; ++i) c.part[i] = part(q, out_q, i < 2, i);
     c.parts = 3;
   } else {
     check_on(*k_in, q, "rotary: k");

@@ -21,8 +21,41 @@
 namespace slapo {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;     // of a CTA, at most
 constexpr int kLeast = -100;      // the least scale's exponent
+
+// Eight values as they are in memory
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void flip(bool negative) {
+    const uint32_t mask = negative ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      w[i].x ^= mask;
+      w[i].y ^= mask;
+      w[i].z ^= mask;
+      w[i].w ^= mask;
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t x[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_floats(x[i], T());
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    } else {
+      Vec8<T>::load(reinterpret_cast<const T*>(w), v);
+    }
+  }
+};
 
 // Eight values of a head from d0 on, to be rotated: cosine and sine of each, or none where nothing is rotated
 struct Turn8 {
@@ -45,50 +78,52 @@ struct Turn8 {
     for (int j = 0; j < 8; ++j) {
       const int d = d0 + j;
       cs[j] = d < rotary ? row[d < half ? d : d - half] : make_float2(1.f, 0.f);
-      if (d < half) cs[j].y = -cs[j].y;
+      if (mode == 2 && d < half) cs[j].y = -cs[j].y;
     }
   }
-  // from a token's entries in shared memory, `stride` float4 between those of a place (modes 1 and 3)
+  // from a token's entries in shared memory, `stride` float4 between those of a place: neighbours', or halves'
+  template <bool kNeighbours>
   __device__ __forceinline__ void take(const float4* token, int stride) {
-    if (mode == 0) return;
-    const int place = (mode == 3 || d0 < half ? d0 : d0 - half) / 8;
+    const int place = (kNeighbours || d0 < half ? d0 : d0 - half) / 8;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (mode == 3 && q >= 2) break;
+    for (int q = 0; q < (kNeighbours ? 2 : 4); ++q) {
       const float4 e = token[q * stride + place];
       cs[2 * q] = make_float2(e.x, e.y);
       cs[2 * q + 1] = make_float2(e.z, e.w);
     }
-    if (mode == 1 && d0 < half) {
+  }
+  __device__ __forceinline__ void neighbours(float (&v)[8]) const {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cs[j].y = -cs[j].y;
+    for (int j = 0; j < 4; ++j) {
+      const float a = v[2 * j], b = v[2 * j + 1];
+      v[2 * j] = turned_value(a, cs[j].x, b, -cs[j].y);
+      v[2 * j + 1] = turned_value(b, cs[j].x, a, cs[j].y);
     }
+  }
+  // (the first half's partners count negatively: their signs are turned, two at a time where they have 16 bits)
+  template <typename T>
+  __device__ __forceinline__ void halves(const T* x, float (&v)[8]) const {
+    Raw8<T> other;
+    other.load(x + (d0 < half ? d0 + half : d0 - half));
+    other.flip(d0 < half);
+    float o[8];
+    other.values(o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = turned_value(v[j], cs[j].x, o[j], cs[j].y);
   }
   // v: the values at d0 of the head `x`
   template <typename T>
   __device__ __forceinline__ void apply(const T* x, float (&v)[8]) const {
-    if (mode == 0) return;
-    if (mode == 3) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = v[2 * j], b = v[2 * j + 1];
-        v[2 * j] = turned_value(a, cs[j].x, b, -cs[j].y);
-        v[2 * j + 1] = turned_value(b, cs[j].x, a, cs[j].y);
-      }
-      return;
-    }
-    float o[8];
-    if (mode == 1) {
-      Vec8<T>::load(x + (d0 < half ? d0 + half : d0 - half), o);
-    } else {
+    if (mode == 1) halves(x, v);
+    else if (mode == 3) neighbours(v);
+    else if (mode == 2) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int d = d0 + j;
-        o[j] = d < rotary ? static_cast<float>(x[d < half ? d + half : d - half]) : 0.f;
+        const float o = d < rotary ? static_cast<float>(x[d < half ? d + half : d - half]) : 0.f;
+        v[j] = turned_value(v[j], cs[j].x, o, cs[j].y);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = turned_value(v[j], cs[j].x, o[j], cs[j].y);
   }
 };
 
@@ -101,20 +136,24 @@ __device__ __forceinline__ int scale_exponent(float top) {
   return e < kLeast ? kLeast : e;
 }
 
-__device__ __forceinline__ uint2 to_codes(const float (&v)[8], float factor) {
+constexpr float kFinite = 3.402823466e38f;
+
+// finite: all of them are (else what is not is NaN: saturation would make a number of an infinity)
+__device__ __forceinline__ uint2 to_codes(const float (&v)[8], float factor, bool finite) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = v[j] * factor;
+  if (!finite) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!(fabsf(v[j]) <= kFinite)) x[j] = __uint_as_float(0x7fffffffu);
+  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t parts[2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int j = 4 * h + 2 * p;
-      // (an infinity as a NaN: saturation would make a number of it)
-      const float a = fabsf(v[j]) <= 3.402823466e38f ? v[j] * factor : __uint_as_float(0x7fffffffu);
-      const float b = fabsf(v[j + 1]) <= 3.402823466e38f ? v[j + 1] * factor : __uint_as_float(0x7fffffffu);
-      parts[p] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    }
-    w[h] = parts[0] | (parts[1] << 16);
+    const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * h], x[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * h + 2], x[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
+    w[h] = low | (high << 16);
   }
   return make_uint2(w[0], w[1]);
 }
@@ -135,127 +174,174 @@ __device__ __forceinline__ void new_tokens(const PagedCache& c, int b, int64_t& 
   start = static_cast<int64_t>(c.lengths[b]) - count;
 }
 
-// Eight values as they are in memory
-template <typename T>
-struct Raw8 {
-  uint4 w[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
+// The largest of all threads' (one barrier: `tops` is read until the next but one call, of the same)
+__device__ __forceinline__ float block_top(float top, float* tops) {
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = tops[0];
+  const int warps = blockDim.x / 32;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void values(float (&v)[8]) const { Vec8<T>::load(reinterpret_cast<const T*>(w), v); }
+  for (int w = 1; w < kThreads / 32; ++w)
+    if (w < warps) top = fmaxf(top, tops[w]);
+  return top;
+}
+
+// A page of one side, some of its heads, and the rows of it that a thread has
+template <typename T>
+struct PagePart {
+  const PagedAppend& a;
+  int h0, h1;
+  int64_t first;                 // the page's first position
+  int held, last;                // its older tokens, and where the new ones end
+  int places, rows, row, d0;
+  bool mine, real;               // whether the thread has rows, and values in them
+  const T* x;                    // its first new row of head h0
+  int64_t head_stride, step;     // ... to the next head, and to its next row
+  uint8_t* codes;                // head h0's
+  float* scales;
+  bool turned, shared;
+  int units, parts;              // float4 of a token's rotation, and of a place
 };
 
-// The heads [h0, h1) of a side of a page.  More than one row to a thread: the rotation's rows of the page's tokens go
-// through shared memory, in the order in which lanes read them (16 bytes of each of the places of a token side by side).
-template <typename T, int kRows>
-__device__ __forceinline__ void append_page(const PagedAppend& a, int64_t tile, int per_cta) {
-  const PagedCache& c = a.cache;
-  extern __shared__ __align__(16) float4 s_rot[];
-  __shared__ float s_top[2][kThreads / 32];
-  const int side = static_cast<int>(tile & 1);
-  tile >>= 1;
-  const int groups = (c.heads + per_cta - 1) / per_cta;
-  const int h0 = static_cast<int>(tile % groups) * per_cta, h1 = min(c.heads, h0 + per_cta);
-  tile /= groups;
-  const int spans = (c.n + c.page - 2) / c.page + 1;
-  const int b = static_cast<int>(tile / spans);
-  int64_t start;
-  int count;
-  new_tokens(c, b, start, count);
-  const int64_t from = start > 0 ? start : 0, end = start + count;      // positions that are written
-  const int64_t number = from / c.page + tile % spans;
-  if (from >= end || number * c.page >= end || number >= c.table_pages) return;
-  const int64_t id = c.table[static_cast<int64_t>(b) * c.table_pages + number];
-  if (id < 0 || id >= c.n_pages) return;
-  const int64_t first = number * c.page;
-  const int held = static_cast<int>(from > first ? from - first : 0);             // the page's older tokens
-  const int last = static_cast<int>(end - first < c.page ? end - first : c.page);
-  const int places = c.pitch / 8, rows = kThreads / places;
-  const int place = threadIdx.x % places, row = threadIdx.x / places;
-  const int d0 = place * 8;
-  const bool mine = row < rows, real = mine && d0 < c.dim;
-  const int64_t* stride = side ? a.v_stride : a.k_stride;
-  const T* x = static_cast<const T*>(side ? a.v : a.k) + b * stride[0] + (first - start) * stride[1] + d0;
+// How a page's values are taken: row by row as they come (0), or all rows of all threads new ones: as they are (1), turned
+// as halves (2) or as neighbours (3) from shared memory.
+template <typename T, int kRows, int kForm>
+__device__ __forceinline__ void append_heads(const PagePart<T>& p, Turn8 turn, const float4* s_rot, float (*s_top)[kThreads / 32]) {
+  const PagedCache& c = p.a.cache;
+  const T* x = p.x;
+  uint8_t* to = p.codes + (p.held + p.row) * c.pitch;
   const int64_t head_bytes = static_cast<int64_t>(c.page) * c.pitch;
-  uint8_t* codes = c.pages + (id * 2 + side) * c.heads * head_bytes + d0;
-  float* scales = c.scales + (id * 2 + side) * c.heads;
-  const bool turned = side == 0 && a.rot != nullptr;
-  Turn8 turn(d0, turned ? a.rotary : 0, a.interleaved);
-  const int half = a.rotary / 2, units = half / 2;                // float4 of a token's rotation
-  const int parts = a.interleaved ? 2 : 4;                        // ... of a place
-  const bool shared = kRows > 1 && turned && half % (2 * parts) == 0;
-  if (shared) {
-    for (int i = threadIdx.x; i < (last - held) * units; i += kThreads) {
-      const int t = i / units, u = i - t * units;
-      const int64_t pos = first + held + t;
-      s_rot[t * units + (u % parts) * (units / parts) + u / parts] =
-          pos < a.rot_rows ? reinterpret_cast<const float4*>(a.rot)[pos * units + u] : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __syncthreads();
-  }
-  auto slot_of = [&](int i) { return held + row + i * rows; };
-
+  auto new_row = [&](int i) { return kForm > 0 || p.held + p.row + i * p.rows < p.last; };
   Raw8<T> next[kRows];
-  auto fetch = [&](int h) {
+  auto fetch = [&] {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (real && slot_of(i) < last) next[i].load(x + h * stride[2] + slot_of(i) * stride[1]);
+    for (int i = 0; i < kRows; ++i) next[i].load(x + i * p.step);
   };
-  fetch(h0);
-  for (int h = h0; h < h1; ++h) {
-    const float old = held > 0 ? scales[h] : 0.f;
+  if constexpr (kForm > 0) fetch();
+  for (int h = p.h0; h < p.h1; ++h) {
+    const float old = kForm == 0 && p.held > 0 ? p.scales[h] : 0.f;
     float v[kRows][8];
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
+      if constexpr (kForm == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      const int slot = slot_of(i);
-      if (!real || slot >= last) continue;
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (!p.real || !new_row(i)) continue;
+        next[i].load(x + i * p.step);
+      }
       next[i].values(v[i]);
-      if (turned) {
-        if (first + slot < a.rot_rows) {
-          if (shared) turn.take(s_rot + (slot - held) * units, units / parts);
-          else if (kRows > 1 || h == h0) turn.read(a.rot, first + slot);
-          turn.apply(x + h * stride[2] + slot * stride[1] - d0, v[i]);
+      if constexpr (kForm >= 2) {
+        if (turn.mode != 0) {
+          turn.take<kForm == 3>(s_rot + (p.row + i * p.rows) * p.units, p.units / p.parts);
+          if constexpr (kForm == 2) turn.halves(x + i * p.step - p.d0, v[i]);
+          else turn.neighbours(v[i]);
+        }
+      } else if (kForm == 0 && p.turned) {
+        const int slot = p.held + p.row + i * p.rows;
+        if (p.first + slot < p.a.rot_rows) {
+          if (p.shared && turn.mode == 3) turn.take<true>(s_rot + (slot - p.held) * p.units, p.units / p.parts);
+          else if (p.shared && turn.mode == 1) turn.take<false>(s_rot + (slot - p.held) * p.units, p.units / p.parts);
+          else if (kRows > 1 || h == p.h0) turn.read(p.a.rot, p.first + slot);
+          turn.apply(x + i * p.step - p.d0, v[i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float size = fabsf(v[i][j]);
-        if (size <= 3.402823466e38f) top = fmaxf(top, size);
-      }
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]));
     }
-    if (h + 1 < h1) fetch(h + 1);
-    top = warp_max(top);
-    float* tops = s_top[h & 1];
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();      // (every thread has read the old scale, and is done with the tops of two heads before)
-    top = tops[0];
+    x += p.head_stride;
+    if (kForm > 0 && h + 1 < p.h1) fetch();        // under the barrier
+    top = block_top(top, s_top[h & 1]);        // (every thread has read the old scale)
+    const bool finite = top <= kFinite;
+    if (!finite) {                             // the largest of those that are
+      top = 0.f;
 #pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, tops[w]);
+      for (int i = 0; i < kRows; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[i][j]) <= kFinite ? fabsf(v[i][j]) : 0.f);
+      __syncthreads();
+      top = block_top(top, s_top[h & 1]);
+    }
     const int e = scale_exponent(top);
-    const float need = power_of_two(e), scale = fmaxf(old, need);
-    const float factor = scale == need ? power_of_two(-e) : 1.f / scale;
-    if (threadIdx.x == 0) scales[h] = scale;
-    uint8_t* to = codes + h * head_bytes;
+    const float need = power_of_two(e), scale = kForm > 0 ? need : fmaxf(old, need);
+    const float factor = kForm > 0 || scale == need ? power_of_two(-e) : 1.f / scale;
+    if (threadIdx.x == 0) p.scales[h] = scale;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
-      if (mine && slot_of(i) < last) *reinterpret_cast<uint2*>(to + slot_of(i) * c.pitch) = to_codes(v[i], factor);
-    if (held > 0 && scale != old && mine) {
+      if (kForm > 0 || (p.mine && new_row(i)))
+        *reinterpret_cast<uint2*>(to + i * p.rows * c.pitch) = to_codes(v[i], factor, finite);
+    if (kForm == 0 && p.held > 0 && scale != old && p.mine) {
       const float ratio = old * factor;
-      for (int slot = row; slot < held; slot += rows) {
-        uint2* at = reinterpret_cast<uint2*>(to + slot * c.pitch);
+      for (int slot = p.row; slot < p.held; slot += p.rows) {
+        uint2* at = reinterpret_cast<uint2*>(to + (slot - p.held - p.row) * c.pitch);
         float w[8];
         from_codes(*at, w);
-        *at = to_codes(w, ratio);
+        *at = to_codes(w, ratio, true);
       }
     }
+    to += head_bytes;
   }
+}
+
+// Some heads of a side of a page.  More than one row to a thread: the rotation's rows of the page's tokens go
+// through shared memory, in the order in which lanes read them (16 bytes of each of the places of a token side by side).
+template <typename T, int kRows>
+__device__ __forceinline__ void append_page(const PagedAppend& a, int tile, int per_cta, int rows) {
+  const PagedCache& c = a.cache;
+  extern __shared__ __align__(16) float4 s_rot[];
+  __shared__ float s_top[2][kThreads / 32];
+  const int side = tile & 1, groups = (c.heads + per_cta - 1) / per_cta, spans = (c.n + c.page - 2) / c.page + 1;
+  int rest = tile >> 1, at = rest / groups;
+  const int h0 = (rest - at * groups) * per_cta;
+  rest = at;
+  at = rest / spans;
+  const int b = at, span = rest - at * spans;
+  int64_t start;
+  int count;
+  new_tokens(c, b, start, count);
+  const int64_t from = start > 0 ? start : 0, end = start + count;      // positions that are written (of 32 bits, but for start)
+  const int64_t number = static_cast<int>(from) / c.page + static_cast<int64_t>(span);
+  if (from >= end || number * c.page >= end || number >= c.table_pages) return;
+  const int64_t id = c.table[static_cast<int64_t>(b) * c.table_pages + number];
+  if (id < 0 || id >= c.n_pages) return;
+  const int64_t first = number * c.page;
+  const int held = static_cast<int>(from > first ? from - first : 0), last = static_cast<int>(end - first < c.page ? end - first : c.page);
+  const int places = c.pitch / 8, place = threadIdx.x % places, row = threadIdx.x / places, d0 = place * 8;
+  const int64_t* stride = side ? a.v_stride : a.k_stride;
+  const bool turned = side == 0 && a.rot != nullptr;
+  const int half = a.rotary / 2, units = half / 2, parts = a.interleaved ? 2 : 4;
+  const PagePart<T> p{a, h0, min(c.heads, h0 + per_cta), first, held, last, places, rows, row, d0, row < rows, row < rows && d0 < c.dim,
+                      static_cast<const T*>(side ? a.v : a.k) + b * stride[0] + (first + held + row - start) * stride[1] +
+                          h0 * stride[2] + d0,
+                      stride[2], rows * stride[1],
+                      c.pages + ((id * 2 + side) * c.heads + h0) * static_cast<int64_t>(c.page) * c.pitch + d0,
+                      c.scales + (id * 2 + side) * c.heads, turned, kRows > 1 && turned && half % (2 * parts) == 0, units, parts};
+  if (p.shared) {
+    const int u = threadIdx.x % units, t0 = threadIdx.x / units, tokens = blockDim.x / units;      // (at most 32 units)
+    const int to = (u % parts) * (units / parts) + u / parts;
+    const float4* from_row = reinterpret_cast<const float4*>(a.rot) + (first + held) * units + u;
+    if (t0 < tokens) {
+#pragma unroll 4
+      for (int t = t0; t < last - held; t += tokens)
+        s_rot[t * units + to] = first + held + t < a.rot_rows ? from_row[t * units] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __syncthreads();
+  }
+  const Turn8 turn(d0, turned ? a.rotary : 0, a.interleaved);
+  if constexpr (kRows > 1) {
+    if (held == 0 && last == kRows * rows && places * rows == static_cast<int>(blockDim.x) && c.pitch == c.dim &&
+        (!turned || (p.shared && first + last <= a.rot_rows))) {
+      if (!turned) append_heads<T, kRows, 1>(p, turn, s_rot, s_top);
+      else if (a.interleaved) append_heads<T, kRows, 3>(p, turn, s_rot, s_top);
+      else append_heads<T, kRows, 2>(p, turn, s_rot, s_top);
+      return;
+    }
+  }
+  append_heads<T, kRows, 0>(p, turn, s_rot, s_top);
 }
 
 // The queries of a token
@@ -269,7 +355,7 @@ __device__ __forceinline__ void append_query(const PagedAppend& a, int64_t token
   const int64_t pos = start + t;
   const bool turned = a.rot != nullptr;
   const bool known = t < count && pos >= 0 && (!turned || pos < a.rot_rows);
-  const int places = c.dim / 8, rows = kThreads / places;
+  const int places = c.dim / 8, rows = blockDim.x / places;
   const int place = threadIdx.x % places, row = threadIdx.x / places;
   if (row >= rows) return;
   Turn8 turn(place * 8, turned ? a.rotary : 0, a.interleaved);
@@ -288,13 +374,13 @@ __device__ __forceinline__ void append_query(const PagedAppend& a, int64_t token
 }
 
 template <typename T, int kRows>
-__global__ void __launch_bounds__(kThreads, kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta) {
-  if (blockIdx.x < tiles) append_page<T, kRows>(a, blockIdx.x, per_cta);
+__global__ void __launch_bounds__(kThreads, kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta, int rows) {
+  if (blockIdx.x < tiles) append_page<T, kRows>(a, static_cast<int>(blockIdx.x), per_cta, rows);
   else append_query<T>(a, blockIdx.x - tiles);
 }
 
 template <typename T, int kRows>
-int launch_rows(const PagedAppend& a, int64_t tiles, int per_cta, unsigned grid, cudaStream_t stream) {
+int launch_rows(const PagedAppend& a, int64_t tiles, int per_cta, int rows, unsigned grid, cudaStream_t stream) {
   auto kernel = paged_append_kernel<T, kRows>;
   int bytes = 0;
   if (kRows > 1 && a.rot != nullptr) {
@@ -310,7 +396,8 @@ int launch_rows(const PagedAppend& a, int64_t tiles, int per_cta, unsigned grid,
     }
   }
   count_launch();
-  kernel<<<grid, kThreads, bytes, stream>>>(a, tiles, per_cta);
+  const int threads = (rows * (a.cache.pitch / 8) + 31) / 32 * 32;
+  kernel<<<grid, threads, bytes, stream>>>(a, tiles, per_cta, rows);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
@@ -347,20 +434,27 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
     a.q = nullptr;
   }
   // as many heads to a CTA as leave each SM some CTAs: they share the rotation's rows
-  int per_cta = 8;
+  int per_cta = 4;
   while (per_cta > 1 && pages * ((c.heads + per_cta - 1) / per_cta) < 6 * sm_count()) per_cta /= 2;
   const int64_t tiles = pages * ((c.heads + per_cta - 1) / per_cta);
   const int64_t ctas = tiles + (a.q != nullptr ? static_cast<int64_t>(c.B) * c.n : 0);
   if (ctas > 0x7fffffff) return 5;
   if (ctas == 0) return 0;
   const unsigned grid = static_cast<unsigned>(ctas);
-  const int rows = kThreads / (c.pitch / 8);
-  const int most = c.n < c.page ? c.n : c.page;           // new tokens of a page
-  const int per = (most + rows - 1) / rows;
-  if (per <= 1) return launch_rows<T, 1>(a, tiles, per_cta, grid, stream);
-  if (per <= 2) return launch_rows<T, 2>(a, tiles, per_cta, grid, stream);
-  if (per <= 4) return launch_rows<T, 4>(a, tiles, per_cta, grid, stream);
-  if (per <= 8) return launch_rows<T, 8>(a, tiles, per_cta, grid, stream);
+  // as many rows of threads as there are new tokens in a page, in powers of two, or a share of that: up to kThreads, no fewer
+  // than half of that where there are tokens enough or the queries' CTAs are in the launch
+  const int places = c.pitch / 8;
+  int rows = 1, per = 1;
+  while (rows < c.n && rows < c.page) rows *= 2;
+  while (rows * places > kThreads) {
+    rows /= 2;
+    per *= 2;
+  }
+  while (per == 1 && rows < c.page && rows * 2 * places <= kThreads / 2) rows *= 2;
+  if (per == 1) return launch_rows<T, 1>(a, tiles, per_cta, rows, grid, stream);
+  if (per == 2) return launch_rows<T, 2>(a, tiles, per_cta, rows, grid, stream);
+  if (per == 4) return launch_rows<T, 4>(a, tiles, per_cta, rows, grid, stream);
+  if (per == 8) return launch_rows<T, 8>(a, tiles, per_cta, rows, grid, stream);
   return 6;
 }
 

@@ -17,21 +17,30 @@ namespace {
 
 // V values as they are in memory: 16 bytes, or a single one
 template <typename T, int V>
-struct __align__(V == 1 ? sizeof(T) : 16) Values {
-  T v[V];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (V == 1) {
-      v[0] = *p;
+struct Values {
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = w; }
+  __device__ __forceinline__ uint32_t& word(int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+  // two values one after the other
+  __device__ __forceinline__ float2 get2(int i) {
+    if constexpr (sizeof(T) == 2) return pair_floats(word(i), T());
+    else return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+  }
+  __device__ __forceinline__ void set2(int i, float a, float b) {
+    if constexpr (sizeof(T) == 2) {
+      word(i) = pair_word(a, b, T());
     } else {
-      *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(p));
+      word(2 * i) = __float_as_uint(a);
+      word(2 * i + 1) = __float_as_uint(b);
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (V == 1) *p = v[0];
-    else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
-  }
-  __device__ __forceinline__ float get(int i) const { return static_cast<float>(v[i]); }
-  __device__ __forceinline__ void set(int i, float x) { v[i] = static_cast<T>(x); }
+};
+template <typename T>
+struct Values<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = v; }
 };
 
 // One place of a head for a thread: V values (16 bytes, or single ones) that are turned with V others, or copied.  Places
@@ -62,10 +71,15 @@ struct RotaryPlace {
   __device__ __forceinline__ void read(const float* table, int64_t pos, int rotary, float sign) {
     if (copy) return;
     const float2* row = reinterpret_cast<const float2*>(table) + pos * (rotary / 2) + entry;
+    if constexpr (V > 1) {
 #pragma unroll
-    for (int j = 0; j < kCs; ++j) {
-      cs[j] = row[j];
-      cs[j].y *= sign;
+      for (int j = 0; j < kCs; j += 2) {
+        const float4 two = *reinterpret_cast<const float4*>(row + j);
+        cs[j] = make_float2(two.x, two.y * sign);
+        cs[j + 1] = make_float2(two.z, two.w * sign);
+      }
+    } else {
+      cs[0] = make_float2(row[0].x, row[0].y * sign);
     }
   }
   __device__ __forceinline__ void load(const T* x, Values<T, V>& m, Values<T, V>& n) const {
@@ -82,70 +96,95 @@ struct RotaryPlace {
   }
   __device__ __forceinline__ void turn(Values<T, V>& m, Values<T, V>& n) const {
     if (copy) return;
+    if constexpr (V == 1) {
+      const float a = static_cast<float>(m.v), b = static_cast<float>(n.v);
+      m.v = static_cast<T>(turned_value(a, cs[0].x, b, -cs[0].y));
+      n.v = static_cast<T>(turned_value(b, cs[0].x, a, cs[0].y));
+    } else if constexpr (kNeighbours) {
 #pragma unroll
-    for (int j = 0; j < kCs; ++j) {
-      float a[2];
-      if constexpr (kNeighbours) { a[0] = m.get(2 * j); a[1] = m.get(2 * j + 1); }
-      else { a[0] = m.get(j); a[1] = n.get(j); }
-      const float x = turned_value(a[0], cs[j].x, a[1], -cs[j].y), y = turned_value(a[1], cs[j].x, a[0], cs[j].y);
-      if constexpr (kNeighbours) { m.set(2 * j, x); m.set(2 * j + 1, y); }
-      else { m.set(j, x); n.set(j, y); }
+      for (int j = 0; j < V / 2; ++j) {
+        const float2 a = m.get2(j);
+        m.set2(j, turned_value(a.x, cs[j].x, a.y, -cs[j].y), turned_value(a.y, cs[j].x, a.x, cs[j].y));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        const float2 a = m.get2(j), b = n.get2(j), c = cs[2 * j], d = cs[2 * j + 1];
+        m.set2(j, turned_value(a.x, c.x, b.x, -c.y), turned_value(a.y, d.x, b.y, -d.y));
+        n.set2(j, turned_value(b.x, c.x, a.x, c.y), turned_value(b.y, d.x, a.y, d.y));
+      }
     }
   }
 };
 
-// Rows of heads that a thread has on their way at a time
-constexpr int kRowsAhead = 3;
+// Rows of heads that a thread has on their way at a time: of 32 or of 16 bytes
+template <bool kTwo> constexpr int kAhead = kTwo ? 2 : 3;
 
+// A CTA has `tokens` tokens one after the other, all heads of each: what an address takes is computed once for all of them.
+// (Addresses by token and head, 64 bits wide, were half of the instructions: 4 x 2048 tokens of 48 heads of 128 49 us.)
 template <typename T, int V, bool kPairs>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall c, int rows) {
+__global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryCall c, int rows, int tokens) {
   using Place = RotaryPlace<T, V, kPairs>;
+  constexpr int kRowsAhead = kAhead<!Place::kNeighbours>;
   Place place(threadIdx.x, c.rotary);
-  for (int64_t token = blockIdx.x; token < c.B * c.S; token += gridDim.x) {
-    const int64_t b = token / c.S, s = token - b * c.S;
-    int64_t pos = c.at.start + s;
-    if (c.at.ids != nullptr) {
-      const int64_t at = b * c.at.batch_stride + s * c.at.token_stride;
-      pos = c.at.ids64 ? static_cast<const int64_t*>(c.at.ids)[at] : static_cast<const int32_t*>(c.at.ids)[at];
-    } else if (c.at.lengths != nullptr) {
-      const int64_t count = c.at.counts != nullptr ? min(max(static_cast<int64_t>(c.at.counts[b]), int64_t{0}), c.S) : c.S;
-      pos = s < count ? c.at.lengths[b] - count + s : -1;
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * tokens;
+  const int n = static_cast<int>(c.S - s0 < tokens ? c.S - s0 : tokens);
+  for (int64_t b = blockIdx.y; b < c.B; b += gridDim.y) {
+    int64_t start = c.at.start, count = c.S;       // positions that follow one another, of the first `count` tokens
+    if (c.at.lengths != nullptr) {
+      if (c.at.counts != nullptr) count = min(max(static_cast<int64_t>(c.at.counts[b]), int64_t{0}), c.S);
+      start = c.at.lengths[b] - count;
     }
-    const bool known = pos >= 0 && pos < c.table_rows;
     for (int row0 = threadIdx.y; row0 < rows; row0 += kRowsAhead * blockDim.y) {
-      Values<T, V> m[kRowsAhead], n[kRowsAhead];
+      const T* x[kRowsAhead];
       T* y[kRowsAhead];
-      bool turn[kRowsAhead];
+      int x_step[kRowsAhead], y_step[kRowsAhead];        // (of more than one token: see launch)
+      bool turn[kRowsAhead], mine[kRowsAhead];
 #pragma unroll
       for (int u = 0; u < kRowsAhead; ++u) {
         int h = row0 + u * blockDim.y;
-        y[u] = nullptr;
-        if (h >= rows) continue;
+        mine[u] = h < rows;
         // the parts' heads are rows one after the other
         int p = 0;
-        while (h >= c.part[p].heads) h -= c.part[p++].heads;
+        while (mine[u] && h >= c.part[p].heads) h -= c.part[p++].heads;
         const RotaryPart& part = c.part[p];
         turn[u] = part.turn;
-        y[u] = static_cast<T*>(part.y) + b * part.y_stride[0] + s * part.y_stride[1] + h * part.y_stride[2];
-        if (part.turn && !known) continue;
-        place.load(static_cast<const T*>(part.x) + b * part.x_stride[0] + s * part.x_stride[1] + h * part.x_stride[2], m[u], n[u]);
+        x[u] = static_cast<const T*>(part.x) + b * part.x_stride[0] + s0 * part.x_stride[1] + h * part.x_stride[2];
+        y[u] = static_cast<T*>(part.y) + b * part.y_stride[0] + s0 * part.y_stride[1] + h * part.y_stride[2];
+        x_step[u] = static_cast<int>(part.x_stride[1]);
+        y_step[u] = static_cast<int>(part.y_stride[1]);
       }
-      if (known && row0 == threadIdx.y) place.read(c.table, pos, c.rotary, c.transposed ? -1.f : 1.f);
-#pragma unroll
-      for (int u = 0; u < kRowsAhead; ++u) {
-        if (y[u] == nullptr) continue;
-        if (turn[u]) {
-          if (known) place.turn(m[u], n[u]);
-          else m[u] = n[u] = Values<T, V>{};        // (a position outside of the table)
+      for (int t = 0; t < n; ++t) {
+        int64_t pos = s0 + t < count ? start + s0 + t : -1;
+        if (c.at.ids != nullptr) {
+          const int64_t at = b * c.at.batch_stride + (s0 + t) * c.at.token_stride;
+          pos = c.at.ids64 ? static_cast<const int64_t*>(c.at.ids)[at] : static_cast<const int32_t*>(c.at.ids)[at];
         }
-        place.store(y[u], m[u], n[u]);
+        const bool known = pos >= 0 && pos < c.table_rows;
+        Values<T, V> m[kRowsAhead], n[kRowsAhead];
+#pragma unroll
+        for (int u = 0; u < kRowsAhead; ++u)
+          if (mine[u] && (known || !turn[u])) place.load(x[u], m[u], n[u]);
+        if (known) place.read(c.table, pos, c.rotary, c.transposed ? -1.f : 1.f);
+#pragma unroll
+        for (int u = 0; u < kRowsAhead; ++u) {
+          if (mine[u]) {
+            if (turn[u]) {
+              if (known) place.turn(m[u], n[u]);
+              else m[u] = n[u] = Values<T, V>{};        // (a position outside of the table)
+            }
+            place.store(y[u], m[u], n[u]);
+          }
+          x[u] += x_step[u];
+          y[u] += y_step[u];
+        }
       }
     }
   }
 }
 
 bool vectors(const RotaryCall& c, int v, int bytes) {
-  if (c.D % v != 0 || c.rotary % (c.interleaved ? v : 2 * v) != 0) return false;
+  if (c.D % v != 0 || c.rotary % (c.interleaved ? v : 2 * v) != 0 || (reinterpret_cast<uintptr_t>(c.table) & 15) != 0) return false;
   for (int p = 0; p < c.parts; ++p) {
     const RotaryPart& part = c.part[p];
     if (((reinterpret_cast<uintptr_t>(part.x) | reinterpret_cast<uintptr_t>(part.y)) & 15) != 0) return false;
@@ -166,17 +205,24 @@ int launch(const RotaryCall& c, cudaStream_t stream) {
   for (int p = 0; p < c.parts; ++p) heads += c.part[p].heads;
   if (places > 256) return 2;
   if (heads == 0) return 0;
-  // as few rounds over the heads as 256 threads take, with as few idle rows in the last one
-  const int most = 256 / places, rounds = (heads + most - 1) / most;
-  const int rows = (heads + rounds - 1) / rounds;
-  const int64_t tokens = c.B * c.S;
-  const unsigned grid = static_cast<unsigned>(tokens < 0x7fffffff ? tokens : 0x7fffffff);
-  const dim3 block(places, rows);
+  // as many rows to a thread as it has on their way at a time, in as few rounds as 256 threads take
+  const int most = 256 / places, ahead = wide && c.interleaved ? kAhead<false> : kAhead<true>;
+  const int each = heads < ahead ? heads : ahead, rounds = (heads + most * each - 1) / (most * each);
+  const int rows = (heads + each * rounds - 1) / (each * rounds);
+  // some tokens to a CTA where that leaves each SM CTAs enough
+  int tokens = 8;
+  for (int p = 0; p < c.parts; ++p)
+    for (const int64_t step : {c.part[p].x_stride[1], c.part[p].y_stride[1]})
+      if (step > 0x7fffffff || step < -0x7fffffff) tokens = 1;
+  while (tokens > 1 && c.B * ((c.S + tokens - 1) / tokens) < 12 * sm_count()) tokens /= 2;
+  const int64_t stretches = (c.S + tokens - 1) / tokens;
+  if (stretches > 0x7fffffff) return 5;
+  const dim3 block(places, rows), grid(static_cast<unsigned>(stretches), static_cast<unsigned>(c.B < 65535 ? c.B : 65535));
   count_launch();
-  if (wide && c.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(c, heads);
-  else if (wide) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(c, heads);
-  else if (c.interleaved) rotary_kernel<T, 1, true><<<grid, block, 0, stream>>>(c, heads);
-  else rotary_kernel<T, 1, false><<<grid, block, 0, stream>>>(c, heads);
+  if (wide && c.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(c, heads, tokens);
+  else if (wide) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(c, heads, tokens);
+  else if (c.interleaved) rotary_kernel<T, 1, true><<<grid, block, 0, stream>>>(c, heads, tokens);
+  else rotary_kernel<T, 1, false><<<grid, block, 0, stream>>>(c, heads, tokens);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
