@@ -26,8 +26,7 @@
 namespace slapo {
 namespace {
 
-// Warps of a CTA by the tiles of 8 rows that each has
-constexpr int warps_of(int tiles) { return tiles == 1 ? 12 : 8; }
+constexpr int kWarps = 8;          // (of up to 255 registers; twelve with one tile of rows each: 54.5 us where eight take 52.5)
 constexpr int kUnit = 32;          // keys: two blocks of 16
 constexpr int kLeastUnits = 2;     // of a warp's share
 
@@ -36,6 +35,7 @@ struct Plan {
   PagedAttention a;
   int group, rows, tiles, tile_rows, warps, words;     // tiles of rows per head; words: of a row's part
   int page_blocks;                                     // log2 of a page's blocks of 16 keys
+  int piece_inverse;                                   // 2^16 / (a token's pieces of 16 bytes), rounded up
   float scale_log2;
 };
 
@@ -59,10 +59,15 @@ __device__ __forceinline__ int64_t warp_sum_long(int64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// (a division of 64 bits takes some hundred instructions)
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+  if (a <= 0x7fffffff) return static_cast<int>(a) / b;
+  return a / b;
+}
 // Units of a warp's share, of `units` per item and all sequences
 __device__ __forceinline__ int64_t share_of(const Plan& p, int64_t units) {
   const int64_t total = units * p.a.cache.heads * p.tiles;
-  return max((total + p.warps - 1) / p.warps, static_cast<int64_t>(kLeastUnits));
+  return max(quotient(total + p.warps - 1, p.warps), static_cast<int64_t>(kLeastUnits));
 }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
@@ -137,8 +142,7 @@ struct Shape {
   static constexpr int kScales = 4 * kBlock;                      // where a unit's four scales are
   static constexpr int kStage = kScales + 16;
   static constexpr int kParts = kPartsOf<T>;
-  static constexpr int kWarps = warps_of(N);
-  static constexpr int kStages = kWide ? (N == 2 ? 3 : 2) : (N == 1 ? 4 : 5);
+  static constexpr int kStages = kWide ? (N <= 2 ? 3 : 2) : 5;
   static constexpr int kTiles = kWide ? 8 : 4;                    // of 16 values of a head
   static constexpr int kValues = kWide ? 16 : 8;                  // consecutive ones that a lane has
   // the queries' operands: in registers for one tile or two, beside the ring for more
@@ -198,14 +202,14 @@ __device__ __forceinline__ int begin_share(const Plan& p, int number, Cursor& at
     at.keys.first_unit = __shfl_sync(0xffffffffu, mine.first_unit, l);
     at.keys.units = __shfl_sync(0xffffffffu, mine.units, l);
     const int64_t in = target - (before + __shfl_sync(0xffffffffu, until, l) - at.keys.units * items);
-    at.item = static_cast<int>(in / at.keys.units);
+    at.item = static_cast<int>(quotient(in, at.keys.units));
     at.unit = static_cast<int>(in - static_cast<int64_t>(at.item) * at.keys.units);
     return static_cast<int>(min(per, all * items - target));
   }
 }
 
 template <bool kWide, int N, bool kSmallPages, typename T>
-__global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(const Plan p) {
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const Plan p) {
   using S = Shape<kWide, N, T>;
   extern __shared__ __align__(128) uint8_t s_ring[];
   const PagedCache& c = p.a.cache;
@@ -218,6 +222,8 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
   int to_issue = left;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(s_ring)) + warp * S::kWarp;
   const int head_bytes = c.page * c.pitch;
+  const int64_t side_bytes = c.heads * static_cast<int64_t>(head_bytes);
+  const uint8_t* lane_pages = c.pages + lane * 16;
   const int items = c.heads * p.tiles;
 
   Cursor in = at;
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
 #pragma unroll
   for (int i = 0; i < S::kCopies; ++i) {
     const int piece = i * 32 + lane;
-    row_of[i] = piece / pieces;        // 16 and more: none
+    row_of[i] = piece * p.piece_inverse >> 16;        // piece / pieces; 16 and more: none
     place[i] = S::place(row_of[i], piece - row_of[i] * pieces);
   }
   // (what lies behind a head's width is zeros from here on: the operands reach to 64 or 128 values)
@@ -273,7 +279,6 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
       // keys that no row sees are zeros: a hidden code may be a NaN
       const int until = in.keys.len - key0;
       const int from = p.a.window > 0 ? in.keys.len - in.keys.count - p.a.window + 1 - key0 : 0;
-      const int64_t side_bytes = c.heads * static_cast<int64_t>(head_bytes);
       const bool every = page[0] >= 0 && page[kPages - 1] >= 0 && until >= kUnit && from <= 0;
 #pragma unroll
       for (int block = 0; block < 2; ++block) {
@@ -282,7 +287,7 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
         const bool known = every || (id >= 0 && (!kSmallPages || (until > 16 * block && from < 16 * block + 16)));
         if (!known) missing |= 1u << (2 * stage + block);
         const int64_t side = (static_cast<int64_t>(known ? id : 0) * 2) * c.heads + h;
-        const uint8_t* k = c.pages + side * head_bytes + (((key0 + 16 * block) & (c.page - 1)) * c.pitch + lane * 16);
+        const uint8_t* k = lane_pages + side * head_bytes + ((key0 + 16 * block) & (c.page - 1)) * c.pitch;
         const uint8_t* v = k + side_bytes;
         const uint32_t k_to = to + 2 * block * S::kBlock, v_to = k_to + S::kBlock;
         if (every) {
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Plan p, int ti
   const int units = __shfl_sync(0xffffffffu, keys.units, b & 31);
   const int64_t per = share_of(p, sum_all);
   const int64_t begin = before * items + static_cast<int64_t>(item) * units;
-  const int w0 = static_cast<int>(begin / per), w1 = static_cast<int>((begin + units - 1) / per);
+  const int w0 = static_cast<int>(begin / per), w1 = static_cast<int>((begin + max(units, 1) - 1) / per);
   pdl_wait();
   if (row >= p.rows || (units > 0 && w0 == w1)) return;
   const int token = row / p.group;
@@ -691,14 +696,14 @@ Plan make_plan(const PagedAttention& a) {
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
   p.page_blocks = 0;
   while ((16 << p.page_blocks) < c.page) ++p.page_blocks;
+  p.piece_inverse = (65536 + c.pitch / 16 - 1) / (c.pitch / 16);        // (exact for the 128 pieces of a block)
   p.words = c.dim + 4;           // (rows on 16 bytes)
   p.scale_log2 = a.scale * kLog2e;
   // units if all sequences fill their rows of the table
   const int64_t units = static_cast<int64_t>(c.B) * c.heads * p.tiles *
                         ((static_cast<int64_t>(c.table_pages) * c.page + kUnit - 1) / kUnit);
-  const int warps = warps_of(p.tile_rows / 8);
-  const int64_t ctas = (units + kLeastUnits * warps - 1) / (kLeastUnits * warps);
-  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * warps;
+  const int64_t ctas = (units + kLeastUnits * kWarps - 1) / (kLeastUnits * kWarps);
+  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * kWarps;
   return p;
 }
 
@@ -716,7 +721,7 @@ int launch_tiles(const Plan& p, cudaStream_t stream) {
     configured[device] = true;
   }
   count_launch();
-  kernel<<<p.warps / S::kWarps, S::kWarps * 32, S::kSmem, stream>>>(p);
+  kernel<<<p.warps / kWarps, kWarps * 32, S::kSmem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 4;
   cudaLaunchConfig_t config{};
   const int tile_rows = p.rows < p.tile_rows ? p.rows : p.tile_rows;
