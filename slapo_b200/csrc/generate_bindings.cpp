@@ -157,7 +157,7 @@ slapo::PagedCache check_cache(const Tensor& pages, const Tensor& scales, const T
     TORCH_CHECK_VALUE(counts->dim() == 1 && counts->size(0) == b && counts->is_contiguous(), what, ": contiguous counts [", b,
                       "] required, not ", counts->sizes());
   }
-  TORCH_CHECK_VALUE(block_table.size(1) * t <= INT_MAX && pages.size(0) <= INT_MAX && pages.size(2) <= 65535 && b <= INT_MAX &&
+  TORCH_CHECK_VALUE(block_table.size(1) * t <= INT_MAX - 256 && pages.size(0) <= INT_MAX && pages.size(2) <= 65535 && b <= INT_MAX &&
                         q_like.size(1) <= INT_MAX - 256 && q_like.size(2) <= 65535,
                     what, ": more tokens, pages or heads than have a number");
   slapo::PagedCache c{};

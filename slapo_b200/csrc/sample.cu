@@ -157,6 +157,25 @@ struct Slice {
   // every bank once
   __device__ __forceinline__ int stretch() const { return ((size + kThreads - 1) / kThreads) | 1; }
 
+  // The least key whose bin is `bin` or one before, found by the lanes of each warp together: comparing keys costs a
+  // fifth of a bin's number.  `top`: the row's largest key.
+  __device__ __forceinline__ unsigned least_key(int bin, unsigned top) const {
+    const unsigned lane = threadIdx.x & 31;
+    auto in = [&](unsigned key) { return key >= top || (key != 0u && row.bin(key) <= bin); };      // (no keys above the top)
+    unsigned base = 0u;                     // at most what is looked for, which is within 32 probes
+#pragma unroll 1
+    for (int shift = 27; shift > 0; shift -= 5) {
+      const unsigned votes = __ballot_sync(0xffffffffu, in(base + (lane << shift)));
+      const unsigned from = votes == 0u ? 32u : __ffs(votes) - 1u;
+      if (from != 0u) base += (from - 1u) << shift;
+    }
+    // (six rounds of five bits and two more)
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i, ++base)
+      if (in(base)) break;
+    return base;
+  }
+
   // Sums over the cluster of a value of each CTA
   __device__ __forceinline__ unsigned long long everywhere(unsigned long long mine) {
     const unsigned long long w = warp_total(mine);
@@ -369,12 +388,14 @@ struct Slice {
 
   // The row by the first CTA alone, from the `number` elements of the bins up to `bin`, at most kList, after count_bins:
   // the token (in all threads of the first CTA).  top_k: 0: all; mass: of all that top_k keeps, or 0: to be summed.
-  __device__ __forceinline__ int finish(int bin, unsigned number, unsigned top_k, double top_p, double min_p, unsigned long long mass, double u) {
+  __device__ __forceinline__ int finish(int bin, unsigned number, unsigned top_k, double top_p, double min_p, unsigned long long mass, double u,
+                                        unsigned top) {
     // Each CTA's into the first one's list, in the order of the indices: behind those of the CTAs before it, each thread a
     // stretch of the slice.  (Barriers: the others' bins are read; the list is whole.  CTAs that are done leave.)
     cluster.barrier_arrive();
     const int t0 = threadIdx.x * stretch(), t1 = min(size, t0 + stretch());
-    auto taken = [&](int i) { return keys[i] != 0u && row.bin(keys[i]) <= bin; };
+    const unsigned least = least_key(bin, top);
+    auto taken = [&](int i) { return keys[i] >= least; };
     const unsigned lower = static_cast<int>(threadIdx.x) <= bin ? mine_before : 0u;
     const unsigned lower_warp = __reduce_add_sync(0xffffffffu, lower);
     if ((threadIdx.x & 31) == 0 && lower_warp != 0u) atomicAdd(&s.before_cta, lower_warp);
@@ -521,13 +542,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
 
   // the last place that is kept
   unsigned long long border = 0ull;
-  const double least = static_cast<double>(min_p);
+  const double least = static_cast<double>(fminf(min_p, 1.f));        // (the largest is kept, and its equals)
   bool binned = false;
   if (top_k > 0 && top_k < c.vocab) {
     const Limit limit{false, static_cast<unsigned>(top_k), 0.0, 0ull};
     at.count_bins(limit);
     if (s.bin >= 0 && s.above_count + s.in_bin <= kList) {
-      const int token = at.finish(s.bin, s.above_count + s.in_bin, static_cast<unsigned>(top_k), top_p, least, 0ull, u);
+      const int token = at.finish(s.bin, s.above_count + s.in_bin, static_cast<unsigned>(top_k), top_p, least, 0ull, u, top);
       if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
       return;
     }
@@ -544,7 +565,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
     }
     at.count_bins(limit);
     if (!binned && s.bin >= 0 && s.above_count + s.in_bin <= kList) {
-      const int token = at.finish(s.bin, s.above_count + s.in_bin, 0u, top_p, least, s.total_mass, u);
+      const int token = at.finish(s.bin, s.above_count + s.in_bin, 0u, top_p, least, s.total_mass, u, top);
       if (rank == 0 && threadIdx.x == 0) c.out[r] = token;
       return;
     }
@@ -552,11 +573,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleCall c, in
   }
   // each thread a stretch of the slice, in the order of the indices
   const int stretch = at.stretch(), t0 = threadIdx.x * stretch, t1 = min(size, t0 + stretch);
+  const unsigned border_key = Slice::key_at(border);
   auto weight = [&](int i) -> unsigned long long {
     const unsigned k = s_keys[i];
-    if (k == 0u || at.place(i) < border) return 0ull;
+    if (k < border_key || k == 0u || (k == border_key && at.place(i) < border)) return 0ull;
     const double f = row.fraction(k);
-    return f >= least || k == top ? Row::held(f) : 0ull;
+    return f >= least ? Row::held(f) : 0ull;
   };
   unsigned long long mine = 0ull, all;
 #pragma unroll 4

@@ -121,8 +121,8 @@ def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None,
     ``rotary_table``: keys - and ``q [B, n, heads, D]`` - are rotated by their positions on the way
     (:func:`slapo_b200.ops.functional.rotary`); without one they stay as they are.  New tokens have positions
     ``lengths[b] - counts[b]`` on; those before position 0 (left padding), behind the block table's end or in a page
-    that there is not are not kept, a query that is none (behind ``counts[b]``, before position 0, behind the
-    rotation's table) is zeros.  A page takes tokens of one sequence: pages that several share have to be full.
+    that there is not are not kept, a query that is none (behind ``counts[b]``, before position 0) is zeros, and so
+    are a query and a key behind the rotation's table.  A page takes tokens of one sequence: pages that several share have to be full.
 
     A value is off by at most 2^-4 of itself, or half of 2^-9 of its page's scale if it is small; values that are
     not finite are held as NaN.  A page's first token sets its scale anew; where a later one is too large for it, the
@@ -248,6 +248,7 @@ class PagedKVCache:
         self._counts = torch.zeros(batch, dtype=torch.int32, device=device)
         self.counts = None          # of the step: None where each sequence brings all of its tokens
         self.fresh = False          # the step's tokens are the first ones of all sequences
+        self.width = 0              # of the step: its most new tokens of a sequence
         self._tables = torch.full((batch, per), -1, dtype=torch.int32)      # the host's copies
         self._tokens = [0] * batch
         self._owned = [[] for _ in range(batch)]
@@ -275,7 +276,7 @@ class PagedKVCache:
             need.append((self._tokens[i] + c + self.page - 1) // self.page - len(self._owned[i]))
         if sum(need) > len(self._free):
             raise RuntimeError(f"the step needs {sum(need)} pages, {len(self._free)} are free")
-        self.fresh = not any(self._tokens)
+        self.fresh, self.width = not any(self._tokens), max(each, default=0)
         for i, c in enumerate(each):
             for _ in range(need[i]):
                 self._tables[i, len(self._owned[i])] = self._free[-1]
@@ -318,6 +319,8 @@ class PagedLayer:
 
     def append(self, k, v, q=None, rotary_table=None, interleaved=False):
         c = self.cache
+        if k.shape[:2] != (c.batch, c.width):
+            raise ValueError(f"the step has room for {c.width} tokens of {c.batch} sequences, not {tuple(k.shape[:2])}")
         return paged_append(c.pages[self.index], c.scales[self.index], k, v, c.block_table, c.lengths, c.counts, q,
                             rotary_table, interleaved)
 

@@ -47,6 +47,7 @@ def sample_reference(logits, uniform, temperature, top_k, top_p, min_p):
 
     temperature, top_p, min_p = (each(v, torch.float64) for v in (temperature, top_p, min_p))
     top_k = each(top_k, torch.int64)
+    min_p = torch.fmin(min_p, torch.ones_like(min_p))        # (the largest is kept, and its equals)
     value, index = torch.sort(x, dim=1, descending=True, stable=True)
     there = value > -float("inf")
     value = value.double()

@@ -397,6 +397,13 @@ def test_sampling_settings_for_each_row():
     got = NF.sample(x, u, torch.tensor([1.0, 0.0, 1.0, 1.0]), torch.tensor([0, 0, 2, 0], dtype=torch.int32),
                     torch.tensor([1.0, 1.0, 1.0, 0.1]), torch.tensor([0.0, 0.0, 0.9, 0.0]))
     assert got.tolist() == [0, 1, 1, 1]
+    # settings beyond their range, which a tensor of them can have: all there is, or the largest
+    one = torch.ones(4)
+    got = NF.sample(x, u, one, torch.full((4,), -3, dtype=torch.int32), 2 * one, -one)
+    assert got.tolist() == [0, 0, 3, 0]
+    for args in ((one, torch.zeros(4, dtype=torch.int32), -one, 0 * one), (one, torch.zeros(4, dtype=torch.int32), one, 2 * one),
+                 (-one, torch.zeros(4, dtype=torch.int32), one, 0 * one)):
+        assert NF.sample(x, u, *args).tolist() == [1, 1, 1, 1]
 
 
 def sample_refusals(device):
@@ -484,6 +491,9 @@ def test_generation_over_pages_is_generation(fused, window):
         FlashAttention(32, 2, causal=True, window=3, sinks=1)(x[:, :1], layer_past=present)
     with pytest.raises(RuntimeError):
         layer(x[:, :1], layer_past=present)
+    for other in (x[:, :2], x[:1, :1]):              # the step has room for one token of two sequences
+        with pytest.raises(ValueError), torch.no_grad():
+            layer(other, layer_past=present)
     with pytest.raises(ValueError):
         FlashAttention(32, 2, rotary=RotaryEmbedding(18, 8))
 

@@ -219,6 +219,28 @@ def test_append_rotates_as_rotary_does(dim, rotated, interleaved, dtype):
         assert torch.equal(pages.view(torch.uint8), other[0].view(torch.uint8))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_many_tokens_is_the_oracle(interleaved):
+    """Ragged, on top of what is there, some behind the rotation's table: queries by a launch of their own."""
+    from slapo_b200.ops.paged import paged_append_reference
+
+    rot = NF.rotary_table(40, 900, device="cuda")
+    k, v = (torch.randn(3, 700, 2, 80, device="cuda").half() for _ in range(2))
+    q = torch.randn(3, 700, 6, 80, device="cuda").half()
+    mine, oracle = (make_cache(3, 32, 2, 80, 32, "cuda") for _ in range(2))
+    for lengths, counts in (([5, 300, 1], [5, 300, 1]), ([705, 950, 1], [700, 650, 0])):
+        lengths, counts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, counts))
+        got = NF.paged_append(mine[0], mine[1], k, v, mine[2], lengths, counts, q, rot, interleaved)
+        want = paged_append_reference(oracle[0], oracle[1], k, v, oracle[2], lengths, counts, q, rot, interleaved)
+        # products and sum in fp32 in another order, then fp16; e4m3: another side of a border now and then
+        assert bool(((got.float() - want.float()).abs() <= 2.0 ** -10 * want.float().abs() + 2.0 ** -22).all())
+        a, b = mine[0].float(), oracle[0].float()
+        assert torch.equal(a.isnan(), b.isnan())
+        a, b = a.nan_to_num(0.0), b.nan_to_num(0.0)
+        assert bool(((a - b).abs() <= 2.0 ** -3 * b.abs() + 2.0 ** -9).all()) and float((a != b).float().mean()) < 1e-3
+        assert torch.equal(mine[1].nan_to_num(0.0), oracle[1].nan_to_num(0.0))
+
+
 # ---------------------------------------------------------------------- #
 # attention
 def _filled(b, lengths, kv, dim, page, seed=0, spread=1.0):
@@ -419,6 +441,8 @@ def test_sampling_rows_of_their_own_and_strides():
     wide = torch.empty(8, 5003, device="cuda")[:, 1:5001].copy_(x)
     assert torch.equal(NF.sample(wide, u, t, k, p, m), want)
     assert torch.equal(NF.sample(x.t().contiguous().t(), u, t, k, p, m), want)
+    for more in ((t, k, p + 1, m), (t, -k, p, m + 1), (-t, k, p, m), (t, k, -p, m)):
+        _sample(x, u, **dict(zip(("temperature", "top_k", "top_p", "min_p"), more)))
     assert NF.sample(x[:0], u[:0]).shape == (0,)
     assert int(NF.sample(x[3], u[3], 0.0)) == int(x[3].argmax())
 
