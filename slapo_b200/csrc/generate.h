@@ -32,6 +32,7 @@ struct RotaryCall {
   int64_t B, S;
   int D, rotary;
   bool interleaved, transposed;      // transposed: the gradient's direction
+  bool beside;                       // the kernel launched before may still run, and says when this one may begin
   int dtype;
 };
 int launch_rotary(const RotaryCall& c, cudaStream_t stream);

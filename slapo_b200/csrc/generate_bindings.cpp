@@ -1,6 +1,7 @@
 // torch bindings of rotation by positions, the paged cache in 8 bits and sampling.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -15,6 +16,11 @@ namespace {
 
 using at::Tensor;
 using c10::optional;
+
+// A new contiguous tensor on the current device, without the dispatcher (half a microsecond less)
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 
 int dtype_code(const Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -80,7 +86,7 @@ std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>
   Tensor k, out_q, out_k;
   slapo::RotaryCall c{};
   if (packed) {
-    out_q = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
+    out_q = empty(q.sizes(), q.scalar_type(), q);
     for (int i = 0; i < 3; ++i) c.part[i] = part(q, out_q, i < 2, i);
     c.parts = 3;
   } else {
@@ -90,8 +96,8 @@ std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>
                           k_in->size(2) <= INT_MAX,
                       "rotary: k [B, S, heads, D] of q's tokens and width required: ", k_in->sizes(), " and ", q.sizes());
     k = heads_in_rows(*k_in);
-    out_q = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
-    out_k = at::empty(k.sizes(), k.options(), at::MemoryFormat::Contiguous);
+    out_q = empty(q.sizes(), q.scalar_type(), q);
+    out_k = empty(k.sizes(), k.scalar_type(), k);
     c.part[0] = part(q, out_q, true);
     c.part[1] = part(k, out_k, true);
     c.parts = 2;
@@ -214,12 +220,12 @@ Tensor paged_append(const Tensor& pages, const Tensor& scales, const Tensor& k_i
                           q_in->size(3) == k_in.size(3) && q_in->size(2) <= 65535,
                       "paged_append: q [B, n, heads, D] of k's tokens and width required: ", q_in->sizes(), " and ", k_in.sizes());
     q = vectors(*q_in);
-    out = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
+    out = empty(q.sizes(), q.scalar_type(), q);
     a.q = q.const_data_ptr();
     a.q_out = out.data_ptr();
     a.q_heads = static_cast<int>(q.size(2));
   } else {
-    out = at::empty({0}, k.options());
+    out = empty({0}, k.scalar_type(), k);
   }
   a.k = k.const_data_ptr();
   a.v = v.const_data_ptr();
@@ -248,7 +254,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& pages, const Tensor& sc
   TORCH_CHECK_VALUE(q_in.size(1) * std::max<int64_t>(q_in.size(2), 1) <= INT_MAX - 256, "paged_attention: too many queries");
   c10::cuda::CUDAGuard guard(q_in.device());
   const Tensor q = vectors(q_in);
-  Tensor out = at::empty(q.sizes(), q.options(), at::MemoryFormat::Contiguous);
+  Tensor out = empty(q.sizes(), q.scalar_type(), q);
   a.q = q.const_data_ptr();
   for (int d = 0; d < 3; ++d) a.q_stride[d] = q.stride(d);
   a.q_heads = static_cast<int>(q.size(2));
@@ -258,7 +264,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& pages, const Tensor& sc
   a.bf16 = q.scalar_type() == at::kBFloat16;
   Tensor scratch;
   if (out.numel() > 0) {
-    scratch = at::empty({slapo::paged_attention_words(a)}, q.options().dtype(at::kFloat));
+    scratch = empty({slapo::paged_attention_words(a)}, at::kFloat, q);
     a.scratch = scratch.data_ptr<float>();
   }
   const int rc = slapo::launch_paged_attention(a, at::cuda::getCurrentCUDAStream().stream());
@@ -298,7 +304,7 @@ Tensor sample(const Tensor& logits_in, const Tensor& uniform, const slapo::Setti
                     min_p.value);
   c10::cuda::CUDAGuard guard(logits_in.device());
   const Tensor logits = logits_in.dim() == 2 && logits_in.stride(1) == 1 ? logits_in : logits_in.reshape({rows, vocab}).contiguous();
-  Tensor out = at::empty(logits_in.sizes().slice(0, logits_in.dim() - 1), logits.options().dtype(at::kLong));
+  Tensor out = empty(logits_in.sizes().slice(0, logits_in.dim() - 1), at::kLong, logits);
   c.logits = logits.const_data_ptr();
   c.row_stride = logits.stride(0);
   c.uniform = uniform.const_data_ptr<float>();

@@ -375,6 +375,7 @@ __device__ __forceinline__ void append_query(const PagedAppend& a, int64_t token
 
 template <typename T, int kRows>
 __global__ void __launch_bounds__(kThreads, kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta, int rows) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // (the queries' kernel waits for nothing of this one)
   if (blockIdx.x < tiles) append_page<T, kRows>(a, static_cast<int>(blockIdx.x), per_cta, rows);
   else append_query<T>(a, blockIdx.x - tiles);
 }
@@ -406,9 +407,11 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
   PagedAppend a = a_in;
   const PagedCache& c = a.cache;
   const int64_t spans = (c.n + c.page - 2) / c.page + 1, pages = c.B * spans * 2;
-  // Many tokens: their queries by the rotation's own kernel, which has more bytes on their way.  (Few: one launch.)
-  if (a.q != nullptr && a.rot != nullptr && static_cast<int64_t>(c.B) * c.n >= 4 * sm_count()) {
-    RotaryCall r{};
+  // Many tokens: their queries by the rotation's own kernel, which has more bytes on their way, beside this one's last CTAs.
+  // (Few: one launch.)
+  RotaryCall r{};
+  const bool apart = a.q != nullptr && a.rot != nullptr && static_cast<int64_t>(c.B) * c.n >= 4 * sm_count();
+  if (apart) {
     RotaryPart& p = r.part[0];
     p.x = a.q;
     p.y = a.q_out;
@@ -429,8 +432,7 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
     r.rotary = a.rotary;
     r.interleaved = a.interleaved;
     r.dtype = a.dtype;
-    const int rc = launch_rotary(r, stream);
-    if (rc != 0) return rc;
+    r.beside = true;
     a.q = nullptr;
   }
   // as many heads to a CTA as leave each SM some CTAs: they share the rotation's rows
@@ -439,7 +441,10 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
   const int64_t tiles = pages * ((c.heads + per_cta - 1) / per_cta);
   const int64_t ctas = tiles + (a.q != nullptr ? static_cast<int64_t>(c.B) * c.n : 0);
   if (ctas > 0x7fffffff) return 5;
-  if (ctas == 0) return 0;
+  if (ctas == 0) {
+    r.beside = false;
+    return apart ? launch_rotary(r, stream) : 0;
+  }
   const unsigned grid = static_cast<unsigned>(ctas);
   // as many rows of threads as there are new tokens in a page, in powers of two, or a share of that: up to kThreads, no fewer
   // than half of that where there are tokens enough or the queries' CTAs are in the launch
@@ -451,11 +456,12 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
     per *= 2;
   }
   while (per == 1 && rows < c.page && rows * 2 * places <= kThreads / 2) rows *= 2;
-  if (per == 1) return launch_rows<T, 1>(a, tiles, per_cta, rows, grid, stream);
-  if (per == 2) return launch_rows<T, 2>(a, tiles, per_cta, rows, grid, stream);
-  if (per == 4) return launch_rows<T, 4>(a, tiles, per_cta, rows, grid, stream);
-  if (per == 8) return launch_rows<T, 8>(a, tiles, per_cta, rows, grid, stream);
-  return 6;
+  int rc = 6;
+  if (per == 1) rc = launch_rows<T, 1>(a, tiles, per_cta, rows, grid, stream);
+  else if (per == 2) rc = launch_rows<T, 2>(a, tiles, per_cta, rows, grid, stream);
+  else if (per == 4) rc = launch_rows<T, 4>(a, tiles, per_cta, rows, grid, stream);
+  else if (per == 8) rc = launch_rows<T, 8>(a, tiles, per_cta, rows, grid, stream);
+  return rc == 0 && apart ? launch_rotary(r, stream) : rc;
 }
 
 }  // namespace

@@ -117,15 +117,16 @@ struct RotaryPlace {
   }
 };
 
-// Rows of heads that a thread has on their way at a time: of 32 or of 16 bytes
-template <bool kTwo> constexpr int kAhead = kTwo ? 2 : 3;
+// Rows of heads that a thread has on their way at a time.  (4 x 2048 packed tokens of 16 heads of 128, and 8 x 2048 of 16 and 2
+// heads, us: three rows and up to 128 registers 39.3 and 33.2, two and 64 39.1 and 37.3, three and 80 42.9 and 39.6, two and
+// 48 53 and 46, four 38.9 and 37.2.)
+constexpr int kRowsAhead = 3;
 
 // A CTA has `tokens` tokens one after the other, all heads of each: what an address takes is computed once for all of them.
 // (Addresses by token and head, 64 bits wide, were half of the instructions: 4 x 2048 tokens of 48 heads of 128 49 us.)
 template <typename T, int V, bool kPairs>
-__global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryCall c, int rows, int tokens) {
+__global__ void __launch_bounds__(256, 2) rotary_kernel(const RotaryCall c, int rows, int tokens) {
   using Place = RotaryPlace<T, V, kPairs>;
-  constexpr int kRowsAhead = kAhead<!Place::kNeighbours>;
   Place place(threadIdx.x, c.rotary);
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * tokens;
   const int n = static_cast<int>(c.S - s0 < tokens ? c.S - s0 : tokens);
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryCall c, int 
       }
     }
   }
+  if (c.beside) asm volatile("griddepcontrol.wait;" ::: "memory");        // (what comes after has to find both done)
 }
 
 bool vectors(const RotaryCall& c, int v, int bytes) {
@@ -206,8 +208,7 @@ int launch(const RotaryCall& c, cudaStream_t stream) {
   if (places > 256) return 2;
   if (heads == 0) return 0;
   // as many rows to a thread as it has on their way at a time, in as few rounds as 256 threads take
-  const int most = 256 / places, ahead = wide && c.interleaved ? kAhead<false> : kAhead<true>;
-  const int each = heads < ahead ? heads : ahead, rounds = (heads + most * each - 1) / (most * each);
+  const int most = 256 / places, each = heads < kRowsAhead ? heads : kRowsAhead, rounds = (heads + most * each - 1) / (most * each);
   const int rows = (heads + each * rounds - 1) / (each * rounds);
   // some tokens to a CTA where that leaves each SM CTAs enough
   int tokens = 8;
@@ -219,11 +220,21 @@ int launch(const RotaryCall& c, cudaStream_t stream) {
   if (stretches > 0x7fffffff) return 5;
   const dim3 block(places, rows), grid(static_cast<unsigned>(stretches), static_cast<unsigned>(c.B < 65535 ? c.B : 65535));
   count_launch();
-  if (wide && c.interleaved) rotary_kernel<T, V, true><<<grid, block, 0, stream>>>(c, heads, tokens);
-  else if (wide) rotary_kernel<T, V, false><<<grid, block, 0, stream>>>(c, heads, tokens);
-  else if (c.interleaved) rotary_kernel<T, 1, true><<<grid, block, 0, stream>>>(c, heads, tokens);
-  else rotary_kernel<T, 1, false><<<grid, block, 0, stream>>>(c, heads, tokens);
-  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = c.beside ? 1 : 0;
+  const cudaError_t done =
+      wide && c.interleaved ? cudaLaunchKernelEx(&config, rotary_kernel<T, V, true>, c, heads, tokens)
+      : wide                ? cudaLaunchKernelEx(&config, rotary_kernel<T, V, false>, c, heads, tokens)
+      : c.interleaved       ? cudaLaunchKernelEx(&config, rotary_kernel<T, 1, true>, c, heads, tokens)
+                            : cudaLaunchKernelEx(&config, rotary_kernel<T, 1, false>, c, heads, tokens);
+  return done == cudaSuccess ? 0 : 4;
 }
 
 }  // namespace

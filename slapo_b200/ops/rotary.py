@@ -120,13 +120,13 @@ def _positions(q, positions):
 
 
 def _rotary(q, k, table, positions, interleaved):
-    from . import functional as NF
-
     if torch.is_tensor(q) and q.is_cuda:
         fn = native.direct("rotary")
         out = None if fn is None else fn(q, k, table, positions, interleaved)
         if out is not None:
             return out
+    from . import functional as NF
+
     _check(q, k, table, positions)
     if NF._native_ok(q):
         tensor = torch.is_tensor(positions)
