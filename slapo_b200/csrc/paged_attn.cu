@@ -3,20 +3,22 @@
 // Row r of a cached head is query t = r / G of query head r % G of its G; it sees the keys up to its own position (and
 // not before its window).  With codes k, v and a page's scales ks, vs: s = ks (q k) scale, o = sum p vs v / sum p.
 //
-// Bound by reading the cache.  A warp works alone, on units of 32 keys of one head: S^T = K Q^T by m16n8k32 of e4m3 numbers
-// (16 keys, 8 rows), the keys' codes as they are and the queries taken apart into two or three, and O^T += V^T P^T by
-// m16n8k16 of fp16 (16 values of a head, 8 rows), codes converted - exactly - on their way into the registers.  The
-// tensor core's order of the contraction is free as long as both operands share it, so that a lane's 16 bytes of a key are its
-// operands of two products, and 16 bytes each of four values' rows, bytes interleaved, those of eight.  Units come by
-// cp.async, 512 bytes of a page side by side at a time (lanes that copied what they read themselves, 64 bytes of each of
-// eight tokens at a time, took 1.3 times as long), into a ring in shared memory of the warp's own: no barriers.  mma.sync and
-// not tcgen05: a unit has one to eight rows of work, and the values pass through registers, since they are converted.
+// Bound by reading the cache and, nearly as much, by the instructions around it.  A warp works alone, on units of 32 keys of
+// one head: S^T = K Q^T by m16n8k16 of fp16 (16 keys, 8 rows), O^T += V^T P^T (16 values of a head, 8 rows), codes
+// converted - exactly - on their way into the registers (products of e4m3 numbers, with the queries taken apart into two or
+// three, are converted by the hardware's own instructions: as many).  The tensor core's order of the contraction is free as
+// long as both operands share it, so that a lane's 16 bytes of a key are its operands of four products, and 16 bytes each of
+// four values' rows, bytes interleaved, those of eight.  Units come by cp.async, 512 bytes of a page side by side at a time
+// (lanes that copied what they read themselves, 64 bytes of each of eight tokens at a time, took 1.3 times as long), into a
+// ring in shared memory of the warp's own: no barriers.  mma.sync and not tcgen05: a unit has one to eight rows of work, and
+// the codes pass through registers, since they are converted.
 //
 // Keys are dealt out over all warps evenly, whatever the sequences' lengths, which are in device memory: each warp counts
 // the units of all sequences and takes its share of their row, at least kLeastUnits; it writes an item (sequence, head,
 // rows) that lies wholly in its share, and leaves its part of the first and the last else, which a second kernel adds up.
 //
-// Roundings: queries to 2^-22 of their row's largest value, probabilities to fp16 (2^-11), all else in fp32.
+// Roundings: queries to fp16 by a power of two per row (exact, but for bf16 values below 2^-28 of the row's largest),
+// probabilities to fp16 (2^-11), all else in fp32.
 #include <cuda_fp8.h>
 
 #include "flash_common.cuh"
@@ -26,7 +28,8 @@
 namespace slapo {
 namespace {
 
-constexpr int kWarps = 8;          // (of up to 255 registers; twelve with one tile of rows each: 54.5 us where eight take 52.5)
+constexpr int kWarps = 8;          // of up to 255 registers.  (16 tokens over 12000 keys of 4 heads, us: eight 52.5, twelve of 168 54.5,
+                                   // sixteen of 128, with one unit on its way to each, 61.)
 constexpr int kUnit = 32;          // keys: two blocks of 16
 constexpr int kLeastUnits = 2;     // of a warp's share
 
@@ -113,27 +116,14 @@ __device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 16 x 8 from 32 e4m3 numbers each
-__device__ __forceinline__ void product8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
-// Queries are taken apart into e4m3 numbers: x = x0 + 2^-5 x1 + 2^-10 x2, each the rest of those before, rounded.  Of a
-// row whose largest value is 2^7 to 2^8, two are bf16's eight bits, and three fp16's eleven, but for values below 2^-22
-// (three: 2^-27) of the largest, which are off by no more than that.
-template <typename T> constexpr int kPartsOf = 3;
-template <> constexpr int kPartsOf<__nv_bfloat16> = 2;
-
 // kWide: heads of 72 to 128, whose tokens are 80 to 128 bytes; else up to 64.  N: tiles of 8 rows.
-template <bool kWide, int N, typename T>
+template <bool kWide, int N>
 struct Shape {
   static constexpr int kChunks = kWide ? 2 : 1;                   // of 64 values of a key
   static constexpr int kPieces = 4 * kChunks;                     // of 16 bytes of a token
@@ -141,13 +131,12 @@ struct Shape {
   static constexpr int kCopies = kPieces / 2;                     // ... of a lane, 16 each
   static constexpr int kScales = 4 * kBlock;                      // where a unit's four scales are
   static constexpr int kStage = kScales + 16;
-  static constexpr int kParts = kPartsOf<T>;
   static constexpr int kStages = kWide ? (N <= 2 ? 3 : 2) : 5;
   static constexpr int kTiles = kWide ? 8 : 4;                    // of 16 values of a head
   static constexpr int kValues = kWide ? 16 : 8;                  // consecutive ones that a lane has
   // the queries' operands: in registers for one tile or two, beside the ring for more
   static constexpr bool kSharedQ = N > 2;
-  static constexpr int kQuery = kSharedQ ? N * kChunks * kParts * 512 : 0;
+  static constexpr int kQuery = kSharedQ ? N * kChunks * 2 * 512 : 0;
   static constexpr int kWarp = kStages * kStage + kQuery;
   static constexpr int kSmem = kWarps * kWarp;
   // where a piece of a token lies in a block
@@ -210,7 +199,7 @@ __device__ __forceinline__ int begin_share(const Plan& p, int number, Cursor& at
 
 template <bool kWide, int N, bool kSmallPages, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const Plan p) {
-  using S = Shape<kWide, N, T>;
+  using S = Shape<kWide, N>;
   extern __shared__ __align__(128) uint8_t s_ring[];
   const PagedCache& c = p.a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -325,7 +314,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
   for (int i = 0; i < S::kStages - 1; ++i) issue(i);
 
   const uint32_t q_at = ring + S::kStages * S::kStage + lane * 16;
-  uint32_t q[S::kSharedQ ? 1 : N][S::kChunks][S::kParts][4];
+  uint32_t q[S::kSharedQ ? 1 : N][S::kChunks][2][4];
   float factor[N][2], m[N][2], l[N][2], o[N][S::kTiles][4];
   int last[N][2];                      // the last key that a row sees, less than 0: none
   // where this lane's operands are in a block: of keys g and g + 8, of values' rows 2 t, 2 t + 1 and eight further
@@ -363,33 +352,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest value in [2^7, 2^8); what is not finite stays so
-        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 7, -100), 121);
+        // the row's largest value in [2^13, 2^14); what is not finite stays so
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127 - 13, -100), 115);
         const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-        for (int j = 0; j < S::kChunks; ++j) {
+        for (int j = 0; j < S::kChunks; ++j)
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[j][k] *= down;
-#pragma unroll
-          for (int part = 0; part < S::kParts; ++part) {
+          for (int half = 0; half < 2; ++half) {
             uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(x[j][k], x[j][k + 1]), __NV_SATFINITE, __NV_E4M3);
-              const float2 held = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3)));
-              x[j][k] = (x[j][k] - held.x) * 32.f;
-              x[j][k + 1] = (x[j][k + 1] - held.y) * 32.f;
-              w[k / 4] = k % 4 == 0 ? pair : w[k / 4] | pair << 16;
+            for (int y = 0; y < 4; ++y) {
+              const __half2 pair = __floats2half2_rn(x[j][8 * half + 2 * y] * down, x[j][8 * half + 2 * y + 1] * down);
+              w[y] = *reinterpret_cast<const uint32_t*>(&pair);
             }
             if constexpr (S::kSharedQ) {
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + ((i * S::kChunks + j) * S::kParts + part) * 512),
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + ((i * S::kChunks + j) * 2 + half) * 512),
                            "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
             } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) q[i][j][part][y] = w[y];
+              for (int y = 0; y < 4; ++y) q[i][j][half][y] = w[y];
             }
           }
-        }
         // the two rows whose scores this lane has
         // (an infinite query's row: NaN)
         const float up = top <= 3.402823466e38f ? __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * p.scale_log2
@@ -418,43 +401,41 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int block = 0; block < 2; ++block) s[i][block][0] = s[i][block][1] = s[i][block][2] = s[i][block][3] = 0.f;
-    uint4 keys[2][2][S::kChunks];
 #pragma unroll
-    for (int block = 0; block < 2; ++block)
+    for (int j = 0; j < S::kChunks; ++j) {
+      uint4 keys[2][2];
 #pragma unroll
-      for (int j = 0; j < S::kChunks; ++j)
+      for (int block = 0; block < 2; ++block)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          keys[block][r][j] = read16(base + 2 * block * S::kBlock + r * 8 * 16 * S::kPieces + (j == 0 ? key_at[0] : key_at[1]));
-    // the queries' least part first: the sum of each part is multiplied on its way to the next
+          keys[block][r] = read16(base + 2 * block * S::kBlock + r * 8 * 16 * S::kPieces + (j == 0 ? key_at[0] : key_at[1]));
 #pragma unroll
-    for (int part = S::kParts - 1; part >= 0; --part) {
+      for (int half = 0; half < 2; ++half) {
+        uint2 a[2][2], b[2][2];        // words 2 half and 2 half + 1 of each block's keys g and g + 8
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+        for (int block = 0; block < 2; ++block) {
+          const uint4 &k0 = keys[block][0], &k1 = keys[block][1];
+          a[block][0] = halves(half == 0 ? k0.x : k0.z);
+          a[block][1] = halves(half == 0 ? k0.y : k0.w);
+          b[block][0] = halves(half == 0 ? k1.x : k1.z);
+          b[block][1] = halves(half == 0 ? k1.y : k1.w);
+        }
 #pragma unroll
-        for (int j = 0; j < S::kChunks; ++j) {
+        for (int i = 0; i < N; ++i) {
           uint32_t w[4];
           if constexpr (S::kSharedQ) {
-            const uint4 x = read16(q_at + ((i * S::kChunks + j) * S::kParts + part) * 512);
+            const uint4 x = read16(q_at + ((i * S::kChunks + j) * 2 + half) * 512);
             w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
           } else {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) w[y] = q[i][j][part][y];
+            for (int y = 0; y < 4; ++y) w[y] = q[i][j][half][y];
           }
 #pragma unroll
-          for (int block = 0; block < 2; ++block) {
-            const uint4 &a = keys[block][0][j], &b = keys[block][1][j];
-            product8(s[i][block], a.x, b.x, a.y, b.y, w[0], w[1]);
-            product8(s[i][block], a.z, b.z, a.w, b.w, w[2], w[3]);
-          }
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int block = 0; block < 2; ++block)
+              product(s[i][block], a[block][y].x, b[block][y].x, a[block][y].y, b[block][y].y, w[2 * y], w[2 * y + 1]);
         }
-      if (part > 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int block = 0; block < 2; ++block)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) s[i][block][y] *= 0.03125f;
       }
     }
     float k_scale[2], v_scale[2];
@@ -709,7 +690,7 @@ Plan make_plan(const PagedAttention& a) {
 
 template <bool kWide, int N, bool kSmallPages, typename T>
 int launch_tiles(const Plan& p, cudaStream_t stream) {
-  using S = Shape<kWide, N, T>;
+  using S = Shape<kWide, N>;
   static_assert(S::kSmem <= 227 * 1024, "a CTA's shared memory");
   auto kernel = paged_attention_kernel<kWide, N, kSmallPages, T>;
   int device = 0;
