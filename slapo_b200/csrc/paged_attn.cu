@@ -77,6 +77,9 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool ok) {
   const int n = ok ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool ok) {
   const int n = ok ? 4 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
@@ -269,25 +272,32 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
       const int until = in.keys.len - key0;
       const int from = p.a.window > 0 ? in.keys.len - in.keys.count - p.a.window + 1 - key0 : 0;
       const bool every = page[0] >= 0 && page[kPages - 1] >= 0 && until >= kUnit && from <= 0;
+      const uint8_t* k = nullptr;
 #pragma unroll
       for (int block = 0; block < 2; ++block) {
         const int id = page[kSmallPages ? block : 0];
         // (a page without a key that is seen may never have been written, its scales neither)
         const bool known = every || (id >= 0 && (!kSmallPages || (until > 16 * block && from < 16 * block + 16)));
-        if (!known) missing |= 1u << (2 * stage + block);
-        const int64_t side = (static_cast<int64_t>(known ? id : 0) * 2) * c.heads + h;
-        const uint8_t* k = lane_pages + side * head_bytes + ((key0 + 16 * block) & (c.page - 1)) * c.pitch;
+        if (kSmallPages || block == 0) {
+          const int64_t side = (static_cast<int64_t>(known ? id : 0) * 2) * c.heads + h;
+          k = lane_pages + side * head_bytes + ((key0 + 16 * block) & (c.page - 1)) * c.pitch;
+          // keys' and values' scale by one lane each
+          if (lane < 2) copy4(to + S::kScales + 8 * block + 4 * lane, c.scales + side + lane * c.heads, known);
+        } else {
+          k += 16 * c.pitch;
+        }
         const uint8_t* v = k + side_bytes;
         const uint32_t k_to = to + 2 * block * S::kBlock, v_to = k_to + S::kBlock;
         if (every) {
 #pragma unroll
           for (int i = 0; i < S::kCopies; ++i) {
             if (row_of[i] < 16) {
-              copy16(k_to + place[i], k + i * 512, true);
-              copy16(v_to + place[i], v + i * 512, true);
+              copy16(k_to + place[i], k + i * 512);
+              copy16(v_to + place[i], v + i * 512);
             }
           }
         } else {
+          if (!known) missing |= 1u << (2 * stage + block);
 #pragma unroll
           for (int i = 0; i < S::kCopies; ++i) {
             if (row_of[i] < 16) {
@@ -298,9 +308,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const P
             }
           }
         }
-        // keys' and values' scale by one lane each
-        if (lane < 2 && (kSmallPages || block == 0))
-          copy4(to + S::kScales + 8 * block + 4 * lane, c.scales + side + lane * c.heads, known);
       }
       step(in);
       if (to_issue > 0) {
