@@ -28,8 +28,10 @@
 namespace slapo {
 namespace {
 
-constexpr int kWarps = 8;          // of up to 255 registers.  (16 tokens over 12000 keys of 4 heads, us: eight 52.5, twelve of 168 54.5,
-                                   // sixteen of 128, with one unit on its way to each, 61.)
+// Warps of a CTA by the tiles of 8 rows that each has: of up to 168 and of up to 255 registers.  (One tile, us, eight warps with
+// three units in the ring of each / twelve with two: 16 tokens over up to 32001 keys of 4 heads 51.9 / 52.1, one over up to 1501
+// of 16 15.1 / 15.3, five with a window of 1001 18.5 / 17.2.  Sixteen with one: 61, 16.6, 20.6.)
+constexpr int warps_of(int tiles) { return tiles == 1 ? 12 : 8; }
 constexpr int kUnit = 32;          // keys: two blocks of 16
 constexpr int kLeastUnits = 2;     // of a warp's share
 
@@ -134,7 +136,8 @@ struct Shape {
   static constexpr int kCopies = kPieces / 2;                     // ... of a lane, 16 each
   static constexpr int kScales = 4 * kBlock;                      // where a unit's four scales are
   static constexpr int kStage = kScales + 16;
-  static constexpr int kStages = kWide ? (N <= 2 ? 3 : 2) : 5;
+  static constexpr int kWarps = warps_of(N);
+  static constexpr int kStages = kWide ? (N == 2 ? 3 : 2) : (N == 1 ? 4 : 5);
   static constexpr int kTiles = kWide ? 8 : 4;                    // of 16 values of a head
   static constexpr int kValues = kWide ? 16 : 8;                  // consecutive ones that a lane has
   // the queries' operands: in registers for one tile or two, beside the ring for more
@@ -201,7 +204,7 @@ __device__ __forceinline__ int begin_share(const Plan& p, int number, Cursor& at
 }
 
 template <bool kWide, int N, bool kSmallPages, typename T>
-__global__ void __launch_bounds__(kWarps * 32, 1) paged_attention_kernel(const Plan p) {
+__global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(const Plan p) {
   using S = Shape<kWide, N>;
   extern __shared__ __align__(128) uint8_t s_ring[];
   const PagedCache& c = p.a.cache;
@@ -690,8 +693,9 @@ Plan make_plan(const PagedAttention& a) {
   // units if all sequences fill their rows of the table
   const int64_t units = static_cast<int64_t>(c.B) * c.heads * p.tiles *
                         ((static_cast<int64_t>(c.table_pages) * c.page + kUnit - 1) / kUnit);
-  const int64_t ctas = (units + kLeastUnits * kWarps - 1) / (kLeastUnits * kWarps);
-  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * kWarps;
+  const int warps = warps_of(p.tile_rows / 8);
+  const int64_t ctas = (units + kLeastUnits * warps - 1) / (kLeastUnits * warps);
+  p.warps = static_cast<int>(ctas < sm_count() ? (ctas > 0 ? ctas : 1) : sm_count()) * warps;
   return p;
 }
 
@@ -709,7 +713,7 @@ int launch_tiles(const Plan& p, cudaStream_t stream) {
     configured[device] = true;
   }
   count_launch();
-  kernel<<<p.warps / kWarps, kWarps * 32, S::kSmem, stream>>>(p);
+  kernel<<<p.warps / S::kWarps, S::kWarps * 32, S::kSmem, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return 4;
   cudaLaunchConfig_t config{};
   const int tile_rows = p.rows < p.tile_rows ? p.rows : p.tile_rows;
