@@ -142,9 +142,10 @@ class FlashAttention(nn.Module):
     ``rotary`` (:class:`slapo_b200.ops.rotary.RotaryEmbedding`): queries and keys are rotated by the tokens'
     positions, those of ``position_ids`` or the ones that follow the cache.
 
-    A cache in generation is a pair of tensors, or a layer of a :class:`slapo_b200.ops.paged.PagedKVCache` that
-    has made room for the tokens: keys and values go into its pages in 8 bits, and tokens attend over these (a
-    prompt's first ones over the keys and values as they are)."""
+    A cache in generation is a pair of tensors, or a layer of a
+    :class:`slapo_b200.ops.paged.PagedKVCache` that has made room for the tokens: keys and values go into
+    its pages in 8 bits, and tokens attend over these (a prompt's first ones over the keys and values as
+    they are)."""
 
     def __init__(self, hidden_size, num_attention_heads, attn_pdrop=0.0, resid_pdrop=0.0,
                  attn_op_name="auto", bias=True, output_proj=True, fused_qkv=False,
@@ -235,15 +236,18 @@ class FlashAttention(nn.Module):
     def _check_paged(self, attention_mask, position_ids):
         op = self.attn_op
         if attention_mask is not None or position_ids is not None:
-            raise NotImplementedError("a paged cache knows its tokens by their lengths: no mask, no position_ids")
+            raise NotImplementedError("a paged cache knows its tokens by their lengths: no mask, no "
+                                      "position_ids")
         if not op.apply_causal_mask or op.sinks or op.rel_bias_table is not None:
-            raise NotImplementedError("a paged cache needs causal attention without sinks or a relative-position table")
+            raise NotImplementedError("a paged cache needs causal attention without sinks or a "
+                                      "relative-position table")
         if self.training and self.attn_pdrop > 0.0:
             raise NotImplementedError("no dropout of attention over a paged cache: call eval()")
 
     def _paged(self, past, q, k, v):
-        table, interleaved = (None, False) if self.rotary is None else (self.rotary.table(q.device),
-                                                                         self.rotary.interleaved)
+        table, interleaved = None, False
+        if self.rotary is not None:
+            table, interleaved = self.rotary.table(q.device), self.rotary.interleaved
         if past.fresh:
             if self.rotary is not None:
                 q, k = self.rotary(q, k)

@@ -2,11 +2,11 @@
 ``csrc/paged_attn.cu``).
 
 ``pages [P, 2, H, T, W]`` of ``float8_e4m3fn``: for keys and values and each head the ``T`` tokens of a page
-(16, 32, 64 or 128), ``W`` the head's width up to a multiple of 16.  ``scales [P, 2, H]`` in fp32: a power of two
-for each page, side and head, the smallest with which the largest value fits (448 times it), at least 2^-100.
-``block_table [B, pages]`` (int32) names a sequence's pages in their order, ``lengths [B]`` (int32) counts its
-tokens, new ones among them.  Of ``n`` new tokens a sequence brings all, or the first ``counts[b]``: they are its
-last ones.
+(16, 32, 64 or 128), ``W`` the head's width up to a multiple of 16.  ``scales [P, 2, H]`` in fp32: a power
+of two for each page, side and head, the smallest with which the largest value fits (448 times it), at least
+2^-100. ``block_table [B, pages]`` (int32) names a sequence's pages in their order, ``lengths [B]`` (int32)
+counts its tokens, new ones among them.  Of ``n`` new tokens a sequence brings all, or the first
+``counts[b]``: they are its last ones.
 
 All of it is in device memory and read there, so that a captured step serves whatever it holds at a replay.
 """
@@ -114,23 +114,26 @@ def paged_append_reference(pages, scales, k, v, block_table, lengths, counts=Non
     return new_q
 
 
-def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None, rotary_table=None, interleaved=False):
-    """New tokens' keys and values ``[B, n, H, D]`` (bf16, fp16 or fp32; slices of a packed projection are read in
-    place) into the cache, in place; returns their queries (or None).
+def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None, rotary_table=None,
+        interleaved=False):
+    """New tokens' keys and values ``[B, n, H, D]`` (bf16, fp16 or fp32; slices of a packed projection are
+    read in place) into the cache, in place; returns their queries (or None).
 
     ``rotary_table``: keys - and ``q [B, n, heads, D]`` - are rotated by their positions on the way
-    (:func:`slapo_b200.ops.functional.rotary`); without one they stay as they are.  New tokens have positions
-    ``lengths[b] - counts[b]`` on; those before position 0 (left padding), behind the block table's end or in a page
-    that there is not are not kept, a query that is none (behind ``counts[b]``, before position 0) is zeros, and so
-    are a query and a key behind the rotation's table.  A page takes tokens of one sequence: pages that several share have to be full.
+    (:func:`slapo_b200.ops.functional.rotary`); without one they stay as they are.  New tokens have
+    positions ``lengths[b] - counts[b]`` on; those before position 0 (left padding), behind the block
+    table's end or in a page that there is not are not kept, a query that is none (behind ``counts[b]``,
+    before position 0) is zeros, and so are a query and a key behind the rotation's table.  A page takes
+    tokens of one sequence: pages that several share have to be full.
 
-    A value is off by at most 2^-4 of itself, or half of 2^-9 of its page's scale if it is small; values that are
-    not finite are held as NaN.  A page's first token sets its scale anew; where a later one is too large for it, the
-    page's codes are rounded to the larger scale."""
+    A value is off by at most 2^-4 of itself, or half of 2^-9 of its page's scale if it is small; values
+    that are not finite are held as NaN.  A page's first token sets its scale anew; where a later one is too
+    large for it, the page's codes are rounded to the larger scale."""
     if torch.is_tensor(k) and k.is_cuda:
         plain_q = rotary_table is None and counts is None       # (queries stay as they are)
         fn = native.direct("paged_append")
-        out = None if fn is None else fn(pages, scales, k, v, block_table, lengths, counts, None if plain_q else q,
+        out = None if fn is None else fn(pages, scales, k, v, block_table, lengths, counts,
+                None if plain_q else q,
                                          rotary_table, interleaved)
         if out is not None:
             return out if q is not None and not plain_q else q
@@ -154,11 +157,13 @@ def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None,
     _check_no_gradient("paged_append", k, v, q)
     if NF._native_ok(k):
         plain_q = rotary_table is None and counts is None
-        out = NF._nodes().paged_append(pages, scales, k, v, block_table, lengths, counts, None if plain_q else q,
+        out = NF._nodes().paged_append(pages, scales, k, v, block_table, lengths, counts,
+                None if plain_q else q,
                                        rotary_table, bool(interleaved))
         return out if q is not None and not plain_q else q
     plain_q = rotary_table is None and counts is None
-    out = paged_append_reference(pages, scales, k, v, block_table, lengths, counts, None if plain_q else q, rotary_table,
+    out = paged_append_reference(pages, scales, k, v, block_table, lengths, counts, None if plain_q else q,
+            rotary_table,
                                  interleaved)
     return q if plain_q else out
 
@@ -196,15 +201,16 @@ def paged_attention_reference(q, pages, scales, block_table, lengths, counts=Non
 
 
 def paged_attention(q, pages, scales, block_table, lengths, counts=None, scale=None, window=None):
-    """Attention of the newest tokens' queries ``[B, n, heads, D]`` (bf16 or fp16) over the cache, which has their own
-    keys already: causal, ``heads`` a multiple of the cache's, which its neighbours share.
+    """Attention of the newest tokens' queries ``[B, n, heads, D]`` (bf16 or fp16) over the cache, which has
+    their own keys already: causal, ``heads`` a multiple of the cache's, which its neighbours share.
 
-    The query of new token ``t`` has position ``lengths[b] - counts[b] + t`` and sees the keys up to it, with a
-    ``window`` that many.  A query without a key - behind ``counts[b]``, before position 0, in an empty sequence - has
-    an output of 0; pages that there are not are not seen.  What is cached has to be finite.
+    The query of new token ``t`` has position ``lengths[b] - counts[b] + t`` and sees the keys up to it,
+    with a ``window`` that many.  A query without a key - behind ``counts[b]``, before position 0, in an
+    empty sequence - has an output of 0; pages that there are not are not seen.  What is cached has to be
+    finite.
 
-    Keys are dealt out evenly over the GPU whatever the lengths; made for few tokens at a time (their keys are read
-    again for every 32 rows of heads and tokens): a prompt's first tokens go through
+    Keys are dealt out evenly over the GPU whatever the lengths; made for few tokens at a time (their keys
+    are read again for every 32 rows of heads and tokens): a prompt's first tokens go through
     :func:`slapo_b200.ops.functional.flash_attention`.  fp32 queries run the PyTorch reference."""
     if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
         raise ValueError(f"a window is a number of keys, 1 and more, not {window!r}")
@@ -227,11 +233,13 @@ def paged_attention(q, pages, scales, block_table, lengths, counts=None, scale=N
 
 
 class PagedKVCache:
-    """Keys and values of ``layers`` attention layers for up to ``batch`` sequences of ``max_tokens`` in ``pages`` pages.
+    """Keys and values of ``layers`` attention layers for up to ``batch`` sequences of ``max_tokens`` in
+    ``pages`` pages.
 
     A step: :meth:`add` makes room for the new tokens of each sequence, then every layer appends and attends
-    (``FlashAttention(..., layer_past=cache.layer(i))``); :meth:`free` gives a sequence's pages back.  The tables on the
-    device keep their addresses, so that the layers' work can be captured and replayed after each :meth:`add`."""
+    (``FlashAttention(..., layer_past=cache.layer(i))``); :meth:`free` gives a sequence's pages back.  The
+    tables on the device keep their addresses, so that the layers' work can be captured and replayed after
+    each :meth:`add`."""
 
     def __init__(self, layers, pages, heads, head_dim, batch, max_tokens, page=64, device=None):
         if page not in PAGE_SIZES:
@@ -263,9 +271,9 @@ class PagedKVCache:
         return self._tokens[sequence]
 
     def add(self, counts):
-        """Room for a step's new tokens: the same number for every sequence, or a list of one for each (0: none in
-        this step; the step's tensors are then as wide as the largest, right-padded).  Refused, with nothing changed,
-        where pages or a sequence's ``max_tokens`` do not suffice."""
+        """Room for a step's new tokens: the same number for every sequence, or a list of one for each (0:
+        none in this step; the step's tensors are then as wide as the largest, right-padded).  Refused, with
+        nothing changed, where pages or a sequence's ``max_tokens`` do not suffice."""
         each = [counts] * self.batch if isinstance(counts, int) else [int(c) for c in counts]
         if len(each) != self.batch or min(each, default=0) < 0:
             raise ValueError(f"a number of new tokens for each of {self.batch} sequences required, not {counts}")
@@ -321,10 +329,12 @@ class PagedLayer:
         c = self.cache
         if k.shape[:2] != (c.batch, c.width):
             raise ValueError(f"the step has room for {c.width} tokens of {c.batch} sequences, not {tuple(k.shape[:2])}")
-        return paged_append(c.pages[self.index], c.scales[self.index], k, v, c.block_table, c.lengths, c.counts, q,
+        return paged_append(c.pages[self.index], c.scales[self.index], k, v, c.block_table, c.lengths,
+                c.counts, q,
                             rotary_table, interleaved)
 
     def attend(self, q, scale=None, window=None):
         c = self.cache
-        return paged_attention(q, c.pages[self.index], c.scales[self.index], c.block_table, c.lengths, c.counts, scale,
+        return paged_attention(q, c.pages[self.index], c.scales[self.index], c.block_table, c.lengths,
+                c.counts, scale,
                                window)

@@ -1,10 +1,10 @@
 """Rotation of queries and keys by their positions (``csrc/rotary.cu``).
 
-A pair ``(a, b)`` of a head at position ``p`` becomes ``(a cos - b sin, b cos + a sin)``, with cosine and sine
-from row ``p`` of a table ``[positions, rotated / 2, 2]`` in fp32, in which the base, a stretched context and a
-factor are.  Pairs are the halves of the rotated part of a head, or neighbours (``interleaved``); what lies
-behind that part stays.  The rotation is computed in fp32 and rounded once; its gradient is the transposed
-rotation, so that nothing is kept but the positions.
+A pair ``(a, b)`` of a head at position ``p`` becomes ``(a cos - b sin, b cos + a sin)``, with cosine and
+sine from row ``p`` of a table ``[positions, rotated / 2, 2]`` in fp32, in which the base, a stretched
+context and a factor are.  Pairs are the halves of the rotated part of a head, or neighbours
+(``interleaved``); what lies behind that part stays.  The rotation is computed in fp32 and rounded once; its
+gradient is the transposed rotation, so that nothing is kept but the positions.
 """
 from __future__ import annotations
 
@@ -89,7 +89,8 @@ def _check(q, k, table, positions):
 
 
 def turn_reference(x, table, pos, interleaved):
-    """``x [B, S, ..., D]`` rotated in fp32; ``pos [S]`` or ``[B, S]``.  Positions outside of the table: zeros."""
+    """``x [B, S, ..., D]`` rotated in fp32; ``pos [S]`` or ``[B, S]``.  Positions outside of the table:
+    zeros."""
     pos = pos.long()
     known = (pos >= 0) & (pos < table.shape[0])
     if table.shape[0]:
@@ -142,9 +143,9 @@ def _rotary(q, k, table, positions, interleaved):
 def rotary(q, k, table, positions=None, interleaved=False):
     """Queries ``[B, S, H, D]`` and keys ``[B, S, heads, D]`` rotated by their positions: two new tensors.
 
-    ``table``: :func:`rotary_table`, of the rotated part of the head; ``positions``: those of the tokens, ``[S]``
-    or ``[B, S]``, the first one's number, or None for 0, 1, ....  A token whose position lies outside of the
-    table (padding: -1) gets zeros and no gradient."""
+    ``table``: :func:`rotary_table`, of the rotated part of the head; ``positions``: those of the tokens,
+    ``[S]`` or ``[B, S]``, the first one's number, or None for 0, 1, ....  A token whose position lies
+    outside of the table (padding: -1) gets zeros and no gradient."""
     return _rotary(q, k, table, positions, interleaved)
 
 
@@ -156,10 +157,11 @@ def rotary_qkvpacked(qkv, table, positions=None, interleaved=False):
 
 class RotaryEmbedding(nn.Module):
     """What :class:`~slapo_b200.ops.attention.FlashAttention` rotates its queries and keys by: a table of
-    ``max_positions`` for the first ``rotary_dim`` values of a head (``base``, ``scaling``: :func:`rotary_table`).
+    ``max_positions`` for the first ``rotary_dim`` values of a head (``base``, ``scaling``:
+    :func:`rotary_table`).
 
-    The table is no parameter and no buffer: it stays in fp32 whatever the model is cast to, and is made on a
-    device when that is first used (before a capture, as a model's first pass is)."""
+    The table is no parameter and no buffer: it stays in fp32 whatever the model is cast to, and is made on
+    a device when that is first used (before a capture, as a model's first pass is)."""
 
     traceable = False
 
@@ -173,7 +175,8 @@ class RotaryEmbedding(nn.Module):
     def table(self, device):
         device = torch.device(device)
         if device not in self._tables:
-            self._tables[device] = rotary_table(self.rotary_dim, self.max_positions, self.base, self.scaling, device)
+            self._tables[device] = rotary_table(self.rotary_dim, self.max_positions, self.base,
+                    self.scaling, device)
         return self._tables[device]
 
     def __getstate__(self):

@@ -42,7 +42,8 @@ def sample_reference(logits, uniform, temperature, top_k, top_p, min_p):
     def each(v, dtype):
         if torch.is_tensor(v):
             return v.reshape(b, 1).to(dtype)
-        return torch.full((b, 1), float(torch.tensor(v, dtype=torch.float32)) if dtype == torch.float64 else v,
+        return torch.full((b, 1), float(torch.tensor(v,
+                dtype=torch.float32)) if dtype == torch.float64 else v,
                           dtype=dtype, device=x.device)
 
     temperature, top_p, min_p = (each(v, torch.float64) for v in (temperature, top_p, min_p))
@@ -71,14 +72,14 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The next token of each row of ``logits [..., vocabulary]``, int64 ``[...]``.
 
     Of the logits over ``temperature`` the ``top_k`` largest are kept (0: all; equals in the order of their
-    indices), of these the shortest beginning of their order that holds a share ``top_p`` of their mass, of these
-    what has at least ``min_p`` times the largest one's probability.  ``uniform``: a random number in [0, 1) for each
-    row, fp32; the token is the first one kept, in the order of indices, at which the sum of probabilities
-    passes it.  Temperature 0 takes the largest, the first of equals.
+    indices), of these the shortest beginning of their order that holds a share ``top_p`` of their mass, of
+    these what has at least ``min_p`` times the largest one's probability.  ``uniform``: a random number in
+    [0, 1) for each row, fp32; the token is the first one kept, in the order of indices, at which the sum of
+    probabilities passes it.  Temperature 0 takes the largest, the first of equals.
 
-    Each setting is one number, or a tensor of one for each row (fp32; ``top_k`` int32).  A logit of -inf or NaN is
-    no token; a row of nothing else gives -1.  Weights are computed in fp64 and held as multiples of 2^-42 of the
-    largest one's, their sums are exact: the same call gives the same token."""
+    Each setting is one number, or a tensor of one for each row (fp32; ``top_k`` int32).  A logit of -inf or
+    NaN is no token; a row of nothing else gives -1.  Weights are computed in fp64 and held as multiples of
+    2^-42 of the largest one's, their sums are exact: the same call gives the same token."""
     if torch.is_tensor(logits) and logits.is_cuda:
         fn = native.direct("sample")
         out = None if fn is None else fn(logits, uniform, temperature, top_k, top_p, min_p)

@@ -1,5 +1,5 @@
-"""Rotation by positions, the paged 8-bit cache and sampling on the CPU: the oracles against definitions written
-apart from them, refusals, the cache's bookkeeping, generation through ``FlashAttention``."""
+"""Rotation by positions, the paged 8-bit cache and sampling on the CPU: the oracles against definitions
+written apart from them, refusals, the cache's bookkeeping, generation through ``FlashAttention``."""
 import copy
 import math
 
@@ -21,7 +21,8 @@ def test_rotation_is_a_complex_product(dim, rotated, interleaved):
     got = NF.rotary(q, k, table, pos, interleaved)
     for x, y in zip((q, k), got):
         part = x[..., :rotated]
-        pairs = part.view(*part.shape[:-1], -1, 2) if interleaved else part.view(*part.shape[:-1], 2, -1).transpose(-1, -2)
+        pairs = part.view(*part.shape[:-1], -1, 2) if interleaved else part.view(*part.shape[:-1], 2,
+                -1).transpose(-1, -2)
         z = torch.view_as_complex(pairs.contiguous()) * torch.view_as_complex(table.double()[pos])[:, :, None]
         z = torch.view_as_real(z)
         want = z.flatten(-2) if interleaved else z.transpose(-1, -2).flatten(-2)
@@ -72,7 +73,8 @@ def test_tables():
     angle = 19 * 1e4 ** (-6 / 8) / 4                                      # the slowest one stretched by the factor
     assert abs(float(ntk[19, 3, 1]) - math.sin(angle)) <= 2.0 ** -23
     yarn = NF.rotary_table(64, 4096, scaling={"type": "yarn", "factor": 4, "original_positions": 1024})
-    plain, stretched = NF.rotary_table(64, 4096), NF.rotary_table(64, 4096, scaling={"type": "linear", "factor": 4})
+    plain, stretched = NF.rotary_table(64, 4096), NF.rotary_table(64, 4096, scaling={"type": "linear",
+            "factor": 4})
     m = 0.1 * math.log(4) + 1
     assert torch.allclose(yarn[:, 0], plain[:, 0] * m, rtol=2.0 ** -22, atol=2.0 ** -22)
     assert torch.allclose(yarn[:, -1], stretched[:, -1] * m, rtol=2.0 ** -22, atol=2.0 ** -22)
@@ -123,11 +125,13 @@ def test_rotary_refusals(index):
 # ---------------------------------------------------------------------- #
 # the paged cache
 def make_cache(b, per, heads, dim, page, device="cpu", seed=0, poison=True, spare=2):
-    """An empty cache, its pages in no order, and a table; ``poison``: codes are NaN until they are written."""
+    """An empty cache, its pages in no order, and a table; ``poison``: codes are NaN until they are
+    written."""
     g = torch.Generator().manual_seed(seed)
     total = b * per + spare
     width = (dim + 15) // 16 * 16
-    pages = torch.full((total, 2, heads, page, width), float("nan") if poison else 0.0).to(torch.float8_e4m3fn).to(device)
+    pages = torch.full((total, 2, heads, page, width),
+            float("nan") if poison else 0.0).to(torch.float8_e4m3fn).to(device)
     scales = torch.full((total, 2, heads), float("nan") if poison else 0.0, device=device)
     table = torch.randperm(total, generator=g)[:b * per].view(b, per).int().to(device)
     return pages, scales, table
@@ -144,14 +148,15 @@ def read_cache(pages, scales, table, b, tokens, dim):
 
 
 def check_cache(pages, scales, table, want, grown=0):
-    """The cache against ``want``: for each sequence keys and values ``[2, tokens, H, D]`` in fp64.  A value is
-    rounded to e4m3, off by 2^-4 of itself or half of 2^-9 of its scale; each growth of its scale can round it again in
-    the last way alone (a power of two)."""
+    """The cache against ``want``: for each sequence keys and values ``[2, tokens, H, D]`` in fp64.  A value
+    is rounded to e4m3, off by 2^-4 of itself or half of 2^-9 of its scale; each growth of its scale can
+    round it again in the last way alone (a power of two)."""
     page = pages.shape[3]
     for b, x in enumerate(want):
         tokens, dim = x.shape[1], x.shape[3]
         got, scale = read_cache(pages, scales, table, b, tokens, dim)
-        bound = torch.maximum(x.abs() * 2.0 ** -4, scale[..., None] * 2.0 ** -10) + grown * scale[..., None] * 2.0 ** -10
+        bound = torch.maximum(x.abs() * 2.0 ** -4, scale[..., None] * 2.0 ** -10) + grown * scale[...,
+                None] * 2.0 ** -10
         assert bool(((got - x).abs() <= bound * (1 + 2.0 ** -10)).all())
         # scales: the smallest power of two for the page's largest value (of rounded ones: with their slack)
         for p in range((tokens + page - 1) // page):
@@ -174,7 +179,8 @@ def append_all(chunks, k, v, q, cache, table_rot, interleaved, counts=None):
         c = None if counts is None else counts[i]
         done = done + (n if c is None else c)
         part = [None if x is None else x[:, at:at + n] for x in (k, v, q)]
-        got = NF.paged_append(pages, scales, part[0], part[1], table, done, c, q=part[2], rotary_table=table_rot,
+        got = NF.paged_append(pages, scales, part[0], part[1], table, done, c, q=part[2],
+                rotary_table=table_rot,
                               interleaved=interleaved)
         out.append(got)
         at += n
@@ -196,7 +202,8 @@ def turned(x, rot, pos, interleaved):
     return x
 
 
-CHUNKS = [([1], 1), ([5], 2), ([40], 1), ([33, 1, 1, 1], 2), ([1] * 20, 3), ([16, 16, 3], 2), ([200, 7, 64], 1)]
+CHUNKS = [([1], 1), ([5], 2), ([40], 1), ([33, 1, 1, 1], 2), ([1] * 20, 3), ([16, 16, 3], 2), ([200, 7, 64],
+        1)]
 
 
 def append_case(chunks, b, page, dim, rotated, interleaved, dtype, device="cpu"):
@@ -204,7 +211,8 @@ def append_case(chunks, b, page, dim, rotated, interleaved, dtype, device="cpu")
     n, heads, q_heads = sum(chunks), 2, 4
     # values whose size jumps, so that scales grow within pages
     size = torch.exp2(torch.randint(-3, 4, (b, n, 1, 1), generator=g).float())
-    k, v, q = ((torch.randn(b, n, h, dim, generator=g) * size).to(dtype).to(device) for h in (heads, heads, q_heads))
+    k, v, q = ((torch.randn(b, n, h, dim, generator=g) * size).to(dtype).to(device) for h in (heads, heads,
+            q_heads))
     cache = make_cache(b, (n + page - 1) // page, heads, dim, page, device)
     rot = NF.rotary_table(rotated, n, device=device) if rotated else None
     out, lengths = append_all(chunks, k, v, q, cache, rot, interleaved)
@@ -229,7 +237,8 @@ def append_case(chunks, b, page, dim, rotated, interleaved, dtype, device="cpu")
 
 
 @pytest.mark.parametrize("chunks,b", CHUNKS)
-@pytest.mark.parametrize("page,dim,rotated,interleaved", [(16, 8, 0, False), (32, 24, 24, False), (16, 80, 40, True),
+@pytest.mark.parametrize("page,dim,rotated,interleaved", [(16, 8, 0, False), (32, 24, 24, False), (16, 80,
+        40, True),
                                                           (64, 64, 20, False)])
 def test_append(chunks, b, page, dim, rotated, interleaved):
     append_case(chunks, b, page, dim, rotated, interleaved, torch.float32)
@@ -247,8 +256,10 @@ def test_append_ragged_and_bad_pages():
         assert bool((q[i, c:] == 0).all()) and bool((q[i, :c] != 0).any(-1).all())
     assert not pages[table[0, 0].long(), :, :, :7].float().isnan().any()
     assert pages[table[0, 0].long(), :, :, 7:].float().isnan().all()
-    assert pages[table[0, 1:].long()].float().isnan().all() and pages[table[2, 2].long()].float().isnan().all()
-    assert not pages[table[1, 0].long()].float().isnan().any() and not pages[table[1, 2].long(), :, :, :8].float().isnan().any()
+    assert pages[table[0, 1:].long()].float().isnan().all() and pages[table[2,
+            2].long()].float().isnan().all()
+    assert not pages[table[1, 0].long()].float().isnan().any() and not pages[table[1, 2].long(), :, :,
+            :8].float().isnan().any()
     assert not pages[table[2, 1].long(), :, :, :4].float().isnan().any()
     # left padding, a table that is too short, no sequences, no tokens
     pages, scales, table = make_cache(1, 1, 1, 8, 16)
@@ -291,14 +302,16 @@ def test_attention_rows_without_a_key():
     q = torch.randn(3, 4, 2, 8)
     lengths = torch.tensor([0, 2, 20], dtype=torch.int32)
     out = NF.paged_attention(q, pages, scales, table, lengths)
-    assert bool((out[0] == 0).all()) and bool((out[1, :2] == 0).all()) and bool((out[1, 2:] != 0).any(-1).all())
+    assert bool((out[0] == 0).all()) and bool((out[1, :2] == 0).all()) and bool((out[1,
+            2:] != 0).any(-1).all())
     counts = torch.tensor([0, 2, 9], dtype=torch.int32)
     out = NF.paged_attention(q, pages, scales, table, lengths, counts)
     assert bool((out[1, 2:] == 0).all()) and bool((out[1, 0] != 0).any(-1).all())
     table[2, 0] = -5                                   # a page that there is not
     first = NF.paged_attention(q, pages, scales, table, lengths, counts)[2]
     only = NF.paged_attention(q[2:], pages, scales, table[2:], lengths[2:], counts[2:], window=4)
-    assert torch.allclose(first[3], only[0, 3], atol=1e-6)         # 17 .. 20 of 20: what the second page holds
+    assert torch.allclose(first[3], only[0, 3],
+            atol=1e-6)         # 17 .. 20 of 20: what the second page holds
 
 
 def paged_refusals(device):
@@ -401,7 +414,8 @@ def test_sampling_settings_for_each_row():
     one = torch.ones(4)
     got = NF.sample(x, u, one, torch.full((4,), -3, dtype=torch.int32), 2 * one, -one)
     assert got.tolist() == [0, 0, 3, 0]
-    for args in ((one, torch.zeros(4, dtype=torch.int32), -one, 0 * one), (one, torch.zeros(4, dtype=torch.int32), one, 2 * one),
+    for args in ((one, torch.zeros(4, dtype=torch.int32), -one, 0 * one), (one, torch.zeros(4,
+            dtype=torch.int32), one, 2 * one),
                  (-one, torch.zeros(4, dtype=torch.int32), one, 0 * one)):
         assert NF.sample(x, u, *args).tolist() == [1, 1, 1, 1]
 
@@ -437,12 +451,14 @@ def test_bookkeeping():
     c = PagedKVCache(2, 7, 2, 16, batch=3, max_tokens=40, page=16)
     assert c.pages[0].shape == (7, 2, 2, 16, 16) and c.block_table.shape == (3, 3) and len(c.pages) == 2
     c.add([17, 0, 16])
-    assert c.fresh and c.free_pages == 4 and c.lengths.tolist() == [17, 0, 16] and c.counts.tolist() == [17, 0, 16]
+    assert c.fresh and c.free_pages == 4 and c.lengths.tolist() == [17, 0, 16] and c.counts.tolist() == [17,
+            0, 16]
     c.add(1)
     assert not c.fresh and c.counts is None and c.lengths.tolist() == [18, 1, 17] and c.free_pages == 2
     used = c.block_table[c.block_table >= 0].tolist()
     assert len(used) == len(set(used)) == 5
-    for bad, error in (([1, 40, 1], ValueError), ([1, 1], ValueError), ([1, -1, 1], ValueError), ([16, 16, 16], RuntimeError)):
+    for bad, error in (([1, 40, 1], ValueError), ([1, 1], ValueError), ([1, -1, 1], ValueError), ([16, 16,
+            16], RuntimeError)):
         before = (c.block_table.clone(), c.lengths.clone(), c.free_pages, [c.tokens(i) for i in range(3)])
         with pytest.raises(error):
             c.add(bad)
@@ -470,11 +486,13 @@ def test_generation_over_pages_is_generation(fused, window):
         cache = PagedKVCache(1, 8, 2, 16, batch=2, max_tokens=32, page=16)
         cache.add(11)
         first, present = layer(x[:, :11], layer_past=cache.layer(0), use_cache=True)
-        assert torch.allclose(first, want[:, :11], atol=1e-5)        # a prompt's first tokens: keys as they are
+        assert torch.allclose(first, want[:, :11],
+                atol=1e-5)        # a prompt's first tokens: keys as they are
         for t in range(11, 20):
             cache.add(1)
             out, present = layer(x[:, t:t + 1], layer_past=present, use_cache=True)
-            # values off by 2^-4 of themselves at most, by an eighth of that in the mean of many; weights by the keys'
+            # values off by 2^-4 of themselves at most, by an eighth of that in the mean of many; weights by
+            # the keys'
             assert (out[:, 0] - want[:, t]).norm() <= 0.1 * want[:, t].norm()
         # the same over a cache of tensors, which keeps rotated keys
         past = None

@@ -1,4 +1,5 @@
-"""Rotation by positions, the paged 8-bit cache, attention over it and sampling on the GPU, against 64 bits."""
+"""Rotation by positions, the paged 8-bit cache, attention over it and sampling on the GPU, against 64
+bits."""
 import math
 
 import pytest
@@ -34,7 +35,8 @@ def test_operands_on_the_host_are_refused():
     for call in (lambda: NF.rotary(q, q.cpu(), table), lambda: NF.rotary(q, q, table.cpu()),
                  lambda: NF.rotary(q, q, table, torch.zeros(2, dtype=torch.long)),
                  lambda: NF.sample(torch.zeros(1, 4, device="cuda"), torch.zeros(1)),
-                 lambda: NF.sample(torch.zeros(1, 4, device="cuda"), torch.zeros(1, device="cuda"), torch.ones(1))):
+                 lambda: NF.sample(torch.zeros(1, 4, device="cuda"), torch.zeros(1, device="cuda"),
+                         torch.ones(1))):
         with pytest.raises(ValueError, match="must be on"):
             call()
     pages, scales, tab = make_cache(1, 1, 1, 8, 16, "cuda")
@@ -66,9 +68,12 @@ def _rotation_bound(x, want, half):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("b,s,heads,kv,dim,rotated", [(1, 1, 1, 1, 2, 2), (2, 3, 5, 1, 8, 8), (3, 17, 16, 16, 128, 128),
-                                                      (2, 33, 8, 2, 80, 40), (1, 100, 3, 3, 72, 72), (1, 5, 2, 1, 256, 256),
-                                                      (2, 7, 40, 8, 96, 20), (1, 9, 300, 1, 24, 10), (5, 2, 4, 4, 7, 6)])
+@pytest.mark.parametrize("b,s,heads,kv,dim,rotated", [(1, 1, 1, 1, 2, 2), (2, 3, 5, 1, 8, 8), (3, 17, 16,
+        16, 128, 128),
+                                                      (2, 33, 8, 2, 80, 40), (1, 100, 3, 3, 72, 72), (1, 5,
+                                                              2, 1, 256, 256),
+                                                      (2, 7, 40, 8, 96, 20), (1, 9, 300, 1, 24, 10), (5, 2,
+                                                              4, 4, 7, 6)])
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotation(b, s, heads, kv, dim, rotated, interleaved, dtype):
     table = NF.rotary_table(rotated, 500, device="cuda")
@@ -93,7 +98,8 @@ def test_rotation(b, s, heads, kv, dim, rotated, interleaved, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("b,s,heads,dim,rotated", [(1, 1, 1, 16, 16), (2, 50, 12, 64, 64), (1, 33, 4, 80, 40), (2, 5, 3, 10, 4)])
+@pytest.mark.parametrize("b,s,heads,dim,rotated", [(1, 1, 1, 16, 16), (2, 50, 12, 64, 64), (1, 33, 4, 80,
+        40), (2, 5, 3, 10, 4)])
 def test_packed_rotation(b, s, heads, dim, rotated, dtype):
     table = NF.rotary_table(rotated, 100, device="cuda")
     qkv = torch.randn(b, s, heads, 3, dim, device="cuda").to(dtype).requires_grad_()
@@ -109,14 +115,17 @@ def test_packed_rotation(b, s, heads, dim, rotated, dtype):
 def test_rotation_strides_and_second_derivatives():
     table = NF.rotary_table(16, 64, device="cuda")
     base = torch.randn(3, 40, 6, 24, device="cuda")
-    for view in (base, base.transpose(0, 1), base[:, ::3], base[:, :, ::2], base.flip(1), base[..., 3:19], base[..., 4:20],
-                 base.expand(2, 3, 40, 6, 24)[:, 0], base.transpose(2, 3)[:, :, :16].contiguous().transpose(2, 3)):
+    for view in (base, base.transpose(0, 1), base[:, ::3], base[:, :, ::2], base.flip(1), base[..., 3:19],
+            base[..., 4:20],
+                 base.expand(2, 3, 40, 6, 24)[:, 0], base.transpose(2, 3)[:, :,
+                         :16].contiguous().transpose(2, 3)):
         for x in (view, view.bfloat16() if view is base else view):
             got = NF.rotary(x, x[:, :, :1], table, 2)
             assert torch.equal(got[0], NF.rotary(x.contiguous(), x[:, :, :1].contiguous(), table, 2)[0])
             assert torch.equal(got[0][:, :, :1], got[1])
     pos = torch.arange(80, device="cuda").view(2, 40).t()[:, 0] % 64
-    assert torch.equal(NF.rotary(base, base, table, pos)[0], NF.rotary(base, base, table, pos.contiguous())[0])
+    assert torch.equal(NF.rotary(base, base, table, pos)[0], NF.rotary(base, base, table,
+            pos.contiguous())[0])
     x = torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True)
     g = torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True)
     dx = torch.autograd.grad(NF.rotary(x, x.detach(), table)[0], x, g, create_graph=True)[0]
@@ -147,8 +156,10 @@ def test_positions_outside_of_the_table():
 # append
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("chunks,b", CHUNKS)
-@pytest.mark.parametrize("page,dim,rotated,interleaved", [(16, 8, 0, False), (32, 24, 24, False), (16, 80, 40, True),
-                                                          (64, 128, 128, False), (128, 128, 50, True), (64, 72, 20, False)])
+@pytest.mark.parametrize("page,dim,rotated,interleaved", [(16, 8, 0, False), (32, 24, 24, False), (16, 80,
+        40, True),
+                                                          (64, 128, 128, False), (128, 128, 50, True), (64,
+                                                                  72, 20, False)])
 def test_append(chunks, b, page, dim, rotated, interleaved, dtype):
     append_case(chunks, b, page, dim, rotated, interleaved, dtype, "cuda")
 
@@ -183,7 +194,8 @@ def test_append_ragged_slices_and_bad_pages():
     results = []
     for q, k, v in ([qkv[..., i, :] for i in range(3)], [qkv[..., i, :].contiguous() for i in range(3)],
                     [qkv[..., i, :].transpose(1, 2).contiguous().transpose(1, 2) for i in range(3)],
-                    [torch.empty(3, 40, 2, 65, device="cuda", dtype=torch.bfloat16)[..., 1:].copy_(qkv[..., i, :])
+                    [torch.empty(3, 40, 2, 65, device="cuda", dtype=torch.bfloat16)[..., 1:].copy_(qkv[...,
+                            i, :])
                      for i in range(3)]):
         pages, scales, table = make_cache(3, 9, 2, 64, 16, "cuda", poison=False)
         table[1, 7] = 1000
@@ -231,7 +243,8 @@ def test_append_of_many_tokens_is_the_oracle(interleaved):
     for lengths, counts in (([5, 300, 1], [5, 300, 1]), ([705, 950, 1], [700, 650, 0])):
         lengths, counts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, counts))
         got = NF.paged_append(mine[0], mine[1], k, v, mine[2], lengths, counts, q, rot, interleaved)
-        want = paged_append_reference(oracle[0], oracle[1], k, v, oracle[2], lengths, counts, q, rot, interleaved)
+        want = paged_append_reference(oracle[0], oracle[1], k, v, oracle[2], lengths, counts, q, rot,
+                interleaved)
         # products and sum in fp32 in another order, then fp16; e4m3: another side of a border now and then
         assert bool(((got.float() - want.float()).abs() <= 2.0 ** -10 * want.float().abs() + 2.0 ** -22).all())
         a, b = mine[0].float(), oracle[0].float()
@@ -261,16 +274,17 @@ def _filled(b, lengths, kv, dim, page, seed=0, spread=1.0):
 
 
 def _attention_bound(q, want, cache, lengths, counts, scale, window):
-    """How far an output may be off.  A score's sum in fp32 is off by 2^-20 of its terms' sizes at most (some 130
-    additions), which changes a weight and the weights' sum by as much of themselves, exp2 by 2^-20 more; weights are
-    rounded to fp16: 2^-11 of themselves, or 2^-25 where they are small, the largest being one; sums in fp32; one
-    rounding to the type."""
+    """How far an output may be off.  A score's sum in fp32 is off by 2^-20 of its terms' sizes at most
+    (some 130 additions), which changes a weight and the weights' sum by as much of themselves, exp2 by
+    2^-20 more; weights are rounded to fp16: 2^-11 of themselves, or 2^-25 where they are small, the largest
+    being one; sums in fp32; one rounding to the type."""
     pages, scales, table = cache
     scale = 1 / math.sqrt(q.shape[3]) if scale is None else scale
     sizes = pages.clone()
     sizes[:, 1] = pages[:, 1].float().abs().to(pages.dtype)
     size = paged_attention_reference(q.double(), sizes, scales, table, lengths, counts, scale, window)
-    values = (pages.float().nan_to_num(0.0).abs() * scales.nan_to_num(0.0)[..., None, None]).amax((0, 3))       # [2, H, W]
+    values = (pages.float().nan_to_num(0.0).abs() * scales.nan_to_num(0.0)[..., None, None]).amax((0,
+            3))       # [2, H, W]
     group = q.shape[2] // pages.shape[2]
     k, v = (x[:, :q.shape[3]].repeat_interleave(group, 0).double() for x in values)
     scores = (q.double().abs() * k).sum(-1, keepdim=True) * scale
@@ -386,7 +400,8 @@ def _sample(x, u, **kw):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (2, 33), (5, 511), (2, 2047), (3, 2048), (4, 5000), (2, 50304),
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (2, 33), (5, 511), (2, 2047), (3, 2048), (4, 5000),
+        (2, 50304),
                                         (1, 128001), (300, 700), (1, 262144)])
 @pytest.mark.parametrize("setting", range(len(SETTINGS)))
 def test_sampling(rows, vocab, setting, dtype):
@@ -420,7 +435,8 @@ def test_sampling_of_odd_rows(kind, vocab):
         x.fill_(-float("inf"))
         x[:, vocab - 1] = -5.0
     u = torch.tensor([0.0, 0.2, 0.5, 0.77, 0.999, 1.0 - 2.0 ** -24], device="cuda")
-    for kw in SETTINGS + [dict(top_k=20, top_p=0.6), dict(top_k=vocab - 1), dict(top_k=vocab // 2, top_p=0.7)]:
+    for kw in SETTINGS + [dict(top_k=20, top_p=0.6), dict(top_k=vocab - 1), dict(top_k=vocab // 2,
+            top_p=0.7)]:
         got = _sample(x, u, **kw)
         if kind == "all_masked":
             assert got[::2].eq(-1).all() and got[1] == -1
@@ -462,7 +478,8 @@ def test_sampled_shares():
 def _layers(dim, heads, window=None, dtype=torch.bfloat16):
     torch.manual_seed(0)
     rot = RotaryEmbedding(dim, 4096)
-    blocks = [FlashAttention(dim * heads, heads, fused_qkv=True, causal=True, window=window, rotary=rot) for _ in range(2)]
+    blocks = [FlashAttention(dim * heads, heads, fused_qkv=True, causal=True, window=window,
+            rotary=rot) for _ in range(2)]
     head = torch.nn.Linear(dim * heads, 1000)
     emb = torch.nn.Embedding(1000, dim * heads)
     return [m.to("cuda", dtype).eval() for m in (*blocks, head, emb)]
@@ -537,7 +554,8 @@ def test_generation_is_near_the_layer_without_a_cache():
 
 def test_training_with_rotation_has_its_gradients():
     """A rotated layer against the same by the oracles, in fp32 through the packed path and in bf16."""
-    rot = RotaryEmbedding(32, 128, interleaved=True, scaling={"type": "yarn", "factor": 4, "original_positions": 32})
+    rot = RotaryEmbedding(32, 128, interleaved=True, scaling={"type": "yarn", "factor": 4,
+            "original_positions": 32})
     layer = FlashAttention(256, 4, fused_qkv=True, causal=True, rotary=rot).to("cuda", torch.bfloat16)
     x = torch.randn(2, 100, 256, device="cuda").bfloat16().requires_grad_()
     out, _ = layer(x)
