@@ -117,11 +117,12 @@ std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>
     check_on(p, q, "rotary: positions");
     TORCH_CHECK_TYPE(p.scalar_type() == at::kLong || p.scalar_type() == at::kInt,
                      "rotary: positions of int64 or int32 required, not ", p.scalar_type());
-    TORCH_CHECK_VALUE((p.dim() == 1 && p.size(0) == c.S) || (p.dim() == 2 && p.size(0) == c.B && p.size(1) == c.S),
-                      "rotary: positions [S] or [B, S] required, not ", p.sizes());
+    TORCH_CHECK_VALUE((p.dim() == 1 && p.size(0) == c.S) ||
+                          (p.dim() == 2 && (p.size(0) == c.B || p.size(0) == 1) && p.size(1) == c.S),
+                      "rotary: positions [S], [1, S] or [B, S] required, not ", p.sizes());
     c.at.ids = p.const_data_ptr();
     c.at.ids64 = p.scalar_type() == at::kLong;
-    c.at.batch_stride = p.dim() == 2 ? p.stride(0) : 0;
+    c.at.batch_stride = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
     c.at.token_stride = p.stride(-1);
   }
   const int rc = slapo::launch_rotary(c, at::cuda::getCurrentCUDAStream().stream());

@@ -241,6 +241,7 @@ class PagedKVCache:
     tables on the device keep their addresses, so that the layers' work can be captured and replayed after
     each :meth:`add`."""
 
+    @torch.inference_mode(False)        # (tensors of inference could not be written outside of it)
     def __init__(self, layers, pages, heads, head_dim, batch, max_tokens, page=64, device=None):
         if page not in PAGE_SIZES:
             raise ValueError(f"pages of {PAGE_SIZES} tokens, not {page}")

@@ -82,8 +82,8 @@ def _check(q, k, table, positions):
     if torch.is_tensor(positions):
         if positions.dtype not in (torch.int64, torch.int32):
             raise TypeError(f"rotary: positions of int64 or int32 required, not {positions.dtype}")
-        if tuple(positions.shape) not in ((q.shape[1],), (q.shape[0], q.shape[1])):
-            raise ValueError(f"rotary: positions [S] or [B, S] required, not {tuple(positions.shape)}")
+        if tuple(positions.shape) not in ((q.shape[1],), (1, q.shape[1]), (q.shape[0], q.shape[1])):
+            raise ValueError(f"rotary: positions [S], [1, S] or [B, S] required, not {tuple(positions.shape)}")
     elif positions is not None and (isinstance(positions, bool) or not isinstance(positions, int)):
         raise TypeError(f"rotary: positions are a tensor, the first one's number or None, not {positions!r}")
 
@@ -144,7 +144,7 @@ def rotary(q, k, table, positions=None, interleaved=False):
     """Queries ``[B, S, H, D]`` and keys ``[B, S, heads, D]`` rotated by their positions: two new tensors.
 
     ``table``: :func:`rotary_table`, of the rotated part of the head; ``positions``: those of the tokens,
-    ``[S]`` or ``[B, S]``, the first one's number, or None for 0, 1, ....  A token whose position lies
+    ``[S]``, ``[1, S]`` or ``[B, S]``, the first one's number, or None for 0, 1, ....  A token whose position lies
     outside of the table (padding: -1) gets zeros and no gradient."""
     return _rotary(q, k, table, positions, interleaved)
 
@@ -175,8 +175,9 @@ class RotaryEmbedding(nn.Module):
     def table(self, device):
         device = torch.device(device)
         if device not in self._tables:
-            self._tables[device] = rotary_table(self.rotary_dim, self.max_positions, self.base,
-                    self.scaling, device)
+            with torch.inference_mode(False):      # (a table of inference could not be kept for a gradient)
+                self._tables[device] = rotary_table(self.rotary_dim, self.max_positions, self.base,
+                                                    self.scaling, device)
         return self._tables[device]
 
     def __getstate__(self):

@@ -516,6 +516,24 @@ def test_generation_over_pages_is_generation(fused, window):
         FlashAttention(32, 2, rotary=RotaryEmbedding(18, 8))
 
 
+def test_inference_mode_and_training_in_turn():
+    layer = FlashAttention(32, 2, fused_qkv=True, causal=True, rotary=RotaryEmbedding(16, 64)).eval()
+    x = torch.randn(2, 6, 32)
+    with torch.inference_mode():
+        cache = PagedKVCache(1, 4, 2, 16, batch=2, max_tokens=32, page=16)
+        cache.add(5)
+        layer(x[:, :5], layer_past=cache.layer(0))
+    out, _ = layer(x)                                  # the table that inference has made
+    assert torch.autograd.grad(out.sum(), layer.qkv.weight)[0].abs().sum() > 0
+    with torch.no_grad():                              # the cache that inference has made
+        cache.add(1)
+        layer(x[:, 5:], layer_past=cache.layer(0))
+    with torch.inference_mode():
+        cache.add(1)
+        layer(x[:, 5:], layer_past=cache.layer(0))
+    assert cache.lengths.tolist() == [7, 7]
+
+
 def test_rotated_layer_takes_positions_and_copies():
     layer = FlashAttention(32, 2, fused_qkv=True, causal=True, rotary=RotaryEmbedding(16, 64))
     x = torch.randn(1, 6, 32)
@@ -523,6 +541,8 @@ def test_rotated_layer_takes_positions_and_copies():
     a, _ = layer(x, position_ids=pos)
     b, _ = layer(x)
     assert torch.allclose(a, b, atol=1e-5)             # (distances alone count)
+    both = torch.cat([x, x])                           # one row of positions for all sequences
+    assert torch.equal(layer(both, position_ids=pos[None])[0], layer(both, position_ids=pos)[0])
     c, _ = layer(x, position_ids=torch.tensor([0, 1, 2, 3, 4, 9]))
     assert not torch.allclose(a[:, -1], c[:, -1], atol=1e-3)
     twin = copy.deepcopy(layer).bfloat16()

@@ -578,6 +578,57 @@ def test_training_with_rotation_has_its_gradients():
         assert (a.double() - b).norm() <= 8 * 2.0 ** -9 * b.norm()
 
 
+def test_inference_mode_and_training_in_turn():
+    layer = FlashAttention(128, 2, fused_qkv=True, causal=True, rotary=RotaryEmbedding(64, 64)).to(
+        "cuda", torch.bfloat16).eval()
+    x = torch.randn(2, 40, 128, device="cuda").bfloat16()
+    with torch.inference_mode():
+        cache = PagedKVCache(1, 8, 2, 64, batch=2, max_tokens=64, page=16, device="cuda")
+        cache.add(39)
+        layer(x[:, :39], layer_past=cache.layer(0))
+    out, _ = layer(x, position_ids=torch.arange(40, device="cuda")[None])
+    assert torch.equal(out, layer(x)[0])
+    assert torch.autograd.grad(out.sum(), layer.qkv.weight)[0].abs().sum() > 0
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            cache.add(1)
+            one, _ = layer(x[:, 39:], layer_past=cache.layer(0))
+            assert bool(one.isfinite().all())
+
+
+def test_prompts_captured_and_replayed():
+    """Append with its queries by a launch of their own, and attention of many rows, from a graph."""
+    rot = NF.rotary_table(64, 900, device="cuda")
+    k, v = (torch.randn(2, 400, 2, 64, device="cuda").half() for _ in range(2))
+    q = torch.randn(2, 400, 4, 64, device="cuda").half()
+    lengths = torch.tensor([400, 450], dtype=torch.int32, device="cuda")
+    cache = make_cache(2, 20, 2, 64, 32, "cuda", poison=False)
+
+    def step():
+        turned_q = NF.paged_append(cache[0], cache[1], k, v, cache[2], lengths, q=q, rotary_table=rot)
+        return turned_q, NF.paged_attention(turned_q, *cache, lengths)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for more in (0, 37):
+        lengths.add_(more)
+        cache[0].zero_()
+        cache[1].zero_()
+        want = step()
+        pages, scales = cache[0].clone(), cache[1].clone()
+        cache[0].zero_()
+        cache[1].zero_()
+        graph.replay()
+        for a, b in zip((*want, pages.float(), scales), (*got, cache[0].float(), cache[1])):
+            assert torch.equal(a, b)
+
+
 def test_streams_of_their_own():
     """Calls on a stream that is not the default one, while the default one is busy."""
     cache = _filled(4, [500] * 4, 4, 64, 64)
