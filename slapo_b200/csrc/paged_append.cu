@@ -205,7 +205,7 @@ struct PagePart {
 };
 
 // How a page's values are taken: row by row as they come (0), or all rows of all threads new ones: as they are (1), turned
-// as halves (2) or as neighbours (3) from shared memory.
+// as halves (2) or as neighbours (3), whole vectors.
 template <typename T, int kRows, int kForm>
 __device__ __forceinline__ void append_heads(const PagePart<T>& p, Turn8 turn, const float4* s_rot, float (*s_top)[kThreads / 32]) {
   const PagedCache& c = p.a.cache;
@@ -234,7 +234,8 @@ __device__ __forceinline__ void append_heads(const PagePart<T>& p, Turn8 turn, c
       next[i].values(v[i]);
       if constexpr (kForm >= 2) {
         if (turn.mode != 0) {
-          turn.take<kForm == 3>(s_rot + (p.row + i * p.rows) * p.units, p.units / p.parts);
+          if constexpr (kRows > 1) turn.take<kForm == 3>(s_rot + (p.row + i * p.rows) * p.units, p.units / p.parts);
+          else if (h == p.h0) turn.read(p.a.rot, p.first + p.row);
           if constexpr (kForm == 2) turn.halves(x + i * p.step - p.d0, v[i]);
           else turn.neighbours(v[i]);
         }
@@ -332,14 +333,12 @@ __device__ __forceinline__ void append_page(const PagedAppend& a, int tile, int 
     __syncthreads();
   }
   const Turn8 turn(d0, turned ? a.rotary : 0, a.interleaved);
-  if constexpr (kRows > 1) {
-    if (held == 0 && last == kRows * rows && places * rows == static_cast<int>(blockDim.x) && c.pitch == c.dim &&
-        (!turned || (p.shared && first + last <= a.rot_rows))) {
-      if (!turned) append_heads<T, kRows, 1>(p, turn, s_rot, s_top);
-      else if (a.interleaved) append_heads<T, kRows, 3>(p, turn, s_rot, s_top);
-      else append_heads<T, kRows, 2>(p, turn, s_rot, s_top);
-      return;
-    }
+  if (held == 0 && last == kRows * rows && places * rows == static_cast<int>(blockDim.x) && c.pitch == c.dim &&
+      (!turned || (half % (2 * parts) == 0 && first + last <= a.rot_rows))) {
+    if (!turned) append_heads<T, kRows, 1>(p, turn, s_rot, s_top);
+    else if (a.interleaved) append_heads<T, kRows, 3>(p, turn, s_rot, s_top);
+    else append_heads<T, kRows, 2>(p, turn, s_rot, s_top);
+    return;
   }
   append_heads<T, kRows, 0>(p, turn, s_rot, s_top);
 }
@@ -373,8 +372,12 @@ __device__ __forceinline__ void append_query(const PagedAppend& a, int64_t token
   }
 }
 
+// (CTAs of an SM, 8 x 1024 tokens of 16 heads of 128, us: 16-bit pages of 64 and 128 37 and 56 with two and one, 34 and 42 with three and
+// two, for some spilling; fp32 44 with two, 53 with three.)
+template <typename T, int kRows> constexpr int kCtas = (kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) + (sizeof(T) == 2 ? 1 : 0);
+
 template <typename T, int kRows>
-__global__ void __launch_bounds__(kThreads, kRows <= 2 ? 3 : kRows <= 4 ? 2 : 1) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta, int rows) {
+__global__ void __launch_bounds__(kThreads, kCtas<T, kRows>) paged_append_kernel(const PagedAppend a, int64_t tiles, int per_cta, int rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // (the queries' kernel waits for nothing of this one)
   if (blockIdx.x < tiles) append_page<T, kRows>(a, static_cast<int>(blockIdx.x), per_cta, rows);
   else append_query<T>(a, blockIdx.x - tiles);
