@@ -10,8 +10,10 @@
 // Rounding: rotation in fp32, then once to e4m3 (at most 2^-4 of the value, the halves of its steps).  Values that are
 // not finite are held as NaN and do not count for the scale.
 //
-// Bound by HBM for prompts (16 bits in, 8 bits out), by latency for a token.  A CTA takes one page of one side of one
-// head: its new values stay in registers between the maximum and their codes.  Other CTAs of the launch rotate queries.
+// Bound by HBM for prompts (16 bits in, 8 bits out), by latency for a token.  A CTA takes one page of one side, and of some
+// heads one after the other: their new values stay in registers between the maximum and their codes, the next head's
+// are read under the barrier.  Other CTAs of the launch rotate queries, or, where tokens are many, rotary.cu's kernel beside it.
+// 8 x 2048 tokens of 16 heads of 128 with their queries, bf16, pages of 64: 80 us (floor 51); one token each 6.6, of which the host has 6.4.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
