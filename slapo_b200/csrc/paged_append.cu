@@ -317,12 +317,13 @@ __device__ __forceinline__ void append_page(const PagedAppend& a, int tile, int 
   const int64_t* stride = side ? a.v_stride : a.k_stride;
   const bool turned = side == 0 && a.rot != nullptr;
   const int half = a.rotary / 2, units = half / 2, parts = a.interleaved ? 2 : 4;
+  const bool whole_places = half % (2 * parts) == 0 && (reinterpret_cast<uintptr_t>(a.rot) & 15) == 0;      // rows as float4
   const PagePart<T> p{a, h0, min(c.heads, h0 + per_cta), first, held, last, places, rows, row, d0, row < rows, row < rows && d0 < c.dim,
                       static_cast<const T*>(side ? a.v : a.k) + b * stride[0] + (first + held + row - start) * stride[1] +
                           h0 * stride[2] + d0,
                       stride[2], rows * stride[1],
                       c.pages + ((id * 2 + side) * c.heads + h0) * static_cast<int64_t>(c.page) * c.pitch + d0,
-                      c.scales + (id * 2 + side) * c.heads, turned, kRows > 1 && turned && half % (2 * parts) == 0, units, parts};
+                      c.scales + (id * 2 + side) * c.heads, turned, kRows > 1 && turned && whole_places, units, parts};
   if (p.shared) {
     const int u = threadIdx.x % units, t0 = threadIdx.x / units, tokens = blockDim.x / units;      // (at most 32 units)
     const int to = (u % parts) * (units / parts) + u / parts;
@@ -336,7 +337,7 @@ __device__ __forceinline__ void append_page(const PagedAppend& a, int tile, int 
   }
   const Turn8 turn(d0, turned ? a.rotary : 0, a.interleaved);
   if (held == 0 && last == kRows * rows && places * rows == static_cast<int>(blockDim.x) && c.pitch == c.dim &&
-      (!turned || (half % (2 * parts) == 0 && first + last <= a.rot_rows))) {
+      (!turned || (whole_places && first + last <= a.rot_rows))) {
     if (!turned) append_heads<T, kRows, 1>(p, turn, s_rot, s_top);
     else if (a.interleaved) append_heads<T, kRows, 3>(p, turn, s_rot, s_top);
     else append_heads<T, kRows, 2>(p, turn, s_rot, s_top);

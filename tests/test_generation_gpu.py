@@ -231,6 +231,28 @@ def test_append_rotates_as_rotary_does(dim, rotated, interleaved, dtype):
         assert torch.equal(pages.view(torch.uint8), other[0].view(torch.uint8))
 
 
+@pytest.mark.parametrize("page,dim,rotated,interleaved", [(64, 128, 128, False), (64, 64, 64, True), (16, 128, 128, False),
+                                                          (32, 80, 40, True), (128, 64, 32, False)])
+def test_a_table_that_starts_anywhere(page, dim, rotated, interleaved):
+    """A table on 8 bytes, not on 16: whole pages, their queries and the rotation alone."""
+    table = NF.rotary_table(rotated, 600, device="cuda")
+    odd = torch.empty(table.numel() + 2, device="cuda")[2:].view(table.shape).copy_(table)
+    assert odd.data_ptr() % 16 == 8
+    k, v = (torch.randn(2, 600, 2, dim, device="cuda").half() for _ in range(2))
+    q = torch.randn(2, 600, 4, dim, device="cuda").half()
+    results = []
+    for rot in (table, odd):
+        for n in (600, 60):
+            cache = make_cache(2, 38, 2, dim, page, "cuda", poison=False)
+            lengths = torch.full((2,), n, dtype=torch.int32, device="cuda")
+            out = NF.paged_append(cache[0], cache[1], k[:, :n], v[:, :n], cache[2], lengths, None, q[:, :n], rot,
+                                  interleaved)
+            results.append((out, cache[0].float(), cache[1], *NF.rotary(q, k, rot, None, interleaved)))
+    for a, b in zip(results[:2], results[2:]):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_append_of_many_tokens_is_the_oracle(interleaved):
     """Ragged, on top of what is there, some behind the rotation's table: queries by a launch of their own."""
