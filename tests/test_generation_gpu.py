@@ -253,6 +253,23 @@ def test_a_table_that_starts_anywhere(page, dim, rotated, interleaved):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rotated", [(96, 128), (128, 96), (95, 128), (97, 128), (127, 96), (300, 96), (128, 94),
+                                       (128, 98), (300, 128)])
+def test_a_pages_rotation_of_any_size_in_shared_memory(n, rotated, dtype):
+    """Keys of pages of 128 as those turned before, to the bit; 47 to 64 KB of the table for a page."""
+    rot = NF.rotary_table(rotated, 320, device="cuda")
+    k, v = (torch.randn(2, n, 3, 128, device="cuda").to(dtype) for _ in range(2))
+    lengths = torch.tensor([n, n + 7], dtype=torch.int32, device="cuda")
+    pos = torch.stack([torch.arange(n), torch.arange(7, n + 7)]).cuda()
+    mine, other = (make_cache(2, 3, 3, 128, 128, "cuda") for _ in range(2))
+    NF.paged_append(mine[0], mine[1], k, v, mine[2], lengths, rotary_table=rot)
+    turned_k = NF.rotary(k.float(), k.float(), rot, pos)[1]
+    NF.paged_append(other[0], other[1], turned_k, v.float(), other[2], lengths)
+    assert torch.equal(mine[0].view(torch.uint8), other[0].view(torch.uint8))
+    assert torch.equal(mine[1].nan_to_num(-1.0), other[1].nan_to_num(-1.0))
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_append_of_many_tokens_is_the_oracle(interleaved):
     """Ragged, on top of what is there, some behind the rotation's table: queries by a launch of their own."""
