@@ -238,8 +238,9 @@ class PagedKVCache:
 
     A step: :meth:`add` makes room for the new tokens of each sequence, then every layer appends and attends
     (``FlashAttention(..., layer_past=cache.layer(i))``); :meth:`free` gives a sequence's pages back.  The
-    tables on the device keep their addresses, so that the layers' work can be captured and replayed after
-    each :meth:`add`."""
+    tables on the device keep their addresses, and layers read from them how many tokens a sequence brings: their
+    work can be captured and replayed after each :meth:`add`, of whatever kind, that brings a sequence at
+    most as many tokens as the captured step is wide."""
 
     @torch.inference_mode(False)        # (tensors of inference could not be written outside of it)
     def __init__(self, layers, pages, heads, head_dim, batch, max_tokens, page=64, device=None):
@@ -254,7 +255,8 @@ class PagedKVCache:
         per = (max_tokens + page - 1) // page
         self.block_table = torch.full((batch, per), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
-        self._counts = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._counts = torch.zeros(batch, dtype=torch.int32, device=device)     # of the step
+        self._each = 0              # what all of them are, None: a list's
         self.counts = None          # of the step: None where each sequence brings all of its tokens
         self.fresh = False          # the step's tokens are the first ones of all sequences
         self.width = 0              # of the step: its most new tokens of a sequence
@@ -296,8 +298,11 @@ class PagedKVCache:
         if isinstance(counts, int):
             self.counts = None
             self.lengths.add_(counts)
+            if self._each != counts:
+                self._counts.fill_(counts)
+                self._each = counts
         else:
-            self.counts = self._counts
+            self.counts, self._each = self._counts, None
             both = torch.tensor([self._tokens, each], dtype=torch.int32).to(self.lengths.device)
             self.lengths.copy_(both[0])
             self._counts.copy_(both[1])
@@ -317,7 +322,8 @@ class PagedKVCache:
 
 
 class PagedLayer:
-    """One layer of a :class:`PagedKVCache`."""
+    """One layer of a :class:`PagedKVCache`.  Its calls always pass the counts' tensor: a captured one has to serve steps
+    in which sequences bring all of its tokens and others."""
 
     def __init__(self, cache, index):
         self.cache, self.index = cache, index
@@ -327,15 +333,15 @@ class PagedLayer:
         return self.cache.fresh
 
     def append(self, k, v, q=None, rotary_table=None, interleaved=False):
+        """The step's keys and values; returns its queries, which stay as they are without a rotation."""
         c = self.cache
         if k.shape[:2] != (c.batch, c.width):
             raise ValueError(f"the step has room for {c.width} tokens of {c.batch} sequences, not {tuple(k.shape[:2])}")
-        return paged_append(c.pages[self.index], c.scales[self.index], k, v, c.block_table, c.lengths,
-                c.counts, q,
-                            rotary_table, interleaved)
+        turned = paged_append(c.pages[self.index], c.scales[self.index], k, v, c.block_table, c.lengths, c._counts,
+                              None if rotary_table is None else q, rotary_table, interleaved)
+        return q if rotary_table is None else turned
 
     def attend(self, q, scale=None, window=None):
         c = self.cache
-        return paged_attention(q, c.pages[self.index], c.scales[self.index], c.block_table, c.lengths,
-                c.counts, scale,
-                               window)
+        return paged_attention(q, c.pages[self.index], c.scales[self.index], c.block_table, c.lengths, c._counts,
+                               scale, window)

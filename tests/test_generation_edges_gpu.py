@@ -1,0 +1,79 @@
+"""Generation over a paged cache at its edges, on the GPU: captured steps of every kind, weights far below the largest,
+values that are not finite beside rotated ones, windows of more than 2^30 keys, settings of any kind."""
+import pytest
+import torch
+
+from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------- #
+# captured steps
+def _layers(rotated, window=None):
+    torch.manual_seed(0)
+    rot = RotaryEmbedding(64, 256) if rotated else None
+    blocks = [FlashAttention(256, 4, fused_qkv=True, causal=True, window=window, rotary=rot) for _ in range(2)]
+    return [b.to("cuda", torch.bfloat16).eval() for b in blocks]
+
+
+def _run(blocks, cache, x):
+    for i, block in enumerate(blocks):
+        x = x + block(x, layer_past=cache.layer(i), use_cache=True)[0]
+    return x
+
+
+def _captured(step):
+    """A graph of a step, its output, and what the step gave before it was captured."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        before = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, out, before
+
+
+def _same(cache, other):
+    for a, b in zip((*cache.pages, *cache.scales), (*other.pages, *other.scales)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(cache.lengths, other.lengths) and torch.equal(cache.block_table, other.block_table)
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+@pytest.mark.parametrize("kept,steps", [(1, [1, [1, 0, 1], [0, 1, 1], 1, [0, 0, 0], 1]),
+                                        ([1, 0, 1], [[1, 0, 1], 1, [0, 1, 0], 1]),
+                                        (3, [3, [1, 3, 0], [3, 2, 1], 3]),
+                                        ([3, 0, 2], [[3, 0, 2], 3, [0, 3, 3], 1])])
+def test_a_captured_step_serves_every_kind_of_step(kept, steps, rotated):
+    """Replayed after steps of every kind: the same as eager ones, codes and scales among it."""
+    blocks = _layers(rotated)
+    width = kept if isinstance(kept, int) else max(kept)
+    prompt = torch.randn(3, 30, 256, device="cuda").bfloat16()
+    xs = torch.randn(len(steps), 3, width, 256, device="cuda").bfloat16()
+
+    def start():
+        cache = PagedKVCache(2, 30, 4, 64, batch=3, max_tokens=128, page=16, device="cuda")
+        cache.add([30, 17, 1])
+        _run(blocks, cache, prompt)
+        return cache
+
+    with torch.no_grad():
+        cache, other = start(), start()
+        x = xs[0].clone()
+        cache.add(kept)
+        graph, out, _ = _captured(lambda: _run(blocks, cache, x))
+        for i, step in enumerate(steps):
+            if i > 0:
+                cache.add(step)
+            x.copy_(xs[i])
+            graph.replay()
+            other.add(step)
+            other.width = width         # (a narrower step, padded: projections of other sizes round in other orders)
+            want = _run(blocks, other, xs[i])
+            each = [step] * 3 if isinstance(step, int) else step
+            for b, n in enumerate(each):
+                assert torch.equal(out[b, :n], want[b, :n])
+            _same(cache, other)
