@@ -145,7 +145,7 @@ class FlashAttention(nn.Module):
     A cache in generation is a pair of tensors, or a layer of a
     :class:`slapo_b200.ops.paged.PagedKVCache` that has made room for the tokens: keys and values go into
     its pages in 8 bits, and tokens attend over these (a prompt's first ones over the keys and values as
-    they are)."""
+    they are, but for a captured step)."""
 
     def __init__(self, hidden_size, num_attention_heads, attn_pdrop=0.0, resid_pdrop=0.0,
                  attn_op_name="auto", bias=True, output_proj=True, fused_qkv=False,

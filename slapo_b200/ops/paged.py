@@ -211,7 +211,8 @@ def paged_attention(q, pages, scales, block_table, lengths, counts=None, scale=N
 
     Keys are dealt out evenly over the GPU whatever the lengths; made for few tokens at a time (their keys
     are read again for every 32 rows of heads and tokens): a prompt's first tokens go through
-    :func:`slapo_b200.ops.functional.flash_attention`.  fp32 queries run the PyTorch reference."""
+    :func:`slapo_b200.ops.functional.flash_attention`.  fp32 queries run the PyTorch reference, which reads lengths
+    on the host: not in a capture."""
     if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
         raise ValueError(f"a window is a number of keys, 1 and more, not {window!r}")
     if torch.is_tensor(q) and q.is_cuda:
@@ -229,6 +230,8 @@ def paged_attention(q, pages, scales, block_table, lengths, counts=None, scale=N
     _check_no_gradient("paged_attention", q)
     if q.dtype in (torch.bfloat16, torch.float16) and NF._native_ok(q):
         return NF._nodes().paged_attention(q, pages, scales, block_table, lengths, counts, scale, window or 0)
+    if q.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"paged_attention: {q.dtype} queries are not captured, bf16 and fp16 are")
     return paged_attention_reference(q, pages, scales, block_table, lengths, counts, scale, window)
 
 
@@ -240,7 +243,8 @@ class PagedKVCache:
     (``FlashAttention(..., layer_past=cache.layer(i))``); :meth:`free` gives a sequence's pages back.  The
     tables on the device keep their addresses, and layers read from them how many tokens a sequence brings: their
     work can be captured and replayed after each :meth:`add`, of whatever kind, that brings a sequence at
-    most as many tokens as the captured step is wide."""
+    most as many tokens as the captured step is wide.  A captured step attends over the pages, a prompt's first
+    tokens among it."""
 
     @torch.inference_mode(False)        # (tensors of inference could not be written outside of it)
     def __init__(self, layers, pages, heads, head_dim, batch, max_tokens, page=64, device=None):
@@ -330,7 +334,9 @@ class PagedLayer:
 
     @property
     def fresh(self):
-        return self.cache.fresh
+        """Whether the step's tokens may attend over its own keys alone: the first ones of all sequences, and no
+        capture, whose replays may come when sequences have others."""
+        return self.cache.fresh and not (self.cache.lengths.is_cuda and torch.cuda.is_current_stream_capturing())
 
     def append(self, k, v, q=None, rotary_table=None, interleaved=False):
         """The step's keys and values; returns its queries, which stay as they are without a rotation."""

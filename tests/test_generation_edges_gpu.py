@@ -77,3 +77,47 @@ def test_a_captured_step_serves_every_kind_of_step(kept, steps, rotated):
             for b, n in enumerate(each):
                 assert torch.equal(out[b, :n], want[b, :n])
             _same(cache, other)
+
+
+@pytest.mark.parametrize("window", [None, 9])
+def test_a_captured_step_of_an_empty_cache_serves_later_ones(window):
+    blocks = _layers(True, window)
+    xs = torch.randn(4, 2, 20, 256, device="cuda").bfloat16()
+
+    def start():
+        return PagedKVCache(2, 20, 4, 64, batch=2, max_tokens=128, page=16, device="cuda")
+
+    with torch.no_grad():
+        cache, other = start(), start()
+        x = xs[0].clone()
+        cache.add(20)
+        graph, out, eager = _captured(lambda: _run(blocks, cache, x))
+        for i, step in enumerate((20, 20, [7, 20])):
+            if i > 0:
+                cache.add(step)
+            x.copy_(xs[i])
+            graph.replay()
+            other.add(step)
+            want = _run(blocks, other, xs[i])
+            if i == 0:          # a prompt's first tokens: over keys as they are where a call is eager, else in 8 bits
+                assert torch.equal(want, eager)
+                assert (out.float() - want.float()).norm() <= 0.1 * want.float().norm()
+                # (what the second layer has kept follows from the first one's output: taken over)
+                for a, b in zip((*other.pages, *other.scales), (*cache.pages, *cache.scales)):
+                    a.copy_(b)
+                continue
+            for b, n in enumerate([step] * 2 if isinstance(step, int) else step):
+                assert torch.equal(out[b, :n], want[b, :n])
+            _same(cache, other)
+
+
+def test_queries_in_32_bits_are_not_captured():
+    layer = FlashAttention(64, 2, fused_qkv=True, causal=True, output_proj=False).cuda().eval()
+    cache = PagedKVCache(1, 4, 2, 32, batch=2, max_tokens=32, page=16, device="cuda")
+    x = torch.randn(2, 3, 64, device="cuda")
+    with torch.no_grad():
+        cache.add(3)
+        want, _ = layer(x, layer_past=cache.layer(0))
+        with pytest.raises(RuntimeError, match="not captured"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            layer(x, layer_past=cache.layer(0))
+        assert torch.equal(layer(x, layer_past=cache.layer(0))[0], want)
