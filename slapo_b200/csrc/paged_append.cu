@@ -94,9 +94,11 @@ struct Turn8 {
       cs[2 * q + 1] = make_float2(e.z, e.w);
     }
   }
-  __device__ __forceinline__ void neighbours(float (&v)[8]) const {
+  // the first `turned` values (those behind stay: a product with 0 would be NaN where one of them is infinite)
+  __device__ __forceinline__ void neighbours(float (&v)[8], int turned = 8) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (2 * j >= turned) break;
       const float a = v[2 * j], b = v[2 * j + 1];
       v[2 * j] = turned_value(a, cs[j].x, b, -cs[j].y);
       v[2 * j + 1] = turned_value(b, cs[j].x, a, cs[j].y);
@@ -117,7 +119,7 @@ struct Turn8 {
   template <typename T>
   __device__ __forceinline__ void apply(const T* x, float (&v)[8]) const {
     if (mode == 1) halves(x, v);
-    else if (mode == 3) neighbours(v);
+    else if (mode == 3) neighbours(v, rotary - d0);
     else if (mode == 2) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -4,6 +4,9 @@ import pytest
 import torch
 
 from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
+from slapo_b200.ops import functional as NF
+from slapo_b200.ops.paged import paged_append_reference
+from test_generation_cpu import make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +124,24 @@ def test_queries_in_32_bits_are_not_captured():
         with pytest.raises(RuntimeError, match="not captured"), torch.cuda.graph(torch.cuda.CUDAGraph()):
             layer(x, layer_past=cache.layer(0))
         assert torch.equal(layer(x, layer_past=cache.layer(0))[0], want)
+
+
+# ---------------------------------------------------------------------- #
+# values beside the rotated ones
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("dim,rotated", [(24, 4), (24, 20), (128, 100), (80, 40)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_values_behind_the_rotated_ones_stay(interleaved, dim, rotated, n):
+    """Infinities and NaN behind the rotated part do not reach their neighbours."""
+    rot = NF.rotary_table(rotated, 64, device="cuda")
+    k, q = (torch.randn(2, n, h, dim, device="cuda") for h in (2, 3))
+    for x in (k, q):
+        x[0, 0, 0, rotated], x[1, n - 1, 1, rotated + 3], x[1, 0, 0, rotated + 1] = float("inf"), float("nan"), -float("inf")
+    lengths = torch.tensor([n, n + 9], dtype=torch.int32, device="cuda")
+    mine, oracle = (make_cache(2, 4, 2, dim, 16, "cuda", poison=False) for _ in range(2))
+    got = NF.paged_append(mine[0], mine[1], k, k, mine[2], lengths, q=q, rotary_table=rot, interleaved=interleaved)
+    want = paged_append_reference(oracle[0], oracle[1], k, k, oracle[2], lengths, q=q, rotary_table=rot, interleaved=interleaved)
+    assert torch.equal(got[..., rotated:].nan_to_num(5.0), q[..., rotated:].nan_to_num(5.0))
+    assert torch.equal(got.isnan(), want.isnan())
+    a, b = mine[0].float(), oracle[0].float()
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(mine[1], oracle[1])
