@@ -17,8 +17,10 @@
 // the units of all sequences and takes its share of their row, at least kLeastUnits; it writes an item (sequence, head,
 // rows) that lies wholly in its share, and leaves its part of the first and the last else, which a second kernel adds up.
 //
-// Roundings: queries to fp16 by a power of two per row (exact, but for bf16 values below 2^-28 of the row's largest),
-// probabilities to fp16 (2^-11), all else in fp32.
+// Roundings: queries to fp16 by a power of two per row (exact, but for bf16 values below 2^-28 of the row's largest);
+// weights, raised by 2^14, to fp16 as the products' operands: 2^-11 of themselves down to 2^-28 of the largest that the warp
+// has seen, below that 2^-39 of it; all else in fp32.  (With the largest as 1, weights below 2^-14 lost bits and those
+// below 2^-25 were none, while the sum had them: 6 % off where 12000 keys shared 1e-3 of the weight.)
 #include <cuda_fp8.h>
 
 #include "flash_common.cuh"
@@ -34,6 +36,8 @@ namespace {
 constexpr int warps_of(int tiles) { return tiles == 1 ? 12 : 8; }
 constexpr int kUnit = 32;          // keys: two blocks of 16
 constexpr int kLeastUnits = 2;     // of a warp's share
+constexpr float kRaise = 14.f;     // log2 of what weights are raised by (fp16 ends at 2^16)
+constexpr float kLower = 1.f / 16384.f;
 
 // What is known of the work before lengths are: the same in both kernels
 struct Plan {
@@ -325,6 +329,7 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
 
   const uint32_t q_at = ring + S::kStages * S::kStage + lane * 16;
   uint32_t q[S::kSharedQ ? 1 : N][S::kChunks][2][4];
+  // m: what a row's scores are measured by, kRaise below its largest; l: the raised weights' sum
   float factor[N][2], m[N][2], l[N][2], o[N][S::kTiles][4];
   int last[N][2];                      // the last key that a row sees, less than 0: none
   // where this lane's operands are in a block: of keys g and g + 8, of values' rows 2 t, 2 t + 1 and eight further
@@ -452,11 +457,11 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
     {
       const float2 x = read8f(base + S::kScales);
       k_scale[0] = k_scale[1] = x.x;
-      v_scale[0] = v_scale[1] = x.y;
+      v_scale[0] = v_scale[1] = x.y * kLower;
       if constexpr (kSmallPages) {
         const float2 y = read8f(base + S::kScales + 8);
         k_scale[1] = y.x;
-        v_scale[1] = y.y;
+        v_scale[1] = y.y * kLower;
       }
     }
 
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
     for (int i = 0; i < N; ++i) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float x[4], top = m[i][k];
+        float x[4], top = -INFINITY;
 #pragma unroll
         for (int block = 0; block < 2; ++block)
 #pragma unroll
@@ -488,10 +493,10 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
         for (int y = 0; y < 4; ++y) top = fmaxf(top, x[y]);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float use = top == -INFINITY ? 0.f : top;
-        grown |= top > m[i][k];
+        const float next = fmaxf(m[i][k], top - kRaise), use = next == -INFINITY ? 0.f : next;
+        grown |= next > m[i][k];
         shrink[i][k] = exp2f(m[i][k] - use);
-        m[i][k] = top;
+        m[i][k] = next;
         float sum = 0.f;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -578,6 +583,7 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
           float sum = l[i][k];
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+          sum *= kLower;
           const int in_tile = i * 8 + 2 * t + k, row = row0 + in_tile;
           if (row >= p.rows) continue;
           const bool none = last[i][k] < 0;         // (masks are not applied where all rows see all keys)

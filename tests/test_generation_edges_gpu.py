@@ -10,6 +10,8 @@ from test_generation_cpu import make_cache
 
 pytestmark = pytest.mark.gpu
 
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
 
 # ---------------------------------------------------------------------- #
 # captured steps
@@ -145,3 +147,47 @@ def test_values_behind_the_rotated_ones_stay(interleaved, dim, rotated, n):
     assert torch.equal(got.isnan(), want.isnan())
     a, b = mine[0].float(), oracle[0].float()
     assert torch.equal(a.isnan(), b.isnan()) and torch.equal(mine[1], oracle[1])
+
+
+# ---------------------------------------------------------------------- #
+# attention
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 12, 40])
+def test_weights_far_below_the_largest_count(n, dtype):
+    """A first key far ahead whose value is zero, and a long row of equal ones: their values by their exact weights.
+
+    So many items that a warp has whole sequences, under one maximum.  A weight is rounded to fp16, 2^-11 of itself
+    whatever its size; a score (up to 19) is off by 2^-20 of itself, and exp2 and the sums in fp32 are far better than
+    2^-12; the output is rounded once."""
+    batch, kv, dim, page, length = 64, 32, 64, 64, 12001
+    per = (length + page - 1) // page
+    pages = torch.zeros(per, 2, kv, page, dim, device="cuda")
+    pages[0, 0, :, 0] = 64.0                                          # keys: the first one, as 1
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pages[:, 1] = torch.rand(per, kv, page, dim, generator=g, device="cuda") * 64.0 + 32.0
+    pages[0, 1, :, 0] = 0.0
+    pages = pages.to(torch.float8_e4m3fn)
+    scales = torch.full((per, 2, kv), 2.0 ** -6, device="cuda")
+    table = torch.arange(per, dtype=torch.int32, device="cuda").repeat(batch, 1)      # (full pages, but for the last: shared)
+    lengths = torch.full((batch,), length, dtype=torch.int32, device="cuda")
+    size = torch.tensor([2.0, 2.0625, 2.125, 2.25, 2.375], device="cuda")[torch.arange(batch, device="cuda") % 5]
+    q = size[:, None, None, None].expand(batch, n, kv, dim).to(dtype)
+    got = NF.paged_attention(q, pages, scales, table, lengths).double()
+    values = (pages[:, 1].double() * 2.0 ** -6).transpose(1, 2).reshape(-1, kv, dim)[:length].cumsum(0)[length - n:]
+    others = torch.arange(length - n, length, device="cuda").double()                  # beside the first
+    for b in range(5):
+        score = float(size[b]) * 8.0
+        want = values / (others + torch.tensor(score, dtype=torch.float64).exp().item())[:, None, None]
+        off = ((got[b::5] - want) / want).abs().max()
+        assert float(off) <= HALF[dtype] + 2.0 ** -11 + 2.0 ** -12 + score * 2.0 ** -20, float(off)
+
+
+@pytest.mark.parametrize("group,length", [(1, 100), (4, 100), (20, 100), (1, 3)])
+def test_values_near_the_types_largest(group, length):
+    """The mean of equal values of 2^120."""
+    pages, scales, table = make_cache(2, 4, 2, 64, 32, "cuda", poison=False)
+    pages[:, 1] = torch.full_like(pages[:, 1].float(), 256.0).to(pages.dtype)
+    scales[:, 0], scales[:, 1] = 1.0, 2.0 ** 112
+    q = torch.zeros(2, 1, 2 * group, 64, device="cuda", dtype=torch.bfloat16)
+    got = NF.paged_attention(q, pages, scales, table, torch.tensor([length, 1], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got.float(), torch.full_like(got, 2.0 ** 120, dtype=torch.float32))
