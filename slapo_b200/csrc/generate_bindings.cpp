@@ -261,7 +261,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& pages, const Tensor& sc
   a.q_heads = static_cast<int>(q.size(2));
   a.out = out.data_ptr();
   a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))));
-  a.window = static_cast<int>(std::min<int64_t>(window, 1 << 30));
+  a.window = static_cast<int>(std::min<int64_t>(window, INT_MAX));        // (positions are below that)
   a.bf16 = q.scalar_type() == at::kBFloat16;
   Tensor scratch;
   if (out.numel() > 0) {

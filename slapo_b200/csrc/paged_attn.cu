@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(warps_of(N) * 32, 1) paged_attention_kernel(co
       missing &= ~(3u << (2 * stage));
       // keys that no row sees are zeros: a hidden code may be a NaN
       const int until = in.keys.len - key0;
-      const int from = p.a.window > 0 ? in.keys.len - in.keys.count - p.a.window + 1 - key0 : 0;
+      // (the first row's first key; no less than 1 - window: a window may have all 31 bits)
+      const int from = p.a.window > 0 ? max(until - in.keys.count, 0) + 1 - p.a.window : 0;
       const bool every = page[0] >= 0 && page[kPages - 1] >= 0 && until >= kUnit && from <= 0;
       const uint8_t* k = nullptr;
 #pragma unroll

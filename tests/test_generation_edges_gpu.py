@@ -191,3 +191,19 @@ def test_values_near_the_types_largest(group, length):
     q = torch.zeros(2, 1, 2 * group, 64, device="cuda", dtype=torch.bfloat16)
     got = NF.paged_attention(q, pages, scales, table, torch.tensor([length, 1], dtype=torch.int32, device="cuda"))
     assert torch.equal(got.float(), torch.full_like(got, 2.0 ** 120, dtype=torch.float32))
+
+
+def test_a_window_of_more_than_two_to_the_thirty_keys():
+    """One page in all places of the table but the first, whose first key outweighs all others."""
+    length, page = (1 << 30) + 1000, 128
+    pages = torch.zeros(2, 2, 1, page, 16, device="cuda")
+    pages[1, 0, 0, 0], pages[1, 1, 0, 0] = 4.0, 1.0
+    pages = pages.to(torch.float8_e4m3fn)
+    scales = torch.ones(2, 2, 1, device="cuda")
+    table = torch.zeros(1, (length + page - 1) // page, dtype=torch.int32, device="cuda")
+    table[0, 0] = 1
+    lengths = torch.tensor([length], dtype=torch.int32, device="cuda")
+    q = torch.full((1, 1, 1, 8), 8.0, device="cuda", dtype=torch.bfloat16)
+    for window in (length, length + 5, (1 << 31) - 1, 1 << 40, None):
+        assert bool((NF.paged_attention(q, pages, scales, table, lengths, window=window) == 1).all()), window
+    assert bool((NF.paged_attention(q, pages, scales, table, lengths, window=length - 1) == 0).all())
