@@ -30,7 +30,7 @@ struct RotaryCall {
   int64_t table_rows;
   RotaryPositions at;
   int64_t B, S;
-  int D, rotary;
+  int D, rotary;            // rotary 0: heads are copied, zeros where a position is none
   bool interleaved, transposed;      // transposed: the gradient's direction
   bool beside;                       // the kernel launched before may still run, and says when this one may begin
   int dtype;

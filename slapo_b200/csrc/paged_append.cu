@@ -418,7 +418,7 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
   // Many tokens: their queries by the rotation's own kernel, which has more bytes on their way, beside this one's last CTAs.
   // (Few: one launch.)
   RotaryCall r{};
-  const bool apart = a.q != nullptr && a.rot != nullptr && static_cast<int64_t>(c.B) * c.n >= 4 * sm_count();
+  const bool apart = a.q != nullptr && static_cast<int64_t>(c.B) * c.n >= 4 * sm_count();
   if (apart) {
     RotaryPart& p = r.part[0];
     p.x = a.q;
@@ -431,7 +431,7 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
     p.turn = true;
     r.parts = 1;
     r.table = a.rot;
-    r.table_rows = a.rot_rows;
+    r.table_rows = a.rot != nullptr ? a.rot_rows : INT64_MAX;
     r.at.lengths = c.lengths;
     r.at.counts = c.counts;
     r.B = c.B;

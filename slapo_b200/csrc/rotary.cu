@@ -243,7 +243,7 @@ int launch(const RotaryCall& c, cudaStream_t stream) {
 
 int launch_rotary(const RotaryCall& c, cudaStream_t stream) {
   if (c.B == 0 || c.S == 0) return 0;
-  if (c.D < 1 || c.D > 256 || c.rotary < 2 || c.rotary % 2 != 0 || c.rotary > c.D) return 1;
+  if (c.D < 1 || c.D > 256 || c.rotary < 0 || c.rotary % 2 != 0 || c.rotary > c.D) return 1;
   switch (c.dtype) {
     case 0: return launch<__nv_bfloat16>(c, stream);
     case 1: return launch<__half>(c, stream);

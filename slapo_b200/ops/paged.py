@@ -115,9 +115,9 @@ def paged_append_reference(pages, scales, k, v, block_table, lengths, counts=Non
 
 
 def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None, rotary_table=None,
-        interleaved=False):
+                 interleaved=False):
     """New tokens' keys and values ``[B, n, H, D]`` (bf16, fp16 or fp32; slices of a packed projection are
-    read in place) into the cache, in place; returns their queries (or None).
+    read in place) into the cache, in place; returns their queries, a new tensor (or None).
 
     ``rotary_table``: keys - and ``q [B, n, heads, D]`` - are rotated by their positions on the way
     (:func:`slapo_b200.ops.functional.rotary`); without one they stay as they are.  New tokens have
@@ -130,13 +130,10 @@ def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None,
     that are not finite are held as NaN.  A page's first token sets its scale anew; where a later one is too
     large for it, the page's codes are rounded to the larger scale."""
     if torch.is_tensor(k) and k.is_cuda:
-        plain_q = rotary_table is None and counts is None       # (queries stay as they are)
         fn = native.direct("paged_append")
-        out = None if fn is None else fn(pages, scales, k, v, block_table, lengths, counts,
-                None if plain_q else q,
-                                         rotary_table, interleaved)
+        out = None if fn is None else fn(pages, scales, k, v, block_table, lengths, counts, q, rotary_table, interleaved)
         if out is not None:
-            return out if q is not None and not plain_q else q
+            return None if q is None else out
     from . import functional as NF
     from .rotary import _check as check_rotary
 
@@ -156,16 +153,10 @@ def paged_append(pages, scales, k, v, block_table, lengths, counts=None, q=None,
         check_rotary(k, k, rotary_table, None)
     _check_no_gradient("paged_append", k, v, q)
     if NF._native_ok(k):
-        plain_q = rotary_table is None and counts is None
-        out = NF._nodes().paged_append(pages, scales, k, v, block_table, lengths, counts,
-                None if plain_q else q,
-                                       rotary_table, bool(interleaved))
-        return out if q is not None and not plain_q else q
-    plain_q = rotary_table is None and counts is None
-    out = paged_append_reference(pages, scales, k, v, block_table, lengths, counts, None if plain_q else q,
-            rotary_table,
-                                 interleaved)
-    return q if plain_q else out
+        out = NF._nodes().paged_append(pages, scales, k, v, block_table, lengths, counts, q, rotary_table,
+                                       bool(interleaved))
+        return None if q is None else out
+    return paged_append_reference(pages, scales, k, v, block_table, lengths, counts, q, rotary_table, interleaved)
 
 
 def paged_attention_reference(q, pages, scales, block_table, lengths, counts=None, scale=None, window=None):

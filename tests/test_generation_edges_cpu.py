@@ -4,7 +4,9 @@ import pytest
 import torch
 
 from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
+from slapo_b200.ops import functional as NF
 from slapo_b200.ops import paged
+from test_generation_cpu import make_cache
 
 
 # ---------------------------------------------------------------------- #
@@ -57,3 +59,45 @@ def test_a_steps_calls_serve_every_kind_of_step(monkeypatch, kept, now, rotated)
                  (cache.scales[0], other.scales[0]), (cache.lengths, other.lengths),
                  (cache.block_table, other.block_table)):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------- #
+# queries beside an append
+def queries_without_rotation(device):
+    """Queries that are none are zeros, with and without counts; the others as they are, in a tensor of their own."""
+    k, q = torch.randn(3, 4, 2, 8, device=device).half(), torch.randn(3, 4, 6, 8, device=device).half()
+    lengths = torch.tensor([1, 4, 9], dtype=torch.int32, device=device)
+    counts = torch.tensor([1, 4, 2], dtype=torch.int32, device=device)
+    token = torch.arange(4, device=device)
+    for each, there in ((None, lengths[:, None] - 4 + token >= 0), (counts, token < counts[:, None])):
+        cache = make_cache(3, 1, 2, 8, 16, device)
+        got = NF.paged_append(cache[0], cache[1], k, k, cache[2], lengths, each, q=q)
+        assert got.data_ptr() != q.data_ptr()
+        assert torch.equal(got, torch.where(there[:, :, None, None], q, torch.zeros_like(q)))
+    assert NF.paged_append(cache[0], cache[1], k, k, cache[2], lengths) is None
+
+
+def query_refusals(device):
+    k, q = torch.randn(2, 3, 2, 16, device=device).half(), torch.randn(2, 3, 4, 16, device=device).half()
+    pages, scales, table = make_cache(2, 2, 2, 16, 16, device)
+    lengths = torch.full((2,), 3, dtype=torch.int32, device=device)
+
+    def append(q):
+        return lambda: NF.paged_append(pages, scales, k, k, table, lengths, q=q)
+
+    yield TypeError, append(q.float())
+    yield ValueError, append(q[:, :2])
+    yield ValueError, append(q[..., :8])
+    yield ValueError, append(q[:, 0])
+    yield RuntimeError, append(q.clone().requires_grad_())
+
+
+def test_queries_without_rotation():
+    queries_without_rotation("cpu")
+
+
+@pytest.mark.parametrize("index", range(5))
+def test_query_refusals(index):
+    error, call = list(query_refusals("cpu"))[index]
+    with pytest.raises(error):
+        call()

@@ -7,6 +7,7 @@ from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
 from slapo_b200.ops import functional as NF
 from slapo_b200.ops.paged import paged_append_reference
 from test_generation_cpu import make_cache
+from test_generation_edges_cpu import queries_without_rotation, query_refusals
 
 pytestmark = pytest.mark.gpu
 
@@ -126,6 +127,29 @@ def test_queries_in_32_bits_are_not_captured():
         with pytest.raises(RuntimeError, match="not captured"), torch.cuda.graph(torch.cuda.CUDAGraph()):
             layer(x, layer_past=cache.layer(0))
         assert torch.equal(layer(x, layer_past=cache.layer(0))[0], want)
+
+
+# ---------------------------------------------------------------------- #
+# queries beside an append, settings of any kind
+def test_queries_without_rotation():
+    queries_without_rotation("cuda")
+
+
+def test_queries_of_many_tokens_without_rotation():
+    q = torch.randn(3, 700, 6, 80, device="cuda").half()
+    k = torch.randn(3, 700, 2, 80, device="cuda").half()
+    lengths = torch.tensor([700, 650, 960], dtype=torch.int32, device="cuda")
+    mine, oracle = (make_cache(3, 32, 2, 80, 32, "cuda", poison=False) for _ in range(2))
+    got = NF.paged_append(mine[0], mine[1], k, k, mine[2], lengths, q=q)
+    assert torch.equal(got, paged_append_reference(oracle[0], oracle[1], k, k, oracle[2], lengths, q=q))
+    assert bool((got[1, :50] == 0).all()) and torch.equal(mine[0].view(torch.uint8), oracle[0].view(torch.uint8))
+
+
+@pytest.mark.parametrize("index", range(5))
+def test_query_refusals(index):
+    error, call = list(query_refusals("cuda"))[index]
+    with pytest.raises(error):
+        call()
 
 
 # ---------------------------------------------------------------------- #
