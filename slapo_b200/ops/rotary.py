@@ -98,7 +98,7 @@ def turn_reference(x, table, pos, interleaved):
     else:
         rows = table.new_zeros(*pos.shape, *table.shape[1:])
     shape = ((1,) if pos.dim() == 1 else ()) + tuple(pos.shape) + (1,) * (x.dim() - 3)
-    cos, sin = (rows[..., j].reshape(shape + (-1,)) for j in (0, 1))
+    cos, sin = (rows[..., j].reshape(shape + (table.shape[1],)) for j in (0, 1))
     known = known.reshape(shape + (1,))
     half = table.shape[1]
     y = x if x.dtype == torch.float64 else x.float()

@@ -101,3 +101,12 @@ def test_query_refusals(index):
     error, call = list(query_refusals("cpu"))[index]
     with pytest.raises(error):
         call()
+
+
+def test_rotation_of_no_tokens():
+    table = NF.rotary_table(8, 4)
+    q, qkv = torch.randn(2, 3, 2, 16), torch.randn(2, 3, 2, 3, 16)
+    for part in (slice(0), (slice(None), slice(0))):
+        for got in NF.rotary(q[part], q[part][:, :, :1], table):
+            assert got.shape[:2] == q[part].shape[:2] and got.shape[3] == 16
+        assert NF.rotary_qkvpacked(qkv[part], table, 9).shape == qkv[part].shape
