@@ -140,7 +140,8 @@ class FlashAttention(nn.Module):
     over a cache as in training.
 
     ``rotary`` (:class:`slapo_b200.ops.rotary.RotaryEmbedding`): queries and keys are rotated by the tokens'
-    positions, those of ``position_ids`` or the ones that follow the cache.
+    positions, those of ``position_ids`` or the ones that follow the cache.  A sequence that is longer than its table is
+    refused, and so is a paged cache whose sequences may get longer.
 
     A cache in generation is a pair of tensors, or a layer of a
     :class:`slapo_b200.ops.paged.PagedKVCache` that has made room for the tokens: keys and values go into
@@ -247,6 +248,8 @@ class FlashAttention(nn.Module):
     def _paged(self, past, q, k, v):
         table, interleaved = None, False
         if self.rotary is not None:
+            # (of all that the cache can hold: a captured step does not come here again)
+            self.rotary.check_positions(past.cache.max_tokens, "a paged cache's sequence")
             table, interleaved = self.rotary.table(q.device), self.rotary.interleaved
         if past.fresh:
             if self.rotary is not None:

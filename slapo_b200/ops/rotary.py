@@ -160,6 +160,10 @@ class RotaryEmbedding(nn.Module):
     ``max_positions`` for the first ``rotary_dim`` values of a head (``base``, ``scaling``:
     :func:`rotary_table`).
 
+    Tokens that follow one another - their first position is a number, or none is given - have to fit the table: more
+    are refused.  Positions in a tensor are not looked at: outside of the table they give zeros
+    (:func:`rotary`).
+
     The table is no parameter and no buffer: it stays in fp32 whatever the model is cast to, and is made on
     a device when that is first used (before a capture, as a model's first pass is)."""
 
@@ -183,10 +187,21 @@ class RotaryEmbedding(nn.Module):
     def __getstate__(self):
         return {**self.__dict__, "_tables": {}}
 
+    def check_positions(self, tokens, what):
+        """Refuses a sequence of more tokens than the table has positions."""
+        if tokens > self.max_positions:
+            raise ValueError(f"{what}: {tokens} tokens, a rotation of {self.max_positions} positions")
+
+    def _check(self, x, positions):
+        if x.shape[1] > 0 and (positions is None or isinstance(positions, int)):
+            self.check_positions((positions or 0) + x.shape[1], "RotaryEmbedding")
+
     def forward(self, q, k, positions=None):
+        self._check(q, positions)
         return rotary(q, k, self.table(q.device), positions, self.interleaved)
 
     def forward_packed(self, qkv, positions=None):
+        self._check(qkv, positions)
         return rotary_qkvpacked(qkv, self.table(qkv.device), positions, self.interleaved)
 
     def extra_repr(self):

@@ -103,6 +103,31 @@ def test_query_refusals(index):
         call()
 
 
+# ---------------------------------------------------------------------- #
+# sequences longer than the rotation's table
+@pytest.mark.parametrize("fused", [False, True])
+def test_a_sequence_longer_than_the_rotations_table_is_refused(fused):
+    layer = FlashAttention(32, 2, fused_qkv=fused, causal=True, rotary=RotaryEmbedding(16, 8)).eval()
+    x = torch.randn(2, 12, 32)
+    with torch.no_grad():
+        layer(x[:, :8])
+        layer(x, position_ids=torch.arange(12).clamp(max=7))       # (positions on the device: zeros behind the table)
+        with pytest.raises(ValueError, match="8 positions"):
+            layer(x)
+        past = layer(x[:, :8], use_cache=True)[1]
+        with pytest.raises(ValueError, match="8 positions"):
+            layer(x[:, 8:9], layer_past=past)
+        # a cache whose sequences can get longer, whatever they have now: a captured step is not asked again
+        cache = PagedKVCache(1, 4, 2, 16, batch=2, max_tokens=9, page=16)
+        cache.add(1)
+        with pytest.raises(ValueError, match="8 positions"):
+            layer(x[:, :1], layer_past=cache.layer(0))
+        cache = PagedKVCache(1, 4, 2, 16, batch=2, max_tokens=8, page=16)
+        for n in (7, 1):
+            cache.add(n)
+            layer(x[:, :n], layer_past=cache.layer(0))
+
+
 def test_rotation_of_no_tokens():
     table = NF.rotary_table(8, 4)
     q, qkv = torch.randn(2, 3, 2, 16), torch.randn(2, 3, 2, 3, 16)
@@ -110,3 +135,14 @@ def test_rotation_of_no_tokens():
         for got in NF.rotary(q[part], q[part][:, :, :1], table):
             assert got.shape[:2] == q[part].shape[:2] and got.shape[3] == 16
         assert NF.rotary_qkvpacked(qkv[part], table, 9).shape == qkv[part].shape
+
+
+def test_a_rotation_past_the_end_of_its_table_is_refused():
+    rot = RotaryEmbedding(8, 8)
+    q = torch.randn(1, 3, 2, 8)
+    rot(q, q, 5), rot(q, q, -2), rot(q[:, :0], q[:, :0], 8)
+    rot.forward_packed(torch.randn(1, 8, 2, 3, 8))
+    for call in (lambda: rot(q, q, 6), lambda: rot(torch.randn(1, 9, 1, 8), torch.randn(1, 9, 1, 8)),
+                 lambda: rot.forward_packed(torch.randn(1, 9, 2, 3, 8))):
+        with pytest.raises(ValueError, match="8 positions"):
+            call()
