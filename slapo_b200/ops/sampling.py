@@ -1,12 +1,30 @@
 """The next token of each row of logits, from given random numbers (``csrc/sample.cu``)."""
 from __future__ import annotations
 
+import math
+import numbers
+import operator
+
 import torch
 
 from . import native
 
 MAX_VOCAB = 1 << 18
 UNIT = 2.0 ** 42            # weights are multiples of 1 / UNIT of the largest one's
+
+
+def _whole(top_k):
+    """A number of tokens as an int: a float of one is taken."""
+    try:
+        return operator.index(top_k)
+    except TypeError:
+        if not isinstance(top_k, numbers.Real):
+            raise TypeError(f"sample: top_k is a number of tokens, not {top_k!r}") from None
+    if not top_k >= 0:
+        raise ValueError(f"sample: top_k of 0 or more required, not {top_k}")
+    if math.isinf(top_k) or top_k != int(top_k):
+        raise TypeError(f"sample: top_k is a number of tokens, not {top_k}")
+    return int(top_k)
 
 
 def _check(logits, uniform, settings):
@@ -29,8 +47,6 @@ def _check(logits, uniform, settings):
         elif not (value >= 0 and (most is None or value <= most)):
             raise ValueError(f"sample: {name} of 0 or more{'' if most is None else ' and at most 1'} required, "
                              f"not {value}")
-        elif dtype == torch.int32 and value != int(value):
-            raise TypeError(f"sample: {name} is a number of tokens, not {value}")
 
 
 def sample_reference(logits, uniform, temperature, top_k, top_p, min_p):
@@ -80,6 +96,8 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Each setting is one number, or a tensor of one for each row (fp32; ``top_k`` int32).  A logit of -inf or
     NaN is no token; a row of nothing else gives -1.  Weights are computed in fp64 and held as multiples of
     2^-42 of the largest one's, their sums are exact: the same call gives the same token."""
+    if type(top_k) is not int and not torch.is_tensor(top_k):
+        top_k = _whole(top_k)
     if torch.is_tensor(logits) and logits.is_cuda:
         fn = native.direct("sample")
         out = None if fn is None else fn(logits, uniform, temperature, top_k, top_p, min_p)

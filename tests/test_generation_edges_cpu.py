@@ -146,3 +146,18 @@ def test_a_rotation_past_the_end_of_its_table_is_refused():
                  lambda: rot.forward_packed(torch.randn(1, 9, 2, 3, 8))):
         with pytest.raises(ValueError, match="8 positions"):
             call()
+
+
+# ---------------------------------------------------------------------- #
+# settings and tables of any kind: the same on the CPU and the GPU
+def whole_numbers(device):
+    x, u = torch.randn(2, 50, device=device), torch.rand(2, device=device)
+    assert torch.equal(NF.sample(x, u, top_k=5.0), NF.sample(x, u, top_k=5))
+    for bad, error in ((1.5, TypeError), (-1.0, ValueError), (float("nan"), ValueError), (float("inf"), TypeError),
+                       ("5", TypeError)):
+        with pytest.raises(error):
+            NF.sample(x, u, top_k=bad)
+
+
+def test_whole_numbers():
+    whole_numbers("cpu")

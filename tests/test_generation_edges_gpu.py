@@ -7,7 +7,7 @@ from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
 from slapo_b200.ops import functional as NF
 from slapo_b200.ops.paged import paged_append_reference
 from test_generation_cpu import make_cache
-from test_generation_edges_cpu import queries_without_rotation, query_refusals
+from test_generation_edges_cpu import queries_without_rotation, query_refusals, whole_numbers
 
 pytestmark = pytest.mark.gpu
 
@@ -150,6 +150,10 @@ def test_query_refusals(index):
     error, call = list(query_refusals("cuda"))[index]
     with pytest.raises(error):
         call()
+
+
+def test_whole_numbers():
+    whole_numbers("cuda")
 
 
 # ---------------------------------------------------------------------- #
