@@ -273,29 +273,33 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& pages, const Tensor& sc
   return out;
 }
 
+// (kept: a copy where rows are not one after the other, alive until the launch)
 template <typename N, typename M>
-slapo::PerRow<M> per_row(const slapo::Setting<N>& s, int64_t rows, at::ScalarType type, const Tensor& logits, const char* name) {
+slapo::PerRow<M> per_row(const slapo::Setting<N>& s, int64_t rows, at::ScalarType type, const Tensor& logits, const char* name,
+                         Tensor& kept) {
   if (!s.rows.has_value()) return {nullptr, static_cast<M>(s.value)};
   check_on(*s.rows, logits, name);
   TORCH_CHECK_TYPE(s.rows->scalar_type() == type, "sample: ", name, " of ", type, " required, not ", s.rows->scalar_type());
-  TORCH_CHECK_VALUE(s.rows->numel() == rows && s.rows->is_contiguous(), "sample: one ", name, " for each of the ", rows,
-                    " rows required");
-  return {static_cast<const M*>(s.rows->const_data_ptr()), M()};
+  TORCH_CHECK_VALUE(s.rows->numel() == rows, "sample: one ", name, " for each of the ", rows, " rows required");
+  if (s.rows->is_contiguous()) return {static_cast<const M*>(s.rows->const_data_ptr()), M()};
+  kept = s.rows->contiguous();
+  return {static_cast<const M*>(kept.const_data_ptr()), M()};
 }
 
-Tensor sample(const Tensor& logits_in, const Tensor& uniform, const slapo::Setting<double>& temperature,
+Tensor sample(const Tensor& logits_in, const Tensor& uniform_in, const slapo::Setting<double>& temperature,
               const slapo::Setting<int64_t>& top_k, const slapo::Setting<double>& top_p, const slapo::Setting<double>& min_p) {
   TORCH_CHECK_VALUE(logits_in.is_cuda() && logits_in.dim() >= 1, "sample: CUDA logits [..., vocabulary] required");
   slapo::SampleCall c{};
   c.dtype = dtype_code(logits_in, "sample");
-  check_on(uniform, logits_in, "sample: random numbers");
-  TORCH_CHECK_TYPE(uniform.scalar_type() == at::kFloat, "sample: random numbers of fp32 required, not ", uniform.scalar_type());
+  check_on(uniform_in, logits_in, "sample: random numbers");
+  TORCH_CHECK_TYPE(uniform_in.scalar_type() == at::kFloat, "sample: random numbers of fp32 required, not ",
+                   uniform_in.scalar_type());
   const int64_t vocab = logits_in.size(-1);
   TORCH_CHECK_VALUE(vocab >= 1 && vocab <= slapo::kSampleVocab, "sample: a vocabulary of 1 to ", slapo::kSampleVocab,
                     " tokens required, not ", vocab);
   const int64_t rows = logits_in.numel() / vocab;
-  TORCH_CHECK_VALUE(uniform.numel() == rows && uniform.is_contiguous(), "sample: one random number for each of the ", rows,
-                    " rows required, not ", uniform.sizes());
+  TORCH_CHECK_VALUE(uniform_in.numel() == rows, "sample: one random number for each of the ", rows, " rows required, not ",
+                    uniform_in.sizes());
   TORCH_CHECK_VALUE(temperature.rows.has_value() || temperature.value >= 0.0, "sample: a temperature of 0 or more required, not ",
                     temperature.value);
   TORCH_CHECK_VALUE(top_k.rows.has_value() || top_k.value >= 0, "sample: top_k is a number of tokens, or 0, not ", top_k.value);
@@ -305,16 +309,17 @@ Tensor sample(const Tensor& logits_in, const Tensor& uniform, const slapo::Setti
                     min_p.value);
   c10::cuda::CUDAGuard guard(logits_in.device());
   const Tensor logits = logits_in.dim() == 2 && logits_in.stride(1) == 1 ? logits_in : logits_in.reshape({rows, vocab}).contiguous();
-  Tensor out = empty(logits_in.sizes().slice(0, logits_in.dim() - 1), at::kLong, logits);
+  const Tensor uniform = uniform_in.is_contiguous() ? uniform_in : uniform_in.contiguous();
+  Tensor kept[4], out = empty(logits_in.sizes().slice(0, logits_in.dim() - 1), at::kLong, logits);
   c.logits = logits.const_data_ptr();
   c.row_stride = logits.stride(0);
   c.uniform = uniform.const_data_ptr<float>();
-  c.temperature = per_row<double, float>(temperature, rows, at::kFloat, logits, "temperature");
+  c.temperature = per_row<double, float>(temperature, rows, at::kFloat, logits, "temperature", kept[0]);
   slapo::Setting<int64_t> most = top_k;
   most.value = std::min<int64_t>(most.value, INT_MAX);
-  c.top_k = per_row<int64_t, int>(most, rows, at::kInt, logits, "top_k");
-  c.top_p = per_row<double, float>(top_p, rows, at::kFloat, logits, "top_p");
-  c.min_p = per_row<double, float>(min_p, rows, at::kFloat, logits, "min_p");
+  c.top_k = per_row<int64_t, int>(most, rows, at::kInt, logits, "top_k", kept[1]);
+  c.top_p = per_row<double, float>(top_p, rows, at::kFloat, logits, "top_p", kept[2]);
+  c.min_p = per_row<double, float>(min_p, rows, at::kFloat, logits, "min_p", kept[3]);
   c.out = out.data_ptr<int64_t>();
   c.rows = rows;
   c.vocab = static_cast<int>(vocab);

@@ -159,5 +159,22 @@ def whole_numbers(device):
             NF.sample(x, u, top_k=bad)
 
 
+def numbers_from_tables(device):
+    """Random numbers and settings that are columns of a table."""
+    g = torch.Generator().manual_seed(4)
+    x = (torch.randn(6, 70, generator=g) * 3).to(device)
+    u = torch.rand(6, 9, generator=g).to(device)
+    t, p, m = (torch.rand(6, 2, generator=g).to(device) for _ in range(3))
+    k = torch.randint(0, 70, (6, 2), generator=g).int().to(device)
+    for i in range(2):
+        got = NF.sample(x, u[:, i], t[:, i], k[:, i], p[:, i], m[:, i])
+        assert torch.equal(got, NF.sample(x, *(a[:, i].contiguous() for a in (u, t, k, p, m))))
+    assert torch.equal(NF.sample(x, u[:1, :1].expand(6, 1)), NF.sample(x, u[:1, 0].repeat(6)))
+
+
 def test_whole_numbers():
     whole_numbers("cpu")
+
+
+def test_numbers_from_tables():
+    numbers_from_tables("cpu")

@@ -7,7 +7,7 @@ from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
 from slapo_b200.ops import functional as NF
 from slapo_b200.ops.paged import paged_append_reference
 from test_generation_cpu import make_cache
-from test_generation_edges_cpu import queries_without_rotation, query_refusals, whole_numbers
+from test_generation_edges_cpu import numbers_from_tables, queries_without_rotation, query_refusals, whole_numbers
 
 pytestmark = pytest.mark.gpu
 
@@ -154,6 +154,10 @@ def test_query_refusals(index):
 
 def test_whole_numbers():
     whole_numbers("cuda")
+
+
+def test_numbers_from_tables():
+    numbers_from_tables("cuda")
 
 
 # ---------------------------------------------------------------------- #
