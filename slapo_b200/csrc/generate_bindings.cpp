@@ -43,14 +43,16 @@ void check_no_gradient(std::initializer_list<const Tensor*> inputs, const char* 
                 " has no gradient: call it under torch.no_grad()");
 }
 
-void check_rotary_table(const Tensor& table, const Tensor& x) {
+// The table as the kernels read it, pair by pair: a copy where its pairs are not one after the other on 8 bytes
+Tensor rotary_rows(const Tensor& table, const Tensor& x) {
   check_on(table, x, "rotary: the table");
   TORCH_CHECK_TYPE(table.scalar_type() == at::kFloat, "rotary: a table of fp32 required, not ", table.scalar_type());
   TORCH_CHECK_VALUE(table.dim() == 3 && table.size(2) == 2 && table.size(1) >= 1 && 2 * table.size(1) <= x.size(-1),
                     "rotary: a table [positions, rotated / 2, 2] of at most the head's ", x.size(-1), " values required, not ",
                     table.sizes());
-  TORCH_CHECK_VALUE(table.is_contiguous() && reinterpret_cast<uintptr_t>(table.const_data_ptr()) % 8 == 0,
-                    "rotary: a contiguous table required");
+  if (table.is_contiguous() && reinterpret_cast<uintptr_t>(table.const_data_ptr()) % 8 == 0) return table;
+  c10::cuda::CUDAGuard guard(x.device());
+  return table.clone(at::MemoryFormat::Contiguous);
 }
 
 Tensor heads_in_rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
@@ -72,14 +74,14 @@ slapo::RotaryPart part(const Tensor& x, const Tensor& y, bool turn, int slice = 
 }
 
 // q [B, S, H, D] and k (heads of its own), or the packed projection [B, S, H, 3, D] alone; new tensors
-std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>& k_in, const Tensor& table,
+std::tuple<Tensor, Tensor> rotary_fwd(const Tensor& q_in, const optional<Tensor>& k_in, const Tensor& table_in,
                                       const optional<Tensor>& positions, int64_t start, bool interleaved, bool transposed) {
   const bool packed = !k_in.has_value();
   TORCH_CHECK_VALUE(q_in.is_cuda() && q_in.dim() == (packed ? 5 : 4) && (!packed || q_in.size(3) == 3),
                     packed ? "rotary: a CUDA tensor [B, S, H, 3, D] required, not "
                            : "rotary: CUDA tensors [B, S, H, D] required, not ", q_in.sizes());
   const int code = dtype_code(q_in, "rotary");
-  check_rotary_table(table, q_in);
+  const Tensor table = rotary_rows(table_in, q_in);
   TORCH_CHECK_VALUE(q_in.size(-1) <= 256 && q_in.size(2) <= INT_MAX, "rotary: heads of at most 256 values required");
   c10::cuda::CUDAGuard guard(q_in.device());
   const Tensor q = heads_in_rows(q_in);
@@ -203,11 +205,12 @@ Tensor paged_append(const Tensor& pages, const Tensor& scales, const Tensor& k_i
   TORCH_CHECK_TYPE(v_in.scalar_type() == k_in.scalar_type(), "paged_append: k and v of one type required");
   TORCH_CHECK_VALUE(v_in.sizes() == k_in.sizes() && k_in.size(2) == pages.size(2), "paged_append: k and v [B, n, ", pages.size(2),
                     ", D] required, not ", k_in.sizes(), " and ", v_in.sizes());
+  Tensor table;
   if (rot.has_value()) {
-    check_rotary_table(*rot, k_in);
-    a.rot = rot->const_data_ptr<float>();
-    a.rot_rows = rot->size(0);
-    a.rotary = static_cast<int>(2 * rot->size(1));
+    table = rotary_rows(*rot, k_in);
+    a.rot = table.const_data_ptr<float>();
+    a.rot_rows = table.size(0);
+    a.rotary = static_cast<int>(2 * table.size(1));
     a.interleaved = interleaved;
   }
   c10::cuda::CUDAGuard guard(k_in.device());

@@ -172,9 +172,34 @@ def numbers_from_tables(device):
     assert torch.equal(NF.sample(x, u[:1, :1].expand(6, 1)), NF.sample(x, u[:1, 0].repeat(6)))
 
 
+def tables_in_other_strides(device):
+    """A rotation's table as a slice of a wider one, transposed, and on 4 bytes."""
+    table = NF.rotary_table(8, 40, device=device)
+    wide = torch.empty(40, 6, 3, device=device)[:, 1:5, 1:].copy_(table)
+    turned = table.permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    odd = torch.empty(table.numel() + 1, device=device)[1:].view(table.shape).copy_(table)
+    x = torch.randn(2, 9, 3, 8, device=device).half()
+    lengths = torch.tensor([9, 30], dtype=torch.int32, device=device)
+    results = []
+    for rot in (table, wide, turned, odd):
+        a, b = (x.clone().requires_grad_() for _ in range(2))
+        y, z = NF.rotary(a, b[:, :, :1], rot, 3)
+        grads = torch.autograd.grad((y, z), (a, b), (x, x[:, :, :1]))
+        pages, scales, tab = make_cache(2, 2, 3, 8, 16, device, poison=False)
+        q = NF.paged_append(pages, scales, x, x, tab, lengths, q=x, rotary_table=rot)
+        results.append((y, z, *grads, NF.rotary_qkvpacked(torch.stack([x, x, x], 3), rot, 3), q, pages.float(), scales))
+    for other in results[1:]:
+        for got, want in zip(other, results[0]):
+            assert torch.equal(got, want)
+
+
 def test_whole_numbers():
     whole_numbers("cpu")
 
 
 def test_numbers_from_tables():
     numbers_from_tables("cpu")
+
+
+def test_tables_in_other_strides():
+    tables_in_other_strides("cpu")

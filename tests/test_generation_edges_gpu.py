@@ -7,7 +7,8 @@ from slapo_b200.op import FlashAttention, PagedKVCache, RotaryEmbedding
 from slapo_b200.ops import functional as NF
 from slapo_b200.ops.paged import paged_append_reference
 from test_generation_cpu import make_cache
-from test_generation_edges_cpu import numbers_from_tables, queries_without_rotation, query_refusals, whole_numbers
+from test_generation_edges_cpu import (numbers_from_tables, queries_without_rotation, query_refusals,
+                                       tables_in_other_strides, whole_numbers)
 
 pytestmark = pytest.mark.gpu
 
@@ -158,6 +159,10 @@ def test_whole_numbers():
 
 def test_numbers_from_tables():
     numbers_from_tables("cuda")
+
+
+def test_tables_in_other_strides():
+    tables_in_other_strides("cuda")
 
 
 # ---------------------------------------------------------------------- #
