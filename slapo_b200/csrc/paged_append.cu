@@ -12,8 +12,9 @@
 //
 // Bound by HBM for prompts (16 bits in, 8 bits out), by latency for a token.  A CTA takes one page of one side, and of some
 // heads one after the other: their new values stay in registers between the maximum and their codes, the next head's
-// are read under the barrier.  Other CTAs of the launch rotate queries, or, where tokens are many, rotary.cu's kernel beside it.
-// 8 x 2048 tokens of 16 heads of 128 with their queries, bf16, pages of 64: 80 us (floor 51); one token each 6.6, of which the host has 6.4.
+// are read under the barrier.  Other CTAs of the launch rotate (or copy) queries, or, where tokens are many, rotary.cu's kernel
+// beside it.
+// 8 x 2048 tokens of 16 heads of 128, bf16, pages of 64: 55 us, with their queries 77 (floor 51); one token each 6.3, the host's time.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -443,7 +444,8 @@ int launch(const PagedAppend& a_in, cudaStream_t stream) {
     r.beside = true;
     a.q = nullptr;
   }
-  // as many heads to a CTA as leave each SM some CTAs: they share the rotation's rows
+  // as many heads to a CTA as leave each SM some CTAs: they share the rotation's rows.  (8 x 2048 tokens of 16 heads of 128 and four
+  // ragged prompts of up to 1001 tokens of 32 heads of 80, us: up to four heads 55 and 29.5, eight 56 and 36, two 64 and 28.)
   int per_cta = 4;
   while (per_cta > 1 && pages * ((c.heads + per_cta - 1) / per_cta) < 6 * sm_count()) per_cta /= 2;
   const int64_t tiles = pages * ((c.heads + per_cta - 1) / per_cta);

@@ -8,8 +8,8 @@
 // thread has one place in the heads - 16 bytes, or for halves the two places of 16 bytes that belong together - and three
 // heads on their way, so that the table's entries are read once per token and thread.  q, k (and v of a packed
 // projection, copied) are parts of one launch.  Heads whose pairs do not fill 16 bytes go value by value.
-// 4 x 2048 packed tokens of 16 heads of 128, bf16: 36 us a direction (5.6 TB/s of 201 MB); 12001 tokens of 32 and 4 heads of 80 with 40
-// rotated as neighbours, fp16: 28.
+// 4 x 2048 packed tokens of 16 heads of 128, bf16: 37 us a direction (5.4 TB/s of 201 MB); 12001 tokens of 32 and 4 heads of 80 with 40
+// rotated as neighbours, fp16: 31, as halves (20 values: value by value) 97.
 #include "common.cuh"
 #include "generate.h"
 #include "kernels.h"
@@ -120,8 +120,8 @@ struct RotaryPlace {
 };
 
 // Rows of heads that a thread has on their way at a time.  (4 x 2048 packed tokens of 16 heads of 128, and 8 x 2048 of 16 and 2
-// heads, us: three rows and up to 128 registers 39.3 and 33.2, two and 64 39.1 and 37.3, three and 80 42.9 and 39.6, two and
-// 48 53 and 46, four 38.9 and 37.2.)
+// heads, us: three rows and up to 128 registers 37.0 and 32.8, two and 64 38.7 and 35.4, three and 80 40.9 and 38.6, four and
+// 128 36.9 and 36.8.)
 constexpr int kRowsAhead = 3;
 
 // A CTA has `tokens` tokens one after the other, all heads of each: what an address takes is computed once for all of them.

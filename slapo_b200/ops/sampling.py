@@ -58,9 +58,9 @@ def sample_reference(logits, uniform, temperature, top_k, top_p, min_p):
     def each(v, dtype):
         if torch.is_tensor(v):
             return v.reshape(b, 1).to(dtype)
-        return torch.full((b, 1), float(torch.tensor(v,
-                dtype=torch.float32)) if dtype == torch.float64 else v,
-                          dtype=dtype, device=x.device)
+        if dtype == torch.float64:          # (a number of the kernel's width)
+            v = float(torch.tensor(v, dtype=torch.float32))
+        return torch.full((b, 1), v, dtype=dtype, device=x.device)
 
     temperature, top_p, min_p = (each(v, torch.float64) for v in (temperature, top_p, min_p))
     top_k = each(top_k, torch.int64)
