@@ -8,7 +8,8 @@
 // do not depend on their order, so that the same call gives the same token.
 //
 // Bound by latency: for few rows some five barriers of a cluster and twenty of a CTA; many rows come in waves of 74 in clusters of
-// four CTAs, each of which waits the same, beside the arithmetic of the weights where top_p needs all.  HBM is read once.  A cluster of CTAs has a row, a slice each in shared memory.  For top_k the largest logit of each thread is
+// four CTAs, each of which waits the same, beside the arithmetic of the weights where top_p needs all.  HBM is read once.
+// A cluster of CTAs has a row, a slice each in shared memory.  For top_k the largest logit of each thread is
 // counted in bins of (largest - x) / temperature, an eighth of a factor 2 wide, and what comes before the end of the bin of the
 // top_k-th goes to the first CTA, which sorts it and finishes the row by itself; the others leave.  top_p without top_k needs all
 // weights in the bins; where what lies before the end of the bin in which its limit falls is at most kList tokens, the first CTA

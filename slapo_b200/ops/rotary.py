@@ -193,7 +193,7 @@ class RotaryEmbedding(nn.Module):
             raise ValueError(f"{what}: {tokens} tokens, a rotation of {self.max_positions} positions")
 
     def _check(self, x, positions):
-        if x.shape[1] > 0 and (positions is None or isinstance(positions, int)):
+        if x.dim() > 1 and x.shape[1] > 0 and (positions is None or isinstance(positions, int)):
             self.check_positions((positions or 0) + x.shape[1], "RotaryEmbedding")
 
     def forward(self, q, k, positions=None):
